@@ -12,7 +12,8 @@ from dataclasses import dataclass
 
 import torch
 
-from . import attention_bf16, blas, experts, native
+from . import attention_bf16, blas, cache8, experts, native
+from .cache8 import Pool8, read_cache
 from .mixers import (act_mul, add_dyt, add_layernorm, add_normed_rmsnorm, add_rmsnorm_scaled, add_row_vector, axpby, channel_decay, channel_gate,  # noqa: F401
                      chunk_scan, chunk_scan_ok, clamped_glu, conv_bias, conv_silu_unit, conv_state_update, decay_scan, embed_sum, gate_relu_squared, gated_group_norm,
                      gelu_tanh, head_gate, head_norm_gate, latent_prepare, latent_rope_prepare, mlstm_gates, mlstm_output, qkv_prepare,
@@ -23,7 +24,7 @@ from .native import NativeError, OutOfBlocks
 __all__ = [
     "NativeError", "OutOfBlocks", "dtype_code", "embed_gather", "add_rmsnorm", "silu_mul", "linear", "linear_silu_mul",
     "silu_mul_is_fused", "qkv_fused_ok", "qkv_norm_rope_kv", "linear_tc", "device_status", "qk_norm_rope_kv", "rope_table", "rope_table_tiled",
-    "attention", "attention_rowwise", "sample", "to_float", "require_cuda_kernels",
+    "attention", "attention_rowwise", "sample", "to_float", "require_cuda_kernels", "Pool8", "read_cache",
 ]
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
@@ -409,7 +410,12 @@ def qk_norm_rope_kv(q_out: torch.Tensor, k_pool: torch.Tensor | None, v_pool: to
                     page_size: int, status: torch.Tensor, stream=None, cos_sin: torch.Tensor | None = None, weights_ahead: bool = False) -> None:
     """Per-head norm of q and k, rotation by position, q written to ``q_out`` [T, nq, d] and the
     new k, v written into their pages. ``k_pool``/``v_pool``: [pages, nkv, page_size, d], or None
-    when this entry only reads another entry's cache (then ``qkv`` holds q alone). ``weights_ahead``: as ``add_rmsnorm``'s, for both norms."""
+    when this entry only reads another entry's cache (then ``qkv`` holds q alone). ``weights_ahead``: as ``add_rmsnorm``'s, for both norms.
+    With 8-bit pools (``Pool8``) keys and values are quantised as they are written."""
+    if isinstance(k_pool, Pool8):
+        cache8.qk_norm_rope_kv(q_out, k_pool, v_pool, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim, eps, positions, row_of_token, page_indptr,
+                               page_indices, page_size, status, stream=stream, cos_sin=cos_sin)
+        return
     _check_dev(q_out, k_pool, v_pool, qkv, q_norm_w, k_norm_w, inv_freq, positions, row_of_token, page_indptr,
                page_indices, status)
     t, nq, d = q_out.shape
@@ -435,7 +441,7 @@ def qkv_fused_ok(x: torch.Tensor, w_qkv: torch.Tensor, nq: int, nkv: int, d: int
     """Whether ``qkv_norm_rope_kv`` takes this projection: a step wide enough for the 2-CTA tcgen05
     kernel to be the faster choice for the q|k|v product, bfloat16, head size 128 rotated whole (or
     not at all), even head counts (a tile's 256 columns are then two whole heads of one kind)."""
-    if TC_GEMM == "0" or not QKV_EPILOGUE or x.dtype != torch.bfloat16 or k_pool is None:
+    if TC_GEMM == "0" or not QKV_EPILOGUE or x.dtype != torch.bfloat16 or k_pool is None or isinstance(k_pool, Pool8):
         return False
     if d != 128 or rotary_dim not in (0, 128) or nq % 2 or nkv % 2 or (q_norm_w is None) != (k_norm_w is None):
         return False
@@ -610,8 +616,14 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     ``extras``: learned sink scores, a cap on the scores, a mask by blocks of positions (``AttentionExtras``).
 
     float32 runs the row-wise kernel, prompts its tiled form (bit-identical however the step was cut). bfloat16 runs the
-    tensor-core kernels when they take this head size, else the row-wise kernel too."""
+    tensor-core kernels when they take this head size, else the row-wise kernel too. 8-bit pools (``Pool8``) have kernels of their own, which take
+    no extras."""
     extras = extras if extras is not None and extras.any else None
+    if isinstance(k_pool, Pool8):
+        if extras is not None:
+            raise ValueError("attention over an 8-bit cache takes no learned sinks, cap, block mask, distance bias or kept first keys")
+        cache8.attention(out, q, k_pool, v_pool, ctx, group, scale, window, sink)
+        return
     if attention_tiled_ok(out, q, k_pool, v_pool, ctx):
         attention_tiled(out, q, k_pool, v_pool, ctx, group, scale, window, sink, extras)
         return

@@ -74,8 +74,10 @@ ATTN_TC = Module("attn_tc", ("attention_tc.cu",))
 def all_modules() -> list[Module]:
     """Every module of the package (what ``__graft_entry__.build`` compiles)."""
     from .attention_bf16 import module_for
+    from .cache8 import CACHE8, module_for as cache8_module_for
 
-    return [HOST, KERNELS, MIXERS, RECURRENCE, EXPERTS, GEMM_TC, ATTN_TC] + [module_for(d) for d in PREBUILT_HEAD_DIMS]
+    return ([HOST, KERNELS, MIXERS, RECURRENCE, EXPERTS, GEMM_TC, ATTN_TC, CACHE8] + [module_for(d) for d in PREBUILT_HEAD_DIMS]
+            + [cache8_module_for(d) for d in PREBUILT_HEAD_DIMS])
 
 
 def log(msg: str) -> None:

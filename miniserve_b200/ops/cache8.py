@@ -1,0 +1,274 @@
+"""The paged cache in 8 bits (``csrc/cache8.cuh``): its pools, the write of a step's keys and values, reading them back, and attention over
+them. ``ops.qk_norm_rope_kv`` and ``ops.attention`` take a ``Pool8`` where they take a pool of bfloat16, and come here."""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from dataclasses import dataclass
+from functools import lru_cache
+
+import torch
+
+from . import build, native
+
+_p, _i, _f, _ll = c_void_p, c_int, c_float, c_longlong
+MIN_PAGE = 8
+EXPONENT_BIAS = 127
+LARGEST, EXPONENTS = 448.0, (-60, 7)
+
+
+@dataclass(frozen=True, eq=False)
+class Pool8:
+    """Keys (or values) of one cache entry in 8 bits. ``codes`` uint8 [pages, kv_heads, page_size, d] (bits of ``torch.float8_e4m3fn``) and
+    ``exponents`` uint8 [pages, kv_heads, page_size]: number i of a head's vector is code_i * 2^(exponent - 127). The writer takes the smallest
+    exponent at which the vector's largest number is at most 448, within 2^-60 and 2^7; a vector with a number that is not finite gets 255 and reads
+    as NaN."""
+
+    codes: torch.Tensor
+    exponents: torch.Tensor
+
+    def __post_init__(self):
+        c, e = self.codes, self.exponents
+        if c.dtype != torch.uint8 or e.dtype != torch.uint8 or c.dim() != 4 or c.shape[:3] != e.shape:
+            raise ValueError(f"an 8-bit pool is uint8 codes [pages, kv_heads, page_size, d] and uint8 exponents of the first three sizes, not "
+                             f"{c.dtype} {tuple(c.shape)} and {e.dtype} {tuple(e.shape)}")
+        if c.shape[3] % 16 or not 16 <= c.shape[3] <= 256:
+            raise ValueError(f"an 8-bit cache takes head sizes that are multiples of 16 up to 256, not {c.shape[3]}")
+        if c.shape[2] < MIN_PAGE or c.shape[2] & (c.shape[2] - 1):
+            raise ValueError(f"an 8-bit cache takes pages of a power of two of at least {MIN_PAGE} tokens, not {c.shape[2]}")
+        if c.device != e.device or not c.is_contiguous() or not e.is_contiguous() or c.data_ptr() % 16 or e.data_ptr() % 8:
+            raise ValueError("an 8-bit pool's tensors lie on one device, contiguous, codes on 16 bytes and exponents on 8")
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Pool8":
+        """A pool of zeros."""
+        return cls(torch.zeros((pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device),
+                   torch.zeros((pages, kv_heads, page_size), dtype=torch.uint8, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def takes(head_dim: int, page_size: int) -> bool:
+    """Whether an 8-bit cache can hold heads of this size in pages of this many tokens."""
+    return head_dim % 16 == 0 and 16 <= head_dim <= 256 and page_size >= MIN_PAGE and page_size & (page_size - 1) == 0
+
+
+CACHE8 = build.Module("cache8", ("cache8.cu",))
+
+
+def module_for(head_dim: int) -> build.Module:
+    return build.Module(f"attn_cache8_d{head_dim}", ("attention_cache8.cu",), defines=(f"MS_HEAD_DIM={head_dim}",))
+
+
+@lru_cache(maxsize=None)
+def _cache_lib():
+    lib = ctypes.CDLL(str(build.ensure_built(CACHE8)))
+    native._declare(lib, "ms_cache8_last_error", [], c_char_p)
+    native._declare(lib, "ms_cache8_set_pdl", [_i], None)
+    native._declare(lib, "ms_cache8_write", [_p] * 14 + [_i] * 5 + [_f, _i, _ll, _p, _p])
+    native._declare(lib, "ms_cache8_read", [_p] * 10 + [_i] * 4 + [_ll, _p, _i, _p])
+    lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
+    return lib
+
+
+def _cache_check(rc: int) -> None:
+    native.kernel_check(rc, lib=_cache_lib() if rc else None, errfn="ms_cache8_last_error")
+
+
+class _Split(ctypes.Structure):
+    """``Split8`` of csrc/attention_cache8.cu."""
+
+    _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part_o", "part_ml", "counters")] + [
+        (n, _i) for n in ("rows", "tiles", "nq", "nkv", "window", "sink", "page_size", "splits")] + [("scale", _f), ("num_pages", _i)]
+
+
+@lru_cache(maxsize=None)
+def _attn_lib(head_dim: int):
+    lib = ctypes.CDLL(str(build.ensure_built(module_for(head_dim))))
+    pre = f"ms_attn_cache8_d{head_dim}_"
+    last_error = native._declare(lib, pre + "last_error", [], c_char_p)
+    native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
+    return native._declare(lib, pre + "split", [_p] * 7 + [_p]), last_error
+
+
+def _on(device: torch.device):
+    """The launches of the block go to ``device``, whichever is current (None: it is)."""
+    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream_of(stream, device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+
+
+def _check_tables(device: torch.device, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError("positions, rows, page tables and the status word are contiguous int32 tensors on the pools' device")
+
+
+def _check_pools(k: Pool8, v: Pool8) -> None:
+    if not isinstance(k, Pool8) or not isinstance(v, Pool8):
+        raise TypeError("keys and values are both in 8 bits or both not")
+    if k.shape != v.shape or k.device != v.device:
+        raise ValueError(f"the pools of keys and values differ: {tuple(k.shape)} on {k.device}, {tuple(v.shape)} on {v.device}")
+    if not k.codes.is_cuda:
+        raise ValueError("kernel operands must be contiguous CUDA tensors")
+
+
+def _launch(device: torch.device, call) -> None:
+    guard = _on(device)
+    if guard is None:
+        call()
+    else:
+        with guard:
+            call()
+
+
+def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim: int, eps: float, positions, row_of_token,
+                    page_indptr, page_indices, page_size: int, status, stream=None, cos_sin=None) -> None:
+    """``ops.qk_norm_rope_kv`` with keys and values quantised into 8-bit pools: what is rounded is the float32 number behind norm and rotation
+    (values: as projected). A token whose position its row's table has no page for raises the status word and is not written."""
+    _check_pools(k_pool, v_pool)
+    t, nq, d = q_out.shape
+    pages, nkv, held, dim = k_pool.shape
+    dev = k_pool.device
+    if held != page_size or dim != d or qkv.shape != (t, (nq + 2 * nkv) * d):
+        raise ValueError(f"q is {tuple(q_out.shape)}, the projection {tuple(qkv.shape)}, the pools {tuple(k_pool.shape)}, the page size {page_size}")
+    for x, n in ((q_out, None), (qkv, None), (q_norm_w, d), (k_norm_w, d)):
+        if x is not None and (x.dtype != torch.bfloat16 or x.device != dev or not x.is_contiguous() or x.data_ptr() % 16 or (n and x.numel() != n)):
+            raise ValueError("an 8-bit cache is written from contiguous bfloat16 tensors on its device, on 16 bytes; norm weights have the head's size")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2 or inv_freq.device != dev or not inv_freq.is_contiguous()):
+        raise ValueError("inv_freq is float32 [rotary_dim / 2] on the pools' device")
+    if inv_freq is None:
+        cos_sin = None
+    if cos_sin is not None and (cos_sin.dtype != torch.float32 or cos_sin.shape != (t, rotary_dim) or not cos_sin.is_contiguous() or cos_sin.device != dev):
+        raise ValueError("cos_sin is float32 [tokens, rotary_dim], contiguous, on the pools' device")
+    _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
+    if positions.numel() < t or row_of_token.numel() < t:
+        raise ValueError(f"{t} tokens need as many positions and rows")
+
+    def ptr(x):
+        return None if x is None else x.data_ptr()
+
+    _launch(dev, lambda: _cache_check(_cache_lib().ms_cache8_write(
+        q_out.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(), qkv.data_ptr(),
+        ptr(q_norm_w), ptr(k_norm_w), ptr(inv_freq), ptr(cos_sin), positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(),
+        page_indices.data_ptr(), t, nq, nkv, d, rotary_dim if inv_freq is not None else 0, float(eps), page_size, pages, status.data_ptr(),
+        _stream_of(stream, dev))))
+
+
+def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: Pool8, positions: torch.Tensor, row_of_token: torch.Tensor,
+               page_indptr: torch.Tensor, page_indices: torch.Tensor, status: torch.Tensor, stream=None) -> None:
+    """The cached keys and values of given tokens as dense rows: ``k_out``, ``v_out`` [N, kv_heads, d], bfloat16 (exact) or float32 (exact), row i what
+    the cache holds at position ``positions[i]`` of row ``row_of_token[i]`` of the page table. A position without a page raises the status word and
+    leaves its row as it was."""
+    _check_pools(k_pool, v_pool)
+    pages, nkv, page_size, d = k_pool.shape
+    dev, n = k_pool.device, k_out.shape[0]
+    if k_out.shape != (n, nkv, d) or v_out.shape != k_out.shape or positions.numel() < n or row_of_token.numel() < n:
+        raise ValueError(f"rows {tuple(k_out.shape)} and {tuple(v_out.shape)} of pools {tuple(k_pool.shape)}, {positions.numel()} positions, {row_of_token.numel()} rows")
+    if k_out.dtype not in (torch.bfloat16, torch.float32) or v_out.dtype != k_out.dtype:
+        raise TypeError(f"a cache is read as bfloat16 or float32, not {k_out.dtype} and {v_out.dtype}")
+    for x in (k_out, v_out):
+        if x.device != dev or not x.is_contiguous() or x.data_ptr() % 16:
+            raise ValueError("the rows are contiguous, on 16 bytes, on the pools' device")
+    _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
+    _launch(dev, lambda: _cache_check(_cache_lib().ms_cache8_read(
+        k_out.data_ptr(), v_out.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(),
+        positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), n, nkv, d, page_size, pages, status.data_ptr(),
+        0 if k_out.dtype == torch.float32 else 1, _stream_of(stream, dev))))
+
+
+# ------------------------------------------------------------------ attention
+ROWS = 16  # query rows (tokens times the heads of a kv head) of a CTA
+
+
+def choose_splits(items: int, keys: int | None, sm_count: int) -> int:
+    """How many ways the keys of an item (a tile of 16 query rows and a kv head) are shared out: two CTAs a multiprocessor, at least 128 keys
+    a split. ``keys`` None (inside a CUDA graph for short contexts): a few thousand are assumed."""
+    by_len = 16 if keys is None else max(1, -(-keys // 128))
+    return max(1, min(2 * sm_count // max(items, 1), by_len, 64))
+
+
+def _workspace(ctx, floats: int, ints: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Partial results and tickets (zero before the first launch, left zero by every launch) of steps that run one after the other. What is outgrown
+    stays alive for graphs that hold its address; a capture that needs more than there is gets its own."""
+    held = ctx.scratch.get("cache8")
+    if held is not None and held[0].numel() >= floats and held[1].numel() >= ints:
+        return held
+    new = (torch.empty(2 * floats, dtype=torch.float32, device=device), torch.zeros(max(4096, 2 * ints), dtype=torch.int32, device=device))
+    ctx.scratch.setdefault("retired", []).append(new)
+    if not torch.cuda.is_current_stream_capturing():
+        ctx.scratch["cache8"] = new
+    return new
+
+
+def _split_plan(ctx, group: int, first: int, rows: int, most: int, keys: int | None, nq: int, nkv: int, d: int, scale: float, window: int, sink: int, page_size: int,
+                pages: int, device) -> _Split:
+    tiles = -(-most * (nq // nkv) // ROWS)
+    items = rows * tiles * nkv
+    splits = choose_splits(items, keys, ctx.sm_count)
+    part_o = part_ml = counters = None
+    if splits > 1:
+        need = items * splits * ROWS
+        buf, tickets = _workspace(ctx, need * (d + 2), items, device)
+        part_o, part_ml, counters = buf.data_ptr(), buf.data_ptr() + 4 * need * d, tickets.data_ptr()
+    skip = 4 * first  # the per-row tables are int32
+    return _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
+                  ctx.status.data_ptr(), part_o, part_ml, counters, rows, tiles, nq, nkv, window, sink, page_size, splits, scale, pages)
+
+
+def _plans(ctx, group: int, key: tuple, device) -> list:
+    """The launches of a step's attention, the same for every layer with these sizes and this window."""
+    nq, nkv, d, scale, window, sink, page_size, pages = key
+    known = ctx.max_kv_len if not ctx.graph_bucket else (ctx.graph_kv_len or None)
+    if known is not None and window:
+        known = min(known, window + ctx.max_q_len)
+    single, out = ctx.leading_single_rows, []
+    for first, rows, most in ((0, single, 1), (single, ctx.num_rows - single, ctx.max_q_len)):
+        if rows > 0:
+            out.append(_split_plan(ctx, group, first, rows, most, known, nq, nkv, d, scale, window, sink, page_size, pages, device))
+    return out
+
+
+def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
+    """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
+    ``group``, window and sink as there. A row's page that its table or the pool does not have raises the status word. Partial results lie in
+    ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
+    if getattr(ctx, "recorder", None) is not None:
+        # a pass that is captured for steps of other lengths too: launched anew for each, between the graphs
+        ctx.recorder.defer(lambda step: attention(out, q, k_pool, v_pool, step, group, scale, window, sink))
+        return
+    t, nq, d = q.shape
+    pages, nkv, page_size, dim = k_pool.shape
+    key = (nq, nkv, d, float(scale), int(window or 0), int(bool(sink)), page_size, pages)
+    plans = ctx.step_cache.get(("cache8", group, key))
+    if plans is None:
+        _check_pools(k_pool, v_pool)
+        if dim != d or nq % nkv or int(window or 0) < 0:
+            raise ValueError(f"{nq} query heads of {d} over pools {tuple(k_pool.shape)}, window {window}")
+        _check_tables(k_pool.device, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
+        plans = ctx.step_cache[("cache8", group, key)] = _plans(ctx, group, key, k_pool.device)
+    dev = k_pool.codes.device
+    if not (out.shape == q.shape and v_pool.shape == k_pool.shape and q.dtype == out.dtype == torch.bfloat16 and q.device == out.device == v_pool.codes.device == dev
+            and q.is_contiguous() and out.is_contiguous()):
+        raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape, and pools of one shape, on one device")
+    split, last_error = _attn_lib(d)
+    stream = ctx.stream
+
+    def launch():
+        for plan in plans:
+            rc = split(ctypes.addressof(plan), out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
+                       v_pool.exponents.data_ptr(), stream)
+            native.LAUNCHES[0] += 1
+            if rc:
+                raise native.NativeError(last_error().decode())
+
+    _launch(dev, launch)
