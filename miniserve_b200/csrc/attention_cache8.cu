@@ -4,13 +4,20 @@
 // Formula: softmax(scale q k^T + causal mask) v; query head h reads kv head h / (heads / kv_heads), the query at position p sees keys 0..p or
 // the last `window` of them, a sink adds exp(0) to the denominator (miniserve/model/attention.py:60-67, 125-133).
 //
-// A CTA takes 16 query rows (consecutive tokens of a request times the query heads of one kv head) and a share of their keys; its four warps
-// take 16-key slices in turn. Codes become float16 (exact: e4m3 has 4 significant bits) and both products run on mma.sync with float32 sums:
+// Both products run on mma.sync with float32 sums, keys (and the head's channels) along the instruction's 16 rows and query rows along its 8
+// columns: S^T = K Q^T, O^T = V^T P^T, so the few query rows of a decode step fill it. Codes become float16 (exact: e4m3 has 4 significant bits):
 //   s_j = (q' . code_j) * qf * 2^ek_j,          q' = q * 2^sh in float16, with sh so that the row's largest |q'| lies in [2^14, 2^15): q's 8
 //                                               significant bits are kept down to 2^-29 of the largest; qf = scale * log2(e) * 2^-sh
-//   m = max_j (s_j + ev_j) - 14                 running, over scores and the values' exponents together
-//   o = sum_j 2^(s_j + ev_j - m) code(v_j),     l = sum_j 2^(s_j - m)
-// so a weight with its value's scale is at most 2^14, a float16 with 11 significant bits down to 2^-28 of the largest; l and o are float32.
+//   m + c >= max_j (s_j + ev_j) - 8             of scores and the values' exponents together, in two parts: m a largest score, c the rest (scores may be so
+//                                               large that an exponent is lost beside them); moves only when it is passed by more than 8
+//   o = sum_j 2^(s_j - m - c + 6 + ev_j) code(v_j),      l = sum_j 2^(s_j - m - c + 6)
+// so a weight with its value's scale is at most 2^14, a float16 with 11 significant bits down to 2^-20 of the largest; l and o are float32.
+//
+// Work: up to 8 or 16 query rows (consecutive tokens of a request times the query heads of a kv head) and a kv head are an item; all items' slices of 32
+// keys in a row are cut into equal runs, one a warp, whatever the requests' lengths. Each warp has a ring of stages of its own, filled by 16-byte
+// copies that run on from item to item. What a warp has of an item that other warps of its CTA share lies in shared memory; the last of them to get
+// there adds the pieces up in the warps' order. Items cut by a CTA's end leave one piece a CTA in global memory for a second small kernel. The
+// lengths are read on the device, so a captured launch serves every context.
 #include "cache8.cuh"
 
 #ifndef MS_HEAD_DIM
@@ -22,29 +29,25 @@ namespace ms {
 constexpr int D = MS_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 up to 256");
 constexpr int CHUNKS = D / 16;                       // 16-byte chunks of a row of codes
-constexpr int KSTEPS = D / 16, DTILES = D / 8;
+constexpr int KSTEPS = D / 16, MTILES = D / 16;    // of q k^T along the head, of v^T p^T down it
 constexpr int WIDE = D / 64, REST = (D % 64) / 16;   // k-steps of q k^T whose codes come four by four, and one by one
 constexpr int VB = D % 128 == 0 ? 16 : (D % 64 == 0 ? 8 : 4), VBLOCKS = D / (8 * VB), VTAIL = D % 32 / 16;  // how a lane reads values: VB bytes a block
-constexpr int QPAD = D + 8;                          // float16 row stride of q in shared memory
-constexpr bool Q_IN_REGS = D <= 128;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int SLICE = 16, WARPS = 4, THREADS = WARPS * 32, STAGES = 3, ROWS = 16;
+constexpr int SLICE = 32, ROWS = 16;                 // keys of a slice; the most query rows of an item
 constexpr int ROW_BYTES = D % 64 == 0 ? D : D + 16;
-constexpr int STAGE_BYTES = 2 * SLICE * ROW_BYTES + 2 * SLICE;  // K codes, V codes, K exponents, V exponents
-static_assert(STAGE_BYTES % 16 == 0, "");
+constexpr int CODE_BYTES = SLICE * ROW_BYTES, STAGE_BYTES = 2 * CODE_BYTES + 2 * SLICE;  // K codes, V codes, K exponents, V exponents
+// Warps of a CTA and stages of a warp's ring: one stage is worked on, the others are on their way.
+constexpr int warps_of(int nt) { return D > 128 ? 4 : (D > 64 && nt == 1 ? 7 : 8); }
+constexpr int stages_of(int nt) { return D > 128 ? 2 : (D <= 64 ? 4 : (nt == 1 ? 3 : 2)); }
+constexpr int PART = D + 4;                          // floats of a row's partial: o, m, l, c (and one that keeps rows on 16 bytes)
+constexpr int MAX_UNITS = 256;                       // (request, tile) pairs of a launch
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;  // 0: zero-filled, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n));
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 8 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(n));
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;\n" ::"r"(dst), "l"(src)); }
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src)); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -55,13 +58,27 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// over the eight lanes of equal lane % 4
+__device__ __forceinline__ float oct_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float oct_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// an 8 x 8 tile of float16 pairs, rows across lane groups, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t at) {
   uint32_t v;
@@ -85,8 +102,8 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[BYTES / 4], uint32_t at)
   if constexpr (BYTES == 4) v[0] = lds32(at);
 }
 
-// Where chunk `chunk` of row `row` of a slice lies. Head sizes of whole 128s and 64 swizzle their chunks so that neither the reads of keys (8 rows,
-// 4 lanes a row) nor those of values (4 rows of every second, the lanes of a row side by side) meet in a bank.
+// Where chunk `chunk` of row `row` of a slice lies: chunks are swizzled so that the reads of keys (8 rows, 4 lanes a row) do not meet in a bank, nor
+// those of values (4 rows of every second, the lanes of a row side by side).
 __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
   if (D % 128 == 0) return row * ROW_BYTES + ((chunk ^ (row & 7)) << 4);
   if (D == 64) return (row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ (2 * ((row >> 1) & 3))) << 4);
@@ -109,323 +126,664 @@ struct Split8 {
   const int* page_indptr;   // [rows + 1]
   const int* page_indices;
   int* status;
-  float* part_o;            // splits > 1: [item][split][16][D] and [item][split][16][2], an item a (row, tile, kv head)
-  float* part_ml;
-  int* counters;            // [items], zero before the first launch, left zero by every launch
-  int rows, tiles;          // tiles of 16 query rows a request has at most
-  int nq, nkv, window, sink, page_size, splits;
+  float* part;              // [2 * ctas][16][PART]: a CTA's partial of the item that began before it, and of the one that goes on behind it
+  int4* cut;                // [ctas]: of the cut item that begins in the CTA, its first query row (counted in tokens x heads of a kv head), rows, kv head and pieces; 0 pieces: none does
+  int rows, tile0, tiles;   // requests; tiles [tile0, tile0 + tiles) of 8 or 16 query rows of each
+  int nq, nkv, window, sink, page_size, ctas;
   float scale;
   int num_pages;
 };
 
-// One slice (16 keys from key0 on) on its way into a stage; keys outside [lo, hi), and those of pages that the table or the pool does not have, are zeros.
-__device__ __forceinline__ void load_slice(uint32_t st, const uint8_t* k_codes, const uint8_t* k_exps, const uint8_t* v_codes, const uint8_t* v_exps,
-                                           const int* pages, int entries, const Split8& p, int kvh, int page_shift, int key0, int lo, int hi, int lane) {
-  // lanes 0 and 1: the pages of the slice's two halves of 8 keys
-  long long base = -1;  // row of the pool that the half's first key lies in
-  if (lane < 2) {
-    const int key = key0 + 8 * lane;
-    if (key + 8 > lo && key < hi) {
-      const int entry = key >> page_shift, page = entry < entries ? pages[entry] : -1;
-      if (page >= 0 && page < p.num_pages)
-        base = (((long long)page * p.nkv + kvh) << page_shift) + (key & ((1 << page_shift) - 1));
-      else
-        atomicExch(p.status, 2);
-    }
-  }
-  const long long base0 = __shfl_sync(0xffffffffu, base, 0), base1 = __shfl_sync(0xffffffffu, base, 1);
-#pragma unroll
-  for (int idx = lane; idx < SLICE * CHUNKS; idx += 32) {
-    const int row = idx / CHUNKS, chunk = idx - row * CHUNKS;
-    const long long b = row < 8 ? base0 : base1;
-    const bool valid = b >= 0 && key0 + row >= lo && key0 + row < hi;
-    const size_t off = valid ? (size_t)(b + (row & 7)) * D + chunk * 16 : 0;
-    cp_async16(st + chunk_at(row, chunk), k_codes + off, valid);
-    cp_async16(st + SLICE * ROW_BYTES + chunk_at(row, chunk), v_codes + off, valid);
-  }
-  if (lane < 4) {  // exponents, 8 at a time
-    const long long b = (lane & 1) ? base1 : base0;
-    const uint8_t* src = lane < 2 ? k_exps : v_exps;
-    cp_async8(st + 2 * SLICE * ROW_BYTES + lane * 8, src + (b >= 0 ? b : 0), b >= 0);
-  }
+// The keys that a tile of query rows sees: those that some row does [lo, hi), those that all do [seen_lo, seen_hi).
+struct Span {
+  int lo, hi, seen_lo, seen_hi, first_slice;
+};
+__device__ __forceinline__ Span span_of(const Split8& p, int start, int row0, int rows_here, int group) {
+  const int first = start + row0 / group, last = start + (row0 + rows_here - 1) / group;
+  Span s;
+  s.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+  s.hi = last + 1;
+  s.seen_lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
+  s.seen_hi = first + 1;
+  s.first_slice = s.lo / SLICE;
+  return s;
 }
 
-__global__ void __launch_bounds__(THREADS)
+constexpr float ABOVE = 6.f, SLACK = 8.f;  // weights are in units of 2^(m + c - ABOVE); m + c is passed by at most SLACK
+constexpr float START = -1e30f, NOTHING = -3e38f;  // c before the first key (m is 0 then); m of a partial without one
+
+// o, m and l of a row, added up: out = o / l (a sink's term in the denominator), zero where no key was seen
+__device__ __forceinline__ float sink_term(int sink, float m, float c) { return sink ? exp2f((ABOVE - c) - m) : 0.f; }
+
+// What a CTA knows of a (request, tile) pair.
+struct Unit {
+  int at;                    // slices of all kv heads before it
+  int n, stride;             // its slices of one kv head; how far apart its kv heads lie in the row of slices (n, or more: see `alone`)
+  int tok0, start, row0, rows_here;
+  int table, entries;        // of its request in page_indices
+};
+
+// NT: tiles of 8 query rows of an item, 1 or 2
+template <int NT>
+__global__ void __launch_bounds__(warps_of(NT) * 32, 1)
 attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_codes,
-                         const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const Split8 p) {
-  const int *cu_q = p.cu_q, *q_start = p.q_start, *page_indptr = p.page_indptr, *page_indices = p.page_indices;
-  pdl_prologue(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
+                         const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const Split8 p, int part_rows) {
+  constexpr int TILE_ROWS = 8 * NT, WARPS = warps_of(NT), THREADS = WARPS * 32, STAGES = stages_of(NT);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ Unit table[MAX_UNITS + 1];
+  __shared__ int scan[3][WARPS], arrived[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, group = p.nq / p.nkv;
-  const int split = blockIdx.x % p.splits, place = blockIdx.x / p.splits, r = place / p.tiles, tile = place - r * p.tiles;
-  const int tok0 = cu_q[r], rows_all = (cu_q[r + 1] - tok0) * group;
-  const int row0 = tile * ROWS;
-  if (row0 >= rows_all) return;
-  const int rows_here = min(ROWS, rows_all - row0), start = q_start[r];
-  const int q_first = start + row0 / group, q_last = start + (row0 + rows_here - 1) / group;
-  const int lo = p.window > 0 ? max(0, q_first - p.window + 1) : 0, hi = q_last + 1;
-  const int first_slice = lo / SLICE, end_slice = (hi + SLICE - 1) / SLICE;
-  const int per_split = (end_slice - first_slice + p.splits - 1) / p.splits;
-  const int s_begin = first_slice + split * per_split, s_end = min(end_slice, s_begin + per_split);
+  const int *cu_q = p.cu_q, *q_start = p.q_start, *page_indptr = p.page_indptr, *page_indices = p.page_indices;
+  if (tid < WARPS) arrived[tid] = 0;
+  pdl_prologue(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
+
+  const int group = p.nq / p.nkv, units = p.rows * p.tiles;
+  // ---- where every tile's slices begin: a scan over the tiles, in order
+  int live, total;
+  {
+    const int each = (units + THREADS - 1) / THREADS, first = tid * each;
+    int slices = 0, count = 0, longest = 0;
+    Unit mine;
+    auto unit_of = [&](int u) {
+      const int r = u / p.tiles, rows_all = (cu_q[r + 1] - cu_q[r]) * group;
+      mine.tok0 = cu_q[r];
+      mine.start = q_start[r];
+      mine.table = page_indptr[r];
+      mine.entries = page_indptr[r + 1] - mine.table;
+      mine.row0 = (p.tile0 + u % p.tiles) * TILE_ROWS;
+      mine.rows_here = min(TILE_ROWS, rows_all - mine.row0);
+      mine.n = 0;
+      if (mine.rows_here > 0) {
+        const Span keys = span_of(p, mine.start, mine.row0, mine.rows_here, group);
+        mine.n = max(1, (keys.hi + SLICE - 1) / SLICE - keys.first_slice);  // (rows that see nothing have a slice, all of it masked)
+      }
+    };
+    for (int u = first; u < min(first + each, units); ++u) {
+      unit_of(u);
+      slices += mine.n;
+      count += mine.n > 0;
+      longest = max(longest, mine.n);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    int s_incl = slices, c_incl = count;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, s_incl, off), b = __shfl_up_sync(0xffffffffu, c_incl, off);
+      if (lane >= off) {
+        s_incl += a;
+        c_incl += b;
+      }
+    }
+    if (lane == 31) {
+      scan[0][warp] = s_incl;
+      scan[1][warp] = c_incl;
+      scan[2][warp] = longest;
+    }
+    __syncthreads();
+    int s_at = s_incl - slices, c_at = c_incl - count;
+    live = total = longest = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) {
+        s_at += scan[0][w];
+        c_at += scan[1][w];
+      }
+      total += scan[0][w];
+      live += scan[1][w];
+      longest = max(longest, scan[2][w]);
+    }
+    // Few short items: a CTA each, whole, so that nothing is left to add up behind.
+    const int alone = live * p.nkv <= p.ctas && longest <= 2 * WARPS ? (longest + WARPS - 1) / WARPS * WARPS : 0;
+    if (alone) total = live * alone;
+    for (int u = first; u < min(first + each, units); ++u) {
+      if (each > 1) unit_of(u);
+      if (mine.n == 0) continue;
+      mine.stride = alone ? alone : mine.n;
+      mine.at = (alone ? c_at * alone : s_at) * p.nkv;
+      table[c_at++] = mine;
+      s_at += mine.n;
+    }
+    total *= p.nkv;
+    if (tid == 0) table[live].at = total;
+    __syncthreads();
+    if (alone) live |= 1 << 30;
+  }
+  const bool alone = live >> 30;
+  live &= (1 << 30) - 1;
+  // ---- this warp's run of slices, [begin, end), and its CTA's
+  const int each = alone ? table[0].stride / WARPS : (total + p.ctas * WARPS - 1) / (p.ctas * WARPS);
+  const int cta_begin = min((int)blockIdx.x * each * WARPS, total), cta_end = min(cta_begin + each * WARPS, total);
+  const int begin = min(cta_begin + warp * each, cta_end), end = min(begin + each, cta_end);
+  auto find = [&](int pos) {  // the last tile that begins at or before `pos`
+    int a = 0, b = live;
+    while (b - a > 1) {
+      const int mid = (a + b) / 2;
+      if (table[mid].at <= pos) a = mid;
+      else b = mid;
+    }
+    return a;
+  };
+  if (tid == 0) {
+    int4 cut = make_int4(0, 0, 0, 0);
+    if (cta_begin < cta_end && !alone) {
+      const Unit& u = table[find(cta_end - 1)];
+      const int kvh = (cta_end - 1 - u.at) / u.n, at = u.at + kvh * u.n;
+      // the item that goes on behind the CTA's end, where it began in this CTA
+      if (at >= cta_begin && at + u.n > cta_end) cut = make_int4(u.tok0 * group + u.row0, u.rows_here, kvh, (at + u.n - 1) / (each * WARPS) - (int)blockIdx.x + 1);
+    }
+    p.cut[blockIdx.x] = cut;
+  }
+  if (begin >= end) return;
+
+  const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE_BYTES;
+  float* heads = reinterpret_cast<float*>(smem + WARPS * STAGES * STAGE_BYTES);  // [warps][part_rows][PART]: of items that began before the warp's run
+  float* tail = reinterpret_cast<float*>(smem + warp * STAGES * STAGE_BYTES);    // of the one that goes on behind it: the ring is done with by then
   const int page_shift = 31 - __clz(p.page_size);
-  const int* pages = page_indices + page_indptr[r];
-  const int entries = page_indptr[r + 1] - page_indptr[r];
 
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  __half* qs = reinterpret_cast<__half*>(smem_raw);
-  __shared__ float q_factor[ROWS];
-  const uint32_t pipe = smem_addr(smem_raw) + (ROWS * QPAD * 2 + 127) / 128 * 128 + warp * ((STAGES * STAGE_BYTES + 127) / 128 * 128);
-
-  const int my_first = s_begin + warp, my_count = my_first < s_end ? (s_end - my_first + WARPS - 1) / WARPS : 0;
-  auto issue = [&](int i) {
-    if (i < my_count)
-      load_slice(pipe + (i % STAGES) * STAGE_BYTES, k_codes, k_exps, v_codes, v_exps, pages, entries, p, kvh, page_shift, (my_first + i * WARPS) * SLICE, lo, hi, lane);
+  // ---- what is asked for: pages one slice ahead of the copies, so that they are known by then (nothing looks at them before)
+  const int span = min(SLICE, p.page_size), boxes = SLICE / span, box = (lane & (boxes - 1)) * span;  // lane i looks after box i: a page's 8, 16 or 32 keys
+  const int first_unit = find(begin);
+  int a_pos = begin, a_left = 0, a_unit = first_unit, a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_entries = 0, a_page = 0;
+  const int* a_pages = page_indices;
+  auto next_item = [&]() {  // the item that a_pos lies in; false: there is none
+    for (;; ++a_unit) {
+      if (a_pos >= end) return false;
+      const Unit& u = table[a_unit];
+      const int past = a_pos - u.at;
+      a_kvh = past / u.stride;
+      if (a_kvh >= p.nkv) continue;
+      const int off = past - a_kvh * u.stride;
+      if (off >= u.n) {  // (behind a lone item's end)
+        a_pos += u.stride - off;
+        --a_unit;
+        continue;
+      }
+      const Span keys = span_of(p, u.start, u.row0, u.rows_here, group);
+      a_lo = keys.lo;
+      a_hi = keys.hi;
+      a_key = (keys.first_slice + off) * SLICE + box;
+      a_pages = page_indices + u.table;
+      a_entries = u.entries;
+      a_left = min(u.n - off, end - a_pos);
+      return true;
+    }
+  };
+  auto look = [&]() {
+    const int entry = a_key >> page_shift;
+    a_page = 0;
+    if (a_key + span > a_lo && a_key < a_hi) a_page = entry < a_entries ? a_pages[entry] : -1;
+  };
+  if (next_item()) look();
+  auto fire = [&](uint32_t st) {  // the slice looked up last, into a stage; then the next one is looked up
+    if (a_left > 0) {
+      if ((unsigned)a_page >= (unsigned)p.num_pages) {
+        if (lane < boxes) atomicExch(p.status, 2);
+        a_page = 0;  // (any page that is there: what comes of it is not used)
+      }
+      const int base = ((a_page * p.nkv + a_kvh) << page_shift) + (a_key & (p.page_size - 1));  // the pool's row at which the lane's box begins
+      const uint32_t kt = st, vt = st + CODE_BYTES, et = st + 2 * CODE_BYTES;
+      int rows8[SLICE / 8];  // where every eight keys begin
+#pragma unroll
+      for (int i = 0; i < SLICE / 8; ++i) rows8[i] = __shfl_sync(0xffffffffu, base, 8 * i / span) + (8 * i & (span - 1));
+      if (8 * CHUNKS % 32 == 0) {
+#pragma unroll
+        for (int i = 0; i < SLICE / 8; ++i) {
+          const size_t at = (size_t)rows8[i] * D + lane * 16;
+#pragma unroll
+          for (int c = 0; c < 8 * CHUNKS / 32; ++c) {
+            const int idx = c * 32 + lane, row = idx / CHUNKS, chunk = idx - row * CHUNKS;
+            cp_async16(kt + chunk_at(8 * i + row, chunk), k_codes + at + c * 512);
+            cp_async16(vt + chunk_at(8 * i + row, chunk), v_codes + at + c * 512);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SLICE / 8; ++i)
+          for (int idx = lane; idx < 8 * CHUNKS; idx += 32) {
+            const int row = idx / CHUNKS, chunk = idx - row * CHUNKS;
+            cp_async16(kt + chunk_at(8 * i + row, chunk), k_codes + (size_t)rows8[i] * D + idx * 16);
+            cp_async16(vt + chunk_at(8 * i + row, chunk), v_codes + (size_t)rows8[i] * D + idx * 16);
+          }
+      }
+      const int mine = __shfl_sync(0xffffffffu, base, 8 * (lane & 3) / span) + (8 * (lane & 3) & (span - 1));
+      if (lane < 8) cp_async8(et + lane * 8, (lane < 4 ? k_exps : v_exps) + mine);  // exponents, 8 a lane: of K, then of V
+      ++a_pos;
+      a_key += SLICE;
+      if (--a_left > 0 || next_item()) look();
+    }
     cp_async_commit();
   };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(i);
+#pragma unroll 1
+  for (int i = 0; i < STAGES; ++i) fire(ring + i * STAGE_BYTES);
 
-  // queries: four rows a warp, to float16 with the row's own power of two
-  for (int i = warp; i < ROWS; i += WARPS) {
-    float x[D / 32 + 1];
-    float most = 0.f;
-    const int row = row0 + i, tok = row / group;
-    const __nv_bfloat16* src = q + ((size_t)(tok0 + tok) * p.nq + kvh * group + (row - tok * group)) * D;
-#pragma unroll
-    for (int c = 0; c < D / 32 + 1; ++c) {
-      const int ch = c * 32 + lane;
-      x[c] = i < rows_here && ch < D ? __bfloat162float(src[ch]) : 0.f;
-      most = fmaxf(most, fabsf(x[c]));
-    }
-    most = warp_max(most);
-    const int field = (__float_as_uint(most) >> 23) & 255;
-    const int sh = most > 0.f && field < 255 ? min(max(14 + 127 - field, -113), 100) : 0;
-    const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-#pragma unroll
-    for (int c = 0; c < D / 32 + 1; ++c) {
-      const int ch = c * 32 + lane;
-      if (ch < D) qs[i * QPAD + ch] = __float2half_rn(x[c] * up);
-    }
-    if (lane == 0) q_factor[i] = p.scale * LOG2E * __uint_as_float((uint32_t)(127 - sh) << 23);
-  }
-  __syncthreads();
-  auto load_q = [&](uint32_t (&a)[4], int kk) {
-    const int ch = channel_of(kk, t);
-    const uint2 top = *reinterpret_cast<const uint2*>(qs + g * QPAD + ch), low = *reinterpret_cast<const uint2*>(qs + (g + 8) * QPAD + ch);
-    a[0] = top.x; a[1] = low.x; a[2] = top.y; a[3] = low.y;
-  };
-  uint32_t qf[Q_IN_REGS ? KSTEPS : 1][4];
-  if (Q_IN_REGS) {
-#pragma unroll
-    for (int kk = 0; kk < (Q_IN_REGS ? KSTEPS : 1); ++kk) load_q(qf[kk], kk);
-  }
-  const float row_factor[2] = {q_factor[g], q_factor[g + 8]};
-  const int q_pos[2] = {start + (row0 + g) / group, start + (row0 + g + 8) / group};
+  // ---- what is computed
+  int unit = first_unit, kvh = 0, item_end = begin, item_begin = 0;
+  int start = 0, row0 = 0, rows_here = 0, tok0 = 0, n = 0;
+  Span it = {};
+  uint32_t qf[NT][KSTEPS][2];
+  float row_factor[NT][2];
+  int q_pos[NT][2];
+  float o[NT][MTILES][4], m_run[NT][2], c_run[NT][2], l_run[NT][2];
+  uint32_t st = ring;
 
-  float o[DTILES][4];
+  for (int pos = begin; pos < end; ++pos) {
+    if (pos >= item_end) {
+      // ---- a new item: its queries, from memory straight into the fragments
+      for (;; ++unit) {
+        kvh = (pos - table[unit].at) / table[unit].stride;
+        if (kvh < p.nkv) break;
+      }
+      {
+        const Unit& u = table[unit];
+        n = u.n;
+        item_begin = u.at + kvh * u.stride;
+        item_end = min(item_begin + n, end);
+        if (pos >= item_begin + n) {  // (behind a lone item's end)
+          pos = item_begin + u.stride - 1;
+          item_end = 0;
+          continue;
+        }
+        start = u.start;
+        row0 = u.row0;
+        rows_here = u.rows_here;
+        tok0 = u.tok0;
+        it = span_of(p, start, row0, rows_here, group);
+      }
+      uint2 raw[NT][KSTEPS];
 #pragma unroll
-  for (int i = 0; i < DTILES; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-
-  for (int i = 0; i < my_count; ++i) {
-    issue(i + STAGES - 1);
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const uint32_t st = pipe + (i % STAGES) * STAGE_BYTES, vt = st + SLICE * ROW_BYTES, et = st + 2 * SLICE * ROW_BYTES;
-    const int key0 = (my_first + i * WARPS) * SLICE;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int j = 0; j < NT; ++j) {
+        const int i = g + 8 * j, row = row0 + i, tok = row / group;
+        const __nv_bfloat16* src = q + ((size_t)(tok0 + tok) * p.nq + kvh * group + (row - tok * group)) * D;
 #pragma unroll
-    for (int grp = 0; grp < WIDE; ++grp) {
-      uint32_t kw[2][4];
-      const int chunk = channel_of(grp * 4, t) >> 4;
-      lds_words<16>(kw[0], st + chunk_at(g, chunk));
-      lds_words<16>(kw[1], st + chunk_at(g + 8, chunk));
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          raw[j][kk] = make_uint2(0u, 0u);
+          if (i < rows_here) raw[j][kk] = *reinterpret_cast<const uint2*>(src + channel_of(kk, t));
+        }
+      }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a[4];
-        if (Q_IN_REGS) {
-          const int kk = grp * 4 + w;
-          a[0] = qf[kk][0]; a[1] = qf[kk][1]; a[2] = qf[kk][2]; a[3] = qf[kk][3];
-        } else {
-          load_q(a, grp * 4 + w);
+      for (int j = 0; j < NT; ++j) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const uint32_t x = raw[j][kk].x, y = raw[j][kk].y;
+          bits = max(bits, max(max((x << 16) & 0x7FFFFFFFu, x & 0x7FFF0000u), max((y << 16) & 0x7FFFFFFFu, y & 0x7FFF0000u)));
+        }
+        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+        // the row's power of two (a query that is not finite leaves its row NaN whatever it is multiplied by)
+        const int field = (int)(bits >> 23), sh = field > 0 && field < 255 ? min(max(14 + 127 - field, -113), 100) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + sh) << 23), down = p.scale * LOG2E * __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          q_pos[j][c] = start + (row0 + 8 * j + 2 * t + c) / group;
+          row_factor[j][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) mma_f16(s[n], a, c8_half2_lo(kw[n][w]), c8_half2_hi(kw[n][w]));
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const uint32_t x = raw[j][kk].x, y = raw[j][kk].y;
+          qf[j][kk][0] = pack_half2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up);
+          qf[j][kk][1] = pack_half2(__uint_as_float(y << 16) * up, __uint_as_float(y & 0xFFFF0000u) * up);
+        }
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+        m_run[j][0] = m_run[j][1] = 0.f;
+        c_run[j][0] = c_run[j][1] = START;
+        l_run[j][0] = l_run[j][1] = 0.f;
       }
+    }
+    // ---- a slice: its halves of 16 keys are two of the instruction's row tiles
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const uint32_t kt = st, vt = kt + CODE_BYTES, et = kt + 2 * CODE_BYTES;
+    float s[2][NT][4];
+    uint32_t vb[2][2];                       // the exponents' bytes of the values g, g + 8, g + 16, g + 24
+    float vf[2][2], kfac[2][2];              // 2^ev and 2^ek (255: infinity, which the codes of such a vector, all zero, make NaN)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        kfac[h][i] = __uint_as_float(lds8(et + 16 * h + 8 * i + g) << 23);
+        vb[h][i] = lds8(et + SLICE + 16 * h + 8 * i + g);
+        vf[h][i] = __uint_as_float(vb[h][i] << 23);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[h][j][0] = s[h][j][1] = s[h][j][2] = s[h][j][3] = 0.f;
+    }
+#pragma unroll
+    for (int grp = 0; grp < WIDE; ++grp) {
+      uint32_t kw[2][2][4];
+      const int chunk = channel_of(grp * 4, t) >> 4;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) lds_words<16>(kw[h][i], kt + chunk_at(16 * h + 8 * i + g, chunk));
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t kf[4] = {c8_half2_lo(kw[h][0][w]), c8_half2_lo(kw[h][1][w]), c8_half2_hi(kw[h][0][w]), c8_half2_hi(kw[h][1][w])};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_f16(s[h][j], kf, qf[j][grp * 4 + w][0], qf[j][grp * 4 + w][1]);
+        }
     }
 #pragma unroll
     for (int rest = 0; rest < REST; ++rest) {
       const int kk = WIDE * 4 + rest;
-      uint32_t a[4];
-      if (Q_IN_REGS) {
-        const int at = Q_IN_REGS ? kk : 0;
-        a[0] = qf[at][0]; a[1] = qf[at][1]; a[2] = qf[at][2]; a[3] = qf[at][3];
-      } else {
-        load_q(a, kk);
-      }
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t w = lds32(st + chunk_at(g + 8 * n, kk) + 4 * t);
-        mma_f16(s[n], a, c8_half2_lo(w), c8_half2_hi(w));
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t top = lds32(kt + chunk_at(16 * h + g, kk) + 4 * t), low = lds32(kt + chunk_at(16 * h + g + 8, kk) + 4 * t);
+        const uint32_t kf[4] = {c8_half2_lo(top), c8_half2_lo(low), c8_half2_hi(top), c8_half2_hi(low)};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_f16(s[h][j], kf, qf[j][kk][0], qf[j][kk][1]);
       }
     }
-    // mask, then the running softmax of rows g and g + 8
-    float kf[4], ev[4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint32_t kb = lds16(et + n * 8 + 2 * t), vb = lds16(et + SLICE + n * 8 + 2 * t);
-      kf[2 * n] = c8_factor(kb & 255);
-      kf[2 * n + 1] = c8_factor(kb >> 8);
-      ev[2 * n] = (vb & 255) == C8_NAN ? __uint_as_float(0x7FFFFFFFu) : (float)((int)(vb & 255) - 127);
-      ev[2 * n + 1] = (vb >> 8) == C8_NAN ? __uint_as_float(0x7FFFFFFFu) : (float)((int)(vb >> 8) - 127);
-    }
-    bool ok[2][4];
-    float m_new[2] = {m_run[0], m_run[1]};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = key0 + n * 8 + 2 * t + (e & 1), qp = q_pos[e >> 1];
-        ok[n][e] = key <= qp && (p.window <= 0 || key > qp - p.window);
-        s[n][e] = s[n][e] * row_factor[e >> 1] * kf[2 * n + (e & 1)];
-        if (ok[n][e]) m_new[e >> 1] = fmaxf(m_new[e >> 1], s[n][e] + ev[2 * n + (e & 1)]);
+    const int key0 = (it.first_slice + pos - item_begin) * SLICE;
+    const bool edge = key0 < it.seen_lo || key0 + SLICE > it.seen_hi;  // some row does not see all of the slice
+    if (edge && (key0 < it.lo || key0 + SLICE > it.hi)) {
+      // values that must not be weighed, not even by zero (they may hold anything)
+      for (int idx = lane; idx < SLICE * CHUNKS; idx += 32) {
+        const int row = idx / CHUNKS, chunk = idx - row * CHUNKS;
+        if (key0 + row < it.lo || key0 + row >= it.hi) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(vt + chunk_at(row, chunk)), "r"(0) : "memory");
       }
-    float alpha[2], m_use[2], row_sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      m_new[j] = quad_max(m_new[j]);
-      m_use[j] = m_new[j] == -INFINITY ? 0.f : m_new[j] - 14.f;
-      alpha[j] = m_run[j] == -INFINITY ? 0.f : exp2f(m_run[j] - m_new[j]);
-      m_run[j] = m_new[j];
+      __syncwarp();
     }
-    uint32_t a[4];
-    float weight[2][4];
+    // scores in units of log2, relative to m, masked; weights 2^(s - m - c + ABOVE) times the values' 2^ev
+    float x[2][NT][4], w[2][NT][4];
+    auto weigh = [&]() {
+      float most = 0.f;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = s[n][e] - m_use[e >> 1];
-        row_sum[e >> 1] += ok[n][e] ? exp2f(x) : 0.f;
-        weight[n][e] = ok[n][e] ? exp2f(x + ev[2 * n + (e & 1)]) : 0.f;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[h][j][e] = ex2(s[h][j][e] + (ABOVE - c_run[j][e & 1]));
+            w[h][j][e] = x[h][j][e] * vf[h][e >> 1];
+          }
+      if (edge) {  // (a value that is NaN, or no value at all, reaches only who sees it)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[h][j][e] = s[h][j][e] == -INFINITY ? 0.f : w[h][j][e];
       }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) l_run[j] = l_run[j] * alpha[j] + row_sum[j];
-    a[0] = pack_half2(weight[0][0], weight[0][1]);
-    a[1] = pack_half2(weight[0][2], weight[0][3]);
-    a[2] = pack_half2(weight[1][0], weight[1][1]);
-    a[3] = pack_half2(weight[1][2], weight[1][3]);
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt) {
-        o[dt][0] *= alpha[0]; o[dt][1] *= alpha[0]; o[dt][2] *= alpha[1]; o[dt][3] *= alpha[1];
-      }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, w[h][j][e]);
+      return most;
+    };
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[h][j][e] = fmaf(s[h][j][e], row_factor[j][e & 1] * kfac[h][e >> 1], -m_run[j][e & 1]);
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * h + g + 8 * (e >> 1), qp = q_pos[j][e & 1];
+            if (key > qp || (p.window > 0 && key <= qp - p.window)) s[h][j][e] = -INFINITY;
+          }
     }
+    // m + c moves only where a weight passes 2^(ABOVE + SLACK)
+    if (__any_sync(0xffffffffu, weigh() > exp2f(ABOVE + SLACK))) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // the largest score, relative to the one before, then the largest score with its exponent, relative to that
+          float up = oct_max(fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]))), c_new = -INFINITY;
+          if (up == -INFINITY || (up < 0.f && c_run[j][c] > START)) up = 0.f;  // (the first key's score is taken whatever its sign)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              s[h][j][2 * i + c] -= up;
+              c_new = fmaxf(c_new, s[h][j][2 * i + c] + (float)((int)vb[h][i] - 127));
+            }
+          c_new = fmaxf(c_run[j][c] - up, oct_max(c_new));
+          const float alpha = ex2((c_run[j][c] - up) - c_new);
+          m_run[j][c] += up;
+          c_run[j][c] = c_new;
+          l_run[j][c] *= alpha;
+#pragma unroll
+          for (int i = 0; i < MTILES; ++i) {
+            o[j][i][c] *= alpha;
+            o[j][i][2 + c] *= alpha;
+          }
+        }
+      weigh();
+    }
+    uint32_t wf[2][NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l_run[j][0] += x[h][j][0] + x[h][j][2];
+        l_run[j][1] += x[h][j][1] + x[h][j][3];
+        wf[h][j][0] = transposed(pack_half2(w[h][j][0], w[h][j][1]));
+        wf[h][j][1] = transposed(pack_half2(w[h][j][2], w[h][j][3]));
+      }
     // values: lane group g's channels of the rows 2t, 2t + 1, 2t + 8, 2t + 9, paired along the keys byte by byte
 #pragma unroll
-    for (int blk = 0; blk < VBLOCKS; ++blk) {
-      uint32_t vw[4][VB / 4];
-      const int ch = blk * 8 * VB + g * VB;
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lds_words<VB>(vw[j], vt + chunk_at(2 * t + (j & 1) + 8 * (j >> 1), ch >> 4) + (ch & 15));
+      for (int blk = 0; blk < VBLOCKS; ++blk) {
+        uint32_t vw[4][VB / 4];
+        const int ch = blk * 8 * VB + g * VB;
 #pragma unroll
-      for (int w = 0; w < VB / 4; ++w) {
-        const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), b1 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
-        const uint32_t c0 = __byte_perm(vw[0][w], vw[1][w], 0x7362), c1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-        const int dt = blk * VB + w * 4;
-        mma_f16(o[dt], a, c8_half2_lo(b0), c8_half2_lo(b1));
-        mma_f16(o[dt + 1], a, c8_half2_hi(b0), c8_half2_hi(b1));
-        mma_f16(o[dt + 2], a, c8_half2_lo(c0), c8_half2_lo(c1));
-        mma_f16(o[dt + 3], a, c8_half2_hi(c0), c8_half2_hi(c1));
+        for (int i = 0; i < 4; ++i) lds_words<VB>(vw[i], vt + chunk_at(16 * h + 2 * t + (i & 1) + 8 * (i >> 1), ch >> 4) + (ch & 15));
+#pragma unroll
+        for (int w = 0; w < VB / 4; ++w) {
+          const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), b1 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
+          const uint32_t c0 = __byte_perm(vw[0][w], vw[1][w], 0x7362), c1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+          const uint32_t va[4] = {c8_half2_lo(b0), c8_half2_hi(b0), c8_half2_lo(b1), c8_half2_hi(b1)};
+          const uint32_t vc[4] = {c8_half2_lo(c0), c8_half2_hi(c0), c8_half2_lo(c1), c8_half2_hi(c1)};
+          const int mt = blk * (VB / 2) + w * 2;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_f16(o[j][mt], va, wf[h][j][0], wf[h][j][1]);
+            mma_f16(o[j][mt + 1], vc, wf[h][j][0], wf[h][j][1]);
+          }
+        }
       }
-    }
-    if (VTAIL) {
-      const int ch = VBLOCKS * 8 * VB + 2 * g;
-      uint32_t vw[4];
+      if (VTAIL) {
+        const int ch = VBLOCKS * 8 * VB + 2 * g;
+        uint32_t vw[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vw[j] = lds16(vt + chunk_at(2 * t + (j & 1) + 8 * (j >> 1), ch >> 4) + (ch & 15));
-      const uint32_t b0 = __byte_perm(vw[0], vw[1], 0x5140), b1 = __byte_perm(vw[2], vw[3], 0x5140);
-      mma_f16(o[DTILES - 2], a, c8_half2_lo(b0), c8_half2_lo(b1));
-      mma_f16(o[DTILES - 1], a, c8_half2_hi(b0), c8_half2_hi(b1));
+        for (int i = 0; i < 4; ++i) vw[i] = lds16(vt + chunk_at(16 * h + 2 * t + (i & 1) + 8 * (i >> 1), ch >> 4) + (ch & 15));
+        const uint32_t b0 = __byte_perm(vw[0], vw[1], 0x5140), b1 = __byte_perm(vw[2], vw[3], 0x5140);
+        const uint32_t va[4] = {c8_half2_lo(b0), c8_half2_hi(b0), c8_half2_lo(b1), c8_half2_hi(b1)};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_f16(o[j][MTILES - 1], va, wf[h][j][0], wf[h][j][1]);
+      }
     }
     __syncwarp();
-  }
-  cp_async_wait<0>();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) l_run[j] = quad_sum(l_run[j]);
-  __syncthreads();  // the pipelines are drained: shared memory becomes the merge area [warps][16][D + 2]
+    fire(st);
+    st = st + STAGE_BYTES == ring + STAGES * STAGE_BYTES ? ring : st + STAGE_BYTES;
 
-  float* merge = reinterpret_cast<float*>(smem_raw);
+    if (pos + 1 < item_end) continue;
+    // ---- this warp's last slice of the item
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float* row = merge + ((size_t)warp * ROWS + g + 8 * j) * (D + 2);
-#pragma unroll
-    for (int dt = 0; dt < DTILES; ++dt)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int from = 2 * t + c;  // the lane group whose channels this column is
-        const int ch = dt < VBLOCKS * VB ? (dt / VB) * 8 * VB + from * VB + dt % VB : VBLOCKS * 8 * VB + 2 * from + (dt - VBLOCKS * VB);
-        row[ch] = o[dt][2 * j + c];
+        l_run[j][c] = oct_sum(l_run[j][c]);
+        if (c_run[j][c] == START) m_run[j][c] = NOTHING;
       }
-    if (t == 0) {
-      row[D] = m_run[j];
-      row[D + 1] = l_run[j];
+    const int seg_begin = max(item_begin, cta_begin), seg_end = min(item_begin + n, cta_end);  // the CTA's share of it
+    const int first_warp = (seg_begin - cta_begin) / each, last_warp = (seg_end - 1 - cta_begin) / each;
+    const bool whole = seg_begin == item_begin && seg_end == item_begin + n;
+    float* piece = p.part + (size_t)(2 * blockIdx.x + (seg_begin == item_begin)) * ROWS * PART;  // (a cut item: began before this CTA, or goes on behind it)
+    __nv_bfloat16* dst = out + ((size_t)tok0 * p.nq + kvh * group) * D;
+    auto row_of = [&](int row) {  // where query row `row` of the item begins in the output
+      const int rho = row0 + row, tok = rho / group;
+      return dst + ((size_t)tok * p.nq + (rho - tok * group)) * D;
+    };
+    // the lane group's channels 2 i and 2 i + 1 of a block
+    auto channel = [&](int i) { return i < VBLOCKS * (VB / 2) ? i / (VB / 2) * 8 * VB + g * VB + i % (VB / 2) * 2 : VBLOCKS * 8 * VB + 2 * g; };
+    if (first_warp == last_warp && whole) {
+      // nobody else has a share of it
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (8 * j + 2 * t + c >= rows_here) continue;
+          const float den = l_run[j][c] + sink_term(p.sink, m_run[j][c], c_run[j][c]), inv = den == 0.f ? 0.f : 1.0f / den;
+          __nv_bfloat16* row = row_of(8 * j + 2 * t + c);
+#pragma unroll
+          for (int i = 0; i < MTILES; ++i)
+            *reinterpret_cast<__nv_bfloat162*>(row + channel(i)) = __floats2bfloat162_rn(o[j][i][c] * inv, o[j][i][2 + c] * inv);
+        }
+      continue;
+    }
+    // its piece: to global memory where it is the CTA's only one, else to shared memory
+    const bool lone = first_warp == last_warp, is_tail = !lone && warp == first_warp;
+    if (is_tail) cp_async_wait<0>();  // (the ring's last, empty groups)
+    float* area = lone ? piece : (is_tail ? tail : heads + (size_t)warp * part_rows * PART);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (8 * j + 2 * t + c >= rows_here) continue;
+        float* row = area + (size_t)(8 * j + 2 * t + c) * PART;
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i) *reinterpret_cast<float2*>(row + channel(i)) = make_float2(o[j][i][c], o[j][i][2 + c]);
+        if (g == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m_run[j][c], l_run[j][c], c_run[j][c], 0.f);
+      }
+    if (lone) continue;
+    __threadfence_block();
+    __syncwarp();
+    int last = 0;
+    if (lane == 0) last = atomicAdd(&arrived[first_warp], 1) == last_warp - first_warp;  // (an item that warps share begins its CTA's share in one warp)
+    if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+    __threadfence_block();
+    const float* first_piece = reinterpret_cast<const float*>(smem + first_warp * STAGES * STAGE_BYTES);
+    for (int row = 0; row < rows_here; ++row) {
+      auto from = [&](int w) { return (w == first_warp ? first_piece : heads + (size_t)w * part_rows * PART) + (size_t)row * PART; };
+      float m = NOTHING, c_all = -INFINITY, l = 0.f, wgt[WARPS];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w)
+        if (w >= first_warp && w <= last_warp) m = fmaxf(m, from(w)[D]);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        wgt[w] = w >= first_warp && w <= last_warp ? (from(w)[D] - m) + from(w)[D + 2] : -INFINITY;
+        c_all = fmaxf(c_all, wgt[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        wgt[w] = ex2(wgt[w] - c_all);
+        if (w >= first_warp && w <= last_warp) l += wgt[w] * from(w)[D + 1];
+      }
+      const float den = l + sink_term(p.sink, m, c_all), inv = den == 0.f ? 0.f : 1.0f / den;
+      for (int c = 4 * lane; c < D; c += 128) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          if (w < first_warp || w > last_warp) continue;
+          const float4 x = *reinterpret_cast<const float4*>(from(w) + c);
+          acc.x += wgt[w] * x.x;
+          acc.y += wgt[w] * x.y;
+          acc.z += wgt[w] * x.z;
+          acc.w += wgt[w] * x.w;
+        }
+        if (whole) {
+          uint2 pk;
+          __nv_bfloat162 lo2 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi2 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+          pk.x = *reinterpret_cast<uint32_t*>(&lo2);
+          pk.y = *reinterpret_cast<uint32_t*>(&hi2);
+          *reinterpret_cast<uint2*>(row_of(row) + c) = pk;
+        } else {
+          *reinterpret_cast<float4*>(piece + (size_t)row * PART + c) = acc;
+        }
+      }
+      if (!whole && lane == 0) *reinterpret_cast<float4*>(piece + (size_t)row * PART + D) = make_float4(m, l, c_all, 0.f);
     }
   }
-  __syncthreads();
-  const size_t item = (size_t)place * p.nkv + kvh;
-  auto store = [&](int row, int c, float acc, float l, float m) {
-    if (p.sink) l += exp2f(14.f - m);  // (the sums are in units of 2^(m - 14))
-    const int rho = row0 + row, tok = rho / group;
-    out[((size_t)(tok0 + tok) * p.nq + kvh * group + (rho - tok * group)) * D + c] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+  cp_async_wait<0>();
+}
+
+// The items that were cut: a CTA's second partial and its successors' first ones, added up in their order. Block (cta, row).
+constexpr int MERGE_THREADS = 128;
+__global__ void __launch_bounds__(MERGE_THREADS)
+attn_cache8_merge_kernel(__nv_bfloat16* __restrict__ out, const Split8 p) {
+  const int4* cuts = p.cut;
+  const float* parts = p.part;
+  pdl_prologue(cuts, parts);
+  const int cta = blockIdx.x, row = blockIdx.y, group = p.nq / p.nkv;
+  const int4 cut = cuts[cta];
+  if (cut.w < 2 || row >= cut.y) return;
+  const int rho = cut.x + row, tok = rho / group;
+  __shared__ float weight[MERGE_THREADS];
+  __shared__ float4 sums[MERGE_THREADS];
+  __shared__ float red[4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto at = [&](int i) { return parts + ((size_t)(2 * (cta + i) + (i == 0)) * ROWS + row) * PART; };
+  // the largest m of all pieces, then the largest m + c
+  auto block_max = [&](float v) {
+    v = warp_max(v);
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   };
-  for (int idx = tid; idx < rows_here * D; idx += THREADS) {
-    const int row = idx / D, c = idx - row * D;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, merge[((size_t)w * ROWS + row) * (D + 2) + D]);
-    float acc = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float* src = merge + ((size_t)w * ROWS + row) * (D + 2);
-      const float wgt = src[D] == -INFINITY ? 0.f : exp2f(src[D] - m);
-      acc += wgt * src[c];
-      l += wgt * src[D + 1];
+  float m = NOTHING, c_all = -INFINITY;
+  for (int i = tid; i < cut.w; i += MERGE_THREADS) m = fmaxf(m, at(i)[D]);
+  m = block_max(m);
+  for (int i = tid; i < cut.w; i += MERGE_THREADS) c_all = fmaxf(c_all, (at(i)[D] - m) + at(i)[D + 2]);
+  c_all = block_max(c_all);
+  constexpr int COLS = D / 4, SHARES = MERGE_THREADS / COLS;  // threads side by side take 4 channels each; shares of them take every SHARES-th piece
+  const int col = tid % COLS, share = tid / COLS;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int first = 0; first < cut.w; first += MERGE_THREADS) {
+    __syncthreads();
+    if (first + tid < cut.w) {
+      const float4 mlc = *reinterpret_cast<const float4*>(at(first + tid) + D);
+      weight[tid] = ex2(((mlc.x - m) + mlc.z) - c_all);
+      l += weight[tid] * mlc.y;
     }
-    if (p.splits == 1) {
-      store(row, c, acc, l, m);
-    } else {
-      const size_t at = (item * p.splits + split) * ROWS + row;
-      p.part_o[at * D + c] = acc;
-      if (c == 0) {
-        p.part_ml[2 * at] = m;
-        p.part_ml[2 * at + 1] = l;
+    __syncthreads();
+    if (share < SHARES) {
+#pragma unroll 4
+      for (int i = share; i < min(MERGE_THREADS, cut.w - first); i += SHARES) {
+        const float4 x = *reinterpret_cast<const float4*>(at(first + i) + 4 * col);
+        const float w = weight[i];
+        acc.x += w * x.x;
+        acc.y += w * x.y;
+        acc.z += w * x.z;
+        acc.w += w * x.w;
       }
     }
   }
-  if (p.splits == 1) return;
-  // the split that finishes last adds them all up (a ticket; nobody waits)
-  __shared__ int last_one;
-  __threadfence();
+  sums[tid] = acc;
+  l = warp_sum(l);
   __syncthreads();
-  if (tid == 0) {
-    const int prev = atomicAdd(p.counters + item, 1);
-    last_one = prev == p.splits - 1;
-    if (last_one) p.counters[item] = 0;
-  }
+  if (lane == 0) red[warp] = l;
   __syncthreads();
-  if (!last_one) return;
-  __threadfence();
-  for (int idx = tid; idx < rows_here * D; idx += THREADS) {
-    const int row = idx / D, c = idx - row * D;
-    float m = -INFINITY, acc = 0.f, l = 0.f;
-    for (int sp = 0; sp < p.splits; ++sp) m = fmaxf(m, __ldcg(p.part_ml + 2 * ((item * p.splits + sp) * ROWS + row)));
-    for (int sp = 0; sp < p.splits; ++sp) {
-      const size_t at = (item * p.splits + sp) * ROWS + row;
-      const float ms = __ldcg(p.part_ml + 2 * at), wgt = ms == -INFINITY ? 0.f : exp2f(ms - m);
-      acc += wgt * __ldcg(p.part_o + at * D + c);
-      l += wgt * __ldcg(p.part_ml + 2 * at + 1);
+  l = (red[0] + red[1]) + (red[2] + red[3]) + sink_term(p.sink, m, c_all);
+  if (share == 0) {
+    for (int i = 1; i < SHARES; ++i) {
+      const float4 x = sums[i * COLS + col];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
     }
-    store(row, c, acc, l, m);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    uint2 pk;
+    pk.x = *reinterpret_cast<uint32_t*>(&lo);
+    pk.y = *reinterpret_cast<uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(out + ((size_t)tok * p.nq + (rho - tok * group) + (size_t)cut.z * group) * D + 4 * col) = pk;
   }
 }
 
@@ -440,32 +798,48 @@ using namespace ms;
 MS_DEFINE_LAST_ERROR(MS_ATTN8_FN(last_error))
 MS_DEFINE_PDL_SWITCH(MS_ATTN8_FN(set_pdl))
 
-static constexpr size_t split_smem() {
-  const size_t pipe = (ROWS * QPAD * 2 + 127) / 128 * 128 + (size_t)WARPS * ((STAGES * STAGE_BYTES + 127) / 128 * 128);
-  const size_t merge = (size_t)WARPS * ROWS * (D + 2) * 4;
-  return pipe > merge ? pipe : merge;
-}
+constexpr int SMEM_MOST = 227 * 1024 - 11 * 1024;  // (the table of tiles is static: 10 KB)
 
-// Rows [0, p->rows) of the geometry in p. Scratch and counters (splits > 1): see Split8.
-MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, void* out, const void* q, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps,
-                                 cudaStream_t stream) {
-  if (p->rows == 0) return 0;
-  MS_CHECK_ARG(p->nq > 0 && p->nkv > 0 && p->nq % p->nkv == 0, "attention: %d query heads are not a multiple of %d kv heads", p->nq, p->nkv);
-  MS_CHECK_ARG(p->page_size >= 8 && (p->page_size & (p->page_size - 1)) == 0, "attention: page_size=%d must be a power of two from 8 on for an 8-bit cache", p->page_size);
-  MS_CHECK_ARG(p->rows > 0 && p->tiles > 0 && p->splits > 0 && (long long)p->rows * p->tiles * p->splits < (1LL << 31) && p->nkv <= 65535,
-               "attention: %d rows of %d tiles, %d splits, %d kv heads are too many for one launch", p->rows, p->tiles, p->splits, p->nkv);
-  MS_CHECK_ARG(p->splits == 1 || (p->part_o && p->part_ml && p->counters), "attention: splits need scratch memory");
-  MS_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_exps % 8 == 0 && (uintptr_t)v_exps % 8 == 0,
-               "attention: an 8-bit cache's tensors must be 16-byte aligned");
+// Floats of partial results that a launch of `ctas` CTAs needs; the table of cut items (4 ints a CTA) lies behind them.
+MS_EXPORT long long MS_ATTN8_FN(part_floats)(int ctas) { return 2LL * ctas * ROWS * PART; }
+MS_EXPORT int MS_ATTN8_FN(max_units)() { return MAX_UNITS; }
+
+template <int NT>
+static int launch_split(const Split8& p, int rows_tile, void* out, const void* q, const void* k_codes,
+                        const void* k_exps, const void* v_codes, const void* v_exps, cudaStream_t stream) {
   static bool configured[64] = {};  // the attribute belongs to a device
   int dev = 0;
   MS_CHECK_CUDA(cudaGetDevice(&dev));
   MS_CHECK_ARG(dev >= 0 && dev < 64, "attention: device index %d is not supported", dev);
   if (!configured[dev]) {
-    MS_CHECK_CUDA(cudaFuncSetAttribute(attn_cache8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)split_smem()));
+    MS_CHECK_CUDA(cudaFuncSetAttribute(attn_cache8_split_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
     configured[dev] = true;
   }
-  MS_LAUNCH(attn_cache8_split_kernel, dim3((unsigned)(p->rows * p->tiles * p->splits), p->nkv), THREADS, split_smem(), stream, (__nv_bfloat16*)out,
-            (const __nv_bfloat16*)q, (const uint8_t*)k_codes, (const uint8_t*)k_exps, (const uint8_t*)v_codes, (const uint8_t*)v_exps, *p);
+  constexpr int ring = warps_of(NT) * stages_of(NT) * STAGE_BYTES;
+  static_assert(ring + warps_of(NT) * 8 * NT * PART * 4 <= SMEM_MOST && 8 * NT * PART * 4 <= stages_of(NT) * STAGE_BYTES, "the rings and the pieces of shared items fit");
+  MS_LAUNCH(attn_cache8_split_kernel<NT>, p.ctas, warps_of(NT) * 32, ring + warps_of(NT) * rows_tile * PART * 4, stream, (__nv_bfloat16*)out, (const __nv_bfloat16*)q,
+            (const uint8_t*)k_codes, (const uint8_t*)k_exps, (const uint8_t*)v_codes, (const uint8_t*)v_exps, p, rows_tile);
+  return 0;
+}
+
+// Rows [0, p->rows) of the geometry in p, in tiles of `tile_rows` (8 or 16) query rows, of which no request has more than `rows_most`.
+MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, int tile_rows, int rows_most, void* out, const void* q, const void* k_codes, const void* k_exps, const void* v_codes,
+                                 const void* v_exps, cudaStream_t stream) {
+  if (p->rows == 0) return 0;
+  MS_CHECK_ARG(p->nq > 0 && p->nkv > 0 && p->nq % p->nkv == 0, "attention: %d query heads are not a multiple of %d kv heads", p->nq, p->nkv);
+  MS_CHECK_ARG(p->page_size >= 8 && (p->page_size & (p->page_size - 1)) == 0, "attention: page_size=%d must be a power of two from 8 on for an 8-bit cache", p->page_size);
+  MS_CHECK_ARG(p->rows > 0 && p->tiles > 0 && (long long)p->rows * p->tiles <= MAX_UNITS, "attention: %d rows of %d tiles are too many for one launch", p->rows, p->tiles);
+  MS_CHECK_ARG(p->ctas > 0 && p->part && p->cut && (tile_rows == 8 || tile_rows == 16) && rows_most > 0, "attention: %d CTAs need scratch memory, tiles %d rows of %d",
+               p->ctas, tile_rows, rows_most);
+  const long long pool_rows = (long long)p->num_pages * p->nkv * p->page_size;
+  MS_CHECK_ARG(pool_rows > 0 && pool_rows < (1LL << 31), "attention: pools of %lld rows", pool_rows);
+  MS_CHECK_ARG((uintptr_t)q % 8 == 0 && (uintptr_t)out % 8 == 0 && (uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_exps % 8 == 0 &&
+                   (uintptr_t)v_exps % 8 == 0 && (uintptr_t)p->part % 16 == 0 && (uintptr_t)p->cut % 16 == 0,
+               "attention: an 8-bit cache's tensors must be 16-byte aligned");
+  const int rows_tile = rows_most < tile_rows ? rows_most : tile_rows;
+  if (int rc = tile_rows == 8 ? launch_split<1>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream)
+                              : launch_split<2>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream))
+    return rc;
+  MS_LAUNCH(attn_cache8_merge_kernel, dim3(p->ctas, rows_tile), MERGE_THREADS, 0, stream, (__nv_bfloat16*)out, *p);
   return 0;
 }

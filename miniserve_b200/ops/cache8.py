@@ -22,8 +22,8 @@ LARGEST, EXPONENTS = 448.0, (-60, 7)
 class Pool8:
     """Keys (or values) of one cache entry in 8 bits. ``codes`` uint8 [pages, kv_heads, page_size, d] (bits of ``torch.float8_e4m3fn``) and
     ``exponents`` uint8 [pages, kv_heads, page_size]: number i of a head's vector is code_i * 2^(exponent - 127). The writer takes the smallest
-    exponent at which the vector's largest number is at most 448, within 2^-60 and 2^7; a vector with a number that is not finite gets 255 and reads
-    as NaN."""
+    exponent at which the vector's largest number is at most 448, within 2^-60 and 2^7; a vector with a number that is not finite gets 255 and zero
+    codes, and reads as NaN."""
 
     codes: torch.Tensor
     exponents: torch.Tensor
@@ -85,17 +85,26 @@ def _cache_check(rc: int) -> None:
 class _Split(ctypes.Structure):
     """``Split8`` of csrc/attention_cache8.cu."""
 
-    _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part_o", "part_ml", "counters")] + [
-        (n, _i) for n in ("rows", "tiles", "nq", "nkv", "window", "sink", "page_size", "splits")] + [("scale", _f), ("num_pages", _i)]
+    _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part", "cut")] + [
+        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i)]
+
+
+class _AttnLib:
+    """The attention kernels of one head size."""
+
+    def __init__(self, head_dim: int):
+        lib = ctypes.CDLL(str(build.ensure_built(module_for(head_dim))))
+        pre = f"ms_attn_cache8_d{head_dim}_"
+        self.last_error = native._declare(lib, pre + "last_error", [], c_char_p)
+        native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
+        self.split = native._declare(lib, pre + "split", [_p, _i, _i] + [_p] * 7)
+        self.part_floats = native._declare(lib, pre + "part_floats", [_i], _ll)
+        self.max_units = native._declare(lib, pre + "max_units", [])()
 
 
 @lru_cache(maxsize=None)
-def _attn_lib(head_dim: int):
-    lib = ctypes.CDLL(str(build.ensure_built(module_for(head_dim))))
-    pre = f"ms_attn_cache8_d{head_dim}_"
-    last_error = native._declare(lib, pre + "last_error", [], c_char_p)
-    native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
-    return native._declare(lib, pre + "split", [_p] * 7 + [_p]), last_error
+def _attn_lib(head_dim: int) -> _AttnLib:
+    return _AttnLib(head_dim)
 
 
 def _on(device: torch.device):
@@ -187,54 +196,38 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
 
 
 # ------------------------------------------------------------------ attention
-ROWS = 16  # query rows (tokens times the heads of a kv head) of a CTA
 
-
-def choose_splits(items: int, keys: int | None, sm_count: int) -> int:
-    """How many ways the keys of an item (a tile of 16 query rows and a kv head) are shared out: two CTAs a multiprocessor, at least 128 keys
-    a split. ``keys`` None (inside a CUDA graph for short contexts): a few thousand are assumed."""
-    by_len = 16 if keys is None else max(1, -(-keys // 128))
-    return max(1, min(2 * sm_count // max(items, 1), by_len, 64))
-
-
-def _workspace(ctx, floats: int, ints: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Partial results and tickets (zero before the first launch, left zero by every launch) of steps that run one after the other. What is outgrown
-    stays alive for graphs that hold its address; a capture that needs more than there is gets its own."""
+def _workspace(ctx, floats: int, device) -> torch.Tensor:
+    """Partial results of steps that run one after the other. What is outgrown stays alive for graphs that hold its address; a capture that needs
+    more than there is gets its own."""
     held = ctx.scratch.get("cache8")
-    if held is not None and held[0].numel() >= floats and held[1].numel() >= ints:
+    if held is not None and held.numel() >= floats:
         return held
-    new = (torch.empty(2 * floats, dtype=torch.float32, device=device), torch.zeros(max(4096, 2 * ints), dtype=torch.int32, device=device))
+    new = torch.empty(floats, dtype=torch.float32, device=device)
     ctx.scratch.setdefault("retired", []).append(new)
     if not torch.cuda.is_current_stream_capturing():
         ctx.scratch["cache8"] = new
     return new
 
 
-def _split_plan(ctx, group: int, first: int, rows: int, most: int, keys: int | None, nq: int, nkv: int, d: int, scale: float, window: int, sink: int, page_size: int,
-                pages: int, device) -> _Split:
-    tiles = -(-most * (nq // nkv) // ROWS)
-    items = rows * tiles * nkv
-    splits = choose_splits(items, keys, ctx.sm_count)
-    part_o = part_ml = counters = None
-    if splits > 1:
-        need = items * splits * ROWS
-        buf, tickets = _workspace(ctx, need * (d + 2), items, device)
-        part_o, part_ml, counters = buf.data_ptr(), buf.data_ptr() + 4 * need * d, tickets.data_ptr()
-    skip = 4 * first  # the per-row tables are int32
-    return _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
-                  ctx.status.data_ptr(), part_o, part_ml, counters, rows, tiles, nq, nkv, window, sink, page_size, splits, scale, pages)
-
-
 def _plans(ctx, group: int, key: tuple, device) -> list:
-    """The launches of a step's attention, the same for every layer with these sizes and this window."""
+    """The launches of a step's attention, the same for every layer with these sizes and this window: ``(plan, query rows of a tile, the most of a request)``."""
     nq, nkv, d, scale, window, sink, page_size, pages = key
-    known = ctx.max_kv_len if not ctx.graph_bucket else (ctx.graph_kv_len or None)
-    if known is not None and window:
-        known = min(known, window + ctx.max_q_len)
-    single, out = ctx.leading_single_rows, []
-    for first, rows, most in ((0, single, 1), (single, ctx.num_rows - single, ctx.max_q_len)):
-        if rows > 0:
-            out.append(_split_plan(ctx, group, first, rows, most, known, nq, nkv, d, scale, window, sink, page_size, pages, device))
+    lib = _attn_lib(d)
+    ctas = ctx.sm_count
+    floats = lib.part_floats(ctas)
+    part = _workspace(ctx, floats + 4 * ctas, device)
+    most = ctx.max_q_len * (nq // nkv)
+    tile_rows = 8 if most <= 8 else 16
+    tiles, out = -(-most // tile_rows), []
+    tiles_each = min(tiles, lib.max_units)
+    rows_each = lib.max_units // tiles_each
+    for first in range(0, ctx.num_rows, rows_each):
+        skip = 4 * first  # the per-row tables are int32
+        for tile0 in range(0, tiles, tiles_each):
+            out.append((_Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
+                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, min(rows_each, ctx.num_rows - first), tile0,
+                               min(tiles_each, tiles - tile0), nq, nkv, window, sink, page_size, ctas, scale, pages), tile_rows, most))
     return out
 
 
@@ -260,15 +253,14 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
     if not (out.shape == q.shape and v_pool.shape == k_pool.shape and q.dtype == out.dtype == torch.bfloat16 and q.device == out.device == v_pool.codes.device == dev
             and q.is_contiguous() and out.is_contiguous()):
         raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape, and pools of one shape, on one device")
-    split, last_error = _attn_lib(d)
-    stream = ctx.stream
+    lib, stream = _attn_lib(d), ctx.stream
 
     def launch():
-        for plan in plans:
-            rc = split(ctypes.addressof(plan), out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
-                       v_pool.exponents.data_ptr(), stream)
-            native.LAUNCHES[0] += 1
+        for plan, tile_rows, most in plans:
+            rc = lib.split(ctypes.addressof(plan), tile_rows, most, out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
+                           v_pool.exponents.data_ptr(), stream)
+            native.LAUNCHES[0] += 2
             if rc:
-                raise native.NativeError(last_error().decode())
+                raise native.NativeError(lib.last_error().decode())
 
     _launch(dev, launch)

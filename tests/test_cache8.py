@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import math
-
 import pytest
 import torch
 
@@ -40,10 +38,3 @@ def test_pools_on_the_host_are_refused_by_the_kernels():
         ops.read_cache(rows, rows, p, p, i, i, i, i, i)
     with pytest.raises(TypeError, match="both"):
         ops.read_cache(rows, rows, p, p.codes, i, i, i, i, i)
-
-
-@pytest.mark.parametrize("items,keys", [(1, 1), (8, 128), (8, 129), (64, 4096), (8, 131072), (1000, 100000), (16, None)])
-def test_splits_leave_every_split_a_share(items, keys):
-    n = cache8.choose_splits(items, keys, 148)
-    assert 1 <= n <= 64 and (n == 1 or items * n <= 2 * 148) and (keys is None or n == 1 or (n - 1) * 128 < keys)
-    assert math.isfinite(n)

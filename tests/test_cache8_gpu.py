@@ -245,6 +245,7 @@ def test_values_and_keys_of_every_size(rows, d):
     q = torch.randn((rows[0][1], 4, d), generator=gen, device=DEV)
     q[:, 1] *= 2.0 ** -100
     q[:, 2] = 0
+    q[:, 3] *= 2.0 ** 60  # (one key takes it all)
     q = q.bfloat16()
     q, out = _attend(pb, 4, d, d ** -0.5, q=q)
     _close(pb, q, out, d ** -0.5)
@@ -265,8 +266,18 @@ def test_what_is_not_finite_reaches_only_who_sees_it():
         assert bool(out.isfinite().all())
         pb.v8.exponents[page, 1, slot] = 127
         pb.k8.exponents[page, 0, slot] = 255
+        pb.k8.codes[page, 0, slot] = 0
         q, out = _attend(pb, 4, d, 0.1)
         assert bool(out[:n, :2].isnan().all()) and bool(out[:n, 2:].isfinite().all()) and bool(out[n:].isfinite().all())
+        if n > 1:  # a later token's key and value: the tokens before it do not see them
+            pb.k8.exponents[page, 0, slot] = 127
+            page, slot = pb.tables[0][102 // 16], 102 % 16
+            pb.v8.codes[page, 0, slot] = 0
+            pb.v8.exponents[page, 0, slot] = 255
+            pb.k8.exponents[page, 1, slot] = 255
+            pb.k8.codes[page, 1, slot] = 0
+            q, out = _attend(pb, 4, d, 0.1)
+            assert bool(out[2:n].isnan().all()) and bool(out[:2].isfinite().all()) and bool(out[n:].isfinite().all())
 
 
 def test_rows_without_keys_are_zero():
