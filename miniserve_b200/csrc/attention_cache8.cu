@@ -127,11 +127,12 @@ struct Split8 {
   const int* page_indices;
   int* status;
   float* part;              // [2 * ctas][16][PART]: a CTA's partial of the item that began before it, and of the one that goes on behind it
-  int4* cut;                // [ctas]: of the cut item that begins in the CTA, its first query row (counted in tokens x heads of a kv head), rows, kv head and pieces; 0 pieces: none does
+  int4* cut;                // [ctas]: for the second kernel, of the cut item that begins in the CTA: its first query row (counted in tokens x heads of a kv head), rows, kv head, pieces; 0: none
   int rows, tile0, tiles;   // requests; tiles [tile0, tile0 + tiles) of 8 or 16 query rows of each
   int nq, nkv, window, sink, page_size, ctas;
   float scale;
   int num_pages;
+  int behind;               // the second kernel runs: an item may be cut
 };
 
 // The keys that a tile of query rows sees: those that some row does [lo, hi), those that all do [seen_lo, seen_hi).
@@ -263,7 +264,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     }
     return a;
   };
-  if (tid == 0) {
+  if (tid == 0 && p.behind) {
     int4 cut = make_int4(0, 0, 0, 0);
     if (cta_begin < cta_end && !alone) {
       const Unit& u = table[find(cta_end - 1)];
@@ -280,51 +281,65 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
   float* tail = reinterpret_cast<float*>(smem + warp * STAGES * STAGE_BYTES);    // of the one that goes on behind it: the ring is done with by then
   const int page_shift = 31 - __clz(p.page_size);
 
-  // ---- what is asked for: pages one slice ahead of the copies, so that they are known by then (nothing looks at them before)
-  const int span = min(SLICE, p.page_size), boxes = SLICE / span, box = (lane & (boxes - 1)) * span;  // lane i looks after box i: a page's 8, 16 or 32 keys
-  const int first_unit = find(begin);
-  int a_pos = begin, a_left = 0, a_unit = first_unit, a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_entries = 0, a_page = 0;
-  const int* a_pages = page_indices;
-  auto next_item = [&]() {  // the item that a_pos lies in; false: there is none
-    for (;; ++a_unit) {
-      if (a_pos >= end) return false;
+  // ---- what is asked for. Pages are looked up 32 at a time, a lane each, and the next 32 while these are used.
+  int a_pos = begin, a_left = 0, a_unit = find(begin), a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_table = 0, a_entries = 0;
+  int window = 0, page_ahead = 0, page_row = 0;  // the first of the 32 table entries; the lane's page of the next ones; the pool's row at which its page of these begins
+  const int first_unit = a_unit;
+  auto page_of = [&](int entry) {
+    const int key = entry << page_shift;
+    if (key + p.page_size <= a_lo || key >= a_hi) return 0;  // (not needed: any page that is there)
+    return entry < a_entries ? page_indices[a_table + entry] : -1;
+  };
+  auto turn = [&]() {  // to the entries looked up last
+    int page = page_ahead;
+    if ((unsigned)page >= (unsigned)p.num_pages) {
+      atomicExch(p.status, 2);
+      page = 0;  // (what comes of it is not used)
+    }
+    page_row = (page * p.nkv + a_kvh) << page_shift;
+    page_ahead = page_of(window + 32 + lane);
+  };
+  auto next_item = [&]() {  // the item that a_pos lies in, if there is one
+    while (a_pos < end) {
       const Unit& u = table[a_unit];
       const int past = a_pos - u.at;
       a_kvh = past / u.stride;
-      if (a_kvh >= p.nkv) continue;
       const int off = past - a_kvh * u.stride;
-      if (off >= u.n) {  // (behind a lone item's end)
+      if (a_kvh >= p.nkv) {
+        ++a_unit;
+      } else if (off >= u.n) {  // (behind a lone item's end)
         a_pos += u.stride - off;
-        --a_unit;
-        continue;
+      } else {
+        const Span keys = span_of(p, u.start, u.row0, u.rows_here, group);
+        a_lo = keys.lo;
+        a_hi = keys.hi;
+        a_key = (keys.first_slice + off) * SLICE;
+        a_table = u.table;
+        a_entries = u.entries;
+        a_left = min(u.n - off, end - a_pos);
+        window = a_key >> page_shift;
+        page_ahead = page_of(window + lane);
+        return;
       }
-      const Span keys = span_of(p, u.start, u.row0, u.rows_here, group);
-      a_lo = keys.lo;
-      a_hi = keys.hi;
-      a_key = (keys.first_slice + off) * SLICE + box;
-      a_pages = page_indices + u.table;
-      a_entries = u.entries;
-      a_left = min(u.n - off, end - a_pos);
-      return true;
     }
   };
-  auto look = [&]() {
-    const int entry = a_key >> page_shift;
-    a_page = 0;
-    if (a_key + span > a_lo && a_key < a_hi) a_page = entry < a_entries ? a_pages[entry] : -1;
-  };
-  if (next_item()) look();
+  bool turned = false;  // (the first look at an item's pages waits until the copies are made)
   auto fire = [&](uint32_t st) {  // the slice looked up last, into a stage; then the next one is looked up
     if (a_left > 0) {
-      if ((unsigned)a_page >= (unsigned)p.num_pages) {
-        if (lane < boxes) atomicExch(p.status, 2);
-        a_page = 0;  // (any page that is there: what comes of it is not used)
+      if (!turned) {
+        turn();
+        turned = true;
+      } else if ((a_key >> page_shift) - window >= 32) {
+        window += 32;
+        turn();
       }
-      const int base = ((a_page * p.nkv + a_kvh) << page_shift) + (a_key & (p.page_size - 1));  // the pool's row at which the lane's box begins
       const uint32_t kt = st, vt = st + CODE_BYTES, et = st + 2 * CODE_BYTES;
-      int rows8[SLICE / 8];  // where every eight keys begin
+      int rows8[SLICE / 8];  // the pool's rows at which every eight keys begin
 #pragma unroll
-      for (int i = 0; i < SLICE / 8; ++i) rows8[i] = __shfl_sync(0xffffffffu, base, 8 * i / span) + (8 * i & (span - 1));
+      for (int i = 0; i < SLICE / 8; ++i) {
+        const int key = a_key + 8 * i;
+        rows8[i] = __shfl_sync(0xffffffffu, page_row, (key >> page_shift) - window) + (key & (p.page_size - 1));
+      }
       if (8 * CHUNKS % 32 == 0) {
 #pragma unroll
         for (int i = 0; i < SLICE / 8; ++i) {
@@ -345,18 +360,21 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
             cp_async16(vt + chunk_at(8 * i + row, chunk), v_codes + (size_t)rows8[i] * D + idx * 16);
           }
       }
-      const int mine = __shfl_sync(0xffffffffu, base, 8 * (lane & 3) / span) + (8 * (lane & 3) & (span - 1));
+      const int mine = (lane & 2) ? ((lane & 1) ? rows8[3] : rows8[2]) : ((lane & 1) ? rows8[1] : rows8[0]);
       if (lane < 8) cp_async8(et + lane * 8, (lane < 4 ? k_exps : v_exps) + mine);  // exponents, 8 a lane: of K, then of V
       ++a_pos;
       a_key += SLICE;
-      if (--a_left > 0 || next_item()) look();
+      if (--a_left == 0) {
+        next_item();
+        turned = false;
+      }
     }
     cp_async_commit();
   };
-#pragma unroll 1
-  for (int i = 0; i < STAGES; ++i) fire(ring + i * STAGE_BYTES);
+  next_item();
 
   // ---- what is computed
+  bool filled = false;
   int unit = first_unit, kvh = 0, item_end = begin, item_begin = 0;
   int start = 0, row0 = 0, rows_here = 0, tok0 = 0, n = 0;
   Span it = {};
@@ -399,6 +417,11 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
           raw[j][kk] = make_uint2(0u, 0u);
           if (i < rows_here) raw[j][kk] = *reinterpret_cast<const uint2*>(src + channel_of(kk, t));
         }
+      }
+      if (!filled) {  // (the first copies go out while the first queries are on their way)
+#pragma unroll 1
+        for (int i = 0; i < STAGES; ++i) fire(ring + i * STAGE_BYTES);
+        filled = true;
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -711,74 +734,95 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
   cp_async_wait<0>();
 }
 
-// The items that were cut: a CTA's second partial and its successors' first ones, added up in their order. Block (cta, row).
+// The items that were cut: a CTA's second partial and its successors' first ones, added up in their order. Block (cta, row). Threads side by side take
+// 4 channels each, shares of them every SHARES-th piece. The first few pieces' sums and numbers are asked for together (their places are there however many
+// there are).
 constexpr int MERGE_THREADS = 128;
 __global__ void __launch_bounds__(MERGE_THREADS)
 attn_cache8_merge_kernel(__nv_bfloat16* __restrict__ out, const Split8 p) {
   const int4* cuts = p.cut;
   const float* parts = p.part;
   pdl_prologue(cuts, parts);
-  const int cta = blockIdx.x, row = blockIdx.y, group = p.nq / p.nkv;
+  constexpr int COLS = D / 4, SHARES = MERGE_THREADS / COLS, EARLY = 4;
+  const int cta = blockIdx.x, row = blockIdx.y, group = p.nq / p.nkv, tid = threadIdx.x, col = tid % COLS, share = tid / COLS;
+  auto at = [&](int i) { return parts + ((size_t)(2 * min(cta + i, p.ctas - 1) + (i == 0)) * ROWS + row) * PART; };
   const int4 cut = cuts[cta];
   if (cut.w < 2 || row >= cut.y) return;
-  const int rho = cut.x + row, tok = rho / group;
-  __shared__ float weight[MERGE_THREADS];
+  float4 head[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) head[i] = *reinterpret_cast<const float4*>(at(i) + D);
+  const float4 mine = *reinterpret_cast<const float4*>(at(share) + 4 * col);
+  // the largest m of all pieces, then the largest m + c, the weights and the sum of the weighed l
   __shared__ float4 sums[MERGE_THREADS];
-  __shared__ float red[4];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  auto at = [&](int i) { return parts + ((size_t)(2 * (cta + i) + (i == 0)) * ROWS + row) * PART; };
-  // the largest m of all pieces, then the largest m + c
-  auto block_max = [&](float v) {
-    v = warp_max(v);
-    __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  };
-  float m = NOTHING, c_all = -INFINITY;
-  for (int i = tid; i < cut.w; i += MERGE_THREADS) m = fmaxf(m, at(i)[D]);
-  m = block_max(m);
-  for (int i = tid; i < cut.w; i += MERGE_THREADS) c_all = fmaxf(c_all, (at(i)[D] - m) + at(i)[D + 2]);
-  c_all = block_max(c_all);
-  constexpr int COLS = D / 4, SHARES = MERGE_THREADS / COLS;  // threads side by side take 4 channels each; shares of them take every SHARES-th piece
-  const int col = tid % COLS, share = tid / COLS;
+  __shared__ float weight[MERGE_THREADS], red[MERGE_THREADS / 32];
+  float m = NOTHING, c_all = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int first = 0; first < cut.w; first += MERGE_THREADS) {
-    __syncthreads();
-    if (first + tid < cut.w) {
-      const float4 mlc = *reinterpret_cast<const float4*>(at(first + tid) + D);
-      weight[tid] = ex2(((mlc.x - m) + mlc.z) - c_all);
-      l += weight[tid] * mlc.y;
+  auto add = [&](const float4& x, float w) {
+    acc.x += w * x.x;
+    acc.y += w * x.y;
+    acc.z += w * x.z;
+    acc.w += w * x.w;
+  };
+  if (cut.w <= EARLY) {
+    float w[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) m = i < cut.w ? fmaxf(m, head[i].x) : m;
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+      w[i] = i < cut.w ? (head[i].x - m) + head[i].z : -INFINITY;
+      c_all = fmaxf(c_all, w[i]);
     }
-    __syncthreads();
-    if (share < SHARES) {
-#pragma unroll 4
-      for (int i = share; i < min(MERGE_THREADS, cut.w - first); i += SHARES) {
-        const float4 x = *reinterpret_cast<const float4*>(at(first + i) + 4 * col);
-        const float w = weight[i];
-        acc.x += w * x.x;
-        acc.y += w * x.y;
-        acc.z += w * x.z;
-        acc.w += w * x.w;
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+      w[i] = ex2(w[i] - c_all);
+      if (i < cut.w) l += w[i] * head[i].y;
+      if (i == share && i < cut.w) add(mine, w[i]);
+    }
+    if (share < SHARES)
+      for (int i = share + SHARES; i < cut.w; i += SHARES) add(*reinterpret_cast<const float4*>(at(i) + 4 * col), ex2(((at(i)[D] - m) + at(i)[D + 2]) - c_all));
+  } else {
+    auto block_max = [&](float v) {
+      v = warp_max(v);
+      __syncthreads();
+      if (tid % 32 == 0) red[tid / 32] = v;
+      __syncthreads();
+      return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    };
+    for (int i = tid; i < cut.w; i += MERGE_THREADS) m = fmaxf(m, at(i)[D]);
+    m = block_max(m);
+    for (int i = tid; i < cut.w; i += MERGE_THREADS) c_all = fmaxf(c_all, (at(i)[D] - m) + at(i)[D + 2]);
+    c_all = block_max(c_all);
+    for (int first = 0; first < cut.w; first += MERGE_THREADS) {
+      __syncthreads();
+      if (first + tid < cut.w) {
+        const float4 h = *reinterpret_cast<const float4*>(at(first + tid) + D);
+        weight[tid] = ex2(((h.x - m) + h.z) - c_all);
+        l += weight[tid] * h.y;
+      }
+      __syncthreads();
+      if (share < SHARES) {
+#pragma unroll 8
+        for (int i = share; i < min(MERGE_THREADS, cut.w - first); i += SHARES) add(*reinterpret_cast<const float4*>(at(first + i) + 4 * col), weight[i]);
       }
     }
+    l = warp_sum(l);
+    __syncthreads();
+    if (tid % 32 == 0) red[tid / 32] = l;
+    __syncthreads();
+    l = (red[0] + red[1]) + (red[2] + red[3]);
   }
   sums[tid] = acc;
-  l = warp_sum(l);
   __syncthreads();
-  if (lane == 0) red[warp] = l;
-  __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]) + sink_term(p.sink, m, c_all);
   if (share == 0) {
-    for (int i = 1; i < SHARES; ++i) {
+    for (int i = 1; i < min(SHARES, cut.w); ++i) {
       const float4 x = sums[i * COLS + col];
       acc.x += x.x;
       acc.y += x.y;
       acc.z += x.z;
       acc.w += x.w;
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int rho = cut.x + row, tok = rho / group;
+    const float den = l + sink_term(p.sink, m, c_all), inv = den == 0.f ? 0.f : 1.0f / den;
     __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     uint2 pk;
     pk.x = *reinterpret_cast<uint32_t*>(&lo);
@@ -803,6 +847,8 @@ constexpr int SMEM_MOST = 227 * 1024 - 11 * 1024;  // (the table of tiles is sta
 // Floats of partial results that a launch of `ctas` CTAs needs; the table of cut items (4 ints a CTA) lies behind them.
 MS_EXPORT long long MS_ATTN8_FN(part_floats)(int ctas) { return 2LL * ctas * ROWS * PART; }
 MS_EXPORT int MS_ATTN8_FN(max_units)() { return MAX_UNITS; }
+// Keys up to which few items (no more than CTAs) run a CTA each, whole: nothing is cut then.
+MS_EXPORT int MS_ATTN8_FN(alone_keys)(int tile_rows) { return SLICE * (2 * (tile_rows == 8 ? warps_of(1) : warps_of(2)) - 1); }
 
 template <int NT>
 static int launch_split(const Split8& p, int rows_tile, void* out, const void* q, const void* k_codes,
@@ -840,6 +886,6 @@ MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, int tile_rows, int rows_most, 
   if (int rc = tile_rows == 8 ? launch_split<1>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream)
                               : launch_split<2>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream))
     return rc;
-  MS_LAUNCH(attn_cache8_merge_kernel, dim3(p->ctas, rows_tile), MERGE_THREADS, 0, stream, (__nv_bfloat16*)out, *p);
+  if (p->behind) MS_LAUNCH(attn_cache8_merge_kernel, dim3(p->ctas, rows_tile), MERGE_THREADS, 0, stream, (__nv_bfloat16*)out, *p);
   return 0;
 }

@@ -86,7 +86,7 @@ class _Split(ctypes.Structure):
     """``Split8`` of csrc/attention_cache8.cu."""
 
     _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part", "cut")] + [
-        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i)]
+        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i), ("behind", _i)]
 
 
 class _AttnLib:
@@ -99,6 +99,7 @@ class _AttnLib:
         native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
         self.split = native._declare(lib, pre + "split", [_p, _i, _i] + [_p] * 7)
         self.part_floats = native._declare(lib, pre + "part_floats", [_i], _ll)
+        self.alone_keys = native._declare(lib, pre + "alone_keys", [_i])
         self.max_units = native._declare(lib, pre + "max_units", [])()
 
 
@@ -220,14 +221,17 @@ def _plans(ctx, group: int, key: tuple, device) -> list:
     most = ctx.max_q_len * (nq // nkv)
     tile_rows = 8 if most <= 8 else 16
     tiles, out = -(-most // tile_rows), []
+    # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
+    keys = min(ctx.max_kv_len, window + ctx.max_q_len) if window else ctx.max_kv_len
+    whole = (keys <= lib.alone_keys(tile_rows) and ctx.num_rows * tiles * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing())
     tiles_each = min(tiles, lib.max_units)
     rows_each = lib.max_units // tiles_each
     for first in range(0, ctx.num_rows, rows_each):
-        skip = 4 * first  # the per-row tables are int32
+        skip, rows = 4 * first, min(rows_each, ctx.num_rows - first)  # the per-row tables are int32
         for tile0 in range(0, tiles, tiles_each):
             out.append((_Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
-                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, min(rows_each, ctx.num_rows - first), tile0,
-                               min(tiles_each, tiles - tile0), nq, nkv, window, sink, page_size, ctas, scale, pages), tile_rows, most))
+                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0,
+                               min(tiles_each, tiles - tile0), nq, nkv, window, sink, page_size, ctas, scale, pages, not whole), tile_rows, most))
     return out
 
 
@@ -259,7 +263,7 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
         for plan, tile_rows, most in plans:
             rc = lib.split(ctypes.addressof(plan), tile_rows, most, out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
                            v_pool.exponents.data_ptr(), stream)
-            native.LAUNCHES[0] += 2
+            native.LAUNCHES[0] += 1 + plan.behind
             if rc:
                 raise native.NativeError(lib.last_error().decode())
 
