@@ -74,6 +74,7 @@ def _cache_lib():
     native._declare(lib, "ms_cache8_set_pdl", [_i], None)
     native._declare(lib, "ms_cache8_write", [_p] * 14 + [_i] * 5 + [_f, _i, _ll, _p, _p])
     native._declare(lib, "ms_cache8_read", [_p] * 10 + [_i] * 4 + [_ll, _p, _i, _p])
+    native._declare(lib, "ms_cache8_unpack", [_p] * 11 + [_i] * 7 + [_ll, _i, _p, _p])
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
 
@@ -211,23 +212,24 @@ def _workspace(ctx, floats: int, device) -> torch.Tensor:
     return new
 
 
-def _plans(ctx, group: int, key: tuple, device) -> list:
-    """The launches of a step's attention, the same for every layer with these sizes and this window: ``(plan, query rows of a tile, the most of a request)``."""
+def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device) -> list:
+    """The launches over rows [0, rows_all) of a step, of at most ``most_tokens`` new tokens each, the same for every layer with these sizes and this window:
+    ``(plan, query rows of a tile, the most of a request)``."""
     nq, nkv, d, scale, window, sink, page_size, pages = key
     lib = _attn_lib(d)
     ctas = ctx.sm_count
     floats = lib.part_floats(ctas)
     part = _workspace(ctx, floats + 4 * ctas, device)
-    most = ctx.max_q_len * (nq // nkv)
+    most = most_tokens * (nq // nkv)
     tile_rows = 8 if most <= 8 else 16
     tiles, out = -(-most // tile_rows), []
     # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
-    keys = min(ctx.max_kv_len, window + ctx.max_q_len) if window else ctx.max_kv_len
-    whole = (keys <= lib.alone_keys(tile_rows) and ctx.num_rows * tiles * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing())
+    keys = min(ctx.max_kv_len, window + most_tokens) if window else ctx.max_kv_len
+    whole = (keys <= lib.alone_keys(tile_rows) and rows_all * tiles * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing())
     tiles_each = min(tiles, lib.max_units)
     rows_each = lib.max_units // tiles_each
-    for first in range(0, ctx.num_rows, rows_each):
-        skip, rows = 4 * first, min(rows_each, ctx.num_rows - first)  # the per-row tables are int32
+    for first in range(0, rows_all, rows_each):
+        skip, rows = 4 * first, min(rows_each, rows_all - first)  # the per-row tables are int32
         for tile0 in range(0, tiles, tiles_each):
             out.append((_Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
                                ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0,
@@ -235,36 +237,112 @@ def _plans(ctx, group: int, key: tuple, device) -> list:
     return out
 
 
+def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool, rows: int, most_tokens: int) -> None:
+    """Rows [0, rows) of the step on the kernel that shares out keys."""
+    d = q.shape[2]
+    pages, nkv, page_size, _ = k_pool.shape
+    key = (q.shape[1], nkv, d, float(scale), int(window or 0), int(bool(sink)), page_size, pages)
+    plans = ctx.step_cache.get(("cache8", group, rows, key))
+    if plans is None:
+        plans = ctx.step_cache[("cache8", group, rows, key)] = _plans(ctx, group, rows, most_tokens, key, k_pool.device)
+    lib = _attn_lib(d)
+    args = (out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(), ctx.stream)
+    for plan, tile_rows, most in plans:
+        native.LAUNCHES[0] += 1 + plan.behind
+        if lib.split(ctypes.addressof(plan), tile_rows, most, *args):
+            raise native.NativeError(lib.last_error().decode())
+
+
+# Query rows (new tokens times heads of a kv head) of a request up to which its keys are shared out over the whole device, read once for every 16 rows. Beyond, a step's pages are
+# unpacked to bfloat16 and attended over by the kernels of a bfloat16 cache, which read them once for 256 rows (64): three times the bytes, once.
+SPLIT_ROWS = 64
+UNPACKED_BYTES = 1 << 30  # of pages unpacked at a time, unless a single request has more
+
+
+class _Unpacked:
+    """A step's context whose pages of one group are the unpacked ones: rows [first, num_rows)."""
+
+    def __init__(self, ctx, group: int, num_rows: int, ids: torch.Tensor):
+        self.__dict__.update(ctx.__dict__)
+        self.num_rows = num_rows
+        self.page_indices = list(ctx.page_indices)
+        self.page_indices[group] = ids
+
+
+def _parts(ctx, group: int, first: int, page_size: int, page_bytes: int) -> list:
+    """Rows [first, num_rows) in parts whose pages fit: ``(first row, row behind, page entries)``."""
+    out, at, entries = [], first, 0
+    for r in range(first, ctx.num_rows):
+        n = -(-(ctx.host_q_start[r] + ctx.host_q_len[r]) // page_size)
+        if entries and (entries + n) * page_bytes > UNPACKED_BYTES:
+            out.append((at, r, entries))
+            at, entries = r, 0
+        entries += n
+    out.append((at, ctx.num_rows, entries))
+    return out
+
+
+def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool, first: int) -> None:
+    """Rows [first, num_rows) of the step over pages unpacked to bfloat16."""
+    from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
+
+    pages, nkv, page_size, d = k_pool.shape
+    dev = k_pool.device
+    key = ("cache8_unpacked", group, first, nkv, page_size, d)
+    parts = ctx.step_cache.get(key)
+    if parts is None:
+        page = nkv * page_size * d
+        parts = _parts(ctx, group, first, page_size, 4 * page)
+        # (a table too short is found on the device, and what is read behind its end is some page that is there)
+        most, table = max(n for _, _, n in parts), ctx.page_indices[group].numel() + sum(n for _, _, n in parts)
+        held = ctx.scratch.get("cache8_pages")
+        if held is None or held[0].numel() < most * page or held[2].numel() < table:
+            held = tuple(torch.empty(most * page, dtype=torch.bfloat16, device=dev) for _ in range(2)) + (torch.zeros(table, dtype=torch.int32, device=dev),)
+            ctx.scratch["cache8_pages"] = held
+        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in held[:2])
+        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, held[2])) for a, b, n in parts])
+    k, v, parts = parts
+    for a, entries, view in parts:
+        _cache_check(_cache_lib().ms_cache8_unpack(
+            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
+            v_pool.exponents.data_ptr(), ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows,
+            entries, nkv, d, int(window or 0), page_size, pages, view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+        if attention_tc_ok(q, k):
+            attention_tc_prefill(out, q, k, v, view, group, scale, window, a, sink)
+        else:
+            attention_bf16.run_prefill(out, q, k, v, view, group, scale, window, a, sink)
+
+
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
     """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
-    ``group``, window and sink as there. A row's page that its table or the pool does not have raises the status word. Partial results lie in
+    ``group``, window and sink as there. Single tokens and drafted ones go to the kernel that shares out keys (``csrc/attention_cache8.cu``); prompts and portions of them to a
+    bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool does not have raises the status word. Workspaces lie in
     ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
+    if not (isinstance(v_pool, Pool8) and k_pool.shape == v_pool.shape):
+        _check_pools(k_pool, v_pool)
+    nq, d = q.shape[1], q.shape[2]
+    nkv, dim = k_pool.shape[1], k_pool.shape[3]
+    dev = q.get_device()
+    if not (out.shape == q.shape and q.dtype == out.dtype == torch.bfloat16 and dev >= 0 and dev == out.get_device() == k_pool.codes.get_device() == v_pool.codes.get_device()
+            and q.is_contiguous() and out.is_contiguous()):
+        raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape, and pools of one shape, on one device")
+    if dim != d or nq % nkv or (window or 0) < 0:
+        raise ValueError(f"{nq} query heads of {d} over pools {tuple(k_pool.shape)}, window {window}")
     if getattr(ctx, "recorder", None) is not None:
         # a pass that is captured for steps of other lengths too: launched anew for each, between the graphs
         ctx.recorder.defer(lambda step: attention(out, q, k_pool, v_pool, step, group, scale, window, sink))
         return
-    t, nq, d = q.shape
-    pages, nkv, page_size, dim = k_pool.shape
-    key = (nq, nkv, d, float(scale), int(window or 0), int(bool(sink)), page_size, pages)
-    plans = ctx.step_cache.get(("cache8", group, key))
-    if plans is None:
-        _check_pools(k_pool, v_pool)
-        if dim != d or nq % nkv or int(window or 0) < 0:
-            raise ValueError(f"{nq} query heads of {d} over pools {tuple(k_pool.shape)}, window {window}")
-        _check_tables(k_pool.device, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
-        plans = ctx.step_cache[("cache8", group, key)] = _plans(ctx, group, key, k_pool.device)
-    dev = k_pool.codes.device
-    if not (out.shape == q.shape and v_pool.shape == k_pool.shape and q.dtype == out.dtype == torch.bfloat16 and q.device == out.device == v_pool.codes.device == dev
-            and q.is_contiguous() and out.is_contiguous()):
-        raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape, and pools of one shape, on one device")
-    lib, stream = _attn_lib(d), ctx.stream
+    dense = ctx.max_q_len * (nq // nkv) > SPLIT_ROWS
 
     def launch():
-        for plan, tile_rows, most in plans:
-            rc = lib.split(ctypes.addressof(plan), tile_rows, most, out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
-                           v_pool.exponents.data_ptr(), stream)
-            native.LAUNCHES[0] += 1 + plan.behind
-            if rc:
-                raise native.NativeError(lib.last_error().decode())
+        single = ctx.leading_single_rows if dense else ctx.num_rows
+        if single:
+            _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single, 1 if dense else ctx.max_q_len)
+        if single < ctx.num_rows:
+            _dense(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single)
 
-    _launch(dev, launch)
+    if torch.cuda.current_device() == dev:
+        launch()
+    else:
+        with torch.cuda.device(dev):
+            launch()

@@ -164,6 +164,11 @@ def test_pages_that_are_not_there():
         out = torch.empty((20, 2, d), dtype=torch.bfloat16, device=DEV)
         ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
         assert pb.status.item() == 2, bad
+        for heads in (8, 16):  # as many query rows as go over unpacked pages
+            pb.status.zero_()
+            q = torch.zeros((20, heads, d), dtype=torch.bfloat16, device=DEV)
+            ops.attention(torch.empty_like(q), q, pb.k8, pb.v8, ku.make_context(pb), 0, 0.1, None)
+            assert pb.status.item() == 2, (bad, heads)
 
 
 # ------------------------------------------------------------------ attention
