@@ -22,6 +22,7 @@ from typing import Sequence
 
 import torch
 
+from ..ops.cache8 import Pool8, read_cache, takes
 from ..parts.base import FixedState, PagedKV, flat_needs
 from ..parts.decoder import EntryCache
 from .blocks import BlockAllocator, BlockTable, OutOfBlocks
@@ -33,8 +34,11 @@ class CacheGroup:
     entries: list[int]  # run entries that own a cache in this group
     allocator: BlockAllocator
     page_size: int
-    k: torch.Tensor | None = None  # [entries, pages + 1, kv_heads, page_size, head_dim]
+    k: torch.Tensor | None = None  # [entries, pages + 1, kv_heads, page_size, head_dim]; in 8 bits the codes
     v: torch.Tensor | None = None
+    k_exponents: torch.Tensor | None = None  # in 8 bits: [entries, pages + 1, kv_heads, page_size]
+    v_exponents: torch.Tensor | None = None
+    eight_bits: bool = False
 
     @property
     def pad_page(self) -> int:
@@ -42,17 +46,26 @@ class CacheGroup:
         return self.allocator.num_blocks
 
     def bytes_per_token(self, itemsize: int) -> int:
-        return (2 if self.need.values else 1) * len(self.entries) * self.need.kv_heads * self.need.head_dim * itemsize
+        vector = vector_bytes(self.need.head_dim, itemsize, self.eight_bits)
+        return (2 if self.need.values else 1) * len(self.entries) * self.need.kv_heads * vector
+
+    def pools(self, index: int) -> tuple:
+        """The pools of keys and values of the group's entry ``index``."""
+        if self.k is None:
+            return None, None
+        if self.eight_bits:
+            return Pool8(self.k[index], self.k_exponents[index]), Pool8(self.v[index], self.v_exponents[index])
+        return self.k[index], self.v[index]
 
 
 @dataclass
 class KVEntryView:
     """What an attention mixer gets: its group's index (to pick the page table from the step
-    context), its own K and V pools [pages + 1, kv_heads, page_size, head_dim]."""
+    context), its own K and V pools [pages + 1, kv_heads, page_size, head_dim] (``Pool8`` where they are in 8 bits)."""
 
     group: int
-    k: torch.Tensor | None
-    v: torch.Tensor | None
+    k: "torch.Tensor | Pool8 | None"
+    v: "torch.Tensor | Pool8 | None"
     page_size: int
 
 
@@ -105,10 +118,28 @@ def window_pages(window: int, page_size: int, step_tokens: int) -> int:
     return -(-(window + step_tokens) // page_size) + 1
 
 
+def vector_bytes(head_dim: int, itemsize: int, eight_bits: bool) -> int:
+    """Bytes of one head's vector in the cache: its numbers, or a code each and an exponent."""
+    return head_dim + 1 if eight_bits else head_dim * itemsize
+
+
+def check_needs8(entry_caches: Sequence[EntryCache], page_size: int) -> None:
+    """Raise unless what the run entries ask of the cache can be held in 8 bits."""
+    for need, _ in group_needs(entry_caches)[0]:
+        if not need.values:
+            raise ValueError("an 8-bit cache holds keys and values, not one latent vector for both")
+        if not takes(need.head_dim, page_size):
+            raise ValueError(f"an 8-bit cache takes head sizes that are multiples of 16 up to 256 and pages of a power of two of at least 8 tokens, not "
+                             f"{need.head_dim} and {page_size}")
+
+
+KV_DTYPES = ("auto", "fp8")  # how keys and values are held: in the model's type, or in 8 bits (``ops.Pool8``)
+
+
 class CacheManager:
     def __init__(self, entry_caches: Sequence[EntryCache], num_pages: "int | Sequence[int]", page_size: int, max_requests: int,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str | None = None,
-                 poison: bool = False, poison_on_free: bool = False, step_tokens: int | None = None):
+                 poison: bool = False, poison_on_free: bool = False, step_tokens: int | None = None, kv_dtype: str = "auto"):
         """``entry_caches``: one per run entry (``DecoderModel.entry_caches``). ``num_pages``:
         pages of ``page_size`` tokens, one number for every group or one per group (in the order
         of ``group_needs``). ``device`` None keeps everything on the host (bookkeeping only, for
@@ -116,7 +147,16 @@ class CacheManager:
         up; ``poison_on_free`` also fills a request's pages with NaN when it gives them back, so
         that a stale key read through a reused page shows up (a debugging aid: it launches a fill
         per release). ``step_tokens``: the most tokens a step brings one request; with it,
-        ``pages_for`` knows that a windowed group never holds a whole long request."""
+        ``pages_for`` knows that a windowed group never holds a whole long request. ``kv_dtype``: "fp8" keeps keys and
+        values in 8 bits (per-request state of fixed size stays as it is)."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype is one of {KV_DTYPES}, not {kv_dtype!r}")
+        eight_bits = kv_dtype == "fp8"
+        if eight_bits:
+            check_needs8(entry_caches, page_size)
+            if dtype != torch.bfloat16:
+                raise ValueError(f"an 8-bit cache belongs to a bfloat16 model, not to one in {dtype}")
+        self.kv_dtype = kv_dtype
         if page_size < 1 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two, got {page_size}")
         needs, _ = group_needs(entry_caches)
@@ -146,7 +186,7 @@ class CacheManager:
                     if g is None:
                         g = len(self.groups)
                         by_need[need] = g
-                        self.groups.append(CacheGroup(need, [], BlockAllocator(per_group[g], page_size), page_size))
+                        self.groups.append(CacheGroup(need, [], BlockAllocator(per_group[g], page_size), page_size, eight_bits=eight_bits))
                     owners[(i, n)] = (g, len(self.groups[g].entries))
                     self.groups[g].entries.append(i)
                 elif isinstance(need, FixedState):
@@ -156,6 +196,10 @@ class CacheManager:
         if self.device is not None:
             for grp in self.groups:
                 shape = (len(grp.entries), grp.allocator.num_blocks + 1, grp.need.kv_heads, page_size, grp.need.head_dim)
+                if eight_bits:
+                    grp.k, grp.v = (torch.full(shape, 0x7F if poison else 0, dtype=torch.uint8, device=self.device) for _ in range(2))
+                    grp.k_exponents, grp.v_exponents = (torch.full(shape[:-1], 255 if poison else 0, dtype=torch.uint8, device=self.device) for _ in range(2))
+                    continue
                 fill = float("nan") if poison else 0.0
                 grp.k = torch.full(shape, fill, dtype=dtype, device=self.device)
                 grp.v = torch.full(shape, fill, dtype=dtype, device=self.device) if grp.need.values else grp.k
@@ -175,8 +219,7 @@ class CacheManager:
             if isinstance(need, PagedKV):
                 g, idx = owners[(owner, n)]
                 grp = self.groups[g]
-                return KVEntryView(g, grp.k[idx] if grp.k is not None else None, grp.v[idx] if grp.v is not None else None,
-                                   page_size)
+                return KVEntryView(g, *grp.pools(idx), page_size)
             return StateEntryView(state_tensors[(owner, n)], tuple(need.shape))
 
         def merged(own, other):
@@ -214,7 +257,8 @@ class CacheManager:
         return sum(g.bytes_per_token(item) for g in self.groups)
 
     def pool_bytes(self) -> int:
-        return sum(g.k.numel() * g.k.element_size() * (2 if g.need.values else 1) for g in self.groups if g.k is not None)
+        return sum((g.k.numel() * g.k.element_size() + (g.k_exponents.numel() if g.eight_bits else 0)) * (2 if g.need.values else 1)
+                   for g in self.groups if g.k is not None)
 
     def state_bytes(self) -> int:
         """Bytes of the per-request state tensors (one slot per request the cache can hold)."""
@@ -258,6 +302,10 @@ class CacheManager:
                 held = [b for b in t.blocks if b >= 0]
                 if held and g.k is not None:
                     idx = torch.tensor(held, dtype=torch.long, device=self.device)
+                    if g.eight_bits:
+                        g.k[:, idx] = g.v[:, idx] = 0x7F
+                        g.k_exponents[:, idx] = g.v_exponents[:, idx] = 255
+                        continue
                     g.k[:, idx] = float("nan")
                     g.v[:, idx] = float("nan")
         for t in rc.tables:
@@ -267,6 +315,34 @@ class CacheManager:
             self._free_slots.append(rc.state_slot)
         rc.state_slot = -1
         rc.released = True
+
+    def read(self, rc: RequestCache, entry: int, start: int = 0, stop: int | None = None, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values that run entry ``entry`` has cached for a request, positions [start, stop) (default: all), as
+        dense rows [n, kv_heads, head_dim] in ``dtype`` (default: the model's): behind norm and rotation, as attention reads them."""
+        if rc.released:
+            raise ValueError("read of a released request cache")
+        view = self._entry_view[entry]
+        if not isinstance(view, KVEntryView):
+            raise ValueError(f"run entry {entry} has no single cache of keys and values")
+        table = rc.tables[view.group]
+        stop = table.num_tokens if stop is None else stop
+        if not 0 <= start <= stop <= table.num_tokens:
+            raise ValueError(f"positions [{start}, {stop}) of a request of {table.num_tokens} tokens")
+        blocks = table.blocks
+        if any(b < 0 for b in blocks[start // self.page_size:-(-stop // self.page_size)]):
+            raise ValueError(f"positions [{start}, {stop}) have left the window: their pages were given back")
+        dtype = dtype or self.dtype
+        n, shape = stop - start, view.k.shape
+        if not isinstance(view.k, Pool8):
+            pos = torch.arange(start, stop, device=self.device)
+            page = torch.tensor(blocks, dtype=torch.long, device=self.device)[pos // self.page_size]
+            return view.k[page, :, pos % self.page_size].to(dtype), view.v[page, :, pos % self.page_size].to(dtype)
+        k, v = (torch.empty((n, shape[1], shape[3]), dtype=dtype, device=self.device) for _ in range(2))
+        if n:
+            i32 = dict(dtype=torch.int32, device=self.device)
+            read_cache(k, v, view.k, view.v, torch.arange(start, stop, **i32), torch.zeros(n, **i32), torch.tensor([0, len(blocks)], **i32),
+                       torch.tensor(blocks, **i32), torch.zeros(1, **i32))
+        return k, v
 
     @property
     def num_free_slots(self) -> int:

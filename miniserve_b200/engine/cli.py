@@ -31,6 +31,8 @@ def add_engine_args(parser: argparse.ArgumentParser) -> None:
                         "(from 16 on also the size halfway to it) or to this number (default: --max-running)")
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                    help="bfloat16: the serving kernels; float32: the whole model in true 32-bit")
+    g.add_argument("--kv-cache-dtype", choices=["auto", "fp8"], default="auto",
+                   help="auto: keys and values in the model's type; fp8: in 8 bits, half the memory a token")
     g.add_argument("--disable-overlap", action="store_true",
                    help="wait for a step's tokens before planning the next one (the host then idles while the GPU works)")
     g.add_argument("--poison-on-free", action="store_true",
@@ -63,6 +65,7 @@ def engine_kwargs(args: argparse.Namespace) -> dict:
         overlap=not args.disable_overlap,
         poison_on_free=args.poison_on_free,
         schedule_policy=args.schedule_policy,
+        kv_cache_dtype=args.kv_cache_dtype,
     )
 
 

@@ -24,7 +24,7 @@ from typing import Sequence
 
 import torch
 
-from ..cache.manager import CacheManager, group_needs, window_pages
+from ..cache.manager import KV_DTYPES, CacheManager, group_needs, vector_bytes, window_pages
 from ..parts.decoder import DecoderModel
 from ..sampling.sampler import Sampler
 from .request import PLACEHOLDER, Request, RequestState, SamplingParams
@@ -77,7 +77,7 @@ class Engine:
                  max_running: int = 64, max_prefill_tokens: int = 8192, chunked_prefill_size: int | None = None,
                  seed: int = 0, cuda_graph: bool = True, cuda_graph_max_bs: int | None = None,
                  kv_mem_fraction: float = 0.9, overlap: bool = True, cache: CacheManager | None = None, step_fn=None,
-                 sampler=None, poison_on_free: bool = False, step_graphs: bool = True, schedule_policy: str = "fcfs"):
+                 sampler=None, poison_on_free: bool = False, step_graphs: bool = True, schedule_policy: str = "fcfs", kv_cache_dtype: str = "auto"):
         """``kv_pool_tokens``: exact size of the cache pool in tokens, rounded down to whole pages
         (default: ``kv_mem_fraction`` of the memory the device has free after the weights, less a
         reserve for activations). ``chunked_prefill_size``: tokens per step, decode tokens included,
@@ -87,7 +87,9 @@ class Engine:
         decode-only steps of up to ``cuda_graph_max_bs`` requests (default ``max_running``).
         ``step_graphs``: with ``cuda_graph``, also capture prompt and mixed steps whose shape comes again.
         ``overlap``: launch each step before reading back the previous one.
-        ``schedule_policy``: "fcfs" or "sjf" (``Scheduler``).
+        ``schedule_policy``: "fcfs" or "sjf" (``Scheduler``). ``kv_cache_dtype``: "auto" keeps keys and values in the
+        model's type, "fp8" in 8 bits with a power of two per token and head (``ops.Pool8``): half the bytes a token, for
+        bfloat16 models whose attention layers are plain grouped-query ones (windows and a sink of score 0 allowed).
         Names and meanings follow miniserve/engine/engine.py:42-77. ``cache``, ``step_fn`` and
         ``sampler`` replace the ones the engine would build (a test can run the whole loop on the
         host against a stand-in step function this way). ``poison_on_free``: a debugging aid, see
@@ -96,15 +98,19 @@ class Engine:
         if chunked_prefill_size is None:
             chunked_prefill_size = DEFAULT_CHUNKED_PREFILL
         step_tokens = chunked_prefill_size if chunked_prefill_size else max_prefill_tokens
+        if kv_cache_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_cache_dtype is one of {KV_DTYPES}, not {kv_cache_dtype!r}")
         if cache is None:
-            num_pages = self._pool_pages(model, kv_pool_tokens, page_size, kv_mem_fraction, step_tokens, max_running)
+            if kv_cache_dtype == "fp8":
+                model.check_cache8(page_size)
+            num_pages = self._pool_pages(model, kv_pool_tokens, page_size, kv_mem_fraction, step_tokens, max_running, kv_cache_dtype == "fp8")
             cache = CacheManager(model.entry_caches, num_pages, page_size, max_running, dtype=model.dtype,
-                                 device=model.device, poison_on_free=poison_on_free, step_tokens=step_tokens)
+                                 device=model.device, poison_on_free=poison_on_free, step_tokens=step_tokens, kv_dtype=kv_cache_dtype)
         self.cache = cache
         self.settings = dict(kv_pool_tokens=kv_pool_tokens, page_size=page_size, max_running=max_running,
                              max_prefill_tokens=max_prefill_tokens, chunked_prefill_size=chunked_prefill_size, seed=seed,
                              cuda_graph=cuda_graph, cuda_graph_max_bs=cuda_graph_max_bs or max_running, overlap=overlap,
-                             schedule_policy=schedule_policy)
+                             schedule_policy=schedule_policy, kv_cache_dtype=getattr(cache, "kv_dtype", "auto"))
         self.step_fn = step_fn if step_fn is not None else StepFunction(model, self.cache)
         self.scheduler = Scheduler(self.cache, max_running, max_prefill_tokens, chunked_prefill_size, schedule_policy)
         self.sampler = sampler if sampler is not None else Sampler(model.device, model.spec.vocab_size, max_running)
@@ -135,14 +141,14 @@ class Engine:
         self._pinned: list[torch.Tensor] = []
 
     @staticmethod
-    def _pool_pages(model, kv_pool_tokens, page_size, fraction, step_tokens, max_running) -> list[int]:
+    def _pool_pages(model, kv_pool_tokens, page_size, fraction, step_tokens, max_running, eight_bits=False) -> list[int]:
         """Pages for each cache group (in ``group_needs`` order). A group that keeps every key gets
         ``kv_pool_tokens`` worth of pages, or its share of the device memory that is left after the
         weights, the per-request state tensors and a reserve for a step's activations; a windowed
         group never needs more than ``max_running`` requests' windows, and gets no more."""
         item = torch.empty((), dtype=model.dtype).element_size()
         needs, states = group_needs(model.entry_caches)
-        page_bytes = [2 * count * need.kv_heads * need.head_dim * item * page_size for need, count in needs]
+        page_bytes = [2 * count * need.kv_heads * vector_bytes(need.head_dim, item, eight_bits) * page_size for need, count in needs]
         bound = [max_running * window_pages(need.window, page_size, step_tokens) if need.window else None for need, _ in needs]
         if kv_pool_tokens is not None:
             if kv_pool_tokens < page_size:
@@ -152,9 +158,9 @@ class Engine:
         free, _ = torch.cuda.mem_get_info(model.device)
         state_bytes = sum(max_running * torch.empty((), dtype=st.dtype).element_size() * _numel(st.shape) for st in states)
         # activations of the largest step: a few [tokens, widest] buffers, and float32 logits of every row; a gigabyte for the rest, and
-        # one for the scratch of recurrent layers over long rows (``csrc/tile_walk.cu`` takes no more)
+        # one for the scratch of recurrent layers over long rows (``csrc/tile_walk.cu`` takes no more), or for pages of an 8-bit cache unpacked for prompts
         widest = max(model.spec.hidden_size * 8, 1)
-        reserve = step_tokens * widest * 4 * 4 + max_running * model.spec.vocab_size * 4 * 3 + (1 << 30) * (2 if states else 1)
+        reserve = step_tokens * widest * 4 * 4 + max_running * model.spec.vocab_size * 4 * 3 + (1 << 30) * (1 + bool(states) + eight_bits)
         usable = int(fraction * (free - reserve - state_bytes))
         windowed = sum(b * pb for b, pb in zip(bound, page_bytes) if b is not None)
         whole = sum(pb for b, pb in zip(bound, page_bytes) if b is None)

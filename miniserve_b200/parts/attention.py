@@ -120,6 +120,10 @@ class GQAttention(Part):
         return self.heads * self.value_dim if self.out_gate == "channel_sigmoid" else (self.heads if self.out_gate else 0)
 
     @property
+    def takes_cache8(self) -> bool:
+        return not self.general
+
+    @property
     def owns_cache(self) -> bool:
         return self.kv_source == "own"
 

@@ -121,6 +121,9 @@ class Part:
     # have recurring step shapes replayed from CUDA graphs (``DecoderModel.shape_static``). A part that
     # reads ``ctx.host_*`` to decide what to launch leaves it False.
     shape_static = False
+    # (mixers) True if the keys and values that this mixer reads and writes may be held in 8 bits (``ops.Pool8``): it
+    # goes through ``ops.qk_norm_rope_kv`` and ``ops.attention`` alone, with a window and a sink of score 0 at most.
+    takes_cache8 = False
 
     def __init__(self, spec: PartSpec, env: BuildEnv):
         self.spec = spec

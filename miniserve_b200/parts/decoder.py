@@ -9,7 +9,7 @@ from typing import Mapping
 import torch
 
 from ..config.spec import ModelSpec
-from .base import BuildEnv, CacheNeed, ResidualStream, WeightDecl, build_part, flat_needs
+from .base import BuildEnv, CacheNeed, PagedKV, ResidualStream, WeightDecl, build_part, flat_needs
 from .block import build_block
 
 
@@ -80,6 +80,18 @@ class DecoderModel:
             return bool(getattr(part, "shape_static", False)) and all(ok(p) for p in subs)
 
         return all(ok(p) for p in [self.embedding, self.final_norm, self.head, *self.layers, *self.transitions])
+
+    def check_cache8(self, page_size: int) -> None:
+        """Raise unless every run entry's keys and values may be held in 8 bits, in pages of ``page_size`` tokens."""
+        from ..cache.manager import check_needs8
+
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"an 8-bit cache belongs to a bfloat16 model, not to one in {self.dtype}")
+        check_needs8(self.entry_caches, page_size)
+        for i, (entry, cache) in enumerate(zip(self.spec.run_order, self.entry_caches)):
+            mixer = self.layers[entry.layer].mixer
+            if any(isinstance(n, PagedKV) for n in flat_needs(cache.need)) and not mixer.takes_cache8:
+                raise ValueError(f"run entry {i}: its mixer ({mixer.spec.kind}) has a part that an 8-bit cache does not go with")
 
     @property
     def dtype(self) -> torch.dtype:

@@ -38,3 +38,71 @@ def test_pools_on_the_host_are_refused_by_the_kernels():
         ops.read_cache(rows, rows, p, p, i, i, i, i, i)
     with pytest.raises(TypeError, match="both"):
         ops.read_cache(rows, rows, p, p.codes, i, i, i, i, i)
+
+
+# ------------------------------------------------------------------ the cache manager
+def _entries(head_dim=64, values=True):
+    from miniserve_b200.parts.base import PagedKV
+    from miniserve_b200.parts.decoder import EntryCache
+
+    return [EntryCache(0, PagedKV(2, head_dim, values=values)), EntryCache(1, PagedKV(2, head_dim, values=values))]
+
+
+def test_the_manager_counts_a_byte_a_number_and_one_a_vector():
+    from miniserve_b200.cache import CacheManager
+
+    cm = CacheManager(_entries(), 6, 16, 2, device="cpu", kv_dtype="fp8")
+    assert cm.bytes_per_token() == 2 * 2 * 2 * 65 and cm.pool_bytes() == 2 * 2 * 7 * 2 * 16 * 65
+    view = cm.entry_views[1]
+    assert isinstance(view.k, ops.Pool8) and view.k.shape == (7, 2, 16, 64) and view.k.codes.data_ptr() != cm.entry_views[0].k.codes.data_ptr()
+    plain = CacheManager(_entries(), 6, 16, 2, device="cpu")
+    assert plain.bytes_per_token() == 2 * 2 * 2 * 128
+
+
+def test_freed_pages_are_poisoned():
+    from miniserve_b200.cache import CacheManager
+
+    cm = CacheManager(_entries(), 3, 16, 2, device="cpu", kv_dtype="fp8", poison_on_free=True)
+    rc = cm.new_request()
+    cm.reserve([(rc, 20)])
+    pages = list(rc.tables[0].blocks)
+    cm.release(rc)
+    for e in (0, 1):
+        k = cm.entry_views[e].k
+        assert bool((k.exponents[pages] == 255).all()) and bool((k.codes[pages] == 0x7F).all())
+        assert not bool((k.exponents == 255).all())
+
+
+@pytest.mark.parametrize("kwargs,what", [(dict(page=4), "at least 8"), (dict(head_dim=40), "multiples of 16"), (dict(values=False), "latent"),
+                                         (dict(dtype=torch.float32), "bfloat16 model"), (dict(kv_dtype="int4"), "kv_dtype")])
+def test_what_an_8_bit_cache_does_not_go_with(kwargs, what):
+    from miniserve_b200.cache import CacheManager
+
+    kwargs = dict(kwargs)
+    page, entries = kwargs.pop("page", 16), _entries(kwargs.pop("head_dim", 64), kwargs.pop("values", True))
+    with pytest.raises(ValueError, match=what):
+        CacheManager(entries, 3, page, 2, device=None, **{"kv_dtype": "fp8", **kwargs})
+
+
+def test_models_with_other_mixers_are_refused():
+    from miniserve_b200.config import preset, resolve
+    from miniserve_b200.parts.decoder import DecoderModel
+
+    def build(name, dtype):
+        return DecoderModel(resolve(preset(name))[2], dtype, "cpu")
+
+    build("tiny-b", torch.bfloat16).check_cache8(16)
+    for name, dtype, what in (("tiny-b", torch.float32, "bfloat16 model"), ("fekulix-tiny", torch.bfloat16, "run entry"), ("mugipel-tiny", torch.bfloat16, "run entry|latent")):
+        with pytest.raises(ValueError, match=what):
+            build(name, dtype).check_cache8(16)
+
+
+def test_the_command_line_has_the_option():
+    import argparse
+
+    from miniserve_b200.engine.cli import add_engine_args, engine_kwargs
+
+    ap = argparse.ArgumentParser()
+    add_engine_args(ap)
+    assert engine_kwargs(ap.parse_args(["--kv-cache-dtype", "fp8"]))["kv_cache_dtype"] == "fp8"
+    assert engine_kwargs(ap.parse_args([]))["kv_cache_dtype"] == "auto"
