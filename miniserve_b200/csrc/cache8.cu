@@ -84,54 +84,62 @@ cache8_write_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_c
   if (lane == 0) (is_v ? v_exps : k_exps)[at] = (uint8_t)b;
 }
 
-// Head sizes 64, 128 and 256 rotated whole or not at all: a block per token, D / 16 lanes per head. A lane holds 8 numbers of the head's first half and the 8 of the second that
-// rotate with them, in 16-byte loads and stores (8 of codes); a head's lanes exchange a sum of squares and a maximum. What hangs on the token alone is fetched once a lane,
-// and its first numbers before the page is looked up (three loads, one behind the other).
-template <int D>
-__global__ void __launch_bounds__(256)
+__device__ __forceinline__ void c8_float4(float (&f)[4], const uint2& v) {  // of bfloat16
+  f[0] = __uint_as_float(v.x << 16);
+  f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+  f[2] = __uint_as_float(v.y << 16);
+  f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint2 c8_bf16x4(const float (&f)[4]) {
+  __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+  return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+}
+
+// Head sizes 64, 128 and 256 rotated whole or not at all: a block per token, D / 8 lanes per head. A lane holds 4 numbers of the head's first half and the 4 of the second that
+// rotate with them; a head's lanes exchange a sum of squares and a maximum. What hangs on the token alone is fetched once a lane, and its first numbers before the
+// page is looked up (three loads, one behind the other). Bound by those chains: with 8 and 8 numbers a lane, 72 registers and 24 warps a multiprocessor, 2,048 tokens of 48 heads took 21 us.
+// TABLE: the angles' cosines and sines are given, or nothing is rotated (the form that makes them itself needs more registers).
+template <int D, bool TABLE>
+__global__ void __launch_bounds__(256, TABLE ? 5 : 1)
 cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_exps, uint8_t* __restrict__ v_codes,
                           uint8_t* __restrict__ v_exps, const __nv_bfloat16* __restrict__ qkv, const __nv_bfloat16* __restrict__ q_norm_w,
                           const __nv_bfloat16* __restrict__ k_norm_w, const float* __restrict__ inv_freq, const float* __restrict__ cos_sin,
                           const int* __restrict__ positions, const int* __restrict__ row_of_token, const int* __restrict__ page_indptr,
                           const int* __restrict__ page_indices, int nq, int nkv, float eps, int page_shift, int num_pages, int* __restrict__ status) {
   pdl_prologue(qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, page_indptr, page_indices);
-  constexpr int LPH = D / 16, HPW = 32 / LPH, HALF = D / 2, BATCH = 2;
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPH, slot = lane / LPH, j0 = sub * 8;
+  constexpr int LPH = D / 8, HPW = 32 / LPH, HALF = D / 2, BATCH = 2;
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPH, slot = lane / LPH, j0 = sub * 4;
   const int heads = nq + 2 * nkv, stride = (int)(blockDim.x >> 5) * HPW;  // heads a pass
-  const __nv_bfloat16* row_in = qkv + (size_t)t * heads * D;
-  uint4 lo_raw[BATCH], hi_raw[BATCH];
+  const __nv_bfloat16* row_in = qkv + (size_t)t * heads * D + j0;
+  uint2 lo_raw[BATCH], hi_raw[BATCH];
   auto fetch = [&](int base) {
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       const __nv_bfloat16* src = row_in + (size_t)min(base + warp * HPW + slot + b * stride, heads - 1) * D;  // past the end: the last head again, unused
-      lo_raw[b] = *reinterpret_cast<const uint4*>(src + j0);
-      hi_raw[b] = *reinterpret_cast<const uint4*>(src + HALF + j0);
+      lo_raw[b] = *reinterpret_cast<const uint2*>(src);
+      hi_raw[b] = *reinterpret_cast<const uint2*>(src + HALF);
     }
   };
   fetch(0);
   const int pos = positions[t], request = row_of_token[t];
   const bool normed = q_norm_w != nullptr;
-  uint4 w_raw[2][2] = {};  // of q and k, both halves
+  uint2 wq_lo = make_uint2(0u, 0u), wq_hi = wq_lo, wk_lo = wq_lo, wk_hi = wq_lo;
   if (normed) {
-    w_raw[0][0] = *reinterpret_cast<const uint4*>(q_norm_w + j0);
-    w_raw[0][1] = *reinterpret_cast<const uint4*>(q_norm_w + HALF + j0);
-    w_raw[1][0] = *reinterpret_cast<const uint4*>(k_norm_w + j0);
-    w_raw[1][1] = *reinterpret_cast<const uint4*>(k_norm_w + HALF + j0);
+    wq_lo = *reinterpret_cast<const uint2*>(q_norm_w + j0);
+    wq_hi = *reinterpret_cast<const uint2*>(q_norm_w + HALF + j0);
+    wk_lo = *reinterpret_cast<const uint2*>(k_norm_w + j0);
+    wk_hi = *reinterpret_cast<const uint2*>(k_norm_w + HALF + j0);
   }
-  float cs[8], sn[8];
-  if (inv_freq == nullptr) {
+  float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
+  if (inv_freq != nullptr) {
+    if (TABLE) {
+      const float4 c = *reinterpret_cast<const float4*>(cos_sin + (size_t)t * D + j0), s = *reinterpret_cast<const float4*>(cos_sin + (size_t)t * D + HALF + j0);
+      cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+      sn[0] = s.x; sn[1] = s.y; sn[2] = s.z; sn[3] = s.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
-  } else if (cos_sin) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 c = reinterpret_cast<const float4*>(cos_sin + (size_t)t * D + j0)[i], s = reinterpret_cast<const float4*>(cos_sin + (size_t)t * D + HALF + j0)[i];
-      cs[4 * i] = c.x; cs[4 * i + 1] = c.y; cs[4 * i + 2] = c.z; cs[4 * i + 3] = c.w;
-      sn[4 * i] = s.x; sn[4 * i + 1] = s.y; sn[4 * i + 2] = s.z; sn[4 * i + 3] = s.w;
+      for (int i = 0; i < 4; ++i) sincosf((float)pos * inv_freq[j0 + i], &sn[i], &cs[i]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sincosf((float)pos * inv_freq[j0 + i], &sn[i], &cs[i]);
   }
   const int page = c8_page(page_indptr, page_indices, request, pos, page_shift, num_pages);
   if (page < 0 && threadIdx.x == 0) atomicExch(status, 2);
@@ -142,21 +150,21 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
     for (int b = 0; b < BATCH; ++b) {
       const int h = base + warp * HPW + slot + b * stride;
       const bool is_q = h < nq, is_v = h >= nq + nkv;
-      float lo[8], hi[8];
-      bf16x8_to_float(lo_raw[b], lo);
-      bf16x8_to_float(hi_raw[b], hi);
+      float lo[4], hi[4];
+      c8_float4(lo, lo_raw[b]);
+      c8_float4(hi, hi_raw[b]);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
+      for (int i = 0; i < 4; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
 #pragma unroll
       for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
       if (!is_v) {
-        float wl[8], wh[8];
+        float wl[4], wh[4];
         const float inv = normed ? 1.0f / sqrtf(ss / (float)D + eps) : 1.f;
-        bf16x8_to_float(w_raw[is_q ? 0 : 1][0], wl);
-        bf16x8_to_float(w_raw[is_q ? 0 : 1][1], wh);
+        c8_float4(wl, is_q ? wq_lo : wk_lo);
+        c8_float4(wh, is_q ? wq_hi : wk_hi);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const float l = normed ? (lo[i] * inv) * wl[i] : lo[i], u = normed ? (hi[i] * inv) * wh[i] : hi[i];
           lo[i] = l * cs[i] - u * sn[i];
           hi[i] = u * cs[i] + l * sn[i];
@@ -164,35 +172,33 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       }
       uint32_t amax = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, max(__float_as_uint(lo[i]) & 0x7FFFFFFFu, __float_as_uint(hi[i]) & 0x7FFFFFFFu));
+      for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(lo[i]) & 0x7FFFFFFFu, __float_as_uint(hi[i]) & 0x7FFFFFFFu));
 #pragma unroll
       for (int off = LPH / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
       if (h >= heads) continue;
       if (is_q) {
-        __nv_bfloat16* dst = q_out + ((size_t)t * nq + h) * D;
-        *reinterpret_cast<uint4*>(dst + j0) = float_to_bf16x8(lo);
-        *reinterpret_cast<uint4*>(dst + HALF + j0) = float_to_bf16x8(hi);
+        __nv_bfloat16* dst = q_out + ((size_t)t * nq + h) * D + j0;
+        *reinterpret_cast<uint2*>(dst) = c8_bf16x4(lo);
+        *reinterpret_cast<uint2*>(dst + HALF) = c8_bf16x4(hi);
         continue;
       }
       if (page < 0) continue;
       const int e = c8_exponent(amax);
       const float inv = c8_inverse(e);
       const size_t at = at0 + ((size_t)(h - nq - (is_v ? nkv : 0)) << page_shift);
-      uint8_t* dst = (is_v ? v_codes : k_codes) + at * D;
-      *reinterpret_cast<uint2*>(dst + j0) = make_uint2(c8_keep(c8_codes4(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv), e),
-                                                       c8_keep(c8_codes4(lo[4] * inv, lo[5] * inv, lo[6] * inv, lo[7] * inv), e));
-      *reinterpret_cast<uint2*>(dst + HALF + j0) = make_uint2(c8_keep(c8_codes4(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv), e),
-                                                              c8_keep(c8_codes4(hi[4] * inv, hi[5] * inv, hi[6] * inv, hi[7] * inv), e));
+      uint8_t* dst = (is_v ? v_codes : k_codes) + at * D + j0;
+      *reinterpret_cast<uint32_t*>(dst) = c8_keep(c8_codes4(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv), e);
+      *reinterpret_cast<uint32_t*>(dst + HALF) = c8_keep(c8_codes4(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv), e);
       if (sub == 0) (is_v ? v_exps : k_exps)[at] = (uint8_t)e;
     }
   }
 }
 
-// 16 codes times a power of two
-__device__ __forceinline__ void c8_numbers16(float (&f)[16], const uint4& raw, float factor) {
-  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+// 8 codes times a power of two
+__device__ __forceinline__ void c8_numbers8(float (&f)[8], const uint2& raw, float factor) {
+  const uint32_t words[2] = {raw.x, raw.y};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const float2 lo = c8_float2(c8_half2_lo(words[i])), hi = c8_float2(c8_half2_hi(words[i]));
     f[4 * i] = lo.x * factor;
     f[4 * i + 1] = lo.y * factor;
@@ -200,25 +206,21 @@ __device__ __forceinline__ void c8_numbers16(float (&f)[16], const uint4& raw, f
     f[4 * i + 3] = hi.y * factor;
   }
 }
-__device__ __forceinline__ void c8_store16(float* dst, const uint4& raw, float factor) {
-  float f[16];
-  c8_numbers16(f, raw, factor);
+__device__ __forceinline__ void c8_store8(float* dst, const uint2& raw, float factor) {
+  float f[8];
+  c8_numbers8(f, raw, factor);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
 }
-__device__ __forceinline__ void c8_store16(__nv_bfloat16* dst, const uint4& raw, float factor) {
-  float f[16];
-  c8_numbers16(f, raw, factor);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float part[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) part[j] = f[8 * i + j];
-    reinterpret_cast<uint4*>(dst)[i] = float_to_bf16x8(part);
-  }
+__device__ __forceinline__ void c8_store8(__nv_bfloat16* dst, const uint2& raw, float factor) {
+  float f[8];
+  c8_numbers8(f, raw, factor);
+  *reinterpret_cast<uint4*>(dst) = float_to_bf16x8(f);
 }
 
-// A thread per 16 numbers of a (token, kv head): K and V.
+// Eight numbers of K and V at a time: neighbours' loads (8 bytes) and stores (16 in bfloat16) lie side by side. A thread takes READ_EACH such pieces of a token, all asked for
+// together, so that where the token lies is looked up once for them. Block (tokens, share of a token).
+constexpr int READ_EACH = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
 cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_exps,
@@ -226,28 +228,40 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
                    const int* __restrict__ row_of_token, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int num_tokens,
                    int nkv, int d, int page_shift, int num_pages, int* __restrict__ status) {
   pdl_prologue(k_codes, k_exps, v_codes, v_exps, positions, row_of_token, page_indptr, page_indices);
-  const int chunks = d >> 4;
-  const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (idx >= (long long)num_tokens * nkv * chunks) return;
-  const int c = (int)(idx % chunks);
-  const long long item = idx / chunks;
-  const int t = (int)(item / nkv), h = (int)(item - (long long)t * nkv), pos = positions[t];
-  const int page = c8_page(page_indptr, page_indices, row_of_token[t], pos, page_shift, num_pages);
+  const int eights = d >> 3, pieces = nkv * eights, threads = (pieces + READ_EACH - 1) / READ_EACH;  // of a token
+  const int tokens = max(1, 256 / threads), mine = threadIdx.x / threads, t = blockIdx.x * tokens + (tokens > 1 ? mine : 0);
+  const int first = tokens > 1 ? threadIdx.x - mine * threads : blockIdx.y * 256 + threadIdx.x;
+  if (t >= num_tokens || first >= threads || (tokens > 1 && mine >= tokens)) return;
+  const int pos = positions[t], page = c8_page(page_indptr, page_indices, row_of_token[t], pos, page_shift, num_pages);
   if (page < 0) {
-    if (c == 0 && h == 0) atomicExch(status, 2);
+    if (first == 0) atomicExch(status, 2);
     return;
   }
-  const size_t at = ((size_t)page * nkv + h) * ((size_t)1 << page_shift) + (pos & ((1 << page_shift) - 1));
-  const uint4 raw[2] = {*reinterpret_cast<const uint4*>(k_codes + at * d + c * 16), *reinterpret_cast<const uint4*>(v_codes + at * d + c * 16)};
-  const int b[2] = {k_exps[at], v_exps[at]};
+  const size_t at0 = ((size_t)page * nkv << page_shift) + (pos & ((1 << page_shift) - 1));
+  uint2 raw[READ_EACH][2];
+  int b[READ_EACH][2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) c8_store16((w ? v_out : k_out) + (size_t)item * d + c * 16, raw[w], c8_factor(b[w]));
+  for (int i = 0; i < READ_EACH; ++i) {
+    const int piece = min(first + i * threads, pieces - 1), h = piece / eights, c = piece - h * eights;  // (the last one again, unused)
+    const size_t at = at0 + ((size_t)h << page_shift);
+    raw[i][0] = *reinterpret_cast<const uint2*>(k_codes + at * d + c * 8);
+    raw[i][1] = *reinterpret_cast<const uint2*>(v_codes + at * d + c * 8);
+    b[i][0] = k_exps[at];
+    b[i][1] = v_exps[at];
+  }
+#pragma unroll
+  for (int i = 0; i < READ_EACH; ++i) {
+    const int piece = first + i * threads;
+    if (piece >= pieces) break;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) c8_store8((w ? v_out : k_out) + ((size_t)t * pieces + piece) * 8, raw[i][w], c8_factor(b[i][w]));
+  }
 }
 
 // The pages that rows [first, rows) of a step list, as bfloat16 pages of their own: entry f of the table becomes page f - indptr[first], and ids[f] says so. Entries that no query of their
 // row looks at (ahead of a window) are left out. What is done to a value vector that is not finite is done for the products that follow, which weigh what a query does
-// not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself zero. Block (entry, share of its page): a thread per 16 numbers of a key
-// and a value, 34 bytes in, 64 out.
+// not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself zero. Block (entry, share of its page), READ_EACH pieces of
+// 8 numbers of K and V a thread.
 __global__ void __launch_bounds__(256)
 cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, const uint8_t* __restrict__ k_codes,
                      const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ cu_q,
@@ -263,8 +277,8 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
         if (((page_indptr[r + 1] - page_indptr[r]) << page_shift) < q_start[r] + cu_q[r + 1] - cu_q[r]) atomicExch(status, 2);
   }
   if (f >= page_indptr[rows]) return;
-  const int chunks = d >> 4, idx = blockIdx.y * 256 + threadIdx.x;
-  if (idx >= nkv * page_size * chunks) return;
+  const int eights = d >> 3, pieces = nkv * page_size * eights, idx0 = blockIdx.y * (256 * READ_EACH) + threadIdx.x;
+  if (idx0 >= pieces) return;
   int a = first, b = rows;  // the row of the entry
   while (b - a > 1) {
     const int mid = (a + b) / 2;
@@ -278,13 +292,26 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
     atomicExch(status, 2);
     return;
   }
-  const int row = idx / chunks;
-  const size_t from = (size_t)page * nkv * page_size, at = (from * chunks + idx) * 16, to = ((size_t)out_page * nkv * page_size * chunks + idx) * 16;
-  const uint4 raw[2] = {*reinterpret_cast<const uint4*>(k_codes + at), *reinterpret_cast<const uint4*>(v_codes + at)};
-  const int eb = k_exps[from + row], vb = v_exps[from + row];
-  const float factor[2] = {c8_factor(vb == C8_NAN ? C8_NAN : eb), vb == C8_NAN ? 0.f : c8_factor(vb)};
+  const size_t from = (size_t)page * nkv * page_size, to = (size_t)out_page * pieces;
+  uint2 raw[READ_EACH][2];
+  int b8[READ_EACH][2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) c8_store16((w ? v_out : k_out) + to, raw[w], factor[w]);
+  for (int i = 0; i < READ_EACH; ++i) {
+    const int idx = min(idx0 + 256 * i, pieces - 1), row = idx / eights;  // (the last one again, unused)
+    const size_t at = (from * eights + idx) * 8;
+    raw[i][0] = *reinterpret_cast<const uint2*>(k_codes + at);
+    raw[i][1] = *reinterpret_cast<const uint2*>(v_codes + at);
+    b8[i][0] = k_exps[from + row];
+    b8[i][1] = v_exps[from + row];
+  }
+#pragma unroll
+  for (int i = 0; i < READ_EACH; ++i) {
+    const int idx = idx0 + 256 * i;
+    if (idx >= pieces) break;
+    const bool fine = b8[i][1] != C8_NAN;
+    c8_store8(k_out + (to + idx) * 8, raw[i][0], c8_factor(fine ? b8[i][0] : C8_NAN));
+    c8_store8(v_out + (to + idx) * 8, raw[i][1], fine ? c8_factor(b8[i][1]) : 0.f);
+  }
 }
 
 }  // namespace ms
@@ -310,10 +337,14 @@ MS_EXPORT int ms_cache8_write(void* q_out, void* k_codes, void* k_exps, void* v_
   MS_CHECK_ARG(nq >= 0 && num_tokens > 0, "cache8_write: nq=%d, %d tokens", nq, num_tokens);
   MS_CHECK_ARG(rot >= 0 && rot <= d && rot % 2 == 0, "cache8_write: rotary_dim=%d must be even and at most the head size %d", rot, d);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0, "cache8_write: pools must be 16-byte aligned");
-  if ((d == 64 || d == 128 || d == 256) && (rot == d || rot == 0 || inv_freq == nullptr) && (q_norm_w != nullptr) == (k_norm_w != nullptr) && (uintptr_t)qkv % 16 == 0 &&
-      (uintptr_t)q_out % 16 == 0 && (uintptr_t)q_norm_w % 16 == 0 && (uintptr_t)k_norm_w % 16 == 0 && (uintptr_t)cos_sin % 16 == 0) {
-    auto kernel = d == 64 ? cache8_write_token_kernel<64> : (d == 128 ? cache8_write_token_kernel<128> : cache8_write_token_kernel<256>);
-    const int a_pass = 32 / (d / 16), warps = ceil_div(nq + 2 * nkv, a_pass) < 8 ? ceil_div(nq + 2 * nkv, a_pass) : 8;  // heads a warp and pass
+  if ((d == 64 || d == 128 || d == 256) && (rot == d || rot == 0 || inv_freq == nullptr) && (q_norm_w != nullptr) == (k_norm_w != nullptr) && (uintptr_t)qkv % 8 == 0 &&
+      (uintptr_t)q_out % 8 == 0 && (uintptr_t)q_norm_w % 8 == 0 && (uintptr_t)k_norm_w % 8 == 0 && (uintptr_t)cos_sin % 16 == 0) {
+    const bool table = cos_sin != nullptr || rot == 0 || inv_freq == nullptr;
+    auto kernel = d == 64    ? (table ? cache8_write_token_kernel<64, true> : cache8_write_token_kernel<64, false>)
+                  : d == 128 ? (table ? cache8_write_token_kernel<128, true> : cache8_write_token_kernel<128, false>)
+                             : (table ? cache8_write_token_kernel<256, true> : cache8_write_token_kernel<256, false>);
+    // as many warps as bring all heads in one trip of two a lane group: the more blocks are resident, the better their chains of loads hide one another
+    const int a_trip = 2 * (32 / (d / 8)), warps = ceil_div(nq + 2 * nkv, a_trip) < 8 ? ceil_div(nq + 2 * nkv, a_trip) : 8;
     MS_LAUNCH(kernel, num_tokens, 32 * warps, 0, stream, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)k_exps, (uint8_t*)v_codes, (uint8_t*)v_exps,
               (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w, rot ? inv_freq : (const float*)nullptr, cos_sin, positions,
               row_of_token, page_indptr, page_indices, nq, nkv, eps, c8_page_shift(page_size), (int)num_pages, status);
@@ -334,8 +365,9 @@ MS_EXPORT int ms_cache8_read(void* k_out, void* v_out, const void* k_codes, cons
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_read: tensors must be 16-byte aligned");
   MS_CHECK_ARG(dtype == MS_F32 || dtype == MS_BF16, "cache8_read: dtype code %d", dtype);
-  const long long items = (long long)num_tokens * nkv * (d / 16);
-  const unsigned grid = (unsigned)((items + 255) / 256);
+  const int threads = ceil_div(nkv * (d / 8), READ_EACH), tokens = threads < 256 ? 256 / threads : 1;
+  const dim3 grid(ceil_div(num_tokens, tokens), ceil_div(threads, 256));
+  MS_CHECK_ARG(grid.y <= 65535, "cache8_read: too many heads (%d)", nkv);
   if (dtype == MS_F32) {
     MS_LAUNCH(cache8_read_kernel<float>, grid, 256, 0, stream, (float*)k_out, (float*)v_out, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
               (const uint8_t*)v_codes, (const uint8_t*)v_exps, positions, row_of_token, page_indptr, page_indices, num_tokens, nkv, d, c8_page_shift(page_size),
@@ -357,7 +389,7 @@ MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, const void* k
   MS_CHECK_ARG(first >= 0 && rows > first && entries > 0, "cache8_unpack: rows %d to %d, %d entries", first, rows, entries);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_unpack: tensors must be 16-byte aligned");
-  const int blocks = ceil_div(nkv * page_size * (d / 16), 256);
+  const int blocks = ceil_div(nkv * page_size * (d / 8), 256 * READ_EACH);
   MS_CHECK_ARG(blocks <= 65535, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
             (const uint8_t*)v_codes, (const uint8_t*)v_exps, cu_q, q_start, page_indptr, page_indices, first, rows, nkv, d, window, c8_page_shift(page_size), (int)num_pages,
