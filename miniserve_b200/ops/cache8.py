@@ -39,6 +39,9 @@ class Pool8:
             raise ValueError(f"an 8-bit cache takes pages of a power of two of at least {MIN_PAGE} tokens, not {c.shape[2]}")
         if c.device != e.device or not c.is_contiguous() or not e.is_contiguous() or c.data_ptr() % 16 or e.data_ptr() % 8:
             raise ValueError("an 8-bit pool's tensors lie on one device, contiguous, codes on 16 bytes and exponents on 8")
+        # what every call asks for: sizes, the device's index (-1: the host), addresses
+        for name, value in (("sizes", tuple(c.shape)), ("index", c.get_device()), ("pointers", (c.data_ptr(), e.data_ptr()))):
+            object.__setattr__(self, name, value)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Pool8":
@@ -109,37 +112,32 @@ def _attn_lib(head_dim: int) -> _AttnLib:
     return _AttnLib(head_dim)
 
 
-def _on(device: torch.device):
-    """The launches of the block go to ``device``, whichever is current (None: it is)."""
-    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
 def _stream_of(stream, device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
 
 
-def _check_tables(device: torch.device, *tensors: torch.Tensor) -> None:
+def _check_tables(index: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
             raise ValueError("positions, rows, page tables and the status word are contiguous int32 tensors on the pools' device")
 
 
 def _check_pools(k: Pool8, v: Pool8) -> None:
     if not isinstance(k, Pool8) or not isinstance(v, Pool8):
         raise TypeError("keys and values are both in 8 bits or both not")
-    if k.shape != v.shape or k.device != v.device:
-        raise ValueError(f"the pools of keys and values differ: {tuple(k.shape)} on {k.device}, {tuple(v.shape)} on {v.device}")
-    if not k.codes.is_cuda:
+    if k.sizes != v.sizes or k.index != v.index:
+        raise ValueError(f"the pools of keys and values differ: {k.sizes} on {k.device}, {v.sizes} on {v.device}")
+    if k.index < 0:
         raise ValueError("kernel operands must be contiguous CUDA tensors")
 
 
-def _launch(device: torch.device, call) -> None:
-    guard = _on(device)
-    if guard is None:
-        call()
+def _launch(index: int, fn, *args) -> None:
+    """``fn(*args)`` with the pools' device as the current one."""
+    if torch.cuda.current_device() == index:
+        _cache_check(fn(*args))
     else:
-        with guard:
-            call()
+        with torch.cuda.device(index):
+            _cache_check(fn(*args))
 
 
 def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim: int, eps: float, positions, row_of_token,
@@ -148,31 +146,29 @@ def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w
     (values: as projected). A token whose position its row's table has no page for raises the status word and is not written."""
     _check_pools(k_pool, v_pool)
     t, nq, d = q_out.shape
-    pages, nkv, held, dim = k_pool.shape
-    dev = k_pool.device
+    pages, nkv, held, dim = k_pool.sizes
+    dev = k_pool.index
     if held != page_size or dim != d or qkv.shape != (t, (nq + 2 * nkv) * d):
-        raise ValueError(f"q is {tuple(q_out.shape)}, the projection {tuple(qkv.shape)}, the pools {tuple(k_pool.shape)}, the page size {page_size}")
-    for x, n in ((q_out, None), (qkv, None), (q_norm_w, d), (k_norm_w, d)):
-        if x is not None and (x.dtype != torch.bfloat16 or x.device != dev or not x.is_contiguous() or x.data_ptr() % 16 or (n and x.numel() != n)):
+        raise ValueError(f"q is {tuple(q_out.shape)}, the projection {tuple(qkv.shape)}, the pools {k_pool.sizes}, the page size {page_size}")
+    pq, px, pw, pk = q_out.data_ptr(), qkv.data_ptr(), None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr()
+    for x, at, n in ((q_out, pq, 0), (qkv, px, 0), (q_norm_w, pw, d), (k_norm_w, pk, d)):
+        if x is not None and (x.dtype is not torch.bfloat16 or x.get_device() != dev or not x.is_contiguous() or at % 16 or (n and x.numel() != n)):
             raise ValueError("an 8-bit cache is written from contiguous bfloat16 tensors on its device, on 16 bytes; norm weights have the head's size")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2 or inv_freq.device != dev or not inv_freq.is_contiguous()):
-        raise ValueError("inv_freq is float32 [rotary_dim / 2] on the pools' device")
-    if inv_freq is None:
-        cos_sin = None
-    if cos_sin is not None and (cos_sin.dtype != torch.float32 or cos_sin.shape != (t, rotary_dim) or not cos_sin.is_contiguous() or cos_sin.device != dev):
-        raise ValueError("cos_sin is float32 [tokens, rotary_dim], contiguous, on the pools' device")
+    freq = table = None
+    if inv_freq is not None:
+        if inv_freq.dtype is not torch.float32 or inv_freq.numel() != rotary_dim // 2 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq is float32 [rotary_dim / 2] on the pools' device")
+        freq = inv_freq.data_ptr()
+        if cos_sin is not None:
+            if cos_sin.dtype is not torch.float32 or cos_sin.shape != (t, rotary_dim) or cos_sin.get_device() != dev or not cos_sin.is_contiguous():
+                raise ValueError("cos_sin is float32 [tokens, rotary_dim], contiguous, on the pools' device")
+            table = cos_sin.data_ptr()
     _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
     if positions.numel() < t or row_of_token.numel() < t:
         raise ValueError(f"{t} tokens need as many positions and rows")
-
-    def ptr(x):
-        return None if x is None else x.data_ptr()
-
-    _launch(dev, lambda: _cache_check(_cache_lib().ms_cache8_write(
-        q_out.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(), qkv.data_ptr(),
-        ptr(q_norm_w), ptr(k_norm_w), ptr(inv_freq), ptr(cos_sin), positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(),
-        page_indices.data_ptr(), t, nq, nkv, d, rotary_dim if inv_freq is not None else 0, float(eps), page_size, pages, status.data_ptr(),
-        _stream_of(stream, dev))))
+    _launch(dev, _cache_lib().ms_cache8_write, pq, *k_pool.pointers, *v_pool.pointers, px, pw, pk, freq, table, positions.data_ptr(), row_of_token.data_ptr(),
+            page_indptr.data_ptr(), page_indices.data_ptr(), t, nq, nkv, d, 0 if freq is None else rotary_dim, eps, page_size, pages, status.data_ptr(),
+            _stream_of(stream, k_pool.device))
 
 
 def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: Pool8, positions: torch.Tensor, row_of_token: torch.Tensor,
@@ -181,20 +177,20 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
     the cache holds at position ``positions[i]`` of row ``row_of_token[i]`` of the page table. A position without a page raises the status word and
     leaves its row as it was."""
     _check_pools(k_pool, v_pool)
-    pages, nkv, page_size, d = k_pool.shape
-    dev, n = k_pool.device, k_out.shape[0]
-    if k_out.shape != (n, nkv, d) or v_out.shape != k_out.shape or positions.numel() < n or row_of_token.numel() < n:
-        raise ValueError(f"rows {tuple(k_out.shape)} and {tuple(v_out.shape)} of pools {tuple(k_pool.shape)}, {positions.numel()} positions, {row_of_token.numel()} rows")
-    if k_out.dtype not in (torch.bfloat16, torch.float32) or v_out.dtype != k_out.dtype:
-        raise TypeError(f"a cache is read as bfloat16 or float32, not {k_out.dtype} and {v_out.dtype}")
-    for x in (k_out, v_out):
-        if x.device != dev or not x.is_contiguous() or x.data_ptr() % 16:
-            raise ValueError("the rows are contiguous, on 16 bytes, on the pools' device")
+    pages, nkv, page_size, d = k_pool.sizes
+    dev, shape = k_pool.index, k_out.shape
+    n = shape[0]
+    if shape != (n, nkv, d) or v_out.shape != shape or positions.numel() < n or row_of_token.numel() < n:
+        raise ValueError(f"rows {tuple(shape)} and {tuple(v_out.shape)} of pools {k_pool.sizes}, {positions.numel()} positions, {row_of_token.numel()} rows")
+    dtype = k_out.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float32) or v_out.dtype is not dtype:
+        raise TypeError(f"a cache is read as bfloat16 or float32, not {dtype} and {v_out.dtype}")
+    pk, pv = k_out.data_ptr(), v_out.data_ptr()
+    if k_out.get_device() != dev or v_out.get_device() != dev or not k_out.is_contiguous() or not v_out.is_contiguous() or pk % 16 or pv % 16:
+        raise ValueError("the rows are contiguous, on 16 bytes, on the pools' device")
     _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
-    _launch(dev, lambda: _cache_check(_cache_lib().ms_cache8_read(
-        k_out.data_ptr(), v_out.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(),
-        positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), n, nkv, d, page_size, pages, status.data_ptr(),
-        0 if k_out.dtype == torch.float32 else 1, _stream_of(stream, dev))))
+    _launch(dev, _cache_lib().ms_cache8_read, pk, pv, *k_pool.pointers, *v_pool.pointers, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(),
+            page_indices.data_ptr(), n, nkv, d, page_size, pages, status.data_ptr(), 0 if dtype is torch.float32 else 1, _stream_of(stream, k_pool.device))
 
 
 # ------------------------------------------------------------------ attention
@@ -214,9 +210,10 @@ def _workspace(ctx, floats: int, device) -> torch.Tensor:
 
 def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device) -> list:
     """The launches over rows [0, rows_all) of a step, of at most ``most_tokens`` new tokens each, the same for every layer with these sizes and this window:
-    ``(plan, query rows of a tile, the most of a request)``."""
+    ``(plan, its address, query rows of a tile, the most of a request, launches)``."""
     nq, nkv, d, scale, window, sink, page_size, pages = key
     lib = _attn_lib(d)
+    _check_tables(device.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
     ctas = ctx.sm_count
     floats = lib.part_floats(ctas)
     part = _workspace(ctx, floats + 4 * ctas, device)
@@ -231,25 +228,24 @@ def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device)
     for first in range(0, rows_all, rows_each):
         skip, rows = 4 * first, min(rows_each, rows_all - first)  # the per-row tables are int32
         for tile0 in range(0, tiles, tiles_each):
-            out.append((_Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
-                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0,
-                               min(tiles_each, tiles - tile0), nq, nkv, window, sink, page_size, ctas, scale, pages, not whole), tile_rows, most))
+            plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
+                          ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, min(tiles_each, tiles - tile0), nq, nkv, window, sink,
+                          page_size, ctas, scale, pages, not whole)
+            out.append((plan, ctypes.addressof(plan), tile_rows, most, 1 if whole else 2))
     return out
 
 
-def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool, rows: int, most_tokens: int) -> None:
+def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, rows: int, most_tokens: int, nq: int) -> None:
     """Rows [0, rows) of the step on the kernel that shares out keys."""
-    d = q.shape[2]
-    pages, nkv, page_size, _ = k_pool.shape
-    key = (q.shape[1], nkv, d, float(scale), int(window or 0), int(bool(sink)), page_size, pages)
-    plans = ctx.step_cache.get(("cache8", group, rows, key))
-    if plans is None:
-        plans = ctx.step_cache[("cache8", group, rows, key)] = _plans(ctx, group, rows, most_tokens, key, k_pool.device)
-    lib = _attn_lib(d)
-    args = (out.data_ptr(), q.data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(), v_pool.exponents.data_ptr(), ctx.stream)
-    for plan, tile_rows, most in plans:
-        native.LAUNCHES[0] += 1 + plan.behind
-        if lib.split(ctypes.addressof(plan), tile_rows, most, *args):
+    pages, nkv, page_size, d = k_pool.sizes
+    key = ("cache8", group, rows, nq, nkv, d, scale, window, sink, page_size, pages)
+    held = ctx.step_cache.get(key)
+    if held is None:
+        held = ctx.step_cache[key] = (_attn_lib(d), _plans(ctx, group, rows, most_tokens, (nq, nkv, d, float(scale), window, int(sink), page_size, pages), k_pool.device))
+    lib, plans = held
+    for plan, at, tile_rows, most, launches in plans:
+        native.LAUNCHES[0] += launches
+        if lib.split(at, tile_rows, most, out.data_ptr(), q.data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.stream):
             raise native.NativeError(lib.last_error().decode())
 
 
@@ -286,7 +282,7 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
     """Rows [first, num_rows) of the step over pages unpacked to bfloat16."""
     from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
 
-    pages, nkv, page_size, d = k_pool.shape
+    pages, nkv, page_size, d = k_pool.sizes
     dev = k_pool.device
     key = ("cache8_unpacked", group, first, nkv, page_size, d)
     parts = ctx.step_cache.get(key)
@@ -304,13 +300,12 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
     k, v, parts = parts
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(
-            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), k_pool.codes.data_ptr(), k_pool.exponents.data_ptr(), v_pool.codes.data_ptr(),
-            v_pool.exponents.data_ptr(), ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows,
-            entries, nkv, d, int(window or 0), page_size, pages, view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows,
+            entries, nkv, d, window, page_size, pages, view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
         if attention_tc_ok(q, k):
-            attention_tc_prefill(out, q, k, v, view, group, scale, window, a, sink)
+            attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
         else:
-            attention_bf16.run_prefill(out, q, k, v, view, group, scale, window, a, sink)
+            attention_bf16.run_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
 
 
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
@@ -318,31 +313,31 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
     ``group``, window and sink as there. Single tokens and drafted ones go to the kernel that shares out keys (``csrc/attention_cache8.cu``); prompts and portions of them to a
     bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool does not have raises the status word. Workspaces lie in
     ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
-    if not (isinstance(v_pool, Pool8) and k_pool.shape == v_pool.shape):
+    if not isinstance(v_pool, Pool8) or k_pool.sizes != v_pool.sizes or k_pool.index != v_pool.index or k_pool.index < 0:
         _check_pools(k_pool, v_pool)
-    nq, d = q.shape[1], q.shape[2]
-    nkv, dim = k_pool.shape[1], k_pool.shape[3]
-    dev = q.get_device()
-    if not (out.shape == q.shape and q.dtype == out.dtype == torch.bfloat16 and dev >= 0 and dev == out.get_device() == k_pool.codes.get_device() == v_pool.codes.get_device()
+    shape = q.shape
+    nq, d = shape[1], shape[2]
+    _, nkv, _, dim = k_pool.sizes
+    dev = k_pool.index
+    if not (out.shape == shape and q.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and q.get_device() == dev and out.get_device() == dev
             and q.is_contiguous() and out.is_contiguous()):
-        raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape, and pools of one shape, on one device")
-    if dim != d or nq % nkv or (window or 0) < 0:
-        raise ValueError(f"{nq} query heads of {d} over pools {tuple(k_pool.shape)}, window {window}")
+        raise ValueError("attention over an 8-bit cache takes contiguous bfloat16 queries and output of one shape on the pools' device")
+    window, heads = window or 0, nq // nkv
+    if dim != d or nq % nkv or window < 0:
+        raise ValueError(f"{nq} query heads of {d} over pools {k_pool.sizes}, window {window}")
     if getattr(ctx, "recorder", None) is not None:
         # a pass that is captured for steps of other lengths too: launched anew for each, between the graphs
         ctx.recorder.defer(lambda step: attention(out, q, k_pool, v_pool, step, group, scale, window, sink))
         return
-    dense = ctx.max_q_len * (nq // nkv) > SPLIT_ROWS
-
-    def launch():
-        single = ctx.leading_single_rows if dense else ctx.num_rows
-        if single:
-            _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single, 1 if dense else ctx.max_q_len)
-        if single < ctx.num_rows:
-            _dense(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single)
-
-    if torch.cuda.current_device() == dev:
-        launch()
-    else:
+    if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
-            launch()
+            attention(out, q, k_pool, v_pool, ctx, group, scale, window, sink)
+        return
+    if ctx.max_q_len * heads <= SPLIT_ROWS:
+        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, ctx.num_rows, ctx.max_q_len, nq)
+        return
+    single = ctx.leading_single_rows
+    if single:
+        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single, 1, nq)
+    if single < ctx.num_rows:
+        _dense(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single)
