@@ -13,10 +13,10 @@
 //   o = sum_j 2^(s_j - m - c + 6 + ev_j) code(v_j),      l = sum_j 2^(s_j - m - c + 6)
 // so a weight with its value's scale is at most 2^14, a float16 with 11 significant bits down to 2^-20 of the largest; l and o are float32.
 //
-// Work: up to 8 or 16 query rows (consecutive tokens of a request times the query heads of a kv head) and a kv head are an item; all items' slices of 32
+// Work: up to 8, 16 or (head sizes up to 64) 24 query rows (consecutive tokens of a request times the query heads of a kv head) and a kv head are an item; all items' slices of 32
 // keys in a row are cut into equal runs, one a warp, whatever the requests' lengths. Each warp has a ring of stages of its own, filled by 16-byte
-// copies that run on from item to item. What a warp has of an item that other warps of its CTA share lies in shared memory; the last of them to get
-// there adds the pieces up in the warps' order. Items cut by a CTA's end leave one piece a CTA in global memory for a second small kernel. The
+// copies that run on from item to item. What a warp has of an item that other warps of its CTA share lies in shared memory until all are done, and the
+// warps add the pieces up together, in the warps' order. Items cut by a CTA's end leave one piece a CTA in global memory for a second small kernel. The
 // lengths are read on the device, so a captured launch serves every context.
 #include "cache8.cuh"
 
@@ -33,12 +33,14 @@ constexpr int KSTEPS = D / 16, MTILES = D / 16;    // of q k^T along the head, o
 constexpr int WIDE = D / 64, REST = (D % 64) / 16;   // k-steps of q k^T whose codes come four by four, and one by one
 constexpr int VB = D % 128 == 0 ? 16 : (D % 64 == 0 ? 8 : 4), VBLOCKS = D / (8 * VB), VTAIL = D % 32 / 16;  // how a lane reads values: VB bytes a block
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int SLICE = 32, ROWS = 16;                 // keys of a slice; the most query rows of an item
+constexpr int MOST_NT = D <= 64 ? 3 : 2;              // tiles of 8 query rows of an item at most: what the registers hold
+constexpr int SLICE = 32, ROWS = 8 * MOST_NT;         // keys of a slice; the most query rows of an item
 constexpr int ROW_BYTES = D % 64 == 0 ? D : D + 16;
 constexpr int CODE_BYTES = SLICE * ROW_BYTES, STAGE_BYTES = 2 * CODE_BYTES + 2 * SLICE;  // K codes, V codes, K exponents, V exponents
-// Warps of a CTA and stages of a warp's ring: one stage is worked on, the others are on their way.
-constexpr int warps_of(int nt) { return D > 128 ? 4 : (D > 64 && nt == 1 ? 7 : 8); }
-constexpr int stages_of(int nt) { return D > 128 ? 2 : (D <= 64 ? 4 : (nt == 1 ? 3 : 2)); }
+// Warps of a CTA and stages of a warp's ring: one stage is worked on, the others are on their way. Head size 128, 64 requests of 1,024 to 3,985 keys: 7 warps of 3 stages
+// 65.0 us, 8 of 2 61.9, 8 of 3 66.1, 9 of 2 65.1.
+constexpr int warps_of(int) { return D > 128 ? 4 : 8; }
+constexpr int stages_of(int) { return D > 64 ? 2 : 4; }
 constexpr int PART = D + 4;                          // floats of a row's partial: o, m, l, c (and one that keeps rows on 16 bytes)
 constexpr int MAX_UNITS = 256;                       // (request, tile) pairs of a launch
 
@@ -95,6 +97,11 @@ __device__ __forceinline__ uint32_t lds8(uint32_t at) {
   asm volatile("ld.shared.u8 %0, [%1];\n" : "=r"(v) : "r"(at));
   return v;
 }
+__device__ __forceinline__ float4 lds_float4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
 template <int BYTES>
 __device__ __forceinline__ void lds_words(uint32_t (&v)[BYTES / 4], uint32_t at) {
   if constexpr (BYTES == 16) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
@@ -126,21 +133,30 @@ struct Split8 {
   const int* page_indptr;   // [rows + 1]
   const int* page_indices;
   int* status;
-  float* part;              // [2 * ctas][16][PART]: a CTA's partial of the item that began before it, and of the one that goes on behind it
+  float* part;              // [2 * ctas][ROWS][PART]: a CTA's partial of the item that began before it, and of the one that goes on behind it
   int4* cut;                // [ctas]: for the second kernel, of the cut item that begins in the CTA: its first query row (counted in tokens x heads of a kv head), rows, kv head, pieces; 0: none
-  int rows, tile0, tiles;   // requests; tiles [tile0, tile0 + tiles) of 8 or 16 query rows of each
+  int rows, tile0, tiles;   // requests; tiles [tile0, tile0 + tiles) of query rows of each
   int nq, nkv, window, sink, page_size, ctas;
   float scale;
   int num_pages;
   int behind;               // the second kernel runs: an item may be cut
 };
 
+// a / b of whole numbers, quotients below 2^20: a multiplication by the reciprocal, off by one at most, put right
+__device__ __forceinline__ int div_small(int a, int b) {
+  int q = (int)((float)a * __frcp_rn((float)b));
+  const int r = a - q * b;
+  if (r < 0) --q;
+  if (r >= b) ++q;
+  return q;
+}
+
 // The keys that a tile of query rows sees: those that some row does [lo, hi), those that all do [seen_lo, seen_hi).
 struct Span {
   int lo, hi, seen_lo, seen_hi, first_slice;
 };
 __device__ __forceinline__ Span span_of(const Split8& p, int start, int row0, int rows_here, int group) {
-  const int first = start + row0 / group, last = start + (row0 + rows_here - 1) / group;
+  const int first = start + div_small(row0, group), last = start + div_small(row0 + rows_here - 1, group);
   Span s;
   s.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
   s.hi = last + 1;
@@ -162,9 +178,14 @@ struct Unit {
   int n, stride;             // its slices of one kv head; how far apart its kv heads lie in the row of slices (n, or more: see `alone`)
   int tok0, start, row0, rows_here;
   int table, entries;        // of its request in page_indices
+  Span keys;
+};
+// An item that several warps of a CTA share.
+struct Joint {
+  int unit, kvh, last_warp, whole, piece;  // piece: which of the CTA's two in global memory, where it is not whole
 };
 
-// NT: tiles of 8 query rows of an item, 1 or 2
+// NT: tiles of 8 query rows of an item
 template <int NT>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1)
 attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_codes,
@@ -172,13 +193,14 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
   constexpr int TILE_ROWS = 8 * NT, WARPS = warps_of(NT), THREADS = WARPS * 32, STAGES = stages_of(NT);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Unit table[MAX_UNITS + 1];
-  __shared__ int scan[3][WARPS], arrived[WARPS];
+  __shared__ int scan[3][WARPS];
+  __shared__ Joint joint[WARPS];  // by the warp that its CTA's share begins in; last_warp 0: none
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int *cu_q = p.cu_q, *q_start = p.q_start, *page_indptr = p.page_indptr, *page_indices = p.page_indices;
-  if (tid < WARPS) arrived[tid] = 0;
+  if (tid < WARPS) joint[tid].last_warp = 0;
   pdl_prologue(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
 
-  const int group = p.nq / p.nkv, units = p.rows * p.tiles;
+  const int group = div_small(p.nq, p.nkv), units = p.rows * p.tiles;
   // ---- where every tile's slices begin: a scan over the tiles, in order
   int live, total;
   {
@@ -186,17 +208,19 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     int slices = 0, count = 0, longest = 0;
     Unit mine;
     auto unit_of = [&](int u) {
-      const int r = u / p.tiles, rows_all = (cu_q[r + 1] - cu_q[r]) * group;
+      const int r = div_small(u, p.tiles);
+      const int tok_end = cu_q[r + 1], table_end = page_indptr[r + 1];
       mine.tok0 = cu_q[r];
       mine.start = q_start[r];
       mine.table = page_indptr[r];
-      mine.entries = page_indptr[r + 1] - mine.table;
-      mine.row0 = (p.tile0 + u % p.tiles) * TILE_ROWS;
+      mine.entries = table_end - mine.table;
+      mine.row0 = (p.tile0 + u - r * p.tiles) * TILE_ROWS;
+      const int rows_all = (tok_end - mine.tok0) * group;
       mine.rows_here = min(TILE_ROWS, rows_all - mine.row0);
       mine.n = 0;
       if (mine.rows_here > 0) {
-        const Span keys = span_of(p, mine.start, mine.row0, mine.rows_here, group);
-        mine.n = max(1, (keys.hi + SLICE - 1) / SLICE - keys.first_slice);  // (rows that see nothing have a slice, all of it masked)
+        mine.keys = span_of(p, mine.start, mine.row0, mine.rows_here, group);
+        mine.n = max(1, (mine.keys.hi + SLICE - 1) / SLICE - mine.keys.first_slice);  // (rows that see nothing have a slice, all of it masked)
       }
     };
     for (int u = first; u < min(first + each, units); ++u) {
@@ -268,13 +292,12 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     int4 cut = make_int4(0, 0, 0, 0);
     if (cta_begin < cta_end && !alone) {
       const Unit& u = table[find(cta_end - 1)];
-      const int kvh = (cta_end - 1 - u.at) / u.n, at = u.at + kvh * u.n;
+      const int kvh = div_small(cta_end - 1 - u.at, u.n), at = u.at + kvh * u.n;
       // the item that goes on behind the CTA's end, where it began in this CTA
       if (at >= cta_begin && at + u.n > cta_end) cut = make_int4(u.tok0 * group + u.row0, u.rows_here, kvh, (at + u.n - 1) / (each * WARPS) - (int)blockIdx.x + 1);
     }
     p.cut[blockIdx.x] = cut;
   }
-  if (begin >= end) return;
 
   const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE_BYTES;
   float* heads = reinterpret_cast<float*>(smem + WARPS * STAGES * STAGE_BYTES);  // [warps][part_rows][PART]: of items that began before the warp's run
@@ -303,17 +326,16 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     while (a_pos < end) {
       const Unit& u = table[a_unit];
       const int past = a_pos - u.at;
-      a_kvh = past / u.stride;
+      a_kvh = div_small(past, u.stride);
       const int off = past - a_kvh * u.stride;
       if (a_kvh >= p.nkv) {
         ++a_unit;
       } else if (off >= u.n) {  // (behind a lone item's end)
         a_pos += u.stride - off;
       } else {
-        const Span keys = span_of(p, u.start, u.row0, u.rows_here, group);
-        a_lo = keys.lo;
-        a_hi = keys.hi;
-        a_key = (keys.first_slice + off) * SLICE;
+        a_lo = u.keys.lo;
+        a_hi = u.keys.hi;
+        a_key = (u.keys.first_slice + off) * SLICE;
         a_table = u.table;
         a_entries = u.entries;
         a_left = min(u.n - off, end - a_pos);
@@ -388,7 +410,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     if (pos >= item_end) {
       // ---- a new item: its queries, from memory straight into the fragments
       for (;; ++unit) {
-        kvh = (pos - table[unit].at) / table[unit].stride;
+        kvh = div_small(pos - table[unit].at, table[unit].stride);
         if (kvh < p.nkv) break;
       }
       {
@@ -405,12 +427,12 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
         row0 = u.row0;
         rows_here = u.rows_here;
         tok0 = u.tok0;
-        it = span_of(p, start, row0, rows_here, group);
+        it = u.keys;
       }
       uint2 raw[NT][KSTEPS];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int i = g + 8 * j, row = row0 + i, tok = row / group;
+        const int i = g + 8 * j, row = row0 + i, tok = div_small(row, group);
         const __nv_bfloat16* src = q + ((size_t)(tok0 + tok) * p.nq + kvh * group + (row - tok * group)) * D;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) {
@@ -438,7 +460,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
         const float up = __uint_as_float((uint32_t)(127 + sh) << 23), down = p.scale * LOG2E * __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          q_pos[j][c] = start + (row0 + 8 * j + 2 * t + c) / group;
+          q_pos[j][c] = start + div_small(row0 + 8 * j + 2 * t + c, group);
           row_factor[j][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
         }
 #pragma unroll
@@ -643,12 +665,12 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
         if (c_run[j][c] == START) m_run[j][c] = NOTHING;
       }
     const int seg_begin = max(item_begin, cta_begin), seg_end = min(item_begin + n, cta_end);  // the CTA's share of it
-    const int first_warp = (seg_begin - cta_begin) / each, last_warp = (seg_end - 1 - cta_begin) / each;
+    const int first_warp = div_small(seg_begin - cta_begin, each), last_warp = div_small(seg_end - 1 - cta_begin, each);
     const bool whole = seg_begin == item_begin && seg_end == item_begin + n;
     float* piece = p.part + (size_t)(2 * blockIdx.x + (seg_begin == item_begin)) * ROWS * PART;  // (a cut item: began before this CTA, or goes on behind it)
     __nv_bfloat16* dst = out + ((size_t)tok0 * p.nq + kvh * group) * D;
     auto row_of = [&](int row) {  // where query row `row` of the item begins in the output
-      const int rho = row0 + row, tok = rho / group;
+      const int rho = row0 + row, tok = div_small(rho, group);
       return dst + ((size_t)tok * p.nq + (rho - tok * group)) * D;
     };
     // the lane group's channels 2 i and 2 i + 1 of a block
@@ -682,56 +704,70 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
         for (int i = 0; i < MTILES; ++i) *reinterpret_cast<float2*>(row + channel(i)) = make_float2(o[j][i][c], o[j][i][2 + c]);
         if (g == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m_run[j][c], l_run[j][c], c_run[j][c], 0.f);
       }
-    if (lone) continue;
-    __threadfence_block();
-    __syncwarp();
-    int last = 0;
-    if (lane == 0) last = atomicAdd(&arrived[first_warp], 1) == last_warp - first_warp;  // (an item that warps share begins its CTA's share in one warp)
-    if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-    __threadfence_block();
-    const float* first_piece = reinterpret_cast<const float*>(smem + first_warp * STAGES * STAGE_BYTES);
-    for (int row = 0; row < rows_here; ++row) {
-      auto from = [&](int w) { return (w == first_warp ? first_piece : heads + (size_t)w * part_rows * PART) + (size_t)row * PART; };
-      float m = NOTHING, c_all = -INFINITY, l = 0.f, wgt[WARPS];
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-        if (w >= first_warp && w <= last_warp) m = fmaxf(m, from(w)[D]);
+    if (is_tail && lane == 0) joint[warp] = {unit, kvh, last_warp, whole, seg_begin == item_begin};
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  // ---- items that warps share: their rows one by one, a row a warp
+  int task = 0;
+  for (int first_warp = 0; first_warp < WARPS; ++first_warp) {
+    const Joint item = joint[first_warp];
+    if (item.last_warp == 0) continue;
+    const Unit& u = table[item.unit];
+    for (int row = 0; row < u.rows_here; ++row) {
+      if (task++ % WARPS != warp) continue;
+      // every lane has all pieces' numbers (no exchanges between lanes: their latency is what a row would take)
+      float4 mlc[WARPS];
+      uint32_t at[WARPS];
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        wgt[w] = w >= first_warp && w <= last_warp ? (from(w)[D] - m) + from(w)[D + 2] : -INFINITY;
+        at[w] = (w == first_warp ? smem_addr(smem) + first_warp * STAGES * STAGE_BYTES : smem_addr(heads) + w * part_rows * PART * 4) + row * PART * 4;
+        mlc[w] = w >= first_warp && w <= item.last_warp ? lds_float4(at[w] + D * 4) : make_float4(NOTHING, 0.f, 0.f, 0.f);
+      }
+      float m = NOTHING, c_all = -INFINITY, l = 0.f, wgt[WARPS];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, mlc[w].x);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        wgt[w] = w >= first_warp && w <= item.last_warp ? (mlc[w].x - m) + mlc[w].z : -INFINITY;
         c_all = fmaxf(c_all, wgt[w]);
       }
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         wgt[w] = ex2(wgt[w] - c_all);
-        if (w >= first_warp && w <= last_warp) l += wgt[w] * from(w)[D + 1];
+        l += wgt[w] * mlc[w].y;
       }
       const float den = l + sink_term(p.sink, m, c_all), inv = den == 0.f ? 0.f : 1.0f / den;
-      for (int c = 4 * lane; c < D; c += 128) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int rho = u.row0 + row, tok = div_small(rho, group);
+      __nv_bfloat16* dst = out + ((size_t)(u.tok0 + tok) * p.nq + item.kvh * group + (rho - tok * group)) * D;
+      float* piece = p.part + ((size_t)(2 * blockIdx.x + item.piece) * ROWS + row) * PART;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 128) {
+        const int c = min(c0 + 4 * lane, D - 4);
+        float4 x[WARPS], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) x[w] = w >= first_warp && w <= item.last_warp ? lds_float4(at[w] + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-          if (w < first_warp || w > last_warp) continue;
-          const float4 x = *reinterpret_cast<const float4*>(from(w) + c);
-          acc.x += wgt[w] * x.x;
-          acc.y += wgt[w] * x.y;
-          acc.z += wgt[w] * x.z;
-          acc.w += wgt[w] * x.w;
+          acc.x += wgt[w] * x[w].x;
+          acc.y += wgt[w] * x[w].y;
+          acc.z += wgt[w] * x[w].z;
+          acc.w += wgt[w] * x[w].w;
         }
-        if (whole) {
+        if (c0 + 4 * lane >= D) continue;
+        if (item.whole) {
           uint2 pk;
           __nv_bfloat162 lo2 = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi2 = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
           pk.x = *reinterpret_cast<uint32_t*>(&lo2);
           pk.y = *reinterpret_cast<uint32_t*>(&hi2);
-          *reinterpret_cast<uint2*>(row_of(row) + c) = pk;
+          *reinterpret_cast<uint2*>(dst + c) = pk;
         } else {
-          *reinterpret_cast<float4*>(piece + (size_t)row * PART + c) = acc;
+          *reinterpret_cast<float4*>(piece + c) = acc;
         }
       }
-      if (!whole && lane == 0) *reinterpret_cast<float4*>(piece + (size_t)row * PART + D) = make_float4(m, l, c_all, 0.f);
+      if (!item.whole && lane == 0) *reinterpret_cast<float4*>(piece + D) = make_float4(m, l, c_all, 0.f);
     }
   }
-  cp_async_wait<0>();
 }
 
 // The items that were cut: a CTA's second partial and its successors' first ones, added up in their order. Block (cta, row). Threads side by side take
@@ -821,7 +857,7 @@ attn_cache8_merge_kernel(__nv_bfloat16* __restrict__ out, const Split8 p) {
       acc.z += x.z;
       acc.w += x.w;
     }
-    const int rho = cut.x + row, tok = rho / group;
+    const int rho = cut.x + row, tok = div_small(rho, group);
     const float den = l + sink_term(p.sink, m, c_all), inv = den == 0.f ? 0.f : 1.0f / den;
     __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     uint2 pk;
@@ -842,13 +878,14 @@ using namespace ms;
 MS_DEFINE_LAST_ERROR(MS_ATTN8_FN(last_error))
 MS_DEFINE_PDL_SWITCH(MS_ATTN8_FN(set_pdl))
 
-constexpr int SMEM_MOST = 227 * 1024 - 11 * 1024;  // (the table of tiles is static: 10 KB)
+constexpr int SMEM_MOST = 227 * 1024 - 16 * 1024;  // (the table of tiles is static: 15 KB)
 
 // Floats of partial results that a launch of `ctas` CTAs needs; the table of cut items (4 ints a CTA) lies behind them.
 MS_EXPORT long long MS_ATTN8_FN(part_floats)(int ctas) { return 2LL * ctas * ROWS * PART; }
 MS_EXPORT int MS_ATTN8_FN(max_units)() { return MAX_UNITS; }
+MS_EXPORT int MS_ATTN8_FN(most_rows)() { return ROWS; }
 // Keys up to which few items (no more than CTAs) run a CTA each, whole: nothing is cut then.
-MS_EXPORT int MS_ATTN8_FN(alone_keys)(int tile_rows) { return SLICE * (2 * (tile_rows == 8 ? warps_of(1) : warps_of(2)) - 1); }
+MS_EXPORT int MS_ATTN8_FN(alone_keys)(int tile_rows) { return SLICE * (2 * (warps_of(tile_rows / 8)) - 1); }
 
 template <int NT>
 static int launch_split(const Split8& p, int rows_tile, void* out, const void* q, const void* k_codes,
@@ -868,14 +905,14 @@ static int launch_split(const Split8& p, int rows_tile, void* out, const void* q
   return 0;
 }
 
-// Rows [0, p->rows) of the geometry in p, in tiles of `tile_rows` (8 or 16) query rows, of which no request has more than `rows_most`.
+// Rows [0, p->rows) of the geometry in p, in tiles of `tile_rows` (a multiple of 8) query rows, of which no request has more than `rows_most`.
 MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, int tile_rows, int rows_most, void* out, const void* q, const void* k_codes, const void* k_exps, const void* v_codes,
                                  const void* v_exps, cudaStream_t stream) {
   if (p->rows == 0) return 0;
   MS_CHECK_ARG(p->nq > 0 && p->nkv > 0 && p->nq % p->nkv == 0, "attention: %d query heads are not a multiple of %d kv heads", p->nq, p->nkv);
   MS_CHECK_ARG(p->page_size >= 8 && (p->page_size & (p->page_size - 1)) == 0, "attention: page_size=%d must be a power of two from 8 on for an 8-bit cache", p->page_size);
   MS_CHECK_ARG(p->rows > 0 && p->tiles > 0 && (long long)p->rows * p->tiles <= MAX_UNITS, "attention: %d rows of %d tiles are too many for one launch", p->rows, p->tiles);
-  MS_CHECK_ARG(p->ctas > 0 && p->part && p->cut && (tile_rows == 8 || tile_rows == 16) && rows_most > 0, "attention: %d CTAs need scratch memory, tiles %d rows of %d",
+  MS_CHECK_ARG(p->ctas > 0 && p->part && p->cut && tile_rows > 0 && tile_rows <= ROWS && tile_rows % 8 == 0 && rows_most > 0, "attention: %d CTAs need scratch memory, tiles %d rows of %d",
                p->ctas, tile_rows, rows_most);
   const long long pool_rows = (long long)p->num_pages * p->nkv * p->page_size;
   MS_CHECK_ARG(pool_rows > 0 && pool_rows < (1LL << 31), "attention: pools of %lld rows", pool_rows);
@@ -883,9 +920,8 @@ MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, int tile_rows, int rows_most, 
                    (uintptr_t)v_exps % 8 == 0 && (uintptr_t)p->part % 16 == 0 && (uintptr_t)p->cut % 16 == 0,
                "attention: an 8-bit cache's tensors must be 16-byte aligned");
   const int rows_tile = rows_most < tile_rows ? rows_most : tile_rows;
-  if (int rc = tile_rows == 8 ? launch_split<1>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream)
-                              : launch_split<2>(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream))
-    return rc;
+  auto launch = tile_rows == 8 ? launch_split<1> : (tile_rows == 16 ? launch_split<2> : launch_split<MOST_NT>);
+  if (int rc = launch(*p, rows_tile, out, q, k_codes, k_exps, v_codes, v_exps, stream)) return rc;
   if (p->behind) MS_LAUNCH(attn_cache8_merge_kernel, dim3(p->ctas, rows_tile), MERGE_THREADS, 0, stream, (__nv_bfloat16*)out, *p);
   return 0;
 }

@@ -104,6 +104,7 @@ class _AttnLib:
         self.split = native._declare(lib, pre + "split", [_p, _i, _i] + [_p] * 7)
         self.part_floats = native._declare(lib, pre + "part_floats", [_i], _ll)
         self.alone_keys = native._declare(lib, pre + "alone_keys", [_i])
+        self.most_rows = native._declare(lib, pre + "most_rows", [])()
         self.max_units = native._declare(lib, pre + "max_units", [])()
 
 
@@ -218,8 +219,9 @@ def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device)
     floats = lib.part_floats(ctas)
     part = _workspace(ctx, floats + 4 * ctas, device)
     most = most_tokens * (nq // nkv)
-    tile_rows = 8 if most <= 8 else 16
-    tiles, out = -(-most // tile_rows), []
+    tiles = -(-most // lib.most_rows)  # as few as there have to be, of one size
+    tile_rows = -(-most // (8 * tiles)) * 8
+    out = []
     # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
     keys = min(ctx.max_kv_len, window + most_tokens) if window else ctx.max_kv_len
     whole = (keys <= lib.alone_keys(tile_rows) and rows_all * tiles * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing())
