@@ -324,6 +324,8 @@ class CacheManager:
         view = self._entry_view[entry]
         if not isinstance(view, KVEntryView):
             raise ValueError(f"run entry {entry} has no single cache of keys and values")
+        if view.k is None:
+            raise ValueError("read of a cache that keeps books alone: it has no pools")
         table = rc.tables[view.group]
         stop = table.num_tokens if stop is None else stop
         if not 0 <= start <= stop <= table.num_tokens:

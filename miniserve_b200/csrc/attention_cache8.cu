@@ -216,7 +216,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
       mine.entries = table_end - mine.table;
       mine.row0 = (p.tile0 + u - r * p.tiles) * TILE_ROWS;
       const int rows_all = (tok_end - mine.tok0) * group;
-      mine.rows_here = min(TILE_ROWS, rows_all - mine.row0);
+      mine.rows_here = min(min(TILE_ROWS, part_rows), rows_all - mine.row0);  // (no more than there is room for)
       mine.n = 0;
       if (mine.rows_here > 0) {
         mine.keys = span_of(p, mine.start, mine.row0, mine.rows_here, group);

@@ -258,34 +258,57 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
   }
 }
 
-// The pages that rows [first, rows) of a step list, as bfloat16 pages of their own: entry f of the table becomes page f - indptr[first], and ids[f] says so. Entries that no query of their
-// row looks at (ahead of a window) are left out. What is done to a value vector that is not finite is done for the products that follow, which weigh what a query does
-// not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself zero. Block (entry, share of its page), READ_EACH pieces of
-// 8 numbers of K and V a thread.
+// The pages that rows [first, rows) of a step need, as bfloat16 pages of their own: the rows' needed pages, counted through, become pages 0, 1, ..., and ids[f] says so of entry f of
+// the table (which may list more pages than a row needs). Pages that no query of their row looks at (ahead of a window) are left as they were. What is done to a value vector that is not
+// finite is done for the products that follow, which weigh what a query does not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself
+// zero. Block (needed page, share of it), READ_EACH pieces of 8 numbers of K and V a thread; every warp finds the page's row for itself, 32 rows a look.
 __global__ void __launch_bounds__(256)
 cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, const uint8_t* __restrict__ k_codes,
                      const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ cu_q,
                      const int* __restrict__ q_start, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int first, int rows, int nkv, int d, int window,
                      int page_shift, int num_pages, int num_ids, int* __restrict__ status) {
   pdl_prologue(k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
-  const int out_page = blockIdx.x, f = page_indptr[first] + out_page, page_size = 1 << page_shift;
-  if (blockIdx.y == 0) {
-    if (threadIdx.x == 0 && f < num_ids) ids[f] = out_page;
-    // (the products behind this trust the tables: rows whose table is too short are found here)
-    if (out_page == 0)
-      for (int r = first + threadIdx.x; r < rows; r += 256)
-        if (((page_indptr[r + 1] - page_indptr[r]) << page_shift) < q_start[r] + cu_q[r + 1] - cu_q[r]) atomicExch(status, 2);
+  const int out_page = blockIdx.x, page_size = 1 << page_shift, lane = threadIdx.x & 31;
+  int a = -1, entry = out_page, start = 0, hi = 0, table = 0, listed = 0;  // the row, which of its pages, its first new token and its end, its place in the table
+  for (int r0 = first; r0 < rows; r0 += 32) {
+    const int r = r0 + lane;
+    int from = 0, end = 0, at = 0, n = 0;
+    if (r < rows) {
+      from = q_start[r];
+      end = from + cu_q[r + 1] - cu_q[r];
+      at = page_indptr[r];
+      n = page_indptr[r + 1] - at;
+    }
+    const int need = (end + page_size - 1) >> page_shift;
+    int incl = need;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += before;
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, incl > entry);
+    if (behind) {
+      const int src = __ffs(behind) - 1;
+      a = r0 + src;
+      entry -= __shfl_sync(0xffffffffu, incl - need, src);
+      start = __shfl_sync(0xffffffffu, from, src);
+      hi = __shfl_sync(0xffffffffu, end, src);
+      table = __shfl_sync(0xffffffffu, at, src);
+      listed = __shfl_sync(0xffffffffu, n, src);
+      break;
+    }
+    entry -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  if (f >= page_indptr[rows]) return;
+  if (a < 0) return;
+  const int f = table + entry;
+  if (entry >= listed || f >= num_ids) {  // (the products behind this trust the tables: one that is too short is found here)
+    atomicExch(status, 2);
+    return;
+  }
+  if (blockIdx.y == 0 && threadIdx.x == 0) ids[f] = out_page;
   const int eights = d >> 3, pieces = nkv * page_size * eights, idx0 = blockIdx.y * (256 * READ_EACH) + threadIdx.x;
   if (idx0 >= pieces) return;
-  int a = first, b = rows;  // the row of the entry
-  while (b - a > 1) {
-    const int mid = (a + b) / 2;
-    if (page_indptr[mid] <= f) a = mid;
-    else b = mid;
-  }
-  const int key = (f - page_indptr[a]) << page_shift, start = q_start[a], hi = start + cu_q[a + 1] - cu_q[a], lo = window > 0 ? max(0, start - window + 1) : 0;
+  const int key = entry << page_shift, lo = window > 0 ? max(0, start - window + 1) : 0;
   if (key + page_size <= lo || key >= hi) return;
   const int page = page_indices[f];
   if ((unsigned)page >= (unsigned)num_pages) {
@@ -380,7 +403,7 @@ MS_EXPORT int ms_cache8_read(void* k_out, void* v_out, const void* k_codes, cons
   return 0;
 }
 
-// Rows [first, rows) list `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; ids has num_ids numbers.
+// Rows [first, rows) need `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; ids has num_ids numbers.
 MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,
                                const int* q_start, const int* page_indptr, const int* page_indices, int first, int rows, int entries, int nkv, int d, int window, int page_size,
                                long long num_pages, int num_ids, int* status, cudaStream_t stream) {

@@ -106,6 +106,8 @@ class Engine:
             num_pages = self._pool_pages(model, kv_pool_tokens, page_size, kv_mem_fraction, step_tokens, max_running, kv_cache_dtype == "fp8")
             cache = CacheManager(model.entry_caches, num_pages, page_size, max_running, dtype=model.dtype,
                                  device=model.device, poison_on_free=poison_on_free, step_tokens=step_tokens, kv_dtype=kv_cache_dtype)
+        elif kv_cache_dtype not in ("auto", getattr(cache, "kv_dtype", "auto")):
+            raise ValueError(f"the cache that was given does not hold keys and values as kv_cache_dtype={kv_cache_dtype!r} asks")
         self.cache = cache
         self.settings = dict(kv_pool_tokens=kv_pool_tokens, page_size=page_size, max_running=max_running,
                              max_prefill_tokens=max_prefill_tokens, chunked_prefill_size=chunked_prefill_size, seed=seed,

@@ -4,6 +4,7 @@ them. ``ops.qk_norm_rope_kv`` and ``ops.attention`` take a ``Pool8`` where they 
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from dataclasses import dataclass
 from functools import lru_cache
@@ -196,13 +197,21 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
 
 # ------------------------------------------------------------------ attention
 
+def _on_stream(ctx, device: torch.device):
+    """Allocations (and their zeroing) in the order of the step's stream, where that is not the current one."""
+    if ctx.stream == torch.cuda.current_stream(device).cuda_stream:
+        return nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream, device=device) if ctx.stream else torch.cuda.default_stream(device))
+
+
 def _workspace(ctx, floats: int, device) -> torch.Tensor:
     """Partial results of steps that run one after the other. What is outgrown stays alive for graphs that hold its address; a capture that needs
     more than there is gets its own."""
     held = ctx.scratch.get("cache8")
     if held is not None and held.numel() >= floats:
         return held
-    new = torch.empty(floats, dtype=torch.float32, device=device)
+    with _on_stream(ctx, device):
+        new = torch.empty(floats, dtype=torch.float32, device=device)
     ctx.scratch.setdefault("retired", []).append(new)
     if not torch.cuda.is_current_stream_capturing():
         ctx.scratch["cache8"] = new
@@ -267,8 +276,8 @@ class _Unpacked:
         self.page_indices[group] = ids
 
 
-def _parts(ctx, group: int, first: int, page_size: int, page_bytes: int) -> list:
-    """Rows [first, num_rows) in parts whose pages fit: ``(first row, row behind, page entries)``."""
+def _parts(ctx, first: int, page_size: int, page_bytes: int) -> list:
+    """Rows [first, num_rows) in parts whose pages fit: ``(first row, row behind, pages)``."""
     out, at, entries = [], first, 0
     for r in range(first, ctx.num_rows):
         n = -(-(ctx.host_q_start[r] + ctx.host_q_len[r]) // page_size)
@@ -280,30 +289,48 @@ def _parts(ctx, group: int, first: int, page_size: int, page_bytes: int) -> list
     return out
 
 
+def _unpacked(ctx, numbers: int, table: int, device: torch.device) -> tuple:
+    """Pages of K and of V (``numbers`` each) and their places in a table of ``table`` entries, for steps that run one after the other; a capture gets its own. All
+    zero at first: the products behind may weigh, by zero, values of pages that were left out, which then have to be numbers; and what they read of a table behind
+    the end of one that is too short has to be a page that is there."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    held = None if capturing else ctx.scratch.get("cache8_pages")
+    if held is not None and held[0].numel() >= numbers and held[2].numel() >= table:
+        return held
+    if held is not None:  # (a context grows portion by portion: twice as much the next time, up to what a step of several rows may take)
+        numbers = max(numbers, min(2 * held[0].numel(), UNPACKED_BYTES // 4))
+        table = max(table, held[2].numel())
+    with _on_stream(ctx, device):
+        new = tuple(torch.zeros(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (torch.zeros(table, dtype=torch.int32, device=device),)
+    if capturing:
+        ctx.scratch.setdefault("retired", []).append(new)
+    else:
+        ctx.scratch["cache8_pages"] = new
+    return new
+
+
 def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool, first: int) -> None:
     """Rows [first, num_rows) of the step over pages unpacked to bfloat16."""
     from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
 
     pages, nkv, page_size, d = k_pool.sizes
-    dev = k_pool.device
     key = ("cache8_unpacked", group, first, nkv, page_size, d)
     parts = ctx.step_cache.get(key)
     if parts is None:
+        _check_tables(k_pool.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
         page = nkv * page_size * d
-        parts = _parts(ctx, group, first, page_size, 4 * page)
-        # (a table too short is found on the device, and what is read behind its end is some page that is there)
-        most, table = max(n for _, _, n in parts), ctx.page_indices[group].numel() + sum(n for _, _, n in parts)
-        held = ctx.scratch.get("cache8_pages")
-        if held is None or held[0].numel() < most * page or held[2].numel() < table:
-            held = tuple(torch.empty(most * page, dtype=torch.bfloat16, device=dev) for _ in range(2)) + (torch.zeros(table, dtype=torch.int32, device=dev),)
-            ctx.scratch["cache8_pages"] = held
-        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in held[:2])
-        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, held[2])) for a, b, n in parts])
+        parts = _parts(ctx, first, page_size, 4 * page)
+        most = max(n for _, _, n in parts)
+        # (behind the table's own entries: what a row whose table is too short reads)
+        *pools, ids = _unpacked(ctx, most * page, ctx.page_indices[group].numel() + sum(n for _, _, n in parts), k_pool.device)
+        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in pools)
+        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, ids)) for a, b, n in parts])
     k, v, parts = parts
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(
-            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows,
-            entries, nkv, d, window, page_size, pages, view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(),
+            ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, entries, nkv, d, window, page_size, pages,
+            view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
         if attention_tc_ok(q, k):
             attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
         else:

@@ -97,6 +97,25 @@ def test_models_with_other_mixers_are_refused():
             build(name, dtype).check_cache8(16)
 
 
+def test_an_engine_s_cache_is_of_the_type_asked_for():
+    from miniserve_b200.cache import CacheManager
+    from miniserve_b200.engine.engine import Engine
+
+    plain = CacheManager(_entries(), 6, 16, 2, device=None)
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        Engine(None, cache=plain, kv_cache_dtype="fp8")
+
+
+def test_a_cache_on_the_host_s_books_alone_has_nothing_to_read():
+    from miniserve_b200.cache import CacheManager
+
+    cm = CacheManager(_entries(), 6, 16, 2, device=None, kv_dtype="fp8")
+    rc = cm.new_request()
+    cm.reserve([(rc, 20)])
+    with pytest.raises(ValueError, match="no pools"):
+        cm.read(rc, 0)
+
+
 def test_the_command_line_has_the_option():
     import argparse
 

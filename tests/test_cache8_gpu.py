@@ -334,6 +334,134 @@ def test_on_another_stream_and_replayed():
         _close(pb, q, out, 0.1)
 
 
+def _spare_entries(pb, spare):
+    """Each row's table goes on behind the pages that it needs; those entries name no page."""
+    tables = [t + [-1] * n for t, n in zip(pb.tables, spare)]
+    indptr = [0]
+    for t in tables:
+        indptr.append(indptr[-1] + len(t))
+    i32 = dict(dtype=torch.int32, device=DEV)
+    pb.page_indptr, pb.page_indices = torch.tensor(indptr, **i32), torch.tensor([p for t in tables for p in t], **i32)
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 8, 128, 16), (8, 2, 64, 8), (16, 2, 80, 32), (2, 1, 128, 256), (2, 2, 128, 128)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_tables_that_list_more_than_a_row_needs(nq, nkv, d, page, window):
+    rows = [(700, 1), (33, 1), (260, 140), (0, 70), (1, 2), (515, 99)]
+    pb = cu.Batch8(rows, page, nkv, d, seed=d)
+    _spare_entries(pb, [3, 0, 5, 1, 0, 2])
+    q, out = _attend(pb, nq, d, 0.1, window)
+    _close(pb, q, out, 0.1, window)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(16, 2, 128), (16, 2, 64)])
+def test_prompts_behind_a_window_over_scratch_that_held_something_else(nq, nkv, d):
+    """Pages that a window has passed are not unpacked; what lies in their place is weighed by zero at most."""
+    for _ in range(3):
+        torch.full((1 << 24,), float("nan"), dtype=torch.bfloat16, device=DEV)  # (given back at once: the next allocations get it)
+    scratch = {}
+    for seed, rows in enumerate(([(700, 1), (333, 90), (1200, 70)], [(64, 40), (1501, 64)], [(4000, 300)], [(10, 64), (90, 33)])):
+        pb = cu.Batch8(rows, 16, nkv, d, seed=seed)
+        for r, (s, n) in enumerate(rows):
+            passed = max(0, s - 50 + 1) // 16
+            pb.page_indices[int(pb.page_indptr[r]):int(pb.page_indptr[r]) + passed] = -1
+        ctx = ku.make_context(pb)
+        ctx.scratch = scratch
+        q, out = _attend(pb, nq, d, 0.1, 50, seed=seed, ctx=ctx)
+        _close(pb, q, out, 0.1, 50)
+
+
+def test_more_requests_than_a_launch_takes():
+    rows = [(3 + 7 * i % 190, 1) for i in range(300)]
+    pb = cu.Batch8(rows, 16, 1, 64, seed=2)
+    q, out = _attend(pb, 4, 64, 0.1)
+    _close(pb, q, out, 0.1)
+    rows = [(3 + 7 * i % 190, 5) for i in range(150)]
+    pb = cu.Batch8(rows, 16, 1, 64, seed=2)
+    q, out = _attend(pb, 8, 64, 0.1)  # 40 query rows a request: two tiles each
+    _close(pb, q, out, 0.1)
+
+
+@pytest.mark.parametrize("rows", [[(5000, 1), (3, 1), (700, 1)], [(900, 90), (0, 33)]])
+def test_two_contexts_on_two_streams(rows):
+    """At once, each with scratch of its own: the bits of a call alone."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    batches = [cu.Batch8(rows, 16, 2, 128, seed=11 + i) for i in range(2)]
+    alone = [_attend(pb, 16, 128, 0.1, seed=i) for i, pb in enumerate(batches)]
+    outs = [torch.full_like(q, float("nan")) for q, _ in alone]
+    contexts = [ku.make_context(pb) for pb in batches]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for pb, side, ctx, (q, _), out in zip(batches, sides, contexts, alone, outs):
+            with torch.cuda.stream(side):
+                ctx.stream = side.cuda_stream
+                ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    torch.cuda.synchronize()
+    for out, (_, want) in zip(outs, alone):
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("rows", [[(900, 1), (37, 1)], [(300, 70), (15, 40)]])
+def test_a_step_s_stream_that_is_not_the_current_one(rows):
+    """``ctx.stream`` says where the kernels go; what they need is made there too."""
+    pb = cu.Batch8(rows, 16, 2, 128, seed=8)
+    q, want = _attend(pb, 16, 128, 0.1)
+    side, out, ctx = torch.cuda.Stream(), torch.full_like(q, float("nan")), ku.make_context(pb)
+    torch.cuda.synchronize()
+    ctx.stream = side.cuda_stream
+    ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    side.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_a_captured_prompt_outlives_larger_ones():
+    """A graph of a prompt over unpacked pages, replayed after a longer prompt of the same scratch."""
+    pb, other = cu.Batch8([(300, 70)], 16, 2, 64, seed=8), cu.Batch8([(3000, 200)], 16, 2, 64, seed=9)
+    ctx = ku.make_context(pb)
+    q, want = _attend(pb, 16, 64, 0.1, ctx=ctx)
+    out, graph = torch.full_like(q, float("nan")), torch.cuda.CUDAGraph()
+    ctx.step_cache.clear()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ctx.stream = torch.cuda.current_stream().cuda_stream
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    larger = ku.make_context(other)
+    larger.scratch = ctx.scratch
+    for _ in range(2):
+        _close(other, *_attend(other, 16, 64, 0.1, ctx=larger), 0.1)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_pages_beyond_4_gb():
+    """Codes whose offset passes 32 bits: written, read, attended over by single tokens and by a prompt."""
+    nkv, d, page = 8, 256, 16
+    rows = [(300, 1), (77, 1), (100, 40)]
+    pb = cu.Batch8(rows, page, nkv, d, seed=5)
+    pages = 2 ** 32 // (nkv * page * d) + pb.num_pages + 5
+    far = pages - pb.num_pages
+    k8, v8 = (ops.Pool8.empty(pages, nkv, page, d) for _ in range(2))
+    for big, small in ((k8, pb.k8), (v8, pb.v8)):
+        big.codes[far:], big.exponents[far:] = small.codes, small.exponents
+    pb.k8, pb.v8 = k8, v8
+    pb.tables = [[p + far for p in t] for t in pb.tables]
+    pb.page_indices += far
+    pb.num_pages = pages
+    q, out = _attend(pb, 16, d, 0.06)
+    _close(pb, q, out, 0.06)
+    qkv, _ = _projection(pb.num_tokens, 16, nkv, d, 3)
+    ops.qk_norm_rope_kv(q, k8, v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+    k, v = (torch.empty((pb.num_tokens, nkv, d), dtype=torch.float32, device=DEV) for _ in range(2))
+    ops.read_cache(k, v, k8, v8, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, pb.status)
+    x = qkv.double().view(pb.num_tokens, 16 + 2 * nkv, d)
+    # half a step: 2^-4 of the number, or half of the smallest code of the vector's scale (2^-10 of 2^e, 448 * 2^e below twice the largest number)
+    for got, want in ((k, x[:, 16:16 + nkv]), (v, x[:, 16 + nkv:])):
+        assert bool(((got.double() - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, want.abs().amax(-1, keepdim=True) * 2.0 ** -9 / 448)).all())
+    assert pb.status.item() == 0 and bool((k8.codes[:far] == 0).all())
+
+
 # ------------------------------------------------------------------ one behind the other
 @pytest.mark.parametrize("nq,nkv,d", [(4, 2, 128), (8, 2, 64)])
 def test_write_attend_read_a_request_in_portions(nq, nkv, d):
