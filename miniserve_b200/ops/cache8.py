@@ -218,8 +218,8 @@ def _workspace(ctx, floats: int, device) -> torch.Tensor:
     return new
 
 
-def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device) -> list:
-    """The launches over rows [0, rows_all) of a step, of at most ``most_tokens`` new tokens each, the same for every layer with these sizes and this window:
+def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:
+    """The launches over ``ranges`` of a step's rows, ``(first, rows, the most new tokens of one)``, the same for every layer with these sizes and this window:
     ``(plan, its address, query rows of a tile, the most of a request, launches)``."""
     nq, nkv, d, scale, window, sink, page_size, pages = key
     lib = _attn_lib(d)
@@ -227,32 +227,50 @@ def _plans(ctx, group: int, rows_all: int, most_tokens: int, key: tuple, device)
     ctas = ctx.sm_count
     floats = lib.part_floats(ctas)
     part = _workspace(ctx, floats + 4 * ctas, device)
-    most = most_tokens * (nq // nkv)
-    tiles = -(-most // lib.most_rows)  # as few as there have to be, of one size
-    tile_rows = -(-most // (8 * tiles)) * 8
     out = []
-    # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
-    keys = min(ctx.max_kv_len, window + most_tokens) if window else ctx.max_kv_len
-    whole = (keys <= lib.alone_keys(tile_rows) and rows_all * tiles * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing())
-    tiles_each = min(tiles, lib.max_units)
-    rows_each = lib.max_units // tiles_each
-    for first in range(0, rows_all, rows_each):
-        skip, rows = 4 * first, min(rows_each, rows_all - first)  # the per-row tables are int32
-        for tile0 in range(0, tiles, tiles_each):
-            plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
-                          ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, min(tiles_each, tiles - tile0), nq, nkv, window, sink,
-                          page_size, ctas, scale, pages, not whole)
-            out.append((plan, ctypes.addressof(plan), tile_rows, most, 1 if whole else 2))
+    for begin, rows_all, most_tokens in ranges:
+        most = most_tokens * (nq // nkv)
+        tiles = -(-most // lib.most_rows)  # as few as there have to be, of one size
+        tile_rows = -(-most // (8 * tiles)) * 8
+        keys = min(ctx.max_kv_len, window + most_tokens) if window else ctx.max_kv_len
+        tiles_each = min(tiles, lib.max_units)
+        rows_each = lib.max_units // tiles_each
+        for first in range(begin, begin + rows_all, rows_each):
+            skip, rows = 4 * first, min(rows_each, begin + rows_all - first)  # the per-row tables are int32
+            for tile0 in range(0, tiles, tiles_each):
+                here = min(tiles_each, tiles - tile0)
+                # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
+                whole = keys <= lib.alone_keys(tile_rows) and rows * here * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing()
+                plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
+                              ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, here, nq, nkv, window, sink, page_size, ctas, scale, pages,
+                              not whole)
+                out.append((plan, ctypes.addressof(plan), tile_rows, most, 1 if whole else 2))
     return out
 
 
-def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, rows: int, most_tokens: int, nq: int) -> None:
-    """Rows [0, rows) of the step on the kernel that shares out keys."""
+def _of_one_size(ctx, first: int, heads: int, lib: _AttnLib) -> list:
+    """Rows [first, num_rows) in ranges that a launch takes whole, as far as that goes: tiles are counted by a range's longest row."""
+    out = []
+    for r in range(first, ctx.num_rows):
+        n = ctx.host_q_len[r]
+        if out:
+            at, rows, most = out[-1]
+            if (rows + 1) * -(-max(n, most) * heads // lib.most_rows) <= lib.max_units:
+                out[-1] = (at, rows + 1, max(n, most))
+                continue
+        out.append((r, 1, n))
+    return [x for x in out if x[2]]
+
+
+def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, first: int, rows: int, most_tokens: int | None, nq: int) -> None:
+    """Rows [first, first + rows) of the step, of at most ``most_tokens`` new tokens (None: of as many as the host's list says), on the kernel that shares out keys."""
     pages, nkv, page_size, d = k_pool.sizes
-    key = ("cache8", group, rows, nq, nkv, d, scale, window, sink, page_size, pages)
+    key = ("cache8", group, first, rows, most_tokens, nq, nkv, d, scale, window, sink, page_size, pages)
     held = ctx.step_cache.get(key)
     if held is None:
-        held = ctx.step_cache[key] = (_attn_lib(d), _plans(ctx, group, rows, most_tokens, (nq, nkv, d, float(scale), window, int(sink), page_size, pages), k_pool.device))
+        lib = _attn_lib(d)
+        ranges = _of_one_size(ctx, first, nq // nkv, lib) if most_tokens is None else [(first, rows, most_tokens)]
+        held = ctx.step_cache[key] = (lib, _plans(ctx, group, ranges, (nq, nkv, d, float(scale), window, int(sink), page_size, pages), k_pool.device))
     lib, plans = held
     for plan, at, tile_rows, most, launches in plans:
         native.LAUNCHES[0] += launches
@@ -260,10 +278,33 @@ def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
             raise native.NativeError(lib.last_error().decode())
 
 
-# Query rows (new tokens times heads of a kv head) of a request up to which its keys are shared out over the whole device, read once for every 16 rows. Beyond, a step's pages are
-# unpacked to bfloat16 and attended over by the kernels of a bfloat16 cache, which read them once for 256 rows (64): three times the bytes, once.
-SPLIT_ROWS = 64
+# Steps of several tokens a request have two ways: the kernel that shares out keys reads the codes again for every 16 query rows of a kv head (24 at head sizes up to 64); or their
+# pages are unpacked to bfloat16 and attended over by a bfloat16 cache's kernels. Measured (one B200, us, keys shared out / unpacked):
+#   head size 128, unpacked for the tcgen05 kernel (256 query rows a tile), by query rows of a request:   64      96     128     256
+#     1 request behind 2,000 tokens                                                                      26/34   26/34   28/36   34/40
+#     16 behind 2,000                                                                                    75/93   99/93  126/89  226/101
+#     1 behind 32,000                                                                                    65/108  87/108 108/108 191/116
+#   others, unpacked for the mma.sync kernel (64 queries a CTA, which walks all their keys), by new tokens of a request:
+#     head size 64, 8 heads a kv head, 4 requests behind 8,000 tokens     32: 79/486   128: 243/488   512: 952/1402
+#                                      4 behind 500                       32: 28/46    128: 52/52     512: 214/157   1,024: 454/345
+#                                      8 from the beginning               32: 28/22    128: 77/32     512: 360/134
+#     head size 80, 2 heads a kv head, 4 behind 3,000                     32: 38/230   512: 282/447   2,048: 1322/1426
+#                                      8 from the beginning               32: 24/24    512: 159/97    2,048: 1372/804
+# So up to SPLIT_ROWS query rows always share out keys; beyond, the tcgen05 kernel takes what it takes, and of other shapes the mma.sync kernel those steps with no more keys behind
+# them than new tokens.
+SPLIT_ROWS = 96
 UNPACKED_BYTES = 1 << 30  # of pages unpacked at a time, unless a single request has more
+
+
+def _shares_out(q, k_pool: Pool8, ctx, first: int) -> bool:
+    """Whether rows [first, num_rows), some of more than SPLIT_ROWS query rows, go to the kernel that shares out keys."""
+    from . import attention_tc_ok  # (this module is imported by theirs)
+
+    key = ("cache8_shares_out", first)
+    more_behind = ctx.step_cache.get(key)
+    if more_behind is None:
+        more_behind = ctx.step_cache[key] = sum(ctx.host_q_start[first:ctx.num_rows]) > sum(ctx.host_q_len[first:ctx.num_rows])
+    return more_behind and not attention_tc_ok(q, k_pool)
 
 
 class _Unpacked:
@@ -339,8 +380,8 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
 
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
     """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
-    ``group``, window and sink as there. Single tokens and drafted ones go to the kernel that shares out keys (``csrc/attention_cache8.cu``); prompts and portions of them to a
-    bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool does not have raises the status word. Workspaces lie in
+    ``group``, window and sink as there. Single tokens, drafted ones and what else the rule at SPLIT_ROWS says go to the kernel that shares out keys
+    (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool does not have raises the status word. Workspaces lie in
     ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
     if not isinstance(v_pool, Pool8) or k_pool.sizes != v_pool.sizes or k_pool.index != v_pool.index or k_pool.index < 0:
         _check_pools(k_pool, v_pool)
@@ -363,10 +404,14 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
             attention(out, q, k_pool, v_pool, ctx, group, scale, window, sink)
         return
     if ctx.max_q_len * heads <= SPLIT_ROWS:
-        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, ctx.num_rows, ctx.max_q_len, nq)
+        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, 0, ctx.num_rows, ctx.max_q_len, nq)
         return
     single = ctx.leading_single_rows
     if single:
-        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single, 1, nq)
-    if single < ctx.num_rows:
+        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, 0, single, 1, nq)
+    if single == ctx.num_rows:
+        return
+    if _shares_out(q, k_pool, ctx, single):
+        _split(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single, ctx.num_rows - single, None, nq)
+    else:
         _dense(out, q, k_pool, v_pool, ctx, group, scale, window, sink, single)

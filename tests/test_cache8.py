@@ -40,6 +40,20 @@ def test_pools_on_the_host_are_refused_by_the_kernels():
         ops.read_cache(rows, rows, p, p.codes, i, i, i, i, i)
 
 
+def test_prompts_are_shared_out_in_ranges_that_a_launch_takes():
+    from types import SimpleNamespace
+
+    lib = SimpleNamespace(most_rows=16, max_units=256)
+    for lens in ([1, 700, 3, 1, 17, 1200, 30], [5] * 300, [0, 0, 9], [5000], [0], []):
+        ctx = SimpleNamespace(num_rows=len(lens) + 2, host_q_len=[1, 1] + lens)
+        ranges = cache8._of_one_size(ctx, 2, 4, lib)
+        seen = [r for first, rows, _ in ranges for r in range(first, first + rows)]
+        assert len(seen) == len(set(seen)) and all(n == 0 or r + 2 in seen for r, n in enumerate(lens))
+        for first, rows, most in ranges:
+            assert most == max(ctx.host_q_len[first:first + rows]) > 0
+            assert rows == 1 or rows * -(-most * 4 // 16) <= 256
+
+
 # ------------------------------------------------------------------ the cache manager
 def _entries(head_dim=64, values=True):
     from miniserve_b200.parts.base import PagedKV

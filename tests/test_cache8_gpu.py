@@ -382,6 +382,17 @@ def test_more_requests_than_a_launch_takes():
     _close(pb, q, out, 0.1)
 
 
+@pytest.mark.parametrize("nq,nkv,d,page", [(8, 1, 64, 16), (4, 2, 80, 16), (2, 1, 256, 16), (2, 1, 128, 256)])
+def test_prompts_behind_long_contexts_of_shapes_that_share_out_keys(nq, nkv, d, page, window=None):
+    """Prompts of very different lengths, one of more tiles than a launch takes, behind more keys than they bring."""
+    rows = [(50, 1), (2500, 701), (9000, 3), (3000, 1), (40, 17), (2000, 1200), (0, 0), (7, 30)]
+    pb = cu.Batch8(rows, page, nkv, d, seed=d)
+    ctx = ku.make_context(pb)
+    q, out = _attend(pb, nq, d, 0.1, ctx=ctx)
+    assert "cache8_pages" not in ctx.scratch
+    _close(pb, q, out, 0.1)
+
+
 @pytest.mark.parametrize("rows", [[(5000, 1), (3, 1), (700, 1)], [(900, 90), (0, 33)]])
 def test_two_contexts_on_two_streams(rows):
     """At once, each with scratch of its own: the bits of a call alone."""
