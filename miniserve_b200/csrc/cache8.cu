@@ -97,10 +97,12 @@ __device__ __forceinline__ uint2 c8_bf16x4(const float (&f)[4]) {
 
 // Head sizes 64, 128 and 256 rotated whole or not at all: a block per token, D / 8 lanes per head. A lane holds 4 numbers of the head's first half and the 4 of the second that
 // rotate with them; a head's lanes exchange a sum of squares and a maximum. What hangs on the token alone is fetched once a lane, and its first numbers before the
-// page is looked up (three loads, one behind the other). Bound by those chains: with 8 and 8 numbers a lane, 72 registers and 24 warps a multiprocessor, 2,048 tokens of 48 heads took 21 us.
+// page is looked up (three loads, one behind the other); a further trip's are asked for ahead of the work on the last. Bound by those chains, not by bytes: written and read back
+// (cache8_read_kernel), 2,048 tokens of 48 heads take 18.9 us (56 MB: 8.5 us at the rate of a copy); without the loads ahead 19.6, with them and five blocks a multiprocessor (which
+// spill) 19.3.
 // TABLE: the angles' cosines and sines are given, or nothing is rotated (the form that makes them itself needs more registers).
 template <int D, bool TABLE>
-__global__ void __launch_bounds__(256, TABLE ? 5 : 1)
+__global__ void __launch_bounds__(256, TABLE ? 4 : 1)
 cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_exps, uint8_t* __restrict__ v_codes,
                           uint8_t* __restrict__ v_exps, const __nv_bfloat16* __restrict__ qkv, const __nv_bfloat16* __restrict__ q_norm_w,
                           const __nv_bfloat16* __restrict__ k_norm_w, const float* __restrict__ inv_freq, const float* __restrict__ cos_sin,
@@ -145,14 +147,20 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
   if (page < 0 && threadIdx.x == 0) atomicExch(status, 2);
   const size_t at0 = ((size_t)max(page, 0) * nkv << page_shift) + (pos & ((1 << page_shift) - 1));
   for (int base = 0; base < heads; base += BATCH * stride) {  // the same trips for every lane: they exchange sums
-    if (base > 0) fetch(base);
+    uint2 lo_now[BATCH], hi_now[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      lo_now[b] = lo_raw[b];
+      hi_now[b] = hi_raw[b];
+    }
+    if (base + BATCH * stride < heads) fetch(base + BATCH * stride);
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       const int h = base + warp * HPW + slot + b * stride;
       const bool is_q = h < nq, is_v = h >= nq + nkv;
       float lo[4], hi[4];
-      c8_float4(lo, lo_raw[b]);
-      c8_float4(hi, hi_raw[b]);
+      c8_float4(lo, lo_now[b]);
+      c8_float4(hi, hi_now[b]);
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
@@ -366,8 +374,8 @@ MS_EXPORT int ms_cache8_write(void* q_out, void* k_codes, void* k_exps, void* v_
     auto kernel = d == 64    ? (table ? cache8_write_token_kernel<64, true> : cache8_write_token_kernel<64, false>)
                   : d == 128 ? (table ? cache8_write_token_kernel<128, true> : cache8_write_token_kernel<128, false>)
                              : (table ? cache8_write_token_kernel<256, true> : cache8_write_token_kernel<256, false>);
-    // as many warps as bring all heads in one trip of two a lane group: the more blocks are resident, the better their chains of loads hide one another
-    const int a_trip = 2 * (32 / (d / 8)), warps = ceil_div(nq + 2 * nkv, a_trip) < 8 ? ceil_div(nq + 2 * nkv, a_trip) : 8;
+    // as many warps as bring all heads in equal trips of two a lane group, 8 at most: 48 heads of 128 in two trips of 6 warps 19.6 us, of 8 warps 21.0 (the sizes above)
+    const int a_trip = 2 * (32 / (d / 8)), trips = ceil_div(nq + 2 * nkv, 8 * a_trip), warps = ceil_div(nq + 2 * nkv, a_trip * trips);
     MS_LAUNCH(kernel, num_tokens, 32 * warps, 0, stream, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)k_exps, (uint8_t*)v_codes, (uint8_t*)v_exps,
               (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w, rot ? inv_freq : (const float*)nullptr, cos_sin, positions,
               row_of_token, page_indptr, page_indices, nq, nkv, eps, c8_page_shift(page_size), (int)num_pages, status);
