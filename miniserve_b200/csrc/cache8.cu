@@ -168,7 +168,7 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
       if (!is_v) {
         float wl[4], wh[4];
-        const float inv = normed ? 1.0f / sqrtf(ss / (float)D + eps) : 1.f;
+        const float inv = normed ? rsqrtf(ss * (1.f / D) + eps) : 1.f;  // (2 steps of float32 at most; a root and a division take 30 instructions more)
         c8_float4(wl, is_q ? wq_lo : wk_lo);
         c8_float4(wh, is_q ? wq_hi : wk_hi);
 #pragma unroll
@@ -179,10 +179,12 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
         }
       }
       uint32_t amax = 0;
+      if (base + warp * HPW + b * stride + HPW > nq) {  // (some head of the warp's is to be quantised)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(lo[i]) & 0x7FFFFFFFu, __float_as_uint(hi[i]) & 0x7FFFFFFFu));
+        for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(lo[i]) & 0x7FFFFFFFu, __float_as_uint(hi[i]) & 0x7FFFFFFFu));
 #pragma unroll
-      for (int off = LPH / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+        for (int off = LPH / 2; off > 0; off >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      }
       if (h >= heads) continue;
       if (is_q) {
         __nv_bfloat16* dst = q_out + ((size_t)t * nq + h) * D + j0;
