@@ -42,6 +42,10 @@ constexpr int CODE_BYTES = SLICE * ROW_BYTES, STAGE_BYTES = 2 * CODE_BYTES + 2 *
 constexpr int warps_of(int) { return D > 128 ? 4 : 8; }
 constexpr int stages_of(int) { return D > 64 ? 2 : 4; }
 constexpr int PART = D + 4;                          // floats of a row's partial: o, m, l, c (and one that keeps rows on 16 bytes)
+// Items that are no more than CTAs get one each, whole, where the longest's warps then have at most this many slices more than in equal runs: that is what cutting costs
+// (pieces, and a second kernel). Measured, us with 0 / 3 / 4 / 6 more: 16 requests of 5 drafted tokens, 4 kv heads of 64, around 2,000 keys 28.1 / 22.9 / 22.9 / 22.9; 16 single
+// tokens, 8 kv heads of 128, at 2,048 keys 20.8 / 17.8 / 17.8 / 17.8; 8 at 1,000 11.6 / 11.3 / 11.3 / 11.3, at 1,500 13.1 / 13.1 / 13.9 / 13.9, at 2,048 15.4 / 15.4 / 15.4 / 17.0.
+constexpr int ALONE_MORE = 3;
 constexpr int MAX_UNITS = 256;                       // (request, tile) pairs of a launch
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -257,8 +261,9 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
       live += scan[1][w];
       longest = max(longest, scan[2][w]);
     }
-    // Few short items: a CTA each, whole, so that nothing is left to add up behind.
-    const int alone = live * p.nkv <= p.ctas && longest <= 2 * WARPS ? (longest + WARPS - 1) / WARPS * WARPS : 0;
+    // Few items, none much longer than an equal share: a CTA each, whole, so that nothing is left to add up behind.
+    const int longest_each = (longest + WARPS - 1) / WARPS, equal_each = (total * p.nkv + p.ctas * WARPS - 1) / (p.ctas * WARPS);
+    const int alone = live * p.nkv <= p.ctas && longest_each <= equal_each + ALONE_MORE ? longest_each * WARPS : 0;
     if (alone) total = live * alone;
     for (int u = first; u < min(first + each, units); ++u) {
       if (each > 1) unit_of(u);
@@ -288,6 +293,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     }
     return a;
   };
+  if (tid == 0 && !p.behind && !alone && total > 0) atomicExch(p.status, 2);  // (other lengths than the host said)
   if (tid == 0 && p.behind) {
     int4 cut = make_int4(0, 0, 0, 0);
     if (cta_begin < cta_end && !alone) {
@@ -884,8 +890,9 @@ constexpr int SMEM_MOST = 227 * 1024 - 16 * 1024;  // (the table of tiles is sta
 MS_EXPORT long long MS_ATTN8_FN(part_floats)(int ctas) { return 2LL * ctas * ROWS * PART; }
 MS_EXPORT int MS_ATTN8_FN(max_units)() { return MAX_UNITS; }
 MS_EXPORT int MS_ATTN8_FN(most_rows)() { return ROWS; }
-// Keys up to which few items (no more than CTAs) run a CTA each, whole: nothing is cut then.
-MS_EXPORT int MS_ATTN8_FN(alone_keys)(int tile_rows) { return SLICE * (2 * (warps_of(tile_rows / 8)) - 1); }
+MS_EXPORT int MS_ATTN8_FN(slice)() { return SLICE; }
+MS_EXPORT int MS_ATTN8_FN(warps)(int tile_rows) { return warps_of(tile_rows / 8); }
+MS_EXPORT int MS_ATTN8_FN(alone_more)() { return ALONE_MORE; }
 
 template <int NT>
 static int launch_split(const Split8& p, int rows_tile, void* out, const void* q, const void* k_codes,

@@ -104,7 +104,8 @@ class _AttnLib:
         native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
         self.split = native._declare(lib, pre + "split", [_p, _i, _i] + [_p] * 7)
         self.part_floats = native._declare(lib, pre + "part_floats", [_i], _ll)
-        self.alone_keys = native._declare(lib, pre + "alone_keys", [_i])
+        self.slice, self.alone_more = (native._declare(lib, pre + name, [])() for name in ("slice", "alone_more"))
+        self.warps = native._declare(lib, pre + "warps", [_i])
         self.most_rows = native._declare(lib, pre + "most_rows", [])()
         self.max_units = native._declare(lib, pre + "max_units", [])()
 
@@ -218,6 +219,22 @@ def _workspace(ctx, floats: int, device) -> torch.Tensor:
     return new
 
 
+def _alone(ctx, lib: _AttnLib, rows: range, tiles: range, tile_rows: int, heads: int, nkv: int, window: int) -> bool:
+    """Whether the kernel gives every item (tile of query rows of a request, and kv head) a CTA of its own, as it will find by the same rule: then none
+    is cut."""
+    if len(ctx.host_q_len) < rows.stop:
+        return False
+    total = longest = 0
+    for r in rows:
+        start, most = ctx.host_q_start[r], ctx.host_q_len[r] * heads
+        for row0 in range(tiles.start * tile_rows, min(tiles.stop * tile_rows, most), tile_rows):
+            low = max(0, start + row0 // heads - window + 1) if window else 0
+            n = max(1, -(-(start + (min(row0 + tile_rows, most) - 1) // heads + 1) // lib.slice) - low // lib.slice)
+            total, longest = total + n, max(longest, n)
+    warps = lib.warps(tile_rows)
+    return -(-longest // warps) <= -(-total * nkv // (ctx.sm_count * warps)) + lib.alone_more
+
+
 def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:
     """The launches over ``ranges`` of a step's rows, ``(first, rows, the most new tokens of one)``, the same for every layer with these sizes and this window:
     ``(plan, its address, query rows of a tile, the most of a request, launches)``."""
@@ -227,20 +244,19 @@ def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:
     ctas = ctx.sm_count
     floats = lib.part_floats(ctas)
     part = _workspace(ctx, floats + 4 * ctas, device)
+    fixed = not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing()  # (a graph may be replayed for other lengths)
     out = []
     for begin, rows_all, most_tokens in ranges:
         most = most_tokens * (nq // nkv)
         tiles = -(-most // lib.most_rows)  # as few as there have to be, of one size
         tile_rows = -(-most // (8 * tiles)) * 8
-        keys = min(ctx.max_kv_len, window + most_tokens) if window else ctx.max_kv_len
         tiles_each = min(tiles, lib.max_units)
         rows_each = lib.max_units // tiles_each
         for first in range(begin, begin + rows_all, rows_each):
             skip, rows = 4 * first, min(rows_each, begin + rows_all - first)  # the per-row tables are int32
             for tile0 in range(0, tiles, tiles_each):
                 here = min(tiles_each, tiles - tile0)
-                # no item is cut: few, and short. (Not inside a graph, which may be replayed for longer ones.)
-                whole = keys <= lib.alone_keys(tile_rows) and rows * here * nkv <= ctas and not ctx.graph_bucket and not torch.cuda.is_current_stream_capturing()
+                whole = fixed and rows * here * nkv <= ctas and _alone(ctx, lib, range(first, first + rows), range(tile0, tile0 + here), tile_rows, nq // nkv, nkv, window)
                 plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, here, nq, nkv, window, sink, page_size, ctas, scale, pages,
                               not whole)

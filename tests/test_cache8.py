@@ -139,3 +139,20 @@ def test_the_command_line_has_the_option():
     add_engine_args(ap)
     assert engine_kwargs(ap.parse_args(["--kv-cache-dtype", "fp8"]))["kv_cache_dtype"] == "fp8"
     assert engine_kwargs(ap.parse_args([]))["kv_cache_dtype"] == "auto"
+
+
+def test_items_that_get_a_cta_each_are_those_that_the_kernel_finds():
+    """The host's rule, against its words: as many slices of 32 keys as an item's rows see, shared by 8 warps, at most 3 more each than in equal runs."""
+    from types import SimpleNamespace
+
+    lib = SimpleNamespace(slice=32, alone_more=3, warps=lambda tile_rows: 8)
+
+    def alone(rows, nkv=8, heads=2, window=0, tiles=1, tile_rows=8, **more):
+        ctx = SimpleNamespace(**{**dict(sm_count=148, host_q_start=[s for s, _ in rows], host_q_len=[n for _, n in rows]), **more})
+        return cache8._alone(ctx, lib, range(len(rows)), range(tiles), tile_rows, heads, nkv, window)
+
+    assert alone([(299, 1)]) and alone([(32 * 32 - 1, 1)]) and not alone([(32 * 32, 1)])  # 32 slices are 4 a warp, equal runs 1
+    assert alone([(2047, 1)] * 16) and not alone([(2047, 1)] * 8)  # 64 slices, 8 a warp; equal runs 7 and 4
+    assert alone([(100000, 1)], window=1024) is False and alone([(100000, 1)], window=900)
+    assert not alone([(299, 1)], host_q_len=[])
+    assert alone([(10, 0), (20, 9)], tiles=3, tile_rows=8)  # rows without tokens have no item
