@@ -42,10 +42,15 @@ constexpr int CODE_BYTES = SLICE * ROW_BYTES, STAGE_BYTES = 2 * CODE_BYTES + 2 *
 constexpr int warps_of(int) { return D > 128 ? 4 : 8; }
 constexpr int stages_of(int) { return D > 64 ? 2 : 4; }
 constexpr int PART = D + 4;                          // floats of a row's partial: o, m, l, c (and one that keeps rows on 16 bytes)
-// Items that are no more than CTAs get one each, whole, where the longest's warps then have at most this many slices more than in equal runs: that is what cutting costs
-// (pieces, and a second kernel). Measured, us with 0 / 3 / 4 / 6 more: 16 requests of 5 drafted tokens, 4 kv heads of 64, around 2,000 keys 28.1 / 22.9 / 22.9 / 22.9; 16 single
-// tokens, 8 kv heads of 128, at 2,048 keys 20.8 / 17.8 / 17.8 / 17.8; 8 at 1,000 11.6 / 11.3 / 11.3 / 11.3, at 1,500 13.1 / 13.1 / 13.9 / 13.9, at 2,048 15.4 / 15.4 / 15.4 / 17.0.
-constexpr int ALONE_MORE = 3;
+// Items that are no more than CTAs get one each, whole, where the longest's warps then have a third and one slice more than in equal runs of `each`, at most three: that is what
+// cutting costs (pieces, and a second kernel). Measured, us whole / cut: one token, 8 kv heads of 128, behind 300 keys (2 slices a warp to 1) 7.4 / 8.1, behind 600 (3 to 1) 8.4 / 8.2;
+// 8 tokens behind 500 (3 to 2) 9.0 / 10.0, 1,000 (5 to 2) 11.3 / 10.3, 1,500 (6 to 3) 14.0 / 11.7; 16 behind 2,048 (9 to 8) 17.8 / 19.7, 4,000 (16 to 14) 26.6 / 29.4; 16
+// requests of 5 drafted tokens, 4 kv heads of 64, behind 1,500 to 2,415 keys (10 to 7) 22.9 / 25.8.
+__host__ __device__ constexpr int alone_most(int each) { return each + (1 + each / 3 < 3 ? 1 + each / 3 : 3); }
+// Slices that going on to an item counts for in the row of slices (its queries, its pages, what is kept of the last one): warps that do have so many fewer. Measured, us with
+// 0 / 1 / 2 / 3 / 4: 8 single tokens, 8 kv heads of 128, at 2,048 keys 15.3 / 14.7 / 14.0 / 14.0 / 14.0; 64 at 200 to 515 keys 19.5 / 18.9 / 18.0 / 18.4 / 18.5, at 1,024 to 3,985
+// 60.5 / 60.9 / 60.0 / 59.9 / 60.6; 4 requests of 5 drafted tokens, 4 kv heads of 64, around 1,600 keys 20.8 / 18.1 / 18.2 / 18.1 / 17.9.
+constexpr int SWITCH = 2;
 constexpr int MAX_UNITS = 256;                       // (request, tile) pairs of a launch
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -229,7 +234,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     };
     for (int u = first; u < min(first + each, units); ++u) {
       unit_of(u);
-      slices += mine.n;
+      slices += mine.n > 0 ? mine.n + SWITCH : 0;
       count += mine.n > 0;
       longest = max(longest, mine.n);
     }
@@ -263,15 +268,15 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     }
     // Few items, none much longer than an equal share: a CTA each, whole, so that nothing is left to add up behind.
     const int longest_each = (longest + WARPS - 1) / WARPS, equal_each = (total * p.nkv + p.ctas * WARPS - 1) / (p.ctas * WARPS);
-    const int alone = live * p.nkv <= p.ctas && longest_each <= equal_each + ALONE_MORE ? longest_each * WARPS : 0;
+    const int alone = live * p.nkv <= p.ctas && longest_each <= alone_most(equal_each) ? longest_each * WARPS : 0;
     if (alone) total = live * alone;
     for (int u = first; u < min(first + each, units); ++u) {
       if (each > 1) unit_of(u);
       if (mine.n == 0) continue;
-      mine.stride = alone ? alone : mine.n;
+      mine.stride = alone ? alone : mine.n + SWITCH;
       mine.at = (alone ? c_at * alone : s_at) * p.nkv;
       table[c_at++] = mine;
-      s_at += mine.n;
+      s_at += mine.n + SWITCH;
     }
     total *= p.nkv;
     if (tid == 0) table[live].at = total;
@@ -298,7 +303,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     int4 cut = make_int4(0, 0, 0, 0);
     if (cta_begin < cta_end && !alone) {
       const Unit& u = table[find(cta_end - 1)];
-      const int kvh = div_small(cta_end - 1 - u.at, u.n), at = u.at + kvh * u.n;
+      const int kvh = div_small(cta_end - 1 - u.at, u.stride), at = u.at + kvh * u.stride;
       // the item that goes on behind the CTA's end, where it began in this CTA
       if (at >= cta_begin && at + u.n > cta_end) cut = make_int4(u.tok0 * group + u.row0, u.rows_here, kvh, (at + u.n - 1) / (each * WARPS) - (int)blockIdx.x + 1);
     }
@@ -892,7 +897,8 @@ MS_EXPORT int MS_ATTN8_FN(max_units)() { return MAX_UNITS; }
 MS_EXPORT int MS_ATTN8_FN(most_rows)() { return ROWS; }
 MS_EXPORT int MS_ATTN8_FN(slice)() { return SLICE; }
 MS_EXPORT int MS_ATTN8_FN(warps)(int tile_rows) { return warps_of(tile_rows / 8); }
-MS_EXPORT int MS_ATTN8_FN(alone_more)() { return ALONE_MORE; }
+MS_EXPORT int MS_ATTN8_FN(alone_most)(int each) { return alone_most(each); }
+MS_EXPORT int MS_ATTN8_FN(switch_slices)() { return SWITCH; }
 
 template <int NT>
 static int launch_split(const Split8& p, int rows_tile, void* out, const void* q, const void* k_codes,

@@ -104,8 +104,8 @@ class _AttnLib:
         native._declare(lib, pre + "set_pdl", [_i], None)(int(native.pdl_enabled()))
         self.split = native._declare(lib, pre + "split", [_p, _i, _i] + [_p] * 7)
         self.part_floats = native._declare(lib, pre + "part_floats", [_i], _ll)
-        self.slice, self.alone_more = (native._declare(lib, pre + name, [])() for name in ("slice", "alone_more"))
-        self.warps = native._declare(lib, pre + "warps", [_i])
+        self.slice, self.switch = (native._declare(lib, pre + name, [])() for name in ("slice", "switch_slices"))
+        self.warps, self.alone_most = (native._declare(lib, pre + name, [_i]) for name in ("warps", "alone_most"))
         self.most_rows = native._declare(lib, pre + "most_rows", [])()
         self.max_units = native._declare(lib, pre + "max_units", [])()
 
@@ -230,9 +230,9 @@ def _alone(ctx, lib: _AttnLib, rows: range, tiles: range, tile_rows: int, heads:
         for row0 in range(tiles.start * tile_rows, min(tiles.stop * tile_rows, most), tile_rows):
             low = max(0, start + row0 // heads - window + 1) if window else 0
             n = max(1, -(-(start + (min(row0 + tile_rows, most) - 1) // heads + 1) // lib.slice) - low // lib.slice)
-            total, longest = total + n, max(longest, n)
+            total, longest = total + n + lib.switch, max(longest, n)
     warps = lib.warps(tile_rows)
-    return -(-longest // warps) <= -(-total * nkv // (ctx.sm_count * warps)) + lib.alone_more
+    return -(-longest // warps) <= lib.alone_most(-(-total * nkv // (ctx.sm_count * warps)))
 
 
 def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:

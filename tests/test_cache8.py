@@ -142,17 +142,17 @@ def test_the_command_line_has_the_option():
 
 
 def test_items_that_get_a_cta_each_are_those_that_the_kernel_finds():
-    """The host's rule, against its words: as many slices of 32 keys as an item's rows see, shared by 8 warps, at most 3 more each than in equal runs."""
+    """The host's rule, against its words: as many slices of 32 keys as an item's rows see and 2 for going on to it, shared by 8 warps; a third and one more than in equal runs, at most 3."""
     from types import SimpleNamespace
 
-    lib = SimpleNamespace(slice=32, alone_more=3, warps=lambda tile_rows: 8)
+    lib = SimpleNamespace(slice=32, alone_most=lambda each: each + min(3, 1 + each // 3), switch=2, warps=lambda tile_rows: 8)
 
     def alone(rows, nkv=8, heads=2, window=0, tiles=1, tile_rows=8, **more):
         ctx = SimpleNamespace(**{**dict(sm_count=148, host_q_start=[s for s, _ in rows], host_q_len=[n for _, n in rows]), **more})
         return cache8._alone(ctx, lib, range(len(rows)), range(tiles), tile_rows, heads, nkv, window)
 
-    assert alone([(299, 1)]) and alone([(32 * 32 - 1, 1)]) and not alone([(32 * 32, 1)])  # 32 slices are 4 a warp, equal runs 1
-    assert alone([(2047, 1)] * 16) and not alone([(2047, 1)] * 8)  # 64 slices, 8 a warp; equal runs 7 and 4
-    assert alone([(100000, 1)], window=1024) is False and alone([(100000, 1)], window=900)
+    assert alone([(299, 1)]) and alone([(16 * 32 - 1, 1)]) and not alone([(16 * 32, 1)])  # 16 slices are 2 a warp, equal runs 1
+    assert alone([(2047, 1)] * 16) and not alone([(2047, 1)] * 8)  # 64 slices are 8 a warp; equal runs 8 and 4
+    assert not alone([(100000, 1)], window=512) and alone([(100000, 1)], window=480)  # 17 slices and 16, where they begin inside one
     assert not alone([(299, 1)], host_q_len=[])
     assert alone([(10, 0), (20, 9)], tiles=3, tile_rows=8)  # rows without tokens have no item
