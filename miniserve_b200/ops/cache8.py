@@ -146,7 +146,8 @@ def _launch(index: int, fn, *args) -> None:
 def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim: int, eps: float, positions, row_of_token,
                     page_indptr, page_indices, page_size: int, status, stream=None, cos_sin=None) -> None:
     """``ops.qk_norm_rope_kv`` with keys and values quantised into 8-bit pools: what is rounded is the float32 number behind norm and rotation
-    (values: as projected). A token whose position its row's table has no page for raises the status word and is not written."""
+    (values: as projected). A token whose position its row's table has no page for raises the status word and is not written; two tokens of a call do
+    not share a place."""
     _check_pools(k_pool, v_pool)
     t, nq, d = q_out.shape
     pages, nkv, held, dim = k_pool.sizes
@@ -414,6 +415,8 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
     if getattr(ctx, "recorder", None) is not None:
         # a pass that is captured for steps of other lengths too: launched anew for each, between the graphs
         ctx.recorder.defer(lambda step: attention(out, q, k_pool, v_pool, step, group, scale, window, sink))
+        return
+    if not shape[0]:
         return
     if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):

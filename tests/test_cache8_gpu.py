@@ -82,6 +82,26 @@ def test_write(nq, nkv, d, page, norm, rot, rows, table):
         assert bool((pool.codes.permute(0, 2, 1, 3)[~written] == 0xA5).all()) and bool((pool.exponents.transpose(1, 2)[~written] == 0xA5).all())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_write_with_one_norm(d, which):
+    rows, nq, nkv, page = [(5, 20)], 4, 2, 16
+    pb = ku.PagedBatch(rows, page, nkv, d, torch.bfloat16)
+    qkv, gen = _projection(20, nq, nkv, d, 4)
+    w = (1 + 0.3 * torch.randn(d, generator=gen, device=DEV)).bfloat16()
+    k8, v8 = ops.Pool8.empty(pb.num_pages, nkv, page, d), ops.Pool8.empty(pb.num_pages, nkv, page, d)
+    q = torch.empty((20, nq, d), dtype=torch.bfloat16, device=DEV)
+    wq, wk = (w, None) if which == "q" else (None, w)
+    ops.qk_norm_rope_kv(q, k8, v8, qkv, wq, wk, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+    x, slack = qkv.double().view(20, nq + 2 * nkv, d), 32 * 2.0 ** -24  # (as in test_write)
+    q64 = _turn64(x[:, :nq], wq, 1e-6, None, None, 0)
+    assert bool(((q.double() - q64).abs() <= 2.0 ** -8 * q64.abs() + slack * q64.abs().amax(-1, keepdim=True)).all())
+    pos = torch.arange(5, 25)
+    pages, slots = torch.tensor([pb.tables[0][p // page] for p in pos.tolist()], device=DEV), (pos % page).to(DEV)
+    cu.check_held(k8.codes[pages, :, slots], k8.exponents[pages, :, slots], _turn64(x[:, nq:nq + nkv], wk, 1e-6, None, None, 0), slack)
+    cu.check_held(v8.codes[pages, :, slots], v8.exponents[pages, :, slots], x[:, nq + nkv:], slack)
+
+
 def test_write_of_values_at_the_format_s_borders():
     """Values (neither normed nor rotated) where rounding, the exponent's choice and its limits show: all bits are known."""
     d, page = 64, 16
@@ -283,6 +303,13 @@ def test_what_is_not_finite_reaches_only_who_sees_it():
             pb.k8.codes[page, 1, slot] = 0
             q, out = _attend(pb, 4, d, 0.1)
             assert bool(out[2:n].isnan().all()) and bool(out[:2].isfinite().all()) and bool(out[n:].isfinite().all())
+
+
+@pytest.mark.parametrize("rows", [[(0, 0)], [(40, 0), (7, 0)]])
+def test_a_step_without_tokens(rows):
+    pb = cu.Batch8(rows, 16, 2, 64, seed=4)
+    q, out = _attend(pb, 8, 64, 0.1)
+    assert out.shape[0] == 0 and pb.status.item() == 0
 
 
 def test_rows_without_keys_are_zero():
