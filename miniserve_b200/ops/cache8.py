@@ -398,8 +398,9 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
     """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
     ``group``, window and sink as there. Single tokens, drafted ones and what else the rule at SPLIT_ROWS says go to the kernel that shares out keys
-    (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool does not have raises the status word. Workspaces lie in
-    ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
+    (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool
+    does not have raises the status word. Workspaces lie in ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the
+    other."""
     if not isinstance(v_pool, Pool8) or k_pool.sizes != v_pool.sizes or k_pool.index != v_pool.index or k_pool.index < 0:
         _check_pools(k_pool, v_pool)
     shape = q.shape
