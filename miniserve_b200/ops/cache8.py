@@ -4,6 +4,7 @@ them. ``ops.qk_norm_rope_kv`` and ``ops.attention`` take a ``Pool8`` where they 
 from __future__ import annotations
 
 import ctypes
+import struct
 from contextlib import nullcontext
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from dataclasses import dataclass
@@ -65,6 +66,7 @@ def takes(head_dim: int, page_size: int) -> bool:
 
 
 CACHE8 = build.Module("cache8", ("cache8.cu",))
+_WRITE, _READ = struct.Struct("16Qq7if").pack, struct.Struct("12Qq6i").pack  # ``Write8`` and ``Read8`` of csrc/cache8.cu
 
 
 def module_for(head_dim: int) -> build.Module:
@@ -76,15 +78,17 @@ def _cache_lib():
     lib = ctypes.CDLL(str(build.ensure_built(CACHE8)))
     native._declare(lib, "ms_cache8_last_error", [], c_char_p)
     native._declare(lib, "ms_cache8_set_pdl", [_i], None)
-    native._declare(lib, "ms_cache8_write", [_p] * 14 + [_i] * 5 + [_f, _i, _ll, _p, _p])
-    native._declare(lib, "ms_cache8_read", [_p] * 10 + [_i] * 4 + [_ll, _p, _i, _p])
+    native._declare(lib, "ms_cache8_write", [c_char_p])
+    native._declare(lib, "ms_cache8_read", [c_char_p])
     native._declare(lib, "ms_cache8_unpack", [_p] * 11 + [_i] * 7 + [_ll, _i, _p, _p])
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
 
 
 def _cache_check(rc: int) -> None:
-    native.kernel_check(rc, lib=_cache_lib() if rc else None, errfn="ms_cache8_last_error")
+    native.LAUNCHES[0] += 1
+    if rc:
+        native.kernel_check(rc, lib=_cache_lib(), errfn="ms_cache8_last_error", launches=0)
 
 
 class _Split(ctypes.Structure):
@@ -119,9 +123,12 @@ def _stream_of(stream, device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
 
 
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
+
 def _check_tables(index: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+        if t.dtype is not _I32 or t.get_device() != index or not t.is_contiguous():
             raise ValueError("positions, rows, page tables and the status word are contiguous int32 tensors on the pools' device")
 
 
@@ -132,15 +139,6 @@ def _check_pools(k: Pool8, v: Pool8) -> None:
         raise ValueError(f"the pools of keys and values differ: {k.sizes} on {k.device}, {v.sizes} on {v.device}")
     if k.index < 0:
         raise ValueError("kernel operands must be contiguous CUDA tensors")
-
-
-def _launch(index: int, fn, *args) -> None:
-    """``fn(*args)`` with the pools' device as the current one."""
-    if torch.cuda.current_device() == index:
-        _cache_check(fn(*args))
-    else:
-        with torch.cuda.device(index):
-            _cache_check(fn(*args))
 
 
 def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim: int, eps: float, positions, row_of_token,
@@ -154,25 +152,27 @@ def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w
     dev = k_pool.index
     if held != page_size or dim != d or qkv.shape != (t, (nq + 2 * nkv) * d):
         raise ValueError(f"q is {tuple(q_out.shape)}, the projection {tuple(qkv.shape)}, the pools {k_pool.sizes}, the page size {page_size}")
-    pq, px, pw, pk = q_out.data_ptr(), qkv.data_ptr(), None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr()
+    pq, px, pw, pk = q_out.data_ptr(), qkv.data_ptr(), 0 if q_norm_w is None else q_norm_w.data_ptr(), 0 if k_norm_w is None else k_norm_w.data_ptr()
     for x, at, n in ((q_out, pq, 0), (qkv, px, 0), (q_norm_w, pw, d), (k_norm_w, pk, d)):
-        if x is not None and (x.dtype is not torch.bfloat16 or x.get_device() != dev or not x.is_contiguous() or at % 16 or (n and x.numel() != n)):
+        if x is not None and (x.dtype is not _BF16 or x.get_device() != dev or not x.is_contiguous() or at % 16 or (n and x.numel() != n)):
             raise ValueError("an 8-bit cache is written from contiguous bfloat16 tensors on its device, on 16 bytes; norm weights have the head's size")
-    freq = table = None
+    freq = table = 0
     if inv_freq is not None:
-        if inv_freq.dtype is not torch.float32 or inv_freq.numel() != rotary_dim // 2 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+        if inv_freq.dtype is not _F32 or inv_freq.numel() != rotary_dim // 2 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
             raise ValueError("inv_freq is float32 [rotary_dim / 2] on the pools' device")
         freq = inv_freq.data_ptr()
         if cos_sin is not None:
-            if cos_sin.dtype is not torch.float32 or cos_sin.shape != (t, rotary_dim) or cos_sin.get_device() != dev or not cos_sin.is_contiguous():
+            if cos_sin.dtype is not _F32 or cos_sin.shape != (t, rotary_dim) or cos_sin.get_device() != dev or not cos_sin.is_contiguous():
                 raise ValueError("cos_sin is float32 [tokens, rotary_dim], contiguous, on the pools' device")
             table = cos_sin.data_ptr()
     _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
     if positions.numel() < t or row_of_token.numel() < t:
         raise ValueError(f"{t} tokens need as many positions and rows")
-    _launch(dev, _cache_lib().ms_cache8_write, pq, *k_pool.pointers, *v_pool.pointers, px, pw, pk, freq, table, positions.data_ptr(), row_of_token.data_ptr(),
-            page_indptr.data_ptr(), page_indices.data_ptr(), t, nq, nkv, d, 0 if freq is None else rotary_dim, eps, page_size, pages, status.data_ptr(),
-            _stream_of(stream, k_pool.device))
+    kc, ke = k_pool.pointers
+    vc, ve = v_pool.pointers
+    _cache_check(_cache_lib().ms_cache8_write(_WRITE(
+        pq, kc, ke, vc, ve, px, pw, pk, freq, table, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
+        status.data_ptr(), _stream_of(stream, k_pool.device), pages, dev, t, nq, nkv, d, rotary_dim if freq else 0, page_size, eps)))
 
 
 def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: Pool8, positions: torch.Tensor, row_of_token: torch.Tensor,
@@ -187,14 +187,17 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
     if shape != (n, nkv, d) or v_out.shape != shape or positions.numel() < n or row_of_token.numel() < n:
         raise ValueError(f"rows {tuple(shape)} and {tuple(v_out.shape)} of pools {k_pool.sizes}, {positions.numel()} positions, {row_of_token.numel()} rows")
     dtype = k_out.dtype
-    if (dtype is not torch.bfloat16 and dtype is not torch.float32) or v_out.dtype is not dtype:
+    if (dtype is not _BF16 and dtype is not _F32) or v_out.dtype is not dtype:
         raise TypeError(f"a cache is read as bfloat16 or float32, not {dtype} and {v_out.dtype}")
     pk, pv = k_out.data_ptr(), v_out.data_ptr()
     if k_out.get_device() != dev or v_out.get_device() != dev or not k_out.is_contiguous() or not v_out.is_contiguous() or pk % 16 or pv % 16:
         raise ValueError("the rows are contiguous, on 16 bytes, on the pools' device")
     _check_tables(dev, positions, row_of_token, page_indptr, page_indices, status)
-    _launch(dev, _cache_lib().ms_cache8_read, pk, pv, *k_pool.pointers, *v_pool.pointers, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(),
-            page_indices.data_ptr(), n, nkv, d, page_size, pages, status.data_ptr(), 0 if dtype is torch.float32 else 1, _stream_of(stream, k_pool.device))
+    kc, ke = k_pool.pointers
+    vc, ve = v_pool.pointers
+    _cache_check(_cache_lib().ms_cache8_read(_READ(
+        pk, pv, kc, ke, vc, ve, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), status.data_ptr(),
+        _stream_of(stream, k_pool.device), pages, dev, n, nkv, d, page_size, 0 if dtype is _F32 else 1)))
 
 
 # ------------------------------------------------------------------ attention
