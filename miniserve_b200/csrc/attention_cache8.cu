@@ -155,15 +155,6 @@ struct Split8 {
   int behind;               // the second kernel runs: an item may be cut
 };
 
-// a / b of whole numbers, quotients below 2^20: a multiplication by the reciprocal, off by one at most, put right
-__device__ __forceinline__ int div_small(int a, int b) {
-  int q = (int)((float)a * __frcp_rn((float)b));
-  const int r = a - q * b;
-  if (r < 0) --q;
-  if (r >= b) ++q;
-  return q;
-}
-
 // The keys that a tile of query rows sees: those that some row does [lo, hi), those that all do [seen_lo, seen_hi).
 struct Span {
   int lo, hi, seen_lo, seen_hi, first_slice;

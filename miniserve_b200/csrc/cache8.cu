@@ -252,7 +252,7 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
   int b[READ_EACH][2];
 #pragma unroll
   for (int i = 0; i < READ_EACH; ++i) {
-    const int piece = min(first + i * threads, pieces - 1), h = piece / eights, c = piece - h * eights;  // (the last one again, unused)
+    const int piece = min(first + i * threads, pieces - 1), h = div_small(piece, eights), c = piece - h * eights;  // (the last one again, unused)
     const size_t at = at0 + ((size_t)h << page_shift);
     raw[i][0] = *reinterpret_cast<const uint2*>(k_codes + at * d + c * 8);
     raw[i][1] = *reinterpret_cast<const uint2*>(v_codes + at * d + c * 8);
@@ -330,7 +330,7 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
   int b8[READ_EACH][2];
 #pragma unroll
   for (int i = 0; i < READ_EACH; ++i) {
-    const int idx = min(idx0 + 256 * i, pieces - 1), row = idx / eights;  // (the last one again, unused)
+    const int idx = min(idx0 + 256 * i, pieces - 1), row = div_small(idx, eights);  // (the last one again, unused)
     const size_t at = (from * eights + idx) * 8;
     raw[i][0] = *reinterpret_cast<const uint2*>(k_codes + at);
     raw[i][1] = *reinterpret_cast<const uint2*>(v_codes + at);
@@ -459,6 +459,7 @@ MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, const void* k
   MS_CHECK_ARG(first >= 0 && rows > first && entries > 0, "cache8_unpack: rows %d to %d, %d entries", first, rows, entries);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_unpack: tensors must be 16-byte aligned");
+  MS_CHECK_ARG((long long)nkv * page_size <= 1 << 20, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   const int blocks = ceil_div(nkv * page_size * (d / 8), 256 * READ_EACH);
   MS_CHECK_ARG(blocks <= 65535, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, (const uint8_t*)k_codes, (const uint8_t*)k_exps,

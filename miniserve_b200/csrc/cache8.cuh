@@ -51,6 +51,15 @@ __device__ __forceinline__ uint32_t c8_half2_hi(uint32_t w) {
 }
 __device__ __forceinline__ float2 c8_float2(uint32_t half2) { return __half22float2(*reinterpret_cast<const __half2*>(&half2)); }
 
+// a / b of whole numbers, quotients below 2^20: a multiplication by the reciprocal, off by one at most, put right
+__device__ __forceinline__ int div_small(int a, int b) {
+  int q = (int)((float)a * __frcp_rn((float)b));
+  const int r = a - q * b;
+  if (r < 0) --q;
+  if (r >= b) ++q;
+  return q;
+}
+
 inline int c8_page_shift(int page_size) {
   int s = 0;
   while ((1 << s) < page_size) ++s;
