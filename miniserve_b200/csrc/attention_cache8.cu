@@ -153,6 +153,7 @@ struct Split8 {
   float scale;
   int num_pages;
   int behind;               // the second kernel runs: an item may be cut
+  int ahead;                // the tables above, and the keys and values of tokens before the step's, were in place before the step's first kernel: read ahead of the wait
 };
 
 // The keys that a tile of query rows sees: those that some row does [lo, hi), those that all do [seen_lo, seen_hi).
@@ -202,7 +203,8 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int *cu_q = p.cu_q, *q_start = p.q_start, *page_indptr = p.page_indptr, *page_indices = p.page_indices;
   if (tid < WARPS) joint[tid].last_warp = 0;
-  pdl_prologue(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
+  pdl_launch_dependents();
+  if (!p.ahead) pdl_wait(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
 
   const int group = div_small(p.nq, p.nkv), units = p.rows * p.tiles;
   // ---- where every tile's slices begin: a scan over the tiles, in order
@@ -293,25 +295,13 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     }
     return a;
   };
-  if (tid == 0 && !p.behind && !alone && total > 0) atomicExch(p.status, 2);  // (other lengths than the host said)
-  if (tid == 0 && p.behind) {
-    int4 cut = make_int4(0, 0, 0, 0);
-    if (cta_begin < cta_end && !alone) {
-      const Unit& u = table[find(cta_end - 1)];
-      const int kvh = div_small(cta_end - 1 - u.at, u.stride), at = u.at + kvh * u.stride;
-      // the item that goes on behind the CTA's end, where it began in this CTA
-      if (at >= cta_begin && at + u.n > cta_end) cut = make_int4(u.tok0 * group + u.row0, u.rows_here, kvh, (at + u.n - 1) / (each * WARPS) - (int)blockIdx.x + 1);
-    }
-    p.cut[blockIdx.x] = cut;
-  }
-
   const uint32_t ring = smem_addr(smem) + warp * STAGES * STAGE_BYTES;
   float* heads = reinterpret_cast<float*>(smem + WARPS * STAGES * STAGE_BYTES);  // [warps][part_rows][PART]: of items that began before the warp's run
   float* tail = reinterpret_cast<float*>(smem + warp * STAGES * STAGE_BYTES);    // of the one that goes on behind it: the ring is done with by then
   const int page_shift = 31 - __clz(p.page_size);
 
   // ---- what is asked for. Pages are looked up 32 at a time, a lane each, and the next 32 while these are used.
-  int a_pos = begin, a_left = 0, a_unit = find(begin), a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_table = 0, a_entries = 0;
+  int a_pos = begin, a_left = 0, a_unit = find(begin), a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_old = 0, a_table = 0, a_entries = 0;
   int window = 0, page_ahead = 0, page_row = 0;  // the first of the 32 table entries; the lane's page of the next ones; the pool's row at which its page of these begins
   const int first_unit = a_unit;
   auto page_of = [&](int entry) {
@@ -341,6 +331,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
       } else {
         a_lo = u.keys.lo;
         a_hi = u.keys.hi;
+        a_old = u.start;
         a_key = (u.keys.first_slice + off) * SLICE;
         a_table = u.table;
         a_entries = u.entries;
@@ -400,9 +391,26 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     cp_async_commit();
   };
   next_item();
+  int filled = 0;  // stages asked for
+  if (p.ahead) {
+    // slices of tokens before the step's; the others, and the queries, come from the kernels before this one
+#pragma unroll 1
+    for (; filled < STAGES && a_left > 0 && a_key + SLICE <= a_old; ++filled) fire(ring + filled * STAGE_BYTES);
+    pdl_wait(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
+  }
+  if (tid == 0 && !p.behind && !alone && total > 0) atomicExch(p.status, 2);  // (other lengths than the host said)
+  if (tid == 0 && p.behind) {
+    int4 cut = make_int4(0, 0, 0, 0);
+    if (cta_begin < cta_end && !alone) {
+      const Unit& u = table[find(cta_end - 1)];
+      const int kvh = div_small(cta_end - 1 - u.at, u.stride), at = u.at + kvh * u.stride;
+      // the item that goes on behind the CTA's end, where it began in this CTA
+      if (at >= cta_begin && at + u.n > cta_end) cut = make_int4(u.tok0 * group + u.row0, u.rows_here, kvh, (at + u.n - 1) / (each * WARPS) - (int)blockIdx.x + 1);
+    }
+    p.cut[blockIdx.x] = cut;
+  }
 
   // ---- what is computed
-  bool filled = false;
   int unit = first_unit, kvh = 0, item_end = begin, item_begin = 0;
   int start = 0, row0 = 0, rows_here = 0, tok0 = 0, n = 0;
   Span it = {};
@@ -446,11 +454,9 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
           if (i < rows_here) raw[j][kk] = *reinterpret_cast<const uint2*>(src + channel_of(kk, t));
         }
       }
-      if (!filled) {  // (the first copies go out while the first queries are on their way)
+      // (the first copies go out while the first queries are on their way)
 #pragma unroll 1
-        for (int i = 0; i < STAGES; ++i) fire(ring + i * STAGE_BYTES);
-        filled = true;
-      }
+      for (; filled < STAGES; ++filled) fire(ring + filled * STAGE_BYTES);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         uint32_t bits = 0;

@@ -50,6 +50,9 @@ class StepContext:
     # launches depend on how the step's tokens are shared among rows hands itself to ``recorder.defer``
     # instead of launching; it is then called with each later step's context, between the graphs.
     recorder: object | None = None
+    # Who makes the context says so: the tables above, and the cache of all tokens before this step's, are in place before the step's first kernel starts (behind
+    # a copy, say, which kernels do not start ahead of). A kernel may then read them while the kernels before it in the step still run.
+    tables_ahead: bool = False
     layout: tuple = ()  # where each field starts in the arena (a replayed graph checks it has not moved)
 
     def buffer(self, role: str, shape: tuple, dtype: torch.dtype, device) -> torch.Tensor:

@@ -222,7 +222,7 @@ class StepFunction:
             max_q_len=max(int(q_len.max()), pad_len if pad_rows else 1), max_kv_len=max(int(kv_end.max()), pad_len if pad_rows else 1),
             decode_only=bool((q_len == 1).all()),
             leading_single_rows=_leading_ones(q_len, pad_rows, pad_len), sm_count=self.sm_count, scratch=self.persistent_scratch,
-            layout=tuple(o))
+            tables_ahead=True, layout=tuple(o))
 
     def reset_after_fault(self) -> None:
         """After a kernel raised the status word: wait for what is in flight, then zero the word and

@@ -95,7 +95,7 @@ class _Split(ctypes.Structure):
     """``Split8`` of csrc/attention_cache8.cu."""
 
     _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part", "cut")] + [
-        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i), ("behind", _i)]
+        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i), ("behind", _i), ("ahead", _i)]
 
 
 class _AttnLib:
@@ -263,7 +263,7 @@ def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:
                 whole = fixed and rows * here * nkv <= ctas and _alone(ctx, lib, range(first, first + rows), range(tile0, tile0 + here), tile_rows, nq // nkv, nkv, window)
                 plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, here, nq, nkv, window, sink, page_size, ctas, scale, pages,
-                              not whole)
+                              not whole, bool(getattr(ctx, "tables_ahead", False)))
                 out.append((plan, ctypes.addressof(plan), tile_rows, most, 1 if whole else 2))
     return out
 

@@ -420,6 +420,27 @@ def test_prompts_behind_long_contexts_of_shapes_that_share_out_keys(nq, nkv, d, 
     _close(pb, q, out, 0.1)
 
 
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 8, 128, 16), (8, 2, 64, 8), (4, 1, 256, 16)])
+@pytest.mark.parametrize("rows", [[(0, 1)], [(2047 + 3 * i, 1) for i in range(8)], [(100, 5), (731, 5), (0, 5)], [(31, 1), (32, 1), (33, 1), (5000, 1)]])
+@pytest.mark.parametrize("window", [None, 40])
+def test_tables_and_older_tokens_ahead_of_the_kernels_before(nq, nkv, d, page, rows, window):
+    """A context that says so (everything is in place: the device has been waited for) gets the same bits, behind a write of the step's own tokens too."""
+    pb = cu.Batch8(rows, page, nkv, d, seed=len(rows))
+    qkv, _ = _projection(pb.num_tokens, nq, nkv, d, 3)
+    outs = []
+    for ahead in (False, True):
+        k8, v8 = (ops.Pool8(p.codes.clone(), p.exponents.clone()) for p in (pb.k8, pb.v8))
+        ctx = ku.make_context(pb)
+        ctx.tables_ahead = ahead
+        q, out = (torch.full((pb.num_tokens, nq, d), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            ops.qk_norm_rope_kv(q, k8, v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+            ops.attention(out, q, k8, v8, ctx, 0, 0.1, window)
+        outs.append(out)
+    assert torch.equal(*outs) and bool(outs[0].isfinite().all()) and pb.status.item() == 0
+
+
 @pytest.mark.parametrize("rows", [[(5000, 1), (3, 1), (700, 1)], [(900, 90), (0, 33)]])
 def test_two_contexts_on_two_streams(rows):
     """At once, each with scratch of its own: the bits of a call alone."""
