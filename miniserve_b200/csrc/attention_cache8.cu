@@ -42,7 +42,7 @@ constexpr int SLICE = 32, ROWS = 8 * MOST_NT;         // keys of a slice; the mo
 constexpr int ROW_BYTES = D % 64 == 0 ? D : D + 16;
 constexpr int CODE_BYTES = SLICE * ROW_BYTES, STAGE_BYTES = 2 * CODE_BYTES + 2 * SLICE;  // K codes, V codes, K exponents, V exponents
 // Warps of a CTA and stages of a warp's ring: one stage is worked on, the others are on their way. Head size 128, 64 requests of 1,024 to 3,985 keys: 7 warps of 3 stages
-// 65.0 us, 8 of 2 61.9, 8 of 3 66.1, 9 of 2 65.1.
+// 65.0 us, 8 of 2 61.9, 8 of 3 66.1, 9 of 2 65.1; 12 of 3 with slices of 16 keys 65.0 where 8 of 2 with 32 take 60.7.
 constexpr int warps_of(int) { return D > 128 ? 4 : 8; }
 constexpr int stages_of(int) { return D > 64 ? 2 : 4; }
 constexpr int PART = D + 4;                          // floats of a row's partial: o, m, l, c (and one that keeps rows on 16 bytes)
