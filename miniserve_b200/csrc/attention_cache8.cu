@@ -152,7 +152,7 @@ struct Split8 {
   int nq, nkv, window, sink, page_size, ctas;
   float scale;
   int num_pages;
-  int behind;               // the second kernel runs: an item may be cut
+  int behind;               // the second kernel runs: an item may be cut. 0 only where kv heads x rows x tiles are no more than CTAs
   int ahead;                // the tables above, and the keys and values of tokens before the step's, were in place before the step's first kernel: read ahead of the wait
 };
 
@@ -263,9 +263,10 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
       live += scan[1][w];
       longest = max(longest, scan[2][w]);
     }
-    // Few items, none much longer than an equal share: a CTA each, whole, so that nothing is left to add up behind.
+    // Few items, none much longer than an equal share: a CTA each, whole, so that nothing is left to add up behind. (Without the second kernel always: there are
+    // no more items than CTAs then, whatever the lengths have become since the host looked at them.)
     const int longest_each = (longest + WARPS - 1) / WARPS, equal_each = (total * p.nkv + p.ctas * WARPS - 1) / (p.ctas * WARPS);
-    const int alone = live * p.nkv <= p.ctas && longest_each <= alone_most(equal_each) ? longest_each * WARPS : 0;
+    const int alone = !p.behind || (live * p.nkv <= p.ctas && longest_each <= alone_most(equal_each)) ? longest_each * WARPS : 0;
     if (alone) total = live * alone;
     for (int u = first; u < min(first + each, units); ++u) {
       if (each > 1) unit_of(u);
@@ -398,7 +399,6 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     for (; filled < STAGES && a_left > 0 && a_key + SLICE <= a_old; ++filled) fire(ring + filled * STAGE_BYTES);
     pdl_wait(q, k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
   }
-  if (tid == 0 && !p.behind && !alone && total > 0) atomicExch(p.status, 2);  // (other lengths than the host said)
   if (tid == 0 && p.behind) {
     int4 cut = make_int4(0, 0, 0, 0);
     if (cta_begin < cta_end && !alone) {
@@ -948,6 +948,7 @@ MS_EXPORT int MS_ATTN8_FN(split)(const Split8* p, int tile_rows, int rows_most, 
   MS_CHECK_ARG(p->rows > 0 && p->tiles > 0 && (long long)p->rows * p->tiles <= MAX_UNITS, "attention: %d rows of %d tiles are too many for one launch", p->rows, p->tiles);
   MS_CHECK_ARG(p->ctas > 0 && p->part && p->cut && tile_rows > 0 && tile_rows <= ROWS && tile_rows % 8 == 0 && rows_most > 0, "attention: %d CTAs need scratch memory, tiles %d rows of %d",
                p->ctas, tile_rows, rows_most);
+  MS_CHECK_ARG(p->behind || (long long)p->rows * p->tiles * p->nkv <= p->ctas, "attention: %d rows of %d tiles and %d kv heads are cut", p->rows, p->tiles, p->nkv);
   const long long pool_rows = (long long)p->num_pages * p->nkv * p->page_size;
   MS_CHECK_ARG(pool_rows > 0 && pool_rows < (1LL << 31), "attention: pools of %lld rows", pool_rows);
   MS_CHECK_ARG((uintptr_t)q % 8 == 0 && (uintptr_t)out % 8 == 0 && (uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_exps % 8 == 0 &&

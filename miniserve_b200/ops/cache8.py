@@ -224,8 +224,8 @@ def _workspace(ctx, floats: int, device) -> torch.Tensor:
 
 
 def _alone(ctx, lib: _AttnLib, rows: range, tiles: range, tile_rows: int, heads: int, nkv: int, window: int) -> bool:
-    """Whether the kernel gives every item (tile of query rows of a request, and kv head) a CTA of its own, as it will find by the same rule: then none
-    is cut."""
+    """Whether the kernel would give every item (tile of query rows of a request, and kv head) a CTA of its own, by its own rule: then none is cut, and the second
+    kernel need not run."""
     if len(ctx.host_q_len) < rows.stop:
         return False
     total = longest = 0
@@ -304,14 +304,15 @@ def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
 #     1 request behind 2,000 tokens                                                                      26/34   26/34   28/36   34/40
 #     16 behind 2,000                                                                                    75/93   99/93  126/89  226/101
 #     1 behind 32,000                                                                                    65/108  87/108 108/108 191/116
-#   others, unpacked for the mma.sync kernel (64 queries a CTA, which walks all their keys), by new tokens of a request:
-#     head size 64, 8 heads a kv head, 4 requests behind 8,000 tokens     32: 79/486   128: 243/488   512: 952/1402
-#                                      4 behind 500                       32: 28/46    128: 52/52     512: 214/157   1,024: 454/345
-#                                      8 from the beginning               32: 28/22    128: 77/32     512: 360/134
-#     head size 80, 2 heads a kv head, 4 behind 3,000                     32: 38/230   512: 282/447   2,048: 1322/1426
-#                                      8 from the beginning               32: 24/24    512: 159/97    2,048: 1372/804
-# So up to SPLIT_ROWS query rows always share out keys; beyond, the tcgen05 kernel takes what it takes, and of other shapes the mma.sync kernel those steps with no more keys behind
-# them than new tokens.
+#   others, unpacked for the mma.sync kernel (64 query rows a CTA, which walks all their keys), by new tokens of a request:
+#     head size 64, 8 heads a kv head, 4 requests behind 3,000 tokens     32: 43/190   128: 111/197   1,024: 919/1034
+#                                      4 behind 500                       32: 25/45    128: 49/51     512: 203/156   1,024: 436/344
+#                                      8 from the beginning               64: 31/20    128: 63/31     512: 315/131
+#     head size 64, 1 head a kv head, 1 from the beginning                512: 31/37   4,096: 313/414;   8 so  512: 86/86   4,096: 2325/2387
+#     head size 80, 2 heads a kv head, 1 from the beginning               512: 33/43   2,048: 121/156;   8 so  512: 115/96  2,048: 917/801;   4 behind 3,000  512: 278/446
+#     head size 256, 4 heads a kv head, 1 from the beginning              256: 20/31   1,024: 72/96;     8 so  256: 92/70   1,024: 585/436;   4 behind 3,000  256: 242/293
+# So up to SPLIT_ROWS query rows always share out keys. Beyond, the tcgen05 kernel takes what it takes. Of other shapes the mma.sync kernel takes steps with no more keys behind them
+# than new tokens where 8 heads and more share a kv head, or where 2 and more do and 4 requests and more come: it has many CTAs then, of few keys each.
 SPLIT_ROWS = 96
 UNPACKED_BYTES = 1 << 30  # of pages unpacked at a time, unless a single request has more
 
@@ -320,7 +321,10 @@ def _shares_out(q, k_pool: Pool8, ctx, first: int) -> bool:
     """Whether rows [first, num_rows), some of more than SPLIT_ROWS query rows, go to the kernel that shares out keys."""
     from . import attention_tc_ok  # (this module is imported by theirs)
 
-    key = ("cache8_shares_out", first)
+    rows, heads = ctx.num_rows - first, q.shape[1] // k_pool.sizes[1]
+    if not (heads >= 8 or (heads >= 2 and rows >= 4)):
+        return not attention_tc_ok(q, k_pool)
+    key = ("cache8_more_behind", first)
     more_behind = ctx.step_cache.get(key)
     if more_behind is None:
         more_behind = ctx.step_cache[key] = sum(ctx.host_q_start[first:ctx.num_rows]) > sum(ctx.host_q_len[first:ctx.num_rows])

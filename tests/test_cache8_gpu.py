@@ -460,6 +460,35 @@ def test_two_contexts_on_two_streams(rows):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_lengths_that_change_on_the_device_alone(captured):
+    """Single tokens go by the lengths on the device: a call (or a graph of one) whose context was first used for short rows serves long ones, and the other way round."""
+    pb = cu.Batch8([(1900, 1), (1500, 1)], 16, 2, 128, seed=8)
+    for first in ((60, 30), (1900, 1500)):
+        ctx = ku.make_context(pb)
+        ctx.host_q_start, ctx.max_kv_len = list(first), max(first) + 1
+        ctx.q_start.copy_(torch.tensor(first, dtype=torch.int32))
+        pb.rows = [(s, 1) for s in first]
+        q, out = _attend(pb, 8, 128, 0.1, ctx=ctx)
+        _close(pb, q, out, 0.1)
+        graph = torch.cuda.CUDAGraph()
+        if captured:
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                ctx.stream = torch.cuda.current_stream().cuda_stream
+                ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+        for now in ((1900, 1500), (12, 1499), (0, 3)):
+            ctx.q_start.copy_(torch.tensor(now, dtype=torch.int32))
+            pb.rows = [(s, 1) for s in now]
+            out.fill_(float("nan"))
+            if captured:
+                graph.replay()
+            else:
+                ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+            torch.cuda.synchronize()
+            _close(pb, q, out, 0.1)
+
+
 @pytest.mark.parametrize("rows", [[(900, 1), (37, 1)], [(300, 70), (15, 40)]])
 def test_a_step_s_stream_that_is_not_the_current_one(rows):
     """``ctx.stream`` says where the kernels go; what they need is made there too."""
@@ -492,6 +521,46 @@ def test_a_captured_prompt_outlives_larger_ones():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(8, 1, 64, 16), (4, 2, 80, 8), (4, 1, 256, 32), (8, 4, 128, 16), (2, 1, 128, 256)])
+@pytest.mark.parametrize("window,sink", [(None, False), (50, True)])
+def test_prompts_over_unpacked_pages(nq, nkv, d, page, window, sink):
+    """Prompts that bring more than lies behind them, the unpacked pages beginning as NaN where they are not written; again with other prompts in the same scratch."""
+    for _ in range(3):
+        torch.full((1 << 24,), float("nan"), dtype=torch.bfloat16, device=DEV)  # (given back at once: the next allocations get it)
+    scratch = {}
+    for seed, rows in enumerate(([(9, 1), (100, 200), (0, 33), (60, 129), (5, 64)], [(0, 128), (1, 100), (130, 300), (0, 0), (2, 97)])):
+        pb = cu.Batch8(rows, page, nkv, d, seed=seed)
+        if window:
+            for r, (s, n) in enumerate(rows):
+                passed = max(0, s - window + 1) // page
+                pb.page_indices[int(pb.page_indptr[r]):int(pb.page_indptr[r]) + passed] = -1
+        ctx = ku.make_context(pb)
+        ctx.scratch = scratch
+        q, out = _attend(pb, nq, d, 0.1, window, sink, ctx=ctx)
+        assert "cache8_pages" in scratch
+        _close(pb, q, out, 0.1, window, sink)
+
+
+def test_a_captured_prompt_over_unpacked_pages_outlives_larger_ones():
+    pb, other = cu.Batch8([(30, 170), (0, 200)], 16, 2, 64, seed=8), cu.Batch8([(300, 2000)], 16, 2, 64, seed=9)
+    ctx = ku.make_context(pb)
+    q, want = _attend(pb, 16, 64, 0.1, ctx=ctx)
+    out, graph = torch.full_like(q, float("nan")), torch.cuda.CUDAGraph()
+    ctx.step_cache.clear()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ctx.stream = torch.cuda.current_stream().cuda_stream
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    larger = ku.make_context(other)
+    larger.scratch = ctx.scratch
+    for _ in range(2):
+        _close(other, *_attend(other, 16, 64, 0.1, ctx=larger), 0.1)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and "cache8_pages" in ctx.scratch
 
 
 def test_pages_beyond_4_gb():
