@@ -268,28 +268,30 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
   }
 }
 
-// The pages that rows [first, rows) of a step need, as bfloat16 pages of their own: the rows' needed pages, counted through, become pages 0, 1, ..., and ids[f] says so of entry f of
-// the table (which may list more pages than a row needs). Pages that no query of their row looks at (ahead of a window) are left as they were. What is done to a value vector that is not
+// The pages that rows [first, rows) of a step look at, as bfloat16 pages of their own, and the tables that say so: a row's pages from the first that its window reaches (page 0 without one)
+// to the last that holds a token, counted through all rows, become pages 0, 1, ... of k_out and v_out; indptr_out[r] + entry is where entry `entry` of row r's table now lies in ids, and
+// ids[i] = i. So what the products behind this look up lies in [0, gridDim.x) whatever the step's own table is like: its rows may begin ahead of the table or inside one
+// another, where a window has given pages back. A page that the table or the pool does not have becomes zeros. What is done to a value vector that is not
 // finite is done for the products that follow, which weigh what a query does not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself
-// zero. Block (needed page, share of it), READ_EACH pieces of 8 numbers of K and V a thread; every warp finds the page's row for itself, 32 rows a look.
+// zero. Block (page, share of it), READ_EACH pieces of 8 numbers of K and V a thread; every warp finds the page's row for itself, 32 rows a look.
 __global__ void __launch_bounds__(256)
-cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, const uint8_t* __restrict__ k_codes,
+cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, int* __restrict__ indptr_out, const uint8_t* __restrict__ k_codes,
                      const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ cu_q,
                      const int* __restrict__ q_start, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int first, int rows, int nkv, int d, int window,
-                     int page_shift, int num_pages, int num_ids, int* __restrict__ status) {
+                     int page_shift, int num_pages, int num_entries, int* __restrict__ status) {
   pdl_prologue(k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
   const int out_page = blockIdx.x, page_size = 1 << page_shift, lane = threadIdx.x & 31;
-  int a = -1, entry = out_page, start = 0, hi = 0, table = 0, listed = 0;  // the row, which of its pages, its first new token and its end, its place in the table
+  int a = -1, entry = out_page, left = 0, ahead = 0, table = 0, listed = 0;  // the row, which of its pages, how many there are behind it, the row's first, its place in the table
   for (int r0 = first; r0 < rows; r0 += 32) {
     const int r = r0 + lane;
-    int from = 0, end = 0, at = 0, n = 0;
+    int need = 0, passed = 0, at = 0, n = 0;
     if (r < rows) {
-      from = q_start[r];
-      end = from + cu_q[r + 1] - cu_q[r];
+      const int from = q_start[r], tokens = cu_q[r + 1] - cu_q[r];
+      passed = window > 0 ? max(0, from - window + 1) >> page_shift : 0;
+      if (tokens > 0) need = max(0, ((from + tokens + page_size - 1) >> page_shift) - passed);
       at = page_indptr[r];
       n = page_indptr[r + 1] - at;
     }
-    const int need = (end + page_size - 1) >> page_shift;
     int incl = need;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -300,32 +302,30 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
     if (behind) {
       const int src = __ffs(behind) - 1;
       a = r0 + src;
+      left = __shfl_sync(0xffffffffu, incl, src) - entry - 1;
       entry -= __shfl_sync(0xffffffffu, incl - need, src);
-      start = __shfl_sync(0xffffffffu, from, src);
-      hi = __shfl_sync(0xffffffffu, end, src);
+      ahead = __shfl_sync(0xffffffffu, passed, src);
       table = __shfl_sync(0xffffffffu, at, src);
       listed = __shfl_sync(0xffffffffu, n, src);
       break;
     }
     entry -= __shfl_sync(0xffffffffu, incl, 31);
   }
+  const bool leads = blockIdx.y == 0 && threadIdx.x == 0;
+  if (leads) ids[out_page] = out_page;
   if (a < 0) return;
-  const int f = table + entry;
-  if (entry >= listed || f >= num_ids) {  // (the products behind this trust the tables: one that is too short is found here)
-    atomicExch(status, 2);
-    return;
+  if (leads && entry == 0) indptr_out[a] = out_page - ahead;
+  if (leads && blockIdx.x == gridDim.x - 1) {  // rows that look at more pages than the launch was made for
+    for (int r = a + 1; r < rows && left == 0; ++r) left = cu_q[r + 1] - cu_q[r];
+    if (left != 0) atomicExch(status, 2);
   }
-  if (blockIdx.y == 0 && threadIdx.x == 0) ids[f] = out_page;
   const int eights = d >> 3, pieces = nkv * page_size * eights, idx0 = blockIdx.y * (256 * READ_EACH) + threadIdx.x;
   if (idx0 >= pieces) return;
-  const int key = entry << page_shift, lo = window > 0 ? max(0, start - window + 1) : 0;
-  if (key + page_size <= lo || key >= hi) return;
-  const int page = page_indices[f];
-  if ((unsigned)page >= (unsigned)num_pages) {
-    atomicExch(status, 2);
-    return;
-  }
-  const size_t from = (size_t)page * nkv * page_size, to = (size_t)out_page * pieces;
+  const int e = ahead + entry, f = table + e;
+  const int page = e < listed && f >= 0 && f < num_entries ? page_indices[f] : -1;
+  const bool there = (unsigned)page < (unsigned)num_pages;
+  if (!there && threadIdx.x == 0) atomicExch(status, 2);
+  const size_t from = (size_t)(there ? page : 0) * nkv * page_size, to = (size_t)out_page * pieces;
   uint2 raw[READ_EACH][2];
   int b8[READ_EACH][2];
 #pragma unroll
@@ -336,6 +336,10 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
     raw[i][1] = *reinterpret_cast<const uint2*>(v_codes + at);
     b8[i][0] = k_exps[from + row];
     b8[i][1] = v_exps[from + row];
+    if (!there) {
+      raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
+      b8[i][0] = b8[i][1] = 0;
+    }
   }
 #pragma unroll
   for (int i = 0; i < READ_EACH; ++i) {
@@ -450,10 +454,11 @@ MS_EXPORT int ms_cache8_read(const Read8* args) {
   return 0;
 }
 
-// Rows [first, rows) need `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; ids has num_ids numbers.
-MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,
+// Rows [first, rows) look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [entries] and, by row, indptr_out. page_indices has
+// num_entries entries.
+MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, int* indptr_out, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,
                                const int* q_start, const int* page_indptr, const int* page_indices, int first, int rows, int entries, int nkv, int d, int window, int page_size,
-                               long long num_pages, int num_ids, int* status, cudaStream_t stream) {
+                               long long num_pages, int num_entries, int* status, cudaStream_t stream) {
   if (entries == 0) return 0;
   if (int rc = c8_check("cache8_unpack", nkv, d, page_size, num_pages)) return rc;
   MS_CHECK_ARG(first >= 0 && rows > first && entries > 0, "cache8_unpack: rows %d to %d, %d entries", first, rows, entries);
@@ -462,8 +467,8 @@ MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, const void* k
   MS_CHECK_ARG((long long)nkv * page_size <= 1 << 20, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   const int blocks = ceil_div(nkv * page_size * (d / 8), 256 * READ_EACH);
   MS_CHECK_ARG(blocks <= 65535, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
-  MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
+  MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, indptr_out, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
             (const uint8_t*)v_codes, (const uint8_t*)v_exps, cu_q, q_start, page_indptr, page_indices, first, rows, nkv, d, window, c8_page_shift(page_size), (int)num_pages,
-            num_ids, status);
+            num_entries, status);
   return 0;
 }

@@ -80,7 +80,7 @@ def _cache_lib():
     native._declare(lib, "ms_cache8_set_pdl", [_i], None)
     native._declare(lib, "ms_cache8_write", [c_char_p])
     native._declare(lib, "ms_cache8_read", [c_char_p])
-    native._declare(lib, "ms_cache8_unpack", [_p] * 11 + [_i] * 7 + [_ll, _i, _p, _p])
+    native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 7 + [_ll, _i, _p, _p])
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
 
@@ -332,41 +332,41 @@ def _shares_out(q, k_pool: Pool8, ctx, first: int) -> bool:
 
 
 class _Unpacked:
-    """A step's context whose pages of one group are the unpacked ones: rows [first, num_rows)."""
+    """A step's context whose pages of one group are the unpacked ones, by tables of their own: rows [first, num_rows)."""
 
-    def __init__(self, ctx, group: int, num_rows: int, ids: torch.Tensor):
+    def __init__(self, ctx, group: int, num_rows: int, indptr: torch.Tensor, ids: torch.Tensor):
         self.__dict__.update(ctx.__dict__)
         self.num_rows = num_rows
-        self.page_indices = list(ctx.page_indices)
-        self.page_indices[group] = ids
+        self.page_indptr, self.page_indices = list(ctx.page_indptr), list(ctx.page_indices)
+        self.page_indptr[group], self.page_indices[group] = indptr, ids
 
 
-def _parts(ctx, first: int, page_size: int, page_bytes: int) -> list:
-    """Rows [first, num_rows) in parts whose pages fit: ``(first row, row behind, pages)``."""
+def _parts(ctx, first: int, window: int, page_size: int, page_bytes: int) -> list:
+    """Rows [first, num_rows) in parts whose pages fit: ``(first row, row behind, pages)``. A row's pages begin with the first that its window reaches."""
     out, at, entries = [], first, 0
     for r in range(first, ctx.num_rows):
-        n = -(-(ctx.host_q_start[r] + ctx.host_q_len[r]) // page_size)
+        start, tokens = ctx.host_q_start[r], ctx.host_q_len[r]
+        n = -(-(start + tokens) // page_size) - (max(0, start - window + 1) // page_size if window else 0) if tokens else 0
         if entries and (entries + n) * page_bytes > UNPACKED_BYTES:
             out.append((at, r, entries))
             at, entries = r, 0
         entries += n
     out.append((at, ctx.num_rows, entries))
-    return out
+    return [x for x in out if x[2]]
 
 
-def _unpacked(ctx, numbers: int, table: int, device: torch.device) -> tuple:
-    """Pages of K and of V (``numbers`` each) and their places in a table of ``table`` entries, for steps that run one after the other; a capture gets its own. All
-    zero at first: the products behind may weigh, by zero, values of pages that were left out, which then have to be numbers; and what they read of a table behind
-    the end of one that is too short has to be a page that is there."""
+def _unpacked(ctx, numbers: int, ints: int, device: torch.device) -> tuple:
+    """Pages of K and of V (``numbers`` each) and ``ints`` entries of tables, for steps that run one after the other; a capture gets its own. What a launch reads of them it has
+    written before."""
     capturing = torch.cuda.is_current_stream_capturing()
     held = None if capturing else ctx.scratch.get("cache8_pages")
-    if held is not None and held[0].numel() >= numbers and held[2].numel() >= table:
+    if held is not None and held[0].numel() >= numbers and held[2].numel() >= ints:
         return held
     if held is not None:  # (a context grows portion by portion: twice as much the next time, up to what a step of several rows may take)
         numbers = max(numbers, min(2 * held[0].numel(), UNPACKED_BYTES // 4))
-        table = max(table, held[2].numel())
+        ints = max(ints, held[2].numel())
     with _on_stream(ctx, device):
-        new = tuple(torch.zeros(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (torch.zeros(table, dtype=torch.int32, device=device),)
+        new = tuple(torch.empty(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (torch.empty(ints, dtype=torch.int32, device=device),)
     if capturing:
         ctx.scratch.setdefault("retired", []).append(new)
     else:
@@ -374,28 +374,28 @@ def _unpacked(ctx, numbers: int, table: int, device: torch.device) -> tuple:
     return new
 
 
-def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool, first: int) -> None:
+def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, first: int) -> None:
     """Rows [first, num_rows) of the step over pages unpacked to bfloat16."""
     from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
 
     pages, nkv, page_size, d = k_pool.sizes
-    key = ("cache8_unpacked", group, first, nkv, page_size, d)
+    key = ("cache8_unpacked", group, first, nkv, page_size, d, window)
     parts = ctx.step_cache.get(key)
     if parts is None:
         _check_tables(k_pool.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
         page = nkv * page_size * d
-        parts = _parts(ctx, first, page_size, 4 * page)
-        most = max(n for _, _, n in parts)
-        # (behind the table's own entries: what a row whose table is too short reads)
-        *pools, ids = _unpacked(ctx, most * page, ctx.page_indices[group].numel() + sum(n for _, _, n in parts), k_pool.device)
+        parts = _parts(ctx, first, window, page_size, 4 * page)
+        most = max((n for _, _, n in parts), default=0)
+        *pools, tables = _unpacked(ctx, most * page, ctx.num_rows + 1 + most, k_pool.device)
         k, v = (x[:most * page].view(most, nkv, page_size, d) for x in pools)
-        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, ids)) for a, b, n in parts])
+        indptr, ids = tables[:ctx.num_rows + 1], tables[ctx.num_rows + 1:ctx.num_rows + 1 + most]
+        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids)) for a, b, n in parts])
     k, v, parts = parts
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(
-            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(), ctx.q_start.data_ptr(),
-            ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, entries, nkv, d, window, page_size, pages,
-            view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), view.page_indptr[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(),
+            ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, entries, nkv, d, window, page_size, pages,
+            ctx.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
         if attention_tc_ok(q, k):
             attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
         else:

@@ -2,8 +2,10 @@
 
 from __future__ import annotations
 
+import ctypes
 import math
 
+import numpy as np
 import torch
 
 from miniserve_b200 import ops
@@ -102,3 +104,49 @@ def attention64(q, k, v, q_positions, scale, window=None, sink=False):
         vh = torch.where(seen.any(0)[:, None], v[:, h // group], 0.0)
         out[:, h], mass[:, h] = p @ vh, p @ vh.abs()
     return out, mass
+
+
+def packed_tables(rows, page: int, window, tables) -> tuple[list, list]:
+    """``page_indptr`` and ``page_indices`` as the engine's packer lays them out for rows (start, q_len) of a group with ``window``: pages that the window had passed when the step began were
+    given back. ``tables``: the pages of every row, from position 0 on."""
+    from miniserve_b200.cache import BlockAllocator
+    from miniserve_b200.ops import native
+
+    alloc = BlockAllocator(sum(len(t) for t in tables) + 1, page)
+    held, name = [], {}
+    for s, n in rows:
+        t = alloc.new_table()
+        t.append_tokens(s)
+        if window:
+            t.release_below(s - window + 1)
+        t.append_tokens(n)
+        held.append(t)
+    for t, pages in zip(held, tables):
+        for block, p in zip(t.blocks, pages):
+            if block >= 0:
+                assert block not in name
+                name[block] = p
+    arr = lambda x: np.asarray(x, dtype=np.int32)  # noqa: E731
+    count, total = len(rows), sum(n for _, n in rows)
+    arena, offsets = np.zeros(8 * total + 64 * count + sum(len(t) for t in tables) + 256, dtype=np.int32), (ctypes.c_longlong * 11)()
+    handles = (ctypes.c_void_p * count)(*[t.handle for t in held])
+    qs, ql, ids, slots, want, pad = arr([s for s, _ in rows]), arr([n for _, n in rows]), arr([0] * total), arr([0] * count), arr([]), arr([0])
+    end = native.host().ms_pack_step(arena.ctypes.data, arena.size, offsets, count, 0, qs.ctypes.data, ql.ctypes.data, ids.ctypes.data, slots.ctypes.data, want.ctypes.data, 0, 1, handles,
+                                     pad.ctypes.data, 0, 0, 0, 1, page)
+    assert end > 0
+    indptr = arena[offsets[8]:offsets[8] + count + 1].tolist()
+    return indptr, [name.get(b, -1) for b in arena[offsets[9]:offsets[9] + indptr[-1]].tolist()]
+
+
+class Packed8(Batch8):
+    """Rows in the packer's layout for a group with ``window``: the pages that it has passed are not in the tables, and poison."""
+
+    def __init__(self, rows, page, kv_heads, d, window, seed=0):
+        super().__init__(rows, page, kv_heads, d, seed)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        indptr, indices = packed_tables(rows, page, window, self.tables)
+        self.page_indptr, self.page_indices = torch.tensor(indptr, **i32), torch.tensor(indices, **i32)
+        gone = sorted({p for t in self.tables for p in t} - set(indices))
+        for pool in (self.k8, self.v8):
+            pool.codes[gone] = 0x7F
+            pool.exponents[gone] = 255
