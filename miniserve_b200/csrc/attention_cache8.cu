@@ -143,8 +143,8 @@ __device__ __forceinline__ int channel_of(int kk, int t) {
 struct Split8 {
   const int* cu_q;          // [rows + 1]
   const int* q_start;       // [rows]
-  const int* page_indptr;   // [rows + 1]
-  const int* page_indices;
+  const int* page_indptr;   // [all_rows + 1]
+  const int* page_indices;  // [num_entries]
   int* status;
   float* part;              // [2 * ctas][ROWS][PART]: a CTA's partial of the item that began before it, and of the one that goes on behind it
   int4* cut;                // [ctas]: for the second kernel, of the cut item that begins in the CTA: its first query row (counted in tokens x heads of a kv head), rows, kv head, pieces; 0: none
@@ -153,6 +153,7 @@ struct Split8 {
   float scale;
   int num_pages;
   int behind;               // the second kernel runs: an item may be cut. 0 only where kv heads x rows x tiles are no more than CTAs
+  int all_rows, num_entries;  // page_indptr[all_rows] is where all rows' tables end
   int ahead;                // the tables above, and the keys and values of tokens before the step's, were in place before the step's first kernel: read ahead of the wait
 };
 
@@ -182,7 +183,7 @@ struct Unit {
   int at;                    // slices of all kv heads before it
   int n, stride;             // its slices of one kv head; how far apart its kv heads lie in the row of slices (n, or more: see `alone`)
   int tok0, start, row0, rows_here;
-  int table, entries;        // of its request in page_indices
+  int table, table_end;      // of its request in page_indices
   Span keys;
 };
 // An item that several warps of a CTA share.
@@ -215,11 +216,12 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     Unit mine;
     auto unit_of = [&](int u) {
       const int r = div_small(u, p.tiles);
-      const int tok_end = cu_q[r + 1], table_end = page_indptr[r + 1];
+      // (without a window a table is whole, and ends where the next begins; with one that says nothing: the step packer in csrc/host_core.cpp)
+      const int tok_end = cu_q[r + 1], table_end = page_indptr[p.window > 0 ? p.all_rows : r + 1];
       mine.tok0 = cu_q[r];
       mine.start = q_start[r];
       mine.table = page_indptr[r];
-      mine.entries = table_end - mine.table;
+      mine.table_end = min(table_end, p.num_entries);
       mine.row0 = (p.tile0 + u - r * p.tiles) * TILE_ROWS;
       const int rows_all = (tok_end - mine.tok0) * group;
       mine.rows_here = min(min(TILE_ROWS, part_rows), rows_all - mine.row0);  // (no more than there is room for)
@@ -302,13 +304,14 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
   const int page_shift = 31 - __clz(p.page_size);
 
   // ---- what is asked for. Pages are looked up 32 at a time, a lane each, and the next 32 while these are used.
-  int a_pos = begin, a_left = 0, a_unit = find(begin), a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_old = 0, a_table = 0, a_entries = 0;
+  int a_pos = begin, a_left = 0, a_unit = find(begin), a_kvh = 0, a_key = 0, a_lo = 0, a_hi = 0, a_old = 0, a_table = 0, a_table_end = 0;
   int window = 0, page_ahead = 0, page_row = 0;  // the first of the 32 table entries; the lane's page of the next ones; the pool's row at which its page of these begins
   const int first_unit = a_unit;
   auto page_of = [&](int entry) {
     const int key = entry << page_shift;
     if (key + p.page_size <= a_lo || key >= a_hi) return 0;  // (not needed: any page that is there)
-    return entry < a_entries ? page_indices[a_table + entry] : -1;
+    const int at = a_table + entry;
+    return at >= 0 && at < a_table_end ? page_indices[at] : -1;
   };
   auto turn = [&]() {  // to the entries looked up last
     int page = page_ahead;
@@ -335,7 +338,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
         a_old = u.start;
         a_key = (u.keys.first_slice + off) * SLICE;
         a_table = u.table;
-        a_entries = u.entries;
+        a_table_end = u.table_end;
         a_left = min(u.n - off, end - a_pos);
         window = a_key >> page_shift;
         page_ahead = page_of(window + lane);

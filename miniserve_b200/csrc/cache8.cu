@@ -10,23 +10,29 @@ namespace ms {
 
 constexpr int C8_MAX_D = 256;
 
-// The page of position `pos` of request `row`; -1 where the table has none, or none that the pool has.
-__device__ __forceinline__ int c8_page(const int* page_indptr, const int* page_indices, int row, int pos, int page_shift, int num_pages) {
-  const int first = page_indptr[row], n = page_indptr[row + 1] - first, entry = pos >> page_shift;
-  if (entry < 0 || entry >= n) return -1;
-  const int page = page_indices[first + entry];
-  return page < num_pages ? page : -1;
-}
+// A step's page tables: `rows` of them in page_indices [entries], entry 0 of row r at page_indptr[r]. Where a window gave pages back that place can lie ahead of the
+// tables or inside another row's entries (csrc/host_core.cpp, the step packer), so that neighbouring places do not tell a row's length: what bounds it is the end of all.
+struct Tables8 {
+  const int *page_indptr, *page_indices;
+  int rows, entries;
+  // The page of position `pos` of request `row`; negative where the tables have none, or none that the pool has.
+  __device__ __forceinline__ int page(int row, int pos, int page_shift, int num_pages) const {
+    if ((unsigned)row >= (unsigned)rows || pos < 0) return -1;
+    const int at = page_indptr[row] + (pos >> page_shift);
+    if (at < 0 || at >= min(page_indptr[rows], entries)) return -1;
+    const int page = page_indices[at];
+    return page < num_pages ? page : -1;
+  }
+};
 
 // A warp per (token, head).
 __global__ void __launch_bounds__(256)
 cache8_write_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_exps, uint8_t* __restrict__ v_codes,
                     uint8_t* __restrict__ v_exps, const __nv_bfloat16* __restrict__ qkv, const __nv_bfloat16* __restrict__ q_norm_w,
                     const __nv_bfloat16* __restrict__ k_norm_w, const float* __restrict__ inv_freq, const float* __restrict__ cos_sin,
-                    const int* __restrict__ positions, const int* __restrict__ row_of_token, const int* __restrict__ page_indptr,
-                    const int* __restrict__ page_indices, int num_tokens, int nq, int nkv, int d, int rot, float eps, int page_shift, int num_pages,
+                    const int* __restrict__ positions, const int* __restrict__ row_of_token, Tables8 tables, int num_tokens, int nq, int nkv, int d, int rot, float eps, int page_shift, int num_pages,
                     int* __restrict__ status) {
-  pdl_prologue(qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, page_indptr, page_indices);
+  pdl_prologue(qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, tables.page_indptr, tables.page_indices);
   __shared__ float held[8][C8_MAX_D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = nq + 2 * nkv;
   const long long item = (long long)blockIdx.x * 8 + warp;
@@ -68,7 +74,7 @@ cache8_write_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_c
     for (int c = lane; c < d; c += 32) dst[c] = __float2bfloat16_rn(x[c]);
     return;
   }
-  const int page = c8_page(page_indptr, page_indices, row_of_token[t], pos, page_shift, num_pages);
+  const int page = tables.page(row_of_token[t], pos, page_shift, num_pages);
   if (page < 0) {
     if (lane == 0) atomicExch(status, 2);
     return;
@@ -106,9 +112,8 @@ __global__ void __launch_bounds__(256, TABLE ? 4 : 1)
 cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ k_exps, uint8_t* __restrict__ v_codes,
                           uint8_t* __restrict__ v_exps, const __nv_bfloat16* __restrict__ qkv, const __nv_bfloat16* __restrict__ q_norm_w,
                           const __nv_bfloat16* __restrict__ k_norm_w, const float* __restrict__ inv_freq, const float* __restrict__ cos_sin,
-                          const int* __restrict__ positions, const int* __restrict__ row_of_token, const int* __restrict__ page_indptr,
-                          const int* __restrict__ page_indices, int nq, int nkv, float eps, int page_shift, int num_pages, int* __restrict__ status) {
-  pdl_prologue(qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, page_indptr, page_indices);
+                          const int* __restrict__ positions, const int* __restrict__ row_of_token, Tables8 tables, int nq, int nkv, float eps, int page_shift, int num_pages, int* __restrict__ status) {
+  pdl_prologue(qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, tables.page_indptr, tables.page_indices);
   constexpr int LPH = D / 8, HPW = 32 / LPH, HALF = D / 2, BATCH = 2;
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPH, slot = lane / LPH, j0 = sub * 4;
   const int heads = nq + 2 * nkv, stride = (int)(blockDim.x >> 5) * HPW;  // heads a pass
@@ -143,7 +148,7 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       for (int i = 0; i < 4; ++i) sincosf((float)pos * inv_freq[j0 + i], &sn[i], &cs[i]);
     }
   }
-  const int page = c8_page(page_indptr, page_indices, request, pos, page_shift, num_pages);
+  const int page = tables.page(request, pos, page_shift, num_pages);
   if (page < 0 && threadIdx.x == 0) atomicExch(status, 2);
   const size_t at0 = ((size_t)max(page, 0) * nkv << page_shift) + (pos & ((1 << page_shift) - 1));
   for (int base = 0; base < heads; base += BATCH * stride) {  // the same trips for every lane: they exchange sums
@@ -235,14 +240,13 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_exps,
                    const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ positions,
-                   const int* __restrict__ row_of_token, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int num_tokens,
-                   int nkv, int d, int page_shift, int num_pages, int* __restrict__ status) {
-  pdl_prologue(k_codes, k_exps, v_codes, v_exps, positions, row_of_token, page_indptr, page_indices);
+                   const int* __restrict__ row_of_token, Tables8 tables, int num_tokens, int nkv, int d, int page_shift, int num_pages, int* __restrict__ status) {
+  pdl_prologue(k_codes, k_exps, v_codes, v_exps, positions, row_of_token, tables.page_indptr, tables.page_indices);
   const int eights = d >> 3, pieces = nkv * eights, threads = (pieces + READ_EACH - 1) / READ_EACH;  // of a token
   const int tokens = max(1, 256 / threads), mine = threadIdx.x / threads, t = blockIdx.x * tokens + (tokens > 1 ? mine : 0);
   const int first = tokens > 1 ? threadIdx.x - mine * threads : blockIdx.y * 256 + threadIdx.x;
   if (t >= num_tokens || first >= threads || (tokens > 1 && mine >= tokens)) return;
-  const int pos = positions[t], page = c8_page(page_indptr, page_indices, row_of_token[t], pos, page_shift, num_pages);
+  const int pos = positions[t], page = tables.page(row_of_token[t], pos, page_shift, num_pages);
   if (page < 0) {
     if (first == 0) atomicExch(status, 2);
     return;
@@ -277,20 +281,20 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
 __global__ void __launch_bounds__(256)
 cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, int* __restrict__ indptr_out, const uint8_t* __restrict__ k_codes,
                      const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ cu_q,
-                     const int* __restrict__ q_start, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int first, int rows, int nkv, int d, int window,
-                     int page_shift, int num_pages, int num_entries, int* __restrict__ status) {
+                     const int* __restrict__ q_start, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int first, int rows, int all_rows, int nkv, int d,
+                     int window, int page_shift, int num_pages, int num_entries, int* __restrict__ status) {
   pdl_prologue(k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
   const int out_page = blockIdx.x, page_size = 1 << page_shift, lane = threadIdx.x & 31;
-  int a = -1, entry = out_page, left = 0, ahead = 0, table = 0, listed = 0;  // the row, which of its pages, how many there are behind it, the row's first, its place in the table
+  int a = -1, entry = out_page, left = 0, ahead = 0, table = 0, stop = 0;  // the row, which of its pages, how many there are behind it, the row's first, where its table lies and ends
   for (int r0 = first; r0 < rows; r0 += 32) {
     const int r = r0 + lane;
-    int need = 0, passed = 0, at = 0, n = 0;
+    int need = 0, passed = 0, at = 0, end = 0;
     if (r < rows) {
       const int from = q_start[r], tokens = cu_q[r + 1] - cu_q[r];
       passed = window > 0 ? max(0, from - window + 1) >> page_shift : 0;
       if (tokens > 0) need = max(0, ((from + tokens + page_size - 1) >> page_shift) - passed);
       at = page_indptr[r];
-      n = page_indptr[r + 1] - at;
+      end = min(page_indptr[window > 0 ? all_rows : r + 1], num_entries);  // (without a window a table is whole, and ends where the next begins)
     }
     int incl = need;
 #pragma unroll
@@ -306,7 +310,7 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
       entry -= __shfl_sync(0xffffffffu, incl - need, src);
       ahead = __shfl_sync(0xffffffffu, passed, src);
       table = __shfl_sync(0xffffffffu, at, src);
-      listed = __shfl_sync(0xffffffffu, n, src);
+      stop = __shfl_sync(0xffffffffu, end, src);
       break;
     }
     entry -= __shfl_sync(0xffffffffu, incl, 31);
@@ -321,8 +325,8 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
   }
   const int eights = d >> 3, pieces = nkv * page_size * eights, idx0 = blockIdx.y * (256 * READ_EACH) + threadIdx.x;
   if (idx0 >= pieces) return;
-  const int e = ahead + entry, f = table + e;
-  const int page = e < listed && f >= 0 && f < num_entries ? page_indices[f] : -1;
+  const int f = table + ahead + entry;
+  const int page = f >= 0 && f < stop ? page_indices[f] : -1;
   const bool there = (unsigned)page < (unsigned)num_pages;
   if (!there && threadIdx.x == 0) atomicExch(status, 2);
   const size_t from = (size_t)(there ? page : 0) * nkv * page_size, to = (size_t)out_page * pieces;
@@ -386,7 +390,7 @@ struct Write8 {
   int* status;
   cudaStream_t stream;
   long long num_pages;
-  int device, num_tokens, nq, nkv, d, rot, page_size;
+  int device, rows, num_entries, num_tokens, nq, nkv, d, rot, page_size;  // rows of page_indptr, entries of page_indices
   float eps;
 };
 struct Read8 {
@@ -396,18 +400,19 @@ struct Read8 {
   int* status;
   cudaStream_t stream;
   long long num_pages;
-  int device, num_tokens, nkv, d, page_size, dtype;
+  int device, rows, num_entries, num_tokens, nkv, d, page_size, dtype;
 };
 
-static_assert(sizeof(Write8) == 168 && sizeof(Read8) == 128, "packed by the caller without gaps");
+static_assert(sizeof(Write8) == 176 && sizeof(Read8) == 136, "packed by the caller without gaps");
 
 MS_EXPORT int ms_cache8_write(const Write8* args) {
   const auto [q_out, k_codes, k_exps, v_codes, v_exps, qkv, q_norm_w, k_norm_w, inv_freq, cos_sin, positions, row_of_token, page_indptr, page_indices, status, stream, num_pages, device,
-              num_tokens, nq, nkv, d, rot, page_size, eps] = *args;
+              rows, num_entries, num_tokens, nq, nkv, d, rot, page_size, eps] = *args;
   if (num_tokens == 0) return 0;
   const OnDevice here(device);
   if (int rc = c8_check("cache8_write", nkv, d, page_size, num_pages)) return rc;
-  MS_CHECK_ARG(nq >= 0 && num_tokens > 0, "cache8_write: nq=%d, %d tokens", nq, num_tokens);
+  MS_CHECK_ARG(nq >= 0 && num_tokens > 0 && rows >= 0, "cache8_write: nq=%d, %d tokens, %d rows", nq, num_tokens, rows);
+  const Tables8 tables = {page_indptr, page_indices, rows, num_entries};
   MS_CHECK_ARG(rot >= 0 && rot <= d && rot % 2 == 0, "cache8_write: rotary_dim=%d must be even and at most the head size %d", rot, d);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0, "cache8_write: pools must be 16-byte aligned");
   if ((d == 64 || d == 128 || d == 256) && (rot == d || rot == 0 || inv_freq == nullptr) && (q_norm_w != nullptr) == (k_norm_w != nullptr) && (uintptr_t)qkv % 8 == 0 &&
@@ -420,55 +425,57 @@ MS_EXPORT int ms_cache8_write(const Write8* args) {
     const int a_trip = 2 * (32 / (d / 8)), trips = ceil_div(nq + 2 * nkv, 8 * a_trip), warps = ceil_div(nq + 2 * nkv, a_trip * trips);
     MS_LAUNCH(kernel, num_tokens, 32 * warps, 0, stream, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)k_exps, (uint8_t*)v_codes, (uint8_t*)v_exps,
               (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w, rot ? inv_freq : (const float*)nullptr, cos_sin, positions,
-              row_of_token, page_indptr, page_indices, nq, nkv, eps, c8_page_shift(page_size), (int)num_pages, status);
+              row_of_token, tables, nq, nkv, eps, c8_page_shift(page_size), (int)num_pages, status);
     return 0;
   }
   const long long items = (long long)num_tokens * (nq + 2 * nkv);
   MS_LAUNCH(cache8_write_kernel, (unsigned)((items + 7) / 8), 256, 0, stream, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)k_exps, (uint8_t*)v_codes,
             (uint8_t*)v_exps, (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w, rot ? inv_freq : (const float*)nullptr,
-            cos_sin, positions, row_of_token, page_indptr, page_indices, num_tokens, nq, nkv, d, rot, eps, c8_page_shift(page_size), (int)num_pages, status);
+            cos_sin, positions, row_of_token, tables, num_tokens, nq, nkv, d, rot, eps, c8_page_shift(page_size), (int)num_pages, status);
   return 0;
 }
 
 MS_EXPORT int ms_cache8_read(const Read8* args) {
-  const auto [k_out, v_out, k_codes, k_exps, v_codes, v_exps, positions, row_of_token, page_indptr, page_indices, status, stream, num_pages, device, num_tokens, nkv, d, page_size,
-              dtype] = *args;
+  const auto [k_out, v_out, k_codes, k_exps, v_codes, v_exps, positions, row_of_token, page_indptr, page_indices, status, stream, num_pages, device, rows, num_entries,
+              num_tokens, nkv, d, page_size, dtype] = *args;
   if (num_tokens == 0) return 0;
   const OnDevice here(device);
   if (int rc = c8_check("cache8_read", nkv, d, page_size, num_pages)) return rc;
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_read: tensors must be 16-byte aligned");
   MS_CHECK_ARG(dtype == MS_F32 || dtype == MS_BF16, "cache8_read: dtype code %d", dtype);
+  MS_CHECK_ARG(num_tokens > 0 && rows >= 0, "cache8_read: %d tokens, %d rows", num_tokens, rows);
+  const Tables8 tables = {page_indptr, page_indices, rows, num_entries};
   const int threads = ceil_div(nkv * (d / 8), READ_EACH), tokens = threads < 256 ? 256 / threads : 1;
   const dim3 grid(ceil_div(num_tokens, tokens), ceil_div(threads, 256));
   MS_CHECK_ARG(grid.y <= 65535, "cache8_read: too many heads (%d)", nkv);
   if (dtype == MS_F32) {
     MS_LAUNCH(cache8_read_kernel<float>, grid, 256, 0, stream, (float*)k_out, (float*)v_out, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
-              (const uint8_t*)v_codes, (const uint8_t*)v_exps, positions, row_of_token, page_indptr, page_indices, num_tokens, nkv, d, c8_page_shift(page_size),
+              (const uint8_t*)v_codes, (const uint8_t*)v_exps, positions, row_of_token, tables, num_tokens, nkv, d, c8_page_shift(page_size),
               (int)num_pages, status);
   } else {
     MS_LAUNCH(cache8_read_kernel<__nv_bfloat16>, grid, 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, (const uint8_t*)k_codes,
-              (const uint8_t*)k_exps, (const uint8_t*)v_codes, (const uint8_t*)v_exps, positions, row_of_token, page_indptr, page_indices, num_tokens, nkv, d,
+              (const uint8_t*)k_exps, (const uint8_t*)v_codes, (const uint8_t*)v_exps, positions, row_of_token, tables, num_tokens, nkv, d,
               c8_page_shift(page_size), (int)num_pages, status);
   }
   return 0;
 }
 
-// Rows [first, rows) look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [entries] and, by row, indptr_out. page_indices has
+// Rows [first, rows) of all_rows look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [entries] and, by row, indptr_out. page_indices has
 // num_entries entries.
 MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, int* indptr_out, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,
-                               const int* q_start, const int* page_indptr, const int* page_indices, int first, int rows, int entries, int nkv, int d, int window, int page_size,
-                               long long num_pages, int num_entries, int* status, cudaStream_t stream) {
+                               const int* q_start, const int* page_indptr, const int* page_indices, int first, int rows, int all_rows, int entries, int nkv, int d, int window,
+                               int page_size, long long num_pages, int num_entries, int* status, cudaStream_t stream) {
   if (entries == 0) return 0;
   if (int rc = c8_check("cache8_unpack", nkv, d, page_size, num_pages)) return rc;
-  MS_CHECK_ARG(first >= 0 && rows > first && entries > 0, "cache8_unpack: rows %d to %d, %d entries", first, rows, entries);
+  MS_CHECK_ARG(first >= 0 && rows > first && all_rows >= rows && entries > 0, "cache8_unpack: rows %d to %d of %d, %d entries", first, rows, all_rows, entries);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_unpack: tensors must be 16-byte aligned");
   MS_CHECK_ARG((long long)nkv * page_size <= 1 << 20, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   const int blocks = ceil_div(nkv * page_size * (d / 8), 256 * READ_EACH);
   MS_CHECK_ARG(blocks <= 65535, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, indptr_out, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
-            (const uint8_t*)v_codes, (const uint8_t*)v_exps, cu_q, q_start, page_indptr, page_indices, first, rows, nkv, d, window, c8_page_shift(page_size), (int)num_pages,
-            num_entries, status);
+            (const uint8_t*)v_codes, (const uint8_t*)v_exps, cu_q, q_start, page_indptr, page_indices, first, rows, all_rows, nkv, d, window, c8_page_shift(page_size),
+            (int)num_pages, num_entries, status);
   return 0;
 }

@@ -66,7 +66,7 @@ def takes(head_dim: int, page_size: int) -> bool:
 
 
 CACHE8 = build.Module("cache8", ("cache8.cu",))
-_WRITE, _READ = struct.Struct("16Qq7if").pack, struct.Struct("12Qq6i").pack  # ``Write8`` and ``Read8`` of csrc/cache8.cu
+_WRITE, _READ = struct.Struct("16Qq9if").pack, struct.Struct("12Qq8i").pack  # ``Write8`` and ``Read8`` of csrc/cache8.cu
 
 
 def module_for(head_dim: int) -> build.Module:
@@ -80,7 +80,7 @@ def _cache_lib():
     native._declare(lib, "ms_cache8_set_pdl", [_i], None)
     native._declare(lib, "ms_cache8_write", [c_char_p])
     native._declare(lib, "ms_cache8_read", [c_char_p])
-    native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 7 + [_ll, _i, _p, _p])
+    native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 8 + [_ll, _i, _p, _p])
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
 
@@ -95,7 +95,7 @@ class _Split(ctypes.Structure):
     """``Split8`` of csrc/attention_cache8.cu."""
 
     _fields_ = [(n, _p) for n in ("cu_q", "q_start", "page_indptr", "page_indices", "status", "part", "cut")] + [
-        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i), ("behind", _i), ("ahead", _i)]
+        (n, _i) for n in ("rows", "tile0", "tiles", "nq", "nkv", "window", "sink", "page_size", "ctas")] + [("scale", _f), ("num_pages", _i), ("behind", _i), ("all_rows", _i), ("num_entries", _i), ("ahead", _i)]
 
 
 class _AttnLib:
@@ -144,8 +144,9 @@ def _check_pools(k: Pool8, v: Pool8) -> None:
 def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w, inv_freq, rotary_dim: int, eps: float, positions, row_of_token,
                     page_indptr, page_indices, page_size: int, status, stream=None, cos_sin=None) -> None:
     """``ops.qk_norm_rope_kv`` with keys and values quantised into 8-bit pools: what is rounded is the float32 number behind norm and rotation
-    (values: as projected). A token whose position its row's table has no page for raises the status word and is not written; two tokens of a call do
-    not share a place."""
+    (values: as projected). ``page_indptr`` [rows + 1], ``page_indices``: entry 0 of row r's table lies at ``page_indptr[r]``, which may be outside the tables where a window gave
+    its pages back; the last number is where all tables end. A token whose position leads outside them, or to no page of the pool, raises the status word and is not written;
+    two tokens of a call do not share a place."""
     _check_pools(k_pool, v_pool)
     t, nq, d = q_out.shape
     pages, nkv, held, dim = k_pool.sizes
@@ -172,14 +173,15 @@ def qk_norm_rope_kv(q_out, k_pool: Pool8, v_pool: Pool8, qkv, q_norm_w, k_norm_w
     vc, ve = v_pool.pointers
     _cache_check(_cache_lib().ms_cache8_write(_WRITE(
         pq, kc, ke, vc, ve, px, pw, pk, freq, table, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
-        status.data_ptr(), _stream_of(stream, k_pool.device), pages, dev, t, nq, nkv, d, rotary_dim if freq else 0, page_size, eps)))
+        status.data_ptr(), _stream_of(stream, k_pool.device), pages, dev, page_indptr.numel() - 1, page_indices.numel(), t, nq,
+        nkv, d, rotary_dim if freq else 0, page_size, eps)))
 
 
 def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: Pool8, positions: torch.Tensor, row_of_token: torch.Tensor,
                page_indptr: torch.Tensor, page_indices: torch.Tensor, status: torch.Tensor, stream=None) -> None:
     """The cached keys and values of given tokens as dense rows: ``k_out``, ``v_out`` [N, kv_heads, d], bfloat16 (exact) or float32 (exact), row i what
-    the cache holds at position ``positions[i]`` of row ``row_of_token[i]`` of the page table. A position without a page raises the status word and
-    leaves its row as it was."""
+    the cache holds at position ``positions[i]`` of row ``row_of_token[i]`` of the page tables (as ``qk_norm_rope_kv`` takes them). A position that leads outside the tables, or to no
+    page of the pool, raises the status word and leaves its row as it was; of a window's group, only positions that were not given back are asked for."""
     _check_pools(k_pool, v_pool)
     pages, nkv, page_size, d = k_pool.sizes
     dev, shape = k_pool.index, k_out.shape
@@ -197,7 +199,7 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
     vc, ve = v_pool.pointers
     _cache_check(_cache_lib().ms_cache8_read(_READ(
         pk, pv, kc, ke, vc, ve, positions.data_ptr(), row_of_token.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), status.data_ptr(),
-        _stream_of(stream, k_pool.device), pages, dev, n, nkv, d, page_size, 0 if dtype is _F32 else 1)))
+        _stream_of(stream, k_pool.device), pages, dev, page_indptr.numel() - 1, page_indices.numel(), n, nkv, d, page_size, 0 if dtype is _F32 else 1)))
 
 
 # ------------------------------------------------------------------ attention
@@ -263,7 +265,7 @@ def _plans(ctx, group: int, ranges: list, key: tuple, device) -> list:
                 whole = fixed and rows * here * nkv <= ctas and _alone(ctx, lib, range(first, first + rows), range(tile0, tile0 + here), tile_rows, nq // nkv, nkv, window)
                 plan = _Split(ctx.cu_q.data_ptr() + skip, ctx.q_start.data_ptr() + skip, ctx.page_indptr[group].data_ptr() + skip, ctx.page_indices[group].data_ptr(),
                               ctx.status.data_ptr(), part.data_ptr(), part.data_ptr() + 4 * floats, rows, tile0, here, nq, nkv, window, sink, page_size, ctas, scale, pages,
-                              not whole, bool(getattr(ctx, "tables_ahead", False)))
+                              not whole, ctx.num_rows - first, ctx.page_indices[group].numel(), bool(getattr(ctx, "tables_ahead", False)))
                 out.append((plan, ctypes.addressof(plan), tile_rows, most, 1 if whole else 2))
     return out
 
@@ -394,8 +396,8 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(
             k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), view.page_indptr[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(),
-            ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, entries, nkv, d, window, page_size, pages,
-            ctx.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, ctx.num_rows, entries, nkv, d, window, page_size,
+            pages, ctx.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
         if attention_tc_ok(q, k):
             attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
         else:
@@ -405,9 +407,9 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:
     """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
     ``group``, window and sink as there. Single tokens, drafted ones and what else the rule at SPLIT_ROWS says go to the kernel that shares out keys
-    (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A row's page that its table or the pool
-    does not have raises the status word. Workspaces lie in ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the
-    other."""
+    (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A page that a row looks at and the tables or
+    the pool do not have raises the status word (without a window a row's table ends where the next one begins). Workspaces lie in ``ctx.scratch``:
+    steps of one context (and graphs captured of them) run one after the other."""
     if not isinstance(v_pool, Pool8) or k_pool.sizes != v_pool.sizes or k_pool.index != v_pool.index or k_pool.index < 0:
         _check_pools(k_pool, v_pool)
     shape = q.shape
