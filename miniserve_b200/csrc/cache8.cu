@@ -461,6 +461,17 @@ MS_EXPORT int ms_cache8_read(const Read8* args) {
   return 0;
 }
 
+// Which capture the stream is part of (never 0), 0: none.
+MS_EXPORT unsigned long long ms_cache8_capture_id(cudaStream_t stream) {
+  cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &state, &id) != cudaSuccess) {
+    cudaGetLastError();  // (the default stream while another one is captured)
+    return 0;
+  }
+  return state == cudaStreamCaptureStatusActive ? id + 1 : 0;
+}
+
 // Rows [first, rows) of all_rows look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [entries] and, by row, indptr_out. page_indices has
 // num_entries entries.
 MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, int* indptr_out, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,

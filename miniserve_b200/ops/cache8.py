@@ -6,7 +6,7 @@ from __future__ import annotations
 import ctypes
 import struct
 from contextlib import nullcontext
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from dataclasses import dataclass
 from functools import lru_cache
 
@@ -81,6 +81,7 @@ def _cache_lib():
     native._declare(lib, "ms_cache8_write", [c_char_p])
     native._declare(lib, "ms_cache8_read", [c_char_p])
     native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 8 + [_ll, _i, _p, _p])
+    native._declare(lib, "ms_cache8_capture_id", [_p], c_ulonglong)
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
 
@@ -205,10 +206,14 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
 # ------------------------------------------------------------------ attention
 
 def _on_stream(ctx, device: torch.device):
-    """Allocations (and their zeroing) in the order of the step's stream, where that is not the current one."""
+    """Allocations in the order of the step's stream, where that is not the current one."""
     if ctx.stream == torch.cuda.current_stream(device).cuda_stream:
         return nullcontext()
-    return torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream, device=device) if ctx.stream else torch.cuda.default_stream(device))
+    return torch.cuda.stream(_stream(ctx, device))
+
+
+def _stream(ctx, device: torch.device) -> torch.cuda.Stream:
+    return torch.cuda.ExternalStream(ctx.stream, device=device) if ctx.stream else torch.cuda.default_stream(device)
 
 
 def _workspace(ctx, floats: int, device) -> torch.Tensor:
@@ -334,11 +339,11 @@ def _shares_out(q, k_pool: Pool8, ctx, first: int) -> bool:
 
 
 class _Unpacked:
-    """A step's context whose pages of one group are the unpacked ones, by tables of their own: rows [first, num_rows)."""
+    """A step's context whose pages of one group are the unpacked ones, by tables of their own: rows [first, num_rows). Plans are its own (those of the context are of all rows)."""
 
-    def __init__(self, ctx, group: int, num_rows: int, indptr: torch.Tensor, ids: torch.Tensor):
+    def __init__(self, ctx, group: int, num_rows: int, indptr: torch.Tensor, ids: torch.Tensor, scratch: dict):
         self.__dict__.update(ctx.__dict__)
-        self.num_rows = num_rows
+        self.num_rows, self.scratch, self.step_cache = num_rows, scratch, {}
         self.page_indptr, self.page_indices = list(ctx.page_indptr), list(ctx.page_indices)
         self.page_indptr[group], self.page_indices[group] = indptr, ids
 
@@ -357,41 +362,42 @@ def _parts(ctx, first: int, window: int, page_size: int, page_bytes: int) -> lis
     return [x for x in out if x[2]]
 
 
-def _unpacked(ctx, numbers: int, ints: int, device: torch.device) -> tuple:
-    """Pages of K and of V (``numbers`` each) and ``ints`` entries of tables, for steps that run one after the other; a capture gets its own. What a launch reads of them it has
-    written before."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    held = None if capturing else ctx.scratch.get("cache8_pages")
+def _unpacked(ctx, scratch: dict, numbers: int, ints: int, device: torch.device) -> tuple:
+    """Pages of K and of V (``numbers`` each), ``ints`` entries of tables and the stream they were made on, kept in ``scratch`` for steps that run one after the other. What a launch
+    reads of them it has written before."""
+    held = scratch.get("cache8_pages")
     if held is not None and held[0].numel() >= numbers and held[2].numel() >= ints:
+        if held[3] != ctx.stream:  # (outgrown, they go back to the stream they came from, which is not to use them before this one is done)
+            for t in held[:3]:
+                t.record_stream(_stream(ctx, device))
         return held
     if held is not None:  # (a context grows portion by portion: twice as much the next time, up to what a step of several rows may take)
         numbers = max(numbers, min(2 * held[0].numel(), UNPACKED_BYTES // 4))
         ints = max(ints, held[2].numel())
     with _on_stream(ctx, device):
-        new = tuple(torch.empty(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (torch.empty(ints, dtype=torch.int32, device=device),)
-    if capturing:
-        ctx.scratch.setdefault("retired", []).append(new)
-    else:
-        ctx.scratch["cache8_pages"] = new
+        new = scratch["cache8_pages"] = tuple(torch.empty(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (
+            torch.empty(ints, dtype=torch.int32, device=device), ctx.stream)
     return new
 
 
 def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, first: int) -> None:
-    """Rows [first, num_rows) of the step over pages unpacked to bfloat16."""
+    """Rows [first, num_rows) of the step over pages unpacked to bfloat16. A captured graph has scratch of its own, the prompt kernels' included, from the graph's memory:
+    what eager steps outgrow may go, and what a kernel finds zero at its start the graph makes so."""
     from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
 
     pages, nkv, page_size, d = k_pool.sizes
-    key = ("cache8_unpacked", group, first, nkv, page_size, d, window)
+    key = ("cache8_unpacked", group, first, nkv, page_size, d, window, ctx.stream, _cache_lib().ms_cache8_capture_id(ctx.stream))
     parts = ctx.step_cache.get(key)
     if parts is None:
         _check_tables(k_pool.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
+        scratch = ctx.step_cache.setdefault(("cache8_scratch", key[-1]), {}) if key[-1] else ctx.scratch
         page = nkv * page_size * d
         parts = _parts(ctx, first, window, page_size, 4 * page)
         most = max((n for _, _, n in parts), default=0)
-        *pools, tables = _unpacked(ctx, most * page, ctx.num_rows + 1 + most, k_pool.device)
-        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in pools)
-        indptr, ids = tables[:ctx.num_rows + 1], tables[ctx.num_rows + 1:ctx.num_rows + 1 + most]
-        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids)) for a, b, n in parts])
+        held = _unpacked(ctx, scratch, most * page, ctx.num_rows + 1 + most, k_pool.device)
+        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in held[:2])
+        indptr, ids = held[2][:ctx.num_rows + 1], held[2][ctx.num_rows + 1:ctx.num_rows + 1 + most]
+        parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids, scratch)) for a, b, n in parts])
     k, v, parts = parts
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(

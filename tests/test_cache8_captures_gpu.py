@@ -1,0 +1,81 @@
+"""The 8-bit cache's attention of one context called eagerly, on another stream and captured, in turn."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from miniserve_b200 import ops
+from tests import cache8_util as cu
+from tests import kernel_util as ku
+from tests.test_cache8_gpu import _attend, _close
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+PROMPTS = [(16, 8, 128, [(30, 170), (0, 200)]), (16, 2, 64, [(30, 170), (0, 200)]), (16, 2, 128, [(900, 1), (37, 1)]), (8, 1, 64, [(700, 90)])]
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", PROMPTS)
+def test_a_context_captured_on_a_side_stream_after_an_eager_call(nq, nkv, d, rows):
+    """All of the step's launches are in the graph, and its scratch stays when a longer prompt needs more."""
+    pb, other = cu.Batch8(rows, 16, nkv, d, seed=8), cu.Batch8([(300, 2000)], 16, nkv, d, seed=9)
+    ctx = ku.make_context(pb)
+    q, want = _attend(pb, nq, d, 0.1, ctx=ctx)
+    _close(pb, q, want, 0.1)
+    out, graph, side = torch.full_like(q, float("nan")), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        ctx.stream = torch.cuda.current_stream().cuda_stream
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    torch.cuda.synchronize()
+    assert bool(out.isnan().all()), "something ran outside the graph"
+    larger = ku.make_context(other)
+    larger.scratch = ctx.scratch
+    for _ in range(2):
+        _close(other, *_attend(other, nq, d, 0.1, ctx=larger), 0.1)
+        torch.full((1 << 24,), float("nan"), dtype=torch.bfloat16, device=DEV)  # (what has been given back is taken)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    ctx.stream = torch.cuda.current_stream().cuda_stream  # and eagerly again
+    out.fill_(float("nan"))
+    ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", PROMPTS)
+def test_two_graphs_of_one_context(nq, nkv, d, rows):
+    """The second is replayed alone, before the first has ever run."""
+    pb = cu.Batch8(rows, 16, nkv, d, seed=8)
+    q, want = _attend(pb, nq, d, 0.1)
+    ctx, outs, graphs = ku.make_context(pb), [torch.full_like(q, float("nan")) for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    ops.attention(torch.empty_like(q), q, pb.k8, pb.v8, ku.make_context(pb), 0, 0.1, None)  # (what is loaded at a first call)
+    torch.cuda.synchronize()
+    for out, graph in zip(outs, graphs):
+        torch.full((1 << 24,), float("nan"), dtype=torch.bfloat16, device=DEV)
+        with torch.cuda.graph(graph):
+            ctx.stream = torch.cuda.current_stream().cuda_stream
+            ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    for i in (1, 0, 1):
+        outs[i].fill_(float("nan"))
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want)
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", PROMPTS)
+def test_a_context_s_stream_may_change(nq, nkv, d, rows):
+    """Both of a prompt's kernels go where ``ctx.stream`` says at the call."""
+    pb = cu.Batch8(rows, 16, nkv, d, seed=8)
+    ctx = ku.make_context(pb)
+    q, want = _attend(pb, nq, d, 0.1, ctx=ctx)
+    side, out, new = torch.cuda.Stream(), torch.full_like(q, float("nan")), torch.randn_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # busy for some milliseconds: what goes elsewhere comes first
+        q.copy_(new)
+        ctx.stream = side.cuda_stream
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    side.synchronize()
+    _close(pb, new, out, 0.1)
