@@ -11,7 +11,8 @@
 //   m + c >= max_j (s_j + ev_j) - 8             of scores and the values' exponents together, in two parts: m a largest score, c the rest (scores may be so
 //                                               large that an exponent is lost beside them); moves only when it is passed by more than 8
 //   o = sum_j 2^(s_j - m - c + 6 + ev_j) code(v_j),      l = sum_j 2^(s_j - m - c + 6)
-// so a weight with its value's scale is at most 2^14, a float16 with 11 significant bits down to 2^-20 of the largest; l and o are float32.
+// so a weight with its value's scale is at most 2^14, a float16 with 11 significant bits down to 2^-20 of the largest; l and o are float32. Exponents ev below the
+// writer's least, -60, count as that in c, and what is left of them scales the weight behind: so no value, however small, makes the weights without their scale leave float32.
 //
 // Work: up to 8, 16 or (head sizes up to 64) 24 query rows (consecutive tokens of a request times the query heads of a kv head) and a kv head are an item; all
 // items' slices of 32 keys in a row are cut into equal runs, one a warp, whatever the requests' lengths (or few items get a CTA each: alone_most). Each warp has a
@@ -497,14 +498,14 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
     const uint32_t kt = st, vt = kt + CODE_BYTES, et = kt + 2 * CODE_BYTES;
     float s[2][NT][4];
     uint32_t vb[2][2];                       // the exponents' bytes of the values g, g + 8, g + 16, g + 24
-    float vf[2][2], kfac[2][2];              // 2^ev and 2^ek (255: infinity, which the codes of such a vector, all zero, make NaN)
+    float vf[2][2], kfac[2][2];              // 2^ev, of the writer's least exponent at least, and 2^ek (255: infinity, which the codes of such a vector, all zero, make NaN)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        kfac[h][i] = __uint_as_float(lds8(et + 16 * h + 8 * i + g) << 23);
+        kfac[h][i] = c8_power(lds8(et + 16 * h + 8 * i + g));
         vb[h][i] = lds8(et + SLICE + 16 * h + 8 * i + g);
-        vf[h][i] = __uint_as_float(vb[h][i] << 23);
+        vf[h][i] = c8_power(max(vb[h][i], (uint32_t)C8_EXP_MIN));
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) s[h][j][0] = s[h][j][1] = s[h][j][2] = s[h][j][3] = 0.f;
@@ -593,8 +594,9 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
             if (key > qp || (p.window > 0 && key <= qp - p.window)) s[h][j][e] = -INFINITY;
           }
     }
-    // m + c moves only where a weight passes 2^(ABOVE + SLACK)
-    if (__any_sync(0xffffffffu, weigh() > exp2f(ABOVE + SLACK))) {
+    // m + c moves only where a weight passes 2^(ABOVE + SLACK); values of exponents below the writer's least come this way too
+    const bool small = min(min(vb[0][0], vb[0][1]), min(vb[1][0], vb[1][1])) < (uint32_t)C8_EXP_MIN;
+    if (__any_sync(0xffffffffu, weigh() > exp2f(ABOVE + SLACK) || small)) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -607,7 +609,7 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               s[h][j][2 * i + c] -= up;
-              c_new = fmaxf(c_new, s[h][j][2 * i + c] + (float)((int)vb[h][i] - 127));
+              c_new = fmaxf(c_new, s[h][j][2 * i + c] + (float)(max((int)vb[h][i], C8_EXP_MIN) - 127));
             }
           c_new = fmaxf(c_run[j][c] - up, oct_max(c_new));
           const float alpha = ex2((c_run[j][c] - up) - c_new);
@@ -621,6 +623,17 @@ attn_cache8_split_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* _
           }
         }
       weigh();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float rest = c8_power(127 - (uint32_t)max(C8_EXP_MIN - (int)vb[h][i], 0));
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            w[h][j][2 * i] *= rest;
+            w[h][j][2 * i + 1] *= rest;
+          }
+        }
     }
     uint32_t wf[2][NT][2];
 #pragma unroll

@@ -25,8 +25,10 @@ __device__ __forceinline__ int c8_exponent(uint32_t amax_bits) {
 }
 // 2^-(b - 127): what numbers are multiplied by before they are rounded to codes; 0 for a vector that is not finite
 __device__ __forceinline__ float c8_inverse(int b) { return b == C8_NAN ? 0.f : __uint_as_float((uint32_t)(254 - b) << 23); }
-// 2^(b - 127); NaN for a vector that is not finite. (Bytes that the writer never makes give powers of two, 0 and 255 aside.)
-__device__ __forceinline__ float c8_factor(int b) { return __uint_as_float(b == C8_NAN ? 0x7FFFFFFFu : (uint32_t)b << 23); }
+// 2^(b - 127), for bytes that the writer never makes too (0 is 2^-127, below float32's normal range); infinity for 255.
+__device__ __forceinline__ float c8_power(uint32_t b) { return __uint_as_float(max(b << 23, 0x00400000u)); }
+// the same, NaN for a vector that is not finite
+__device__ __forceinline__ float c8_factor(int b) { return b == C8_NAN ? __uint_as_float(0x7FFFFFFFu) : c8_power((uint32_t)b); }
 
 // two numbers to two codes (the first in the low byte), rounded to nearest, ties to even, saturating
 __device__ __forceinline__ uint32_t c8_codes2(float x0, float x1) {

@@ -25,7 +25,7 @@ class Pool8:
     """Keys (or values) of one cache entry in 8 bits. ``codes`` uint8 [pages, kv_heads, page_size, d] (bits of ``torch.float8_e4m3fn``) and
     ``exponents`` uint8 [pages, kv_heads, page_size]: number i of a head's vector is code_i * 2^(exponent - 127). The writer takes the smallest
     exponent at which the vector's largest number is at most 448, within 2^-60 and 2^7; a vector with a number that is not finite gets 255 and zero
-    codes, and reads as NaN."""
+    codes, and reads as NaN. Other exponents follow the formula too: 0, an empty pool's, is 2^-127."""
 
     codes: torch.Tensor
     exponents: torch.Tensor

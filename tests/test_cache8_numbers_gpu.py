@@ -1,0 +1,78 @@
+"""The 8-bit cache's numbers: exponents that the writer never makes, the norm's rounding, weights of 11 bits, places that other tests do not look at."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from miniserve_b200 import ops
+from tests import cache8_util as cu
+from tests import kernel_util as ku
+from tests.test_cache8_gpu import _attend, _close
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+# ways through attention: one token (a CTA an item, and cut), drafted tokens, prompts that share out keys, prompts over unpacked pages
+WAYS = [(4, 2, 128, [(100, 1), (33, 1)]), (4, 2, 64, [(5000, 1)]), (8, 2, 64, [(60, 5), (700, 4)]), (8, 1, 64, [(700, 90)]), (16, 2, 128, [(20, 200)]), (8, 1, 80, [(20, 200)])]
+
+
+# ------------------------------------------------------------------ exponents below the writer's
+@pytest.mark.parametrize("nq,nkv,d,rows", WAYS)
+@pytest.mark.parametrize("sink", [False, True])
+def test_a_pool_of_zeros_gives_zeros(nq, nkv, d, rows, sink):
+    pb = cu.Batch8(rows, 16, nkv, d, seed=3)
+    pb.k8, pb.v8 = (ops.Pool8.empty(pb.num_pages, nkv, 16, d) for _ in range(2))
+    q, out = _attend(pb, nq, d, 0.1, sink=sink)
+    assert pb.status.item() == 0 and bool((out == 0).all())
+    k, v = (torch.full((pb.num_tokens, nkv, d), 3.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.read_cache(k, v, pb.k8, pb.v8, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, pb.status)
+    assert bool((k == 0).all()) and bool((v == 0).all())
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", WAYS)
+def test_zero_vectors_of_exponent_zero_among_others(nq, nkv, d, rows):
+    """The first pages of every row as an empty pool has them, the others as the writer makes them."""
+    pb = cu.Batch8(rows, 16, nkv, d, seed=3)
+    for t in pb.tables:
+        for pool in (pb.k8, pb.v8):
+            pool.codes[t[:2]] = 0
+            pool.exponents[t[:2]] = 0
+    q, out = _attend(pb, nq, d, 0.1)
+    _close(pb, q, out, 0.1)
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", WAYS)
+@pytest.mark.parametrize("least,most", [(0, 1), (0, 67), (1, 40), (30, 135)])
+def test_exponents_below_the_writer_s(nq, nkv, d, rows, least, most):
+    """Values of any exponent: finite, and where they are smaller than what the writer makes within 2^-82 a key of the formula: a weight's half step at the end of float16 is 2^-25, a code
+    below 2^9, and the weights' sum, in units of the least exponent's 2^-60 and the 2^6 that weights are kept below, 2^66 or more."""
+    pb = cu.Batch8(rows, 16, nkv, d, seed=3)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    e = torch.randint(least, most, pb.v8.exponents.shape, generator=gen, device=DEV, dtype=torch.uint8)
+    pb.v8.exponents.copy_(torch.where(pb.v8.exponents == 255, pb.v8.exponents, e))
+    q, out = _attend(pb, nq, d, 0.1)
+    at = 0
+    for r, (s, n) in enumerate(rows):
+        k, v = pb.dense64(r)
+        want, mass = cu.attention64(q[at:at + n], k, v, list(range(s, s + n)), 0.1)
+        off = (out[at:at + n].double() - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * mass + (s + n) * 2.0 ** -82)
+        assert bool(out[at:at + n].isfinite().all()) and bool((off <= 0).all())
+        at += n
+    assert pb.status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_exponent_is_read_by_the_formula(dtype):
+    """code * 2^(b - 127) for every byte b but 255, where the type holds it (2^-133 and 2^-149 are the smallest numbers)."""
+    d, page = 16, 256
+    pool = ops.Pool8.empty(1, 1, page, d)
+    pool.exponents[0, 0] = torch.arange(256, device=DEV, dtype=torch.uint8)
+    pool.codes[0, 0] = torch.tensor([0x38, 0xB8, 0x7E, 0x08] * 4, device=DEV, dtype=torch.uint8)  # 1, -1, 448, 2^-6
+    pb = ku.PagedBatch([(0, 256)], page, 1, d, torch.bfloat16)
+    pb.page_indices.zero_()
+    k, v = (torch.empty((256, 1, d), dtype=dtype, device=DEV) for _ in range(2))
+    ops.read_cache(k, v, pool, pool, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, pb.status)
+    want = torch.tensor([1.0, -1.0, 448.0, 2.0 ** -6] * 4, dtype=torch.float64, device=DEV) * torch.exp2(torch.arange(255, device=DEV).double() - 127)[:, None]
+    want = torch.where(want.abs() < 2.0 ** 128, want, want.sign() * float("inf"))
+    assert torch.equal(k[:255, 0].double(), want) and torch.equal(v[:255, 0].double(), want) and bool(k[255].isnan().all())
