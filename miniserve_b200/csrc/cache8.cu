@@ -173,7 +173,7 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       for (int off = LPH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
       if (!is_v) {
         float wl[4], wh[4];
-        const float inv = normed ? rsqrtf(ss * (1.f / D) + eps) : 1.f;  // (2 steps of float32 at most; a root and a division take 30 instructions more)
+        const float inv = normed ? 1.0f / sqrtf(ss * (1.f / D) + eps) : 1.f;
         c8_float4(wl, is_q ? wq_lo : wk_lo);
         c8_float4(wh, is_q ? wq_hi : wk_hi);
 #pragma unroll

@@ -76,3 +76,30 @@ def test_every_exponent_is_read_by_the_formula(dtype):
     want = torch.tensor([1.0, -1.0, 448.0, 2.0 ** -6] * 4, dtype=torch.float64, device=DEV) * torch.exp2(torch.arange(255, device=DEV).double() - 127)[:, None]
     want = torch.where(want.abs() < 2.0 ** 128, want, want.sign() * float("inf"))
     assert torch.equal(k[:255, 0].double(), want) and torch.equal(v[:255, 0].double(), want) and bool(k[255].isnan().all())
+
+
+# ------------------------------------------------------------------ the norm
+@pytest.mark.parametrize("nq,nkv,d", [(16, 8, 128), (8, 2, 64), (8, 4, 256), (6, 3, 48)])
+def test_the_norm_is_rounded_as_a_root_and_a_division(nq, nkv, d):
+    """1 / sqrt(mean + eps) in float32, each operation to the nearest, as the package's other norms have it: of whole numbers up to 15 the sum of squares is exact in any order, so
+    that every bit of the queries (and of keys, to the code) is known."""
+    tokens, page = 4096, 16
+    pb = ku.PagedBatch([(0, tokens)], page, nkv, d, torch.bfloat16)
+    gen = torch.Generator(device=DEV).manual_seed(d)
+    x = torch.randint(-15, 16, (tokens, nq + 2 * nkv, d), generator=gen, device=DEV).bfloat16()
+    wq, wk = ((1 + 0.3 * torch.randn(d, generator=gen, device=DEV)).bfloat16() for _ in range(2))
+    k8, v8 = (ops.Pool8.empty(pb.num_pages, nkv, page, d) for _ in range(2))
+    q = torch.empty((tokens, nq, d), dtype=torch.bfloat16, device=DEV)
+    ops.qk_norm_rope_kv(q, k8, v8, x.view(tokens, -1), wq, wk, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+    f = x.float().cpu()
+    mean = f.square().sum(-1, keepdim=True) / d
+    inv = 1.0 / (mean + torch.tensor(1e-6, dtype=torch.float32)).sqrt()
+    want = f * inv * torch.cat([wq.float().cpu().expand(nq, d), wk.float().cpu().expand(nkv, d), torch.ones(nkv, d)])
+    assert torch.equal(q.cpu(), want[:, :nq].bfloat16())
+    pages = torch.tensor(pb.tables[0], device=DEV)[torch.arange(tokens, device=DEV) // page]
+    held = cu.values64(k8.codes[pages, :, pb.positions.long() % page], k8.exponents[pages, :, pb.positions.long() % page]).cpu()
+    key = want[:, nq:nq + nkv].double()
+    e = cu.exponent64(key)[..., None]
+    y = key * torch.exp2(-e)
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -40))).clamp_min(-6) - 3)
+    assert torch.equal(held, torch.round(y / step) * step * torch.exp2(e))
