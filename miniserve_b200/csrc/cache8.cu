@@ -15,11 +15,13 @@ constexpr int C8_MAX_D = 256;
 struct Tables8 {
   const int *page_indptr, *page_indices;
   int rows, entries;
+  // Where they end: asked for early, so that nothing waits for it behind the row and its beginning.
+  __device__ __forceinline__ int end() const { return min(page_indptr[rows], entries); }
   // The page of position `pos` of request `row`; negative where the tables have none, or none that the pool has.
-  __device__ __forceinline__ int page(int row, int pos, int page_shift, int num_pages) const {
+  __device__ __forceinline__ int page(int row, int pos, int end, int page_shift, int num_pages) const {
     if ((unsigned)row >= (unsigned)rows || pos < 0) return -1;
     const int at = page_indptr[row] + (pos >> page_shift);
-    if (at < 0 || at >= min(page_indptr[rows], entries)) return -1;
+    if (at < 0 || at >= end) return -1;
     const int page = page_indices[at];
     return page < num_pages ? page : -1;
   }
@@ -74,7 +76,7 @@ cache8_write_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_c
     for (int c = lane; c < d; c += 32) dst[c] = __float2bfloat16_rn(x[c]);
     return;
   }
-  const int page = tables.page(row_of_token[t], pos, page_shift, num_pages);
+  const int page = tables.page(row_of_token[t], pos, tables.end(), page_shift, num_pages);
   if (page < 0) {
     if (lane == 0) atomicExch(status, 2);
     return;
@@ -127,8 +129,8 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       hi_raw[b] = *reinterpret_cast<const uint2*>(src + HALF);
     }
   };
+  const int pos = positions[t], request = row_of_token[t], tables_end = tables.end();
   fetch(0);
-  const int pos = positions[t], request = row_of_token[t];
   const bool normed = q_norm_w != nullptr;
   uint2 wq_lo = make_uint2(0u, 0u), wq_hi = wq_lo, wk_lo = wq_lo, wk_hi = wq_lo;
   if (normed) {
@@ -148,7 +150,7 @@ cache8_write_token_kernel(__nv_bfloat16* __restrict__ q_out, uint8_t* __restrict
       for (int i = 0; i < 4; ++i) sincosf((float)pos * inv_freq[j0 + i], &sn[i], &cs[i]);
     }
   }
-  const int page = tables.page(request, pos, page_shift, num_pages);
+  const int page = tables.page(request, pos, tables_end, page_shift, num_pages);
   if (page < 0 && threadIdx.x == 0) atomicExch(status, 2);
   const size_t at0 = ((size_t)max(page, 0) * nkv << page_shift) + (pos & ((1 << page_shift) - 1));
   for (int base = 0; base < heads; base += BATCH * stride) {  // the same trips for every lane: they exchange sums
@@ -246,7 +248,7 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
   const int tokens = max(1, 256 / threads), mine = threadIdx.x / threads, t = blockIdx.x * tokens + (tokens > 1 ? mine : 0);
   const int first = tokens > 1 ? threadIdx.x - mine * threads : blockIdx.y * 256 + threadIdx.x;
   if (t >= num_tokens || first >= threads || (tokens > 1 && mine >= tokens)) return;
-  const int pos = positions[t], page = tables.page(row_of_token[t], pos, page_shift, num_pages);
+  const int pos = positions[t], request = row_of_token[t], page = tables.page(request, pos, tables.end(), page_shift, num_pages);
   if (page < 0) {
     if (first == 0) atomicExch(status, 2);
     return;
