@@ -108,6 +108,8 @@ class Engine:
                                  device=model.device, poison_on_free=poison_on_free, step_tokens=step_tokens, kv_dtype=kv_cache_dtype)
         elif kv_cache_dtype not in ("auto", getattr(cache, "kv_dtype", "auto")):
             raise ValueError(f"the cache that was given does not hold keys and values as kv_cache_dtype={kv_cache_dtype!r} asks")
+        elif getattr(cache, "kv_dtype", "auto") == "fp8" and step_fn is None:
+            model.check_cache8(cache.page_size)
         self.cache = cache
         self.settings = dict(kv_pool_tokens=kv_pool_tokens, page_size=page_size, max_running=max_running,
                              max_prefill_tokens=max_prefill_tokens, chunked_prefill_size=chunked_prefill_size, seed=seed,

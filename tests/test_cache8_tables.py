@@ -53,3 +53,19 @@ def test_parts_are_cut_by_the_bytes_of_their_pages(monkeypatch):
     ctx = SimpleNamespace(num_rows=4, host_q_start=[0, 160, 1600, 0], host_q_len=[16, 16, 32, 5])
     assert cache8._parts(ctx, 0, 0, 16, 100) == [(0, 1, 1), (1, 2, 11), (2, 3, 102), (3, 4, 1)]
     assert cache8._parts(ctx, 0, 40, 16, 100) == [(0, 3, 1 + 4 + 5), (3, 4, 1)]
+
+
+def test_an_engine_with_a_cache_of_its_caller_s_checks_the_model_too():
+    """The error is the one of an engine that makes its own cache, before any step."""
+    import torch
+
+    from miniserve_b200.cache import CacheManager
+    from miniserve_b200.config import preset, resolve
+    from miniserve_b200.engine.engine import Engine
+    from miniserve_b200.parts.decoder import DecoderModel
+
+    model = DecoderModel(resolve(preset("fekulix-tiny"))[2], torch.bfloat16, "cpu")
+    cache = CacheManager(model.entry_caches, 8, 16, 2, device=None, kv_dtype="fp8")
+    for dtype in ("auto", "fp8"):
+        with pytest.raises(ValueError, match="run entry"):
+            Engine(model, cache=cache, kv_cache_dtype=dtype)
