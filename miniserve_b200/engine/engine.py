@@ -25,6 +25,7 @@ from typing import Sequence
 import torch
 
 from ..cache.manager import KV_DTYPES, CacheManager, group_needs, vector_bytes, window_pages
+from ..ops.cache8 import UNPACKED_BYTES
 from ..parts.decoder import DecoderModel
 from ..sampling.sampler import Sampler
 from .request import PLACEHOLDER, Request, RequestState, SamplingParams
@@ -169,6 +170,11 @@ class Engine:
         windowed = sum(b * pb for b, pb in zip(bound, page_bytes) if b is not None)
         whole = sum(pb for b, pb in zip(bound, page_bytes) if b is None)
         pages = (usable - windowed) // max(whole, 1) if whole else 0
+        if eight_bits and whole:
+            # (a single long request's pages are unpacked all at once, whatever they take beyond that gigabyte: at most all of the pool's)
+            one = max(4 * need.kv_heads * need.head_dim * page_size for need, _ in needs if not need.window)
+            if pages * one > UNPACKED_BYTES:
+                pages = (usable - windowed + UNPACKED_BYTES) // (whole + one)
         if usable <= windowed or (whole and pages < 1):
             raise RuntimeError(f"no device memory left for the cache pool ({free} bytes free)")
         return [pages if b is None else b for b in bound]

@@ -362,22 +362,27 @@ def _parts(ctx, first: int, window: int, page_size: int, page_bytes: int) -> lis
     return [x for x in out if x[2]]
 
 
-def _unpacked(ctx, scratch: dict, numbers: int, ints: int, device: torch.device) -> tuple:
-    """Pages of K and of V (``numbers`` each), ``ints`` entries of tables and the stream they were made on, kept in ``scratch`` for steps that run one after the other. What a launch
-    reads of them it has written before."""
-    held = scratch.get("cache8_pages")
+def _unpacked(ctx, capture: int, numbers: int, ints: int, device: torch.device) -> tuple:
+    """Pages of K and of V (``numbers`` each) and ``ints`` entries of tables for steps that run one after the other, and the scratch that they are kept in. What a launch reads of them it
+    has written before. ``capture``: which one, 0: none."""
+    scratch = ctx.step_cache.setdefault(("cache8_scratch", capture), {}) if capture else ctx.scratch
+    held = scratch.get("cache8_pages")  # with the stream they were made on
     if held is not None and held[0].numel() >= numbers and held[2].numel() >= ints:
         if held[3] != ctx.stream:  # (outgrown, they go back to the stream they came from, which is not to use them before this one is done)
             for t in held[:3]:
                 t.record_stream(_stream(ctx, device))
-        return held
+        return *held[:3], scratch
     if held is not None:  # (a context grows portion by portion: twice as much the next time, up to what a step of several rows may take)
-        numbers = max(numbers, min(2 * held[0].numel(), UNPACKED_BYTES // 4))
-        ints = max(ints, held[2].numel())
+        numbers = max(numbers, min(2 * held[0].numel(), UNPACKED_BYTES // 4)) if held[0].numel() < numbers else held[0].numel()
+        ints = max(ints, 2 * held[2].numel())
+        # the old ones go first: here, and what the step keeps of them
+        del scratch["cache8_pages"], held
+        for key in [x for x in ctx.step_cache if x[0] == "cache8_unpacked" and x[-1] == capture]:
+            del ctx.step_cache[key]
     with _on_stream(ctx, device):
-        new = scratch["cache8_pages"] = tuple(torch.empty(numbers, dtype=torch.bfloat16, device=device) for _ in range(2)) + (
-            torch.empty(ints, dtype=torch.int32, device=device), ctx.stream)
-    return new
+        new = tuple(torch.empty(n, dtype=t, device=device) for n, t in ((numbers, torch.bfloat16), (numbers, torch.bfloat16), (ints, torch.int32)))
+    scratch["cache8_pages"] = *new, ctx.stream
+    return *new, scratch
 
 
 def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int, sink: bool, first: int) -> None:
@@ -390,13 +395,12 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
     parts = ctx.step_cache.get(key)
     if parts is None:
         _check_tables(k_pool.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
-        scratch = ctx.step_cache.setdefault(("cache8_scratch", key[-1]), {}) if key[-1] else ctx.scratch
         page = nkv * page_size * d
         parts = _parts(ctx, first, window, page_size, 4 * page)
         most = max((n for _, _, n in parts), default=0)
-        held = _unpacked(ctx, scratch, most * page, ctx.num_rows + 1 + most, k_pool.device)
-        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in held[:2])
-        indptr, ids = held[2][:ctx.num_rows + 1], held[2][ctx.num_rows + 1:ctx.num_rows + 1 + most]
+        *pools, tables, scratch = _unpacked(ctx, key[-1], most * page, ctx.num_rows + 1 + most, k_pool.device)
+        k, v = (x[:most * page].view(most, nkv, page_size, d) for x in pools)
+        indptr, ids = tables[:ctx.num_rows + 1], tables[ctx.num_rows + 1:ctx.num_rows + 1 + most]
         parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids, scratch)) for a, b, n in parts])
     k, v, parts = parts
     for a, entries, view in parts:

@@ -79,3 +79,33 @@ def test_a_context_s_stream_may_change(nq, nkv, d, rows):
         ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
     side.synchronize()
     _close(pb, new, out, 0.1)
+
+
+def test_scratch_that_grows_gives_the_old_back_first():
+    """A longer prompt's pages take the place of a shorter one's; a step whose groups' pages are of two sizes keeps the larger alone."""
+    pb, longer = cu.Batch8([(3000, 3100)], 16, 8, 128, seed=8), cu.Batch8([(9000, 9100)], 16, 8, 128, seed=9)
+    wide = cu.Batch8([(3000, 3100)], 16, 16, 128, seed=10)
+    ctx = ku.make_context(pb)
+    ctx.page_indptr.append(wide.page_indptr)
+    ctx.page_indices.append(wide.page_indices)
+    q, out = _attend(pb, 16, 128, 0.1, ctx=ctx)
+    held = lambda c: sum(t.numel() * t.element_size() for t in c.scratch["cache8_pages"][:3])  # noqa: E731
+    rest = lambda c: sum(t.numel() * t.element_size() for t in c.scratch.values() if isinstance(t, torch.Tensor)) + (1 << 20)  # noqa: E731  (the prompt kernel's own)
+    first = held(ctx)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    ops.attention(out, q, wide.k8, wide.v8, ctx, 1, 0.1, None)
+    again = torch.empty_like(q)
+    ops.attention(again, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    assert held(ctx) >= 2 * first - 65536 and torch.cuda.max_memory_allocated() <= before - first + held(ctx) + again.numel() * 2 + rest(ctx)
+    _close(pb, q, again, 0.1)
+    larger = ku.make_context(longer)
+    larger.scratch = ctx.scratch
+    q, out = torch.randn((9100, 16, 128), device=DEV).bfloat16(), torch.empty((9100, 16, 128), dtype=torch.bfloat16, device=DEV)
+    ctx.step_cache.clear()
+    torch.cuda.synchronize()
+    before, old = torch.cuda.memory_allocated(), held(ctx)
+    torch.cuda.reset_peak_memory_stats()
+    ops.attention(out, q, longer.k8, longer.v8, larger, 0, 0.1, None)
+    assert held(larger) > old and torch.cuda.max_memory_allocated() <= before - old + held(larger) + rest(larger)

@@ -69,3 +69,27 @@ def test_an_engine_with_a_cache_of_its_caller_s_checks_the_model_too():
     for dtype in ("auto", "fp8"):
         with pytest.raises(ValueError, match="run entry"):
             Engine(model, cache=cache, kv_cache_dtype=dtype)
+
+
+@pytest.mark.parametrize("free_gb", [4, 20, 170])
+def test_the_pool_leaves_room_for_a_request_as_long_as_it(free_gb, monkeypatch):
+    """What a step needs beside the pool fits at the start: a gigabyte of unpacked pages, or the longest request's if that is more."""
+    import torch
+
+    from miniserve_b200.engine.engine import Engine
+    from miniserve_b200.parts.base import PagedKV
+    from miniserve_b200.parts.decoder import EntryCache
+
+    free = free_gb << 30
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (free, free))
+    for layers, heads, dim in ((2, 8, 128), (28, 8, 128), (4, 2, 64)):
+        model = SimpleNamespace(dtype=torch.bfloat16, device="cuda", entry_caches=[EntryCache(i, PagedKV(heads, dim)) for i in range(layers)],
+                                spec=SimpleNamespace(hidden_size=1024, vocab_size=50000))
+        reserve = 2048 * 8192 * 16 + 8 * 50000 * 12 + (1 << 30)
+        pages, = Engine._pool_pages(model, None, 16, 0.9, 2048, 8, True)
+        pool, unpacked = pages * 16 * layers * heads * 2 * (dim + 1), pages * 16 * heads * dim * 4
+        room = 0.9 * (free - reserve - (1 << 30))
+        assert pool + max(0, unpacked - (1 << 30)) <= room
+        assert pool + max(0, unpacked - (1 << 30)) >= room - 16 * layers * heads * 4 * (dim + 1) - 16 * heads * dim * 4 - 1, "all but a page of the room is used"
+        plain, = Engine._pool_pages(model, None, 16, 0.9, 2048, 8)
+        assert plain == int(0.9 * (free - reserve)) // (2 * layers * heads * dim * 2 * 16)
