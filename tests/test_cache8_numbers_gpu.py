@@ -8,7 +8,7 @@ import torch
 from miniserve_b200 import ops
 from tests import cache8_util as cu
 from tests import kernel_util as ku
-from tests.test_cache8_gpu import _attend, _close
+from tests.test_cache8_gpu import _attend, _close, _projection
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -103,3 +103,100 @@ def test_the_norm_is_rounded_as_a_root_and_a_division(nq, nkv, d):
     y = key * torch.exp2(-e)
     step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -40))).clamp_min(-6) - 3)
     assert torch.equal(held, torch.round(y / step) * step * torch.exp2(e))
+
+
+# ------------------------------------------------------------------ weights of 11 bits
+def _close11(pb, q, out, scale, window=None, sink=False):
+    """The kernel that shares out keys against 64 bits: the output's rounding (2^-8 of it), the weights' in float16 (2^-11 of what they carry), and 2^-14 of that for scores to float32
+    (2^-20 of a weight for each unit of sum |q k| scale log2(e), which stays below 64 here), sums of a few thousand terms and weights below float16's normal range (2^-31 of the largest)."""
+    at = 0
+    for r, (s, n) in enumerate(pb.rows):
+        if n:
+            k, v = pb.dense64(r)
+            want, mass = cu.attention64(q[at:at + n], k, v, list(range(s, s + n)), scale, window, sink)
+            off = (out[at:at + n].double() - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -14) * mass + 1e-30)
+            assert bool((off <= 0).all()), (r, s, n, off.max().item())
+        at += n
+    assert pb.status.item() == 0
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 8, 128, 16), (32, 4, 64, 16), (5, 1, 80, 16), (4, 4, 256, 32), (3, 3, 16, 8), (6, 2, 48, 64)])
+@pytest.mark.parametrize("rows", [[(299, 1)], [(15, 1), (1000, 1), (0, 1), (64, 1)], [(2000 + 37 * i, 1) for i in range(9)], [(100, 5), (731, 5), (0, 5)], [(20000, 1)]])
+@pytest.mark.parametrize("window,sink", [(None, False), (100, True)])
+def test_single_and_drafted_tokens_keep_11_bits_of_a_weight(nq, nkv, d, page, rows, window, sink):
+    pb = cu.Batch8(rows, page, nkv, d, seed=nq + len(rows))
+    q, out = _attend(pb, nq, d, 0.5 * d ** -0.5, window, sink)
+    _close11(pb, q, out, 0.5 * d ** -0.5, window, sink)
+
+
+@pytest.mark.parametrize("nq,d,rows", [(4, 64, [(131071, 1)]), (4, 128, [(147000, 1)]), (8, 64, [(140000, 2)]), (1, 128, [(150000, 1)])])
+def test_one_kv_head_and_a_context_cut_into_more_than_128_pieces(nq, d, rows):
+    pb = cu.Batch8(rows, 16, 1, d, seed=5)
+    q, out = _attend(pb, nq, d, d ** -0.5)
+    _close11(pb, q, out, d ** -0.5)
+
+
+# ------------------------------------------------------------------ places that other tests do not look at
+def test_a_number_beside_ones_that_saturate():
+    d, page = 64, 16
+    v = torch.zeros((1, d))
+    v[0, :3] = torch.tensor([1e30, -1e30, 3.0])  # exponent 7: 3 is 1.5 * 2^-6 of 2^7, a code
+    qkv = torch.cat([torch.zeros((1, 2 * d)), v], -1).bfloat16().to(DEV)
+    pb = ku.PagedBatch([(0, 1)], page, 1, d, torch.bfloat16)
+    k8, v8 = ops.Pool8.empty(pb.num_pages, 1, page, d), ops.Pool8.empty(pb.num_pages, 1, page, d)
+    q = torch.empty((1, 1, d), dtype=torch.bfloat16, device=DEV)
+    ops.qk_norm_rope_kv(q, k8, v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+    assert cu.values64(v8.codes, v8.exponents)[pb.tables[0][0], 0, 0, :4].tolist() == [57344, -57344, 3, 0]
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(16, 8, 128), (16, 2, 64)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_prompts_unpacked_in_several_parts(nq, nkv, d, window, monkeypatch):
+    """As many rows at a time as have room, here for some 20 pages: the bits of all at once."""
+    from miniserve_b200.ops import cache8
+
+    rows = [(9, 1), (100, 200), (0, 333), (60, 129), (5, 64), (0, 0), (2, 97)]
+    pb = cu.Batch8(rows, 16, nkv, d, seed=2)
+    q, want = _attend(pb, nq, d, 0.1, window)
+    _close(pb, q, want, 0.1, window)
+    monkeypatch.setattr(cache8, "UNPACKED_BYTES", 20 * 4 * nkv * 16 * d)
+    ctx = ku.make_context(pb)
+    _, out = _attend(pb, nq, d, 0.1, window, ctx=ctx, q=q)
+    assert ctx.scratch["cache8_pages"][0].numel() <= 32 * nkv * 16 * d  # (the longest row has 21 pages)
+    _close(pb, q, out, 0.1, window)
+
+
+# ------------------------------------------------------------------ tables read ahead
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 8, 128, 16), (8, 2, 64, 8), (4, 1, 256, 16), (4, 1, 64, 8), (2, 1, 128, 64)])
+@pytest.mark.parametrize("rows", [[(0, 1)], [(2047 + 3 * i, 1) for i in range(8)], [(100, 5), (731, 5), (0, 5)], [(31, 1), (32, 1), (33, 1), (5000, 1)], [(6 + i, 1) for i in range(40)]])
+@pytest.mark.parametrize("window", [None, 40])
+def test_what_is_read_ahead_is_never_a_step_s_own(nq, nkv, d, page, rows, window):
+    """Every pass writes other tokens into slots that held poison or the pass before's, and attends at once: a slot read before its own write would show in the pass that it belongs to."""
+    pb = cu.Batch8(rows, page, nkv, d, seed=len(rows))
+    pos = pb.positions.long()
+    pages = torch.tensor([pb.tables[r][p // page] for r, p in zip(pb.row_of_token.tolist(), pos.tolist())], device=DEV)
+    for pool in (pb.k8, pb.v8):  # the step's own slots: nothing has been written there yet
+        pool.codes[pages, :, pos % page] = 0x7F
+        pool.exponents[pages, :, pos % page] = 255
+    projections = [_projection(pb.num_tokens, nq, nkv, d, 3 + i)[0] for i in range(4)]
+    got = []
+    for ahead in (False, True):
+        k8, v8 = (ops.Pool8(p.codes.clone(), p.exponents.clone()) for p in (pb.k8, pb.v8))
+        ctx = ku.make_context(pb)
+        ctx.tables_ahead = ahead
+        outs = [torch.full((pb.num_tokens, nq, d), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in projections]
+        q = torch.full_like(outs[0], float("nan"))
+        warm = ops.Pool8(k8.codes.clone(), k8.exponents.clone())
+        ops.attention(torch.empty_like(q), torch.zeros_like(q), warm, warm, ctx, 0, 0.1, window)  # (the plan is made)
+        torch.cuda.synchronize()
+        for qkv, out in zip(projections, outs):
+            ops.qk_norm_rope_kv(q, k8, v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+            ops.attention(out, q, k8, v8, ctx, 0, 0.1, window)
+        got.append(outs)
+        pb.k8, held = k8, pb.k8
+        pb.v8, held_v = v8, pb.v8
+        _close(pb, q, outs[-1], 0.1, window)
+        pb.k8, pb.v8 = held, held_v
+    for plain, early in zip(*got):
+        assert bool(plain.isfinite().all()) and torch.equal(plain, early)
+    assert pb.status.item() == 0
