@@ -276,15 +276,16 @@ cache8_read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* 
 
 // The pages that rows [first, rows) of a step look at, as bfloat16 pages of their own, and the tables that say so: a row's pages from the first that its window reaches (page 0 without one)
 // to the last that holds a token, counted through all rows, become pages 0, 1, ... of k_out and v_out; indptr_out[r] + entry is where entry `entry` of row r's table now lies in ids, and
-// ids[i] = i. So what the products behind this look up lies in [0, gridDim.x) whatever the step's own table is like: its rows may begin ahead of the table or inside one
-// another, where a window has given pages back. A page that the table or the pool does not have becomes zeros. What is done to a value vector that is not
+// ids[i] = i, 0 behind the last. So what the products behind this look up lies in [0, gridDim.x) whatever the step's own table is like: its rows may begin ahead of the table or inside one
+// another, where a window has given pages back. A page that the table or the pool does not have becomes zeros. Rows that look at more pages than the launch was made for (the host counted
+// other lengths) raise the status word and look at some of these. What is done to a value vector that is not
 // finite is done for the products that follow, which weigh what a query does not see by zero: its key becomes NaN (a score that is masked where it is not seen), the value itself
 // zero. Block (page, share of it), READ_EACH pieces of 8 numbers of K and V a thread; every warp finds the page's row for itself, 32 rows a look.
 __global__ void __launch_bounds__(256)
 cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ ids, int* __restrict__ indptr_out, const uint8_t* __restrict__ k_codes,
                      const uint8_t* __restrict__ k_exps, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ v_exps, const int* __restrict__ cu_q,
                      const int* __restrict__ q_start, const int* __restrict__ page_indptr, const int* __restrict__ page_indices, int first, int rows, int all_rows, int nkv, int d,
-                     int window, int page_shift, int num_pages, int num_entries, int* __restrict__ status) {
+                     int window, int page_shift, int num_pages, int num_entries, int num_ids, int* __restrict__ status) {
   pdl_prologue(k_codes, k_exps, v_codes, v_exps, cu_q, q_start, page_indptr, page_indices);
   const int out_page = blockIdx.x, page_size = 1 << page_shift, lane = threadIdx.x & 31;
   int a = -1, entry = out_page, left = 0, ahead = 0, table = 0, stop = 0;  // the row, which of its pages, how many there are behind it, the row's first, where its table lies and ends
@@ -319,11 +320,17 @@ cache8_unpack_kernel(__nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restric
   }
   const bool leads = blockIdx.y == 0 && threadIdx.x == 0;
   if (leads) ids[out_page] = out_page;
+  if (blockIdx.y == 0)
+    for (int i = gridDim.x + blockIdx.x * 256 + threadIdx.x; i < num_ids; i += gridDim.x * 256) ids[i] = 0;
   if (a < 0) return;
   if (leads && entry == 0) indptr_out[a] = out_page - ahead;
-  if (leads && blockIdx.x == gridDim.x - 1) {  // rows that look at more pages than the launch was made for
-    for (int r = a + 1; r < rows && left == 0; ++r) left = cu_q[r + 1] - cu_q[r];
-    if (left != 0) atomicExch(status, 2);
+  if (leads && blockIdx.x == gridDim.x - 1) {
+    for (int r = a + 1; r < rows; ++r) {
+      if (cu_q[r + 1] == cu_q[r]) continue;
+      indptr_out[r] = window > 0 ? -(max(0, q_start[r] - window + 1) >> page_shift) : 0;
+      left = 1;
+    }
+    if (left > 0) atomicExch(status, 2);
   }
   const int eights = d >> 3, pieces = nkv * page_size * eights, idx0 = blockIdx.y * (256 * READ_EACH) + threadIdx.x;
   if (idx0 >= pieces) return;
@@ -474,14 +481,15 @@ MS_EXPORT unsigned long long ms_cache8_capture_id(cudaStream_t stream) {
   return state == cudaStreamCaptureStatusActive ? id + 1 : 0;
 }
 
-// Rows [first, rows) of all_rows look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [entries] and, by row, indptr_out. page_indices has
-// num_entries entries.
+// Rows [first, rows) of all_rows look at `entries` pages, which k_out and v_out [entries, nkv, page_size, d] hold; their tables are ids [num_ids] and, by row, indptr_out. page_indices has
+// num_entries entries; ids that many more than pages, so that no row of lengths other than the host's leaves it.
 MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, int* indptr_out, const void* k_codes, const void* k_exps, const void* v_codes, const void* v_exps, const int* cu_q,
                                const int* q_start, const int* page_indptr, const int* page_indices, int first, int rows, int all_rows, int entries, int nkv, int d, int window,
-                               int page_size, long long num_pages, int num_entries, int* status, cudaStream_t stream) {
+                               int page_size, long long num_pages, int num_entries, int num_ids, int* status, cudaStream_t stream) {
   if (entries == 0) return 0;
   if (int rc = c8_check("cache8_unpack", nkv, d, page_size, num_pages)) return rc;
-  MS_CHECK_ARG(first >= 0 && rows > first && all_rows >= rows && entries > 0, "cache8_unpack: rows %d to %d of %d, %d entries", first, rows, all_rows, entries);
+  MS_CHECK_ARG(first >= 0 && rows > first && all_rows >= rows && entries > 0 && num_ids >= entries, "cache8_unpack: rows %d to %d of %d, %d entries, %d ids", first, rows, all_rows, entries,
+               num_ids);
   MS_CHECK_ARG((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                "cache8_unpack: tensors must be 16-byte aligned");
   MS_CHECK_ARG((long long)nkv * page_size <= 1 << 20, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
@@ -489,6 +497,6 @@ MS_EXPORT int ms_cache8_unpack(void* k_out, void* v_out, int* ids, int* indptr_o
   MS_CHECK_ARG(blocks <= 65535, "cache8_unpack: pages of %d tokens and %d heads are too large", page_size, nkv);
   MS_LAUNCH(cache8_unpack_kernel, dim3(entries, blocks), 256, 0, stream, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, ids, indptr_out, (const uint8_t*)k_codes, (const uint8_t*)k_exps,
             (const uint8_t*)v_codes, (const uint8_t*)v_exps, cu_q, q_start, page_indptr, page_indices, first, rows, all_rows, nkv, d, window, c8_page_shift(page_size),
-            (int)num_pages, num_entries, status);
+            (int)num_pages, num_entries, num_ids, status);
   return 0;
 }

@@ -80,7 +80,7 @@ def _cache_lib():
     native._declare(lib, "ms_cache8_set_pdl", [_i], None)
     native._declare(lib, "ms_cache8_write", [c_char_p])
     native._declare(lib, "ms_cache8_read", [c_char_p])
-    native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 8 + [_ll, _i, _p, _p])
+    native._declare(lib, "ms_cache8_unpack", [_p] * 12 + [_i] * 8 + [_ll, _i, _i, _p, _p])
     native._declare(lib, "ms_cache8_capture_id", [_p], c_ulonglong)
     lib.ms_cache8_set_pdl(int(native.pdl_enabled()))
     return lib
@@ -398,16 +398,17 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
         page = nkv * page_size * d
         parts = _parts(ctx, first, window, page_size, 4 * page)
         most = max((n for _, _, n in parts), default=0)
-        *pools, tables, scratch = _unpacked(ctx, key[-1], most * page, ctx.num_rows + 1 + most, k_pool.device)
+        rows, num_ids = ctx.num_rows + 1, most + ctx.page_indices[group].numel()
+        *pools, tables, scratch = _unpacked(ctx, key[-1], most * page, rows + num_ids, k_pool.device)
         k, v = (x[:most * page].view(most, nkv, page_size, d) for x in pools)
-        indptr, ids = tables[:ctx.num_rows + 1], tables[ctx.num_rows + 1:ctx.num_rows + 1 + most]
+        indptr, ids = tables[:rows], tables[rows:rows + num_ids]
         parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids, scratch)) for a, b, n in parts])
     k, v, parts = parts
     for a, entries, view in parts:
         _cache_check(_cache_lib().ms_cache8_unpack(
             k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), view.page_indptr[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(),
             ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, ctx.num_rows, entries, nkv, d, window, page_size,
-            pages, ctx.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            pages, ctx.page_indices[group].numel(), view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
         if attention_tc_ok(q, k):
             attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
         else:
@@ -418,8 +419,9 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, 
     """``ops.attention`` over an 8-bit cache: causal attention of the step's new tokens (bfloat16 queries and output) over the pages of cache group
     ``group``, window and sink as there. Single tokens, drafted ones and what else the rule at SPLIT_ROWS says go to the kernel that shares out keys
     (``csrc/attention_cache8.cu``); other prompts to a bfloat16 cache's kernels, over pages unpacked first. A page that a row looks at and the tables or
-    the pool do not have raises the status word (without a window a row's table ends where the next one begins). Workspaces lie in ``ctx.scratch``:
-    steps of one context (and graphs captured of them) run one after the other."""
+    the pool do not have raises the status word (without a window a row's table ends where the next one begins). Single and drafted
+    tokens go by the lengths on the device; other prompts' pages are counted by ``ctx.host_q_start`` and ``ctx.host_q_len``, and rows that turn out to have more of
+    them raise the status word. Workspaces lie in ``ctx.scratch``: steps of one context (and graphs captured of them) run one after the other."""
     if not isinstance(v_pool, Pool8) or k_pool.sizes != v_pool.sizes or k_pool.index != v_pool.index or k_pool.index < 0:
         _check_pools(k_pool, v_pool)
     shape = q.shape

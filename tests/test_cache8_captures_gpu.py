@@ -109,3 +109,36 @@ def test_scratch_that_grows_gives_the_old_back_first():
     torch.cuda.reset_peak_memory_stats()
     ops.attention(out, q, longer.k8, longer.v8, larger, 0, 0.1, None)
     assert held(larger) > old and torch.cuda.max_memory_allocated() <= before - old + held(larger) + rest(larger)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(16, 8, 128), (16, 2, 64)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_a_captured_prompt_s_beginning_that_changes_on_the_device(nq, nkv, d, window):
+    """As many pages or fewer as the host counted: right. More: the status word, and nothing outside the scratch is looked at."""
+    pb = cu.Batch8([(400, 500), (500, 400), (0, 150)], 16, nkv, d, seed=8)
+    whole, ctx = list(pb.rows), ku.make_context(pb)
+    first = [(200, 500), (100, 400), (0, 150)]
+    ctx.host_q_start = [s for s, _ in first]
+    ctx.q_start.copy_(torch.tensor(ctx.host_q_start, dtype=torch.int32))
+    pb.rows = first
+    q, out = _attend(pb, nq, d, 0.1, window, ctx=ctx)
+    assert "cache8_pages" in ctx.scratch
+    _close(pb, q, out, 0.1, window)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ctx.stream = torch.cuda.current_stream().cuda_stream
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, window)
+    fits = [[200, 100, 0], [0, 300, 0], [0, 0, 0], [100, 200, 0]]
+    for starts in fits + ([] if window else [[s for s, _ in whole], [400, 100, 0], [0, 500, 0], [200, 101 + 16, 0]]) + [[0, 1, 0]]:
+        ctx.q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        pages = sum(-(-(s + n) // 16) - (max(0, s - (window or 0) + 1) // 16 if window else 0) for s, (_, n) in zip(starts, whole))
+        counted = sum(-(-(s + n) // 16) - (max(0, s - (window or 0) + 1) // 16 if window else 0) for s, n in first)
+        assert pb.status.item() == (2 if pages > counted else 0), starts
+        pb.status.zero_()
+        if pages <= counted:
+            pb.rows = [(s, n) for s, (_, n) in zip(starts, whole)]
+            _close(pb, q, out, 0.1, window)
