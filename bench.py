@@ -16,7 +16,8 @@ engine runs on one GPU: for N > 1 it prints a line that says so and exits with 2
 requests with prompts of 128 to 4,096 tokens and 128 output tokens; Qwen3-32B shapes: 16 requests
 with 8,192-token prompts and 128 output tokens, in a pool too small for all of them) through
 ``Engine.generate`` and print one line with tokens per second, the mean time of decode and of
-mixed steps, their fraction of the measured peaks, and the number of preemptions.
+mixed steps, their fraction of the measured peaks, and the number of preemptions. ``--kv-cache-dtype fp8`` measures
+these and the default run with keys and values in 8 bits.
 
 ``--config fekulix`` measures the Fekulix design (random weights, the layer sizes of Qwen3-0.6B and
 Qwen3-1.7B) beside the Qwen3 model of the same width, depth, feed-forward size and vocabulary: one
@@ -268,6 +269,11 @@ def time_prefill(engine, tokens: int, repeats: int = 5, warmup: int = 6):
     return statistics.median(times)
 
 
+def kv_held(args) -> dict:
+    """What a line's config says of keys and values that are not held in the model's type."""
+    return {} if args.kv_cache_dtype == "auto" else {"kv_cache_dtype": args.kv_cache_dtype}
+
+
 def run_ours(args) -> dict:
     import torch
 
@@ -278,7 +284,7 @@ def run_ours(args) -> dict:
     raw = qwen3_06b_config(args.layers)
     pool_tokens = 64 * (CONTEXT + DECODE_TOKENS) + 4096
     llm = LLM(random=raw, weights_seed=0, dtype="bfloat16", kv_pool_tokens=pool_tokens, page_size=16,
-              max_running=64, chunked_prefill_size=2048, cuda_graph=not args.no_graph)
+              max_running=64, chunked_prefill_size=2048, cuda_graph=not args.no_graph, kv_cache_dtype=args.kv_cache_dtype)
     eng = llm.engine
     model = llm.model
     weight_bytes = model.weight_bytes()
@@ -326,7 +332,7 @@ def run_ours(args) -> dict:
             "head_dim": raw["head_dim"], "intermediate": raw["intermediate_size"], "vocab": raw["vocab_size"],
             "tied_head": raw["tie_word_embeddings"], "global_batch": args.batch, "seq_len": CONTEXT,
             "decode_tokens": DECODE_TOKENS, "page_size": 16, "kv_pool_tokens": pool_tokens,
-            "cuda_graph": eng.graphs is not None, "parallelism": "single GPU",
+            "cuda_graph": eng.graphs is not None, "parallelism": "single GPU", **kv_held(args),
             "l2": "inputs larger than L2 (1.19 GB of weights and the KV cache are read every step)",
         },
         "e2e": {"value": round(e2e_value, 1), "unit": "tokens/s", "h2d_bytes_per_step": int(h2d),
@@ -593,7 +599,7 @@ def run_workload(args) -> dict:
     need = sum(len(p) + wl["new_tokens"] for p in prompts)
     pool_tokens = wl["pool_pages"] * 16 if wl["pool_pages"] else need + 4096
     llm = LLM(random=raw, weights_seed=0, dtype="bfloat16", kv_pool_tokens=pool_tokens, page_size=16, max_running=64,
-              chunked_prefill_size=2048)
+              chunked_prefill_size=2048, kv_cache_dtype=args.kv_cache_dtype)
     eng = llm.engine
     eng.capture_graphs(("greedy",), context_lengths=(wl["prompt"][0], wl["prompt"][1] + wl["new_tokens"]))
     weight_bytes, kv_per_token = llm.model.weight_bytes(), eng.cache.bytes_per_token()
@@ -635,7 +641,7 @@ def run_workload(args) -> dict:
     result = {
         "impl": "ours", "workload": f"Qwen3-{args.config.upper()} shapes, {wl['requests']} requests, prompts {wl['prompt'][0]}..{wl['prompt'][1]}, "
                                     f"{wl['new_tokens']} output tokens each, chunk budget 2048",
-        "layers": layers, "layers_full_model": full_layers, "dtype": "bf16", "kv_pool_tokens": pool_tokens,
+        "layers": layers, "layers_full_model": full_layers, "dtype": "bf16", "kv_pool_tokens": pool_tokens, **kv_held(args),
         "tokens_needed_at_once": need, "seconds": round(seconds, 3),
         "value": round((sum(map(len, prompts)) + out_tokens) / seconds, 1), "unit": "tokens/s (prompt + output)",
         "output_tokens_per_s": round(out_tokens / seconds, 1), "steps": len(times),
@@ -742,6 +748,8 @@ def main() -> int:
     ap.add_argument("--config", choices=["0.6b", "8b", "32b", "fekulix", "mugipel", "rofozen", "kovusun", "vumedra", "tunadra"], default="0.6b",
                     help="0.6b: the benchmark line; 8b, 32b: the larger workloads through Engine.generate (a line of their own); "
                          "fekulix, mugipel, rofozen, kovusun, vumedra, tunadra: prefill and decode of that design beside Qwen3 at equal sizes (a line of its own)")
+    ap.add_argument("--kv-cache-dtype", choices=["auto", "fp8"], default="auto",
+                    help="with --config 0.6b, 8b or 32b: fp8 holds keys and values in 8 bits (named in config)")
     ap.add_argument("--kernels", action="store_true", help="with --config fekulix, mugipel, rofozen, kovusun, vumedra or tunadra: also device time per kernel of a prompt step and a decode step")
     ap.add_argument("--only", choices=["all", "decode", "prefill"], default="all",
                     help="measure only the decode steps or only the prefill (for profiling); the line then lacks the other parts")
