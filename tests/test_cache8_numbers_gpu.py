@@ -200,3 +200,60 @@ def test_what_is_read_ahead_is_never_a_step_s_own(nq, nkv, d, page, rows, window
     for plain, early in zip(*got):
         assert bool(plain.isfinite().all()) and torch.equal(plain, early)
     assert pb.status.item() == 0
+
+
+def _close_wide(pb, q, out, scale):
+    """``_close`` for scores of any size. Scores to float32: 2^-20 of a weight for each unit of sum |q k| scale log2(e), here up to some thousands (queries and keys are scaled by 8 each: 128
+    channels of 12 x 12 make 2,600), where that text takes 64. And one key may take nearly all: a weight with its value's scale is kept to 2^-25 (half of float16's smallest step), the
+    row's largest is 2^6 or more, so that a key's part is off by 2^-31 of a largest code (448) at most, in the scale of the largest's value, whatever it carries itself."""
+    at = 0
+    for r, (s, n) in enumerate(pb.rows):
+        k, v = pb.dense64(r)
+        mine = q[at:at + n]
+        want, mass = cu.attention64(mine, k, v, list(range(s, s + n)), scale)
+        group = mine.shape[1] // k.shape[1]
+        size = torch.stack([(mine[:, h].double().abs() @ k[:, h // group].abs().T).amax(1) for h in range(mine.shape[1])], 1) * scale * 1.4427
+        e = pb.v8.exponents[torch.tensor(pb.tables[r], device=DEV)].permute(0, 2, 1).reshape(-1, k.shape[1])[:s + n].amax(0).double() - 127
+        lost = ((s + n) * 448 * 2.0 ** -31 * torch.exp2(e)).repeat_interleave(group)[None, :, None]
+        off = (out[at:at + n].double() - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -20 * size.clamp_min(64)[..., None]) * mass + lost)
+        assert bool((off <= 0).all()), (r, s, n, off.max().item())
+        at += n
+    assert pb.status.item() == 0
+
+
+def _pages_in_order(pb, first):
+    """The same batch with its rows' pages one behind the other from page ``first`` on, as an allocator that begins there gives them."""
+    order = [p for t in pb.tables for p in t]
+    rest = [p for p in range(pb.num_pages) if p not in set(order)]
+    place = rest[:first] + order + rest[first:]
+    at = torch.tensor(place, device=DEV)
+    pb.k8, pb.v8 = (ops.Pool8(x.codes[at].contiguous(), x.exponents[at].contiguous()) for x in (pb.k8, pb.v8))
+    new = {p: i for i, p in enumerate(place)}
+    pb.tables = [[new[p] for p in t] for t in pb.tables]
+    pb.page_indices = torch.tensor([p for t in pb.tables for p in t], dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 1, 64, 8), (4, 1, 64, 16), (8, 1, 128, 16), (4, 2, 64, 8), (16, 8, 128, 16)])
+@pytest.mark.parametrize("first", [0, 1, 2, 3])
+@pytest.mark.parametrize("rows", [[(36, 1)], [(32 + 5 * i, 1) for i in range(12)], [(33, 5), (64, 3), (1000, 1)], [(2000 + i, 1) for i in range(40)]])
+def test_a_step_s_own_slots_beside_ones_that_were_read_ahead(nq, nkv, d, page, first, rows):
+    """The kernels wait behind one that takes long, with what they read ahead long there: exponents of neighbouring slots, pages and heads share 32 bytes of memory, and the write in between
+    changes some of them."""
+    pb = cu.Batch8(rows, page, nkv, d, seed=len(rows))
+    _pages_in_order(pb, first)
+    slow = ku.PagedBatch([(2500, 1)], 16, 1, 64, torch.float32)
+    slow.k_pool.zero_(), slow.v_pool.zero_()
+    busy = torch.zeros((1, 1, 64), device=DEV)
+    ctx = ku.make_context(pb)
+    ctx.tables_ahead = True
+    q, out = (torch.full((pb.num_tokens, nq, d), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.attention(torch.empty_like(q), torch.zeros_like(q), pb.k8, pb.v8, ctx, 0, 0.1, None)  # (the plan is made)
+    for i in range(3):
+        qkv = _projection(pb.num_tokens, nq, nkv, d, 3 + i)[0]
+        qkv *= (1.0, 8.0, 0.125)[i]  # (other exponents)
+        torch.cuda.synchronize()
+        ops.attention_rowwise(busy, busy, slow.k_pool, slow.v_pool, slow.positions, slow.row_of_token, slow.page_indptr, slow.page_indices, 0.1, None, slow.status)
+        ops.qk_norm_rope_kv(q, pb.k8, pb.v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+        ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+        torch.cuda.synchronize()
+        _close_wide(pb, q, out, 0.1)
