@@ -20,9 +20,9 @@
 // memory until all are done, and the warps add the pieces up together, in the warps' order. Items cut by a CTA's end leave one piece a CTA in global memory for a
 // second small kernel. The lengths are read on the device, so a captured launch serves every context.
 //
-// What bounds it: the codes' bytes for full batches (64 requests of 1,024 to 3,985 keys, 8 kv heads of 128: 60 us, 5.5 TB/s, 0.84 of a copy), then the fixed
+// What bounds it: the codes' bytes for full batches (64 requests of 1,024 to 3,985 keys, 8 kv heads of 128: 61 us, 5.4 TB/s, 0.83 of a copy), then the fixed
 // latencies of a slice's chain with two warps a scheduler; for few keys the three dependent trips to memory before the first slice (4 us) and the second kernel
-// (one token behind 299 keys 7.4 us, 8 behind 2,048 13.9).
+// (one token behind 299 keys 7.5 us, 8 behind 2,048 14.3).
 #include "cache8.cuh"
 
 #ifndef MS_HEAD_DIM

@@ -318,7 +318,8 @@ def _split(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
 #     head size 64, 1 head a kv head, 1 from the beginning                512: 31/37   4,096: 313/414;   8 so  512: 86/86   4,096: 2325/2387
 #     head size 80, 2 heads a kv head, 1 from the beginning               512: 33/43   2,048: 121/156;   8 so  512: 115/96  2,048: 917/801;   4 behind 3,000  512: 278/446
 #     head size 256, 4 heads a kv head, 1 from the beginning              256: 20/31   1,024: 72/96;     8 so  256: 92/70   1,024: 585/436;   4 behind 3,000  256: 242/293
-# So up to SPLIT_ROWS query rows always share out keys. Beyond, the tcgen05 kernel takes what it takes. Of other shapes the mma.sync kernel takes steps with no more keys behind them
+# So up to SPLIT_ROWS query rows always share out keys. Beyond, the tcgen05 kernel takes what it takes: right for many requests and for many keys; a lone request of 128 or 256 query rows behind
+# 2,000 keys is 6 to 8 us slower for it. Of other shapes the mma.sync kernel takes steps with no more keys behind them
 # than new tokens where 8 heads and more share a kv head, or where 2 and more do and 4 requests and more come: it has many CTAs then, of few keys each.
 SPLIT_ROWS = 96
 UNPACKED_BYTES = 1 << 30  # of pages unpacked at a time, unless a single request has more
