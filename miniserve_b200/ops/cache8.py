@@ -206,7 +206,7 @@ def read_cache(k_out: torch.Tensor, v_out: torch.Tensor, k_pool: Pool8, v_pool: 
 # ------------------------------------------------------------------ attention
 
 def _on_stream(ctx, device: torch.device):
-    """Allocations in the order of the step's stream, where that is not the current one."""
+    """Allocations (and their zeroing) in the order of the step's stream, where that is not the current one."""
     if ctx.stream == torch.cuda.current_stream(device).cuda_stream:
         return nullcontext()
     return torch.cuda.stream(_stream(ctx, device))
@@ -392,9 +392,10 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
     from . import attention_bf16, attention_tc_ok, attention_tc_prefill  # (this module is imported by theirs)
 
     pages, nkv, page_size, d = k_pool.sizes
-    key = ("cache8_unpacked", group, first, nkv, page_size, d, window, ctx.stream, _cache_lib().ms_cache8_capture_id(ctx.stream))
-    parts = ctx.step_cache.get(key)
+    key = ("cache8_unpacked", group, first, q.shape[1], nkv, page_size, d, window, ctx.stream, _cache_lib().ms_cache8_capture_id(ctx.stream))
+    parts, scope = ctx.step_cache.get(key), nullcontext()
     if parts is None:
+        scope = _on_stream(ctx, k_pool.device)  # (what the prompt kernels make at a first call is made, and zeroed, there)
         _check_tables(k_pool.index, ctx.cu_q, ctx.q_start, ctx.page_indptr[group], ctx.page_indices[group], ctx.status)
         page = nkv * page_size * d
         parts = _parts(ctx, first, window, page_size, 4 * page)
@@ -405,15 +406,16 @@ def _dense(out, q, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, 
         indptr, ids = tables[:rows], tables[rows:rows + num_ids]
         parts = ctx.step_cache[key] = (k, v, [(a, n, _Unpacked(ctx, group, b, indptr, ids, scratch)) for a, b, n in parts])
     k, v, parts = parts
-    for a, entries, view in parts:
-        _cache_check(_cache_lib().ms_cache8_unpack(
-            k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), view.page_indptr[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(),
-            ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, ctx.num_rows, entries, nkv, d, window, page_size,
-            pages, ctx.page_indices[group].numel(), view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
-        if attention_tc_ok(q, k):
-            attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
-        else:
-            attention_bf16.run_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
+    with scope:
+        for a, entries, view in parts:
+            _cache_check(_cache_lib().ms_cache8_unpack(
+                k.data_ptr(), v.data_ptr(), view.page_indices[group].data_ptr(), view.page_indptr[group].data_ptr(), *k_pool.pointers, *v_pool.pointers, ctx.cu_q.data_ptr(),
+                ctx.q_start.data_ptr(), ctx.page_indptr[group].data_ptr(), ctx.page_indices[group].data_ptr(), a, view.num_rows, ctx.num_rows, entries, nkv, d, window, page_size,
+                pages, ctx.page_indices[group].numel(), view.page_indices[group].numel(), ctx.status.data_ptr(), ctx.stream))
+            if attention_tc_ok(q, k):
+                attention_tc_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
+            else:
+                attention_bf16.run_prefill(out, q, k, v, view, group, scale, window or None, a, sink)
 
 
 def attention(out: torch.Tensor, q: torch.Tensor, k_pool: Pool8, v_pool: Pool8, ctx, group: int, scale: float, window: int | None, sink: bool = False) -> None:

@@ -142,3 +142,17 @@ def test_a_captured_prompt_s_beginning_that_changes_on_the_device(nq, nkv, d, wi
         if pages <= counted:
             pb.rows = [(s, n) for s, (_, n) in zip(starts, whole)]
             _close(pb, q, out, 0.1, window)
+
+
+@pytest.mark.parametrize("nq,nkv,d,rows", PROMPTS + [(16, 8, 128, [(9000, 300)])])
+def test_a_stream_of_its_own_while_the_current_one_is_busy(nq, nkv, d, rows):
+    """All that a first call makes, counters that a kernel finds zero among it, is made on the step's stream: what lies on the current one may come much later."""
+    pb = cu.Batch8(rows, 16, nkv, d, seed=8)
+    q, want = _attend(pb, nq, d, 0.1)
+    side, out, ctx = torch.cuda.Stream(), torch.full_like(q, float("nan")), ku.make_context(pb)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    ctx.stream = side.cuda_stream
+    ops.attention(out, q, pb.k8, pb.v8, ctx, 0, 0.1, None)
+    with torch.cuda.stream(side):
+        assert torch.equal(out, want)
