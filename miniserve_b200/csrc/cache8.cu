@@ -15,15 +15,15 @@ constexpr int C8_MAX_D = 256;
 struct Tables8 {
   const int *page_indptr, *page_indices;
   int rows, entries;
-  // Where they end: asked for early, so that nothing waits for it behind the row and its beginning.
-  __device__ __forceinline__ int end() const { return min(page_indptr[rows], entries); }
+  // Where they end: asked for early, so that nothing waits for it behind the row and its beginning. (Of a page_indptr with room for more rows than there are the next row's
+  // beginning still says so of whole tables.)
+  __device__ __forceinline__ int end() const { return page_indptr[rows]; }
   // The page of position `pos` of request `row`; negative where the tables have none, or none that the pool has.
   __device__ __forceinline__ int page(int row, int pos, int end, int page_shift, int num_pages) const {
     if ((unsigned)row >= (unsigned)rows || pos < 0) return -1;
-    const int at = page_indptr[row] + (pos >> page_shift);
-    if (at < 0 || at >= end) return -1;
-    const int page = page_indices[at];
-    return page < num_pages ? page : -1;
+    const int at = page_indptr[row] + (pos >> page_shift), next = page_indptr[row + 1];
+    const int page = at >= 0 && at < entries ? page_indices[at] : -1;  // (asked for before the end is known)
+    return at < max(end, next) && page < num_pages ? page : -1;
   }
 };
 
@@ -106,7 +106,7 @@ __device__ __forceinline__ uint2 c8_bf16x4(const float (&f)[4]) {
 // Head sizes 64, 128 and 256 rotated whole or not at all: a block per token, D / 8 lanes per head. A lane holds 4 numbers of the head's first half and the 4 of the second that
 // rotate with them; a head's lanes exchange a sum of squares and a maximum. What hangs on the token alone is fetched once a lane, and its first numbers before the
 // page is looked up (three loads, one behind the other); a further trip's are asked for ahead of the work on the last. Bound by those chains, not by bytes: written and read back
-// (cache8_read_kernel), 2,048 tokens of 48 heads take 17.7 us (56 MB: 8.5 us at the rate of a copy), 777 tokens of 40 heads of 64 6.2; without the loads ahead 19.5 and 6.4, with
+// (cache8_read_kernel), 2,048 tokens of 48 heads take 17.8 us (56 MB: 8.5 us at the rate of a copy), 777 tokens of 40 heads of 64 6.4; without the loads ahead the first take 19.5, with
 // five blocks a multiprocessor 17.2 and 7.1.
 // TABLE: the angles' cosines and sines are given, or nothing is rotated (the form that makes them itself needs more registers).
 template <int D, bool TABLE>
@@ -430,7 +430,7 @@ MS_EXPORT int ms_cache8_write(const Write8* args) {
     auto kernel = d == 64    ? (table ? cache8_write_token_kernel<64, true> : cache8_write_token_kernel<64, false>)
                   : d == 128 ? (table ? cache8_write_token_kernel<128, true> : cache8_write_token_kernel<128, false>)
                              : (table ? cache8_write_token_kernel<256, true> : cache8_write_token_kernel<256, false>);
-    // as many warps as bring all heads in equal trips of two a lane group, 8 at most: 48 heads of 128 in two trips of 6 warps 17.7 us, of 8 warps 19.9 (the sizes above)
+    // as many warps as bring all heads in equal trips of two a lane group, 8 at most: 48 heads of 128 in two trips of 6 warps 17.8 us, of 8 warps 19.9 (the sizes above)
     const int a_trip = 2 * (32 / (d / 8)), trips = ceil_div(nq + 2 * nkv, 8 * a_trip), warps = ceil_div(nq + 2 * nkv, a_trip * trips);
     MS_LAUNCH(kernel, num_tokens, 32 * warps, 0, stream, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)k_exps, (uint8_t*)v_codes, (uint8_t*)v_exps,
               (const __nv_bfloat16*)qkv, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w, rot ? inv_freq : (const float*)nullptr, cos_sin, positions,

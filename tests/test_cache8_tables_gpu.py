@@ -137,3 +137,26 @@ def test_exactly_the_pages_that_are_there_are_written():
         ops.qk_norm_rope_kv(q, pb.k8, pb.v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
         changed = (pb.k8.codes != before).any(-1).any(1).any(-1)
         assert pb.status.item() == 2 and changed.nonzero().flatten().tolist() == [pb.tables[0][0]], bad
+
+
+@pytest.mark.parametrize("tail", [0, -7, 1 << 30])
+def test_tables_with_room_for_more_rows(tail):
+    """Whole tables in a ``page_indptr`` of more places than the step has rows, whatever stands in the places behind."""
+    rows, nkv, d, page = [(0, 20), (40, 1), (7, 30)], 2, 64, 16
+    pb = cu.Batch8(rows, page, nkv, d, seed=3)
+    pb.page_indptr = torch.cat([pb.page_indptr, torch.full((5,), tail, dtype=torch.int32, device=DEV)])
+    k, v = (torch.empty((pb.num_tokens, nkv, d), dtype=torch.float32, device=DEV) for _ in range(2))
+    ops.read_cache(k, v, pb.k8, pb.v8, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, pb.status)
+    at = 0
+    for r, (s, n) in enumerate(rows):
+        k64, v64 = pb.dense64(r)
+        assert torch.equal(k[at:at + n].double(), k64[s:]) and torch.equal(v[at:at + n].double(), v64[s:])
+        at += n
+    qkv, _ = _projection(pb.num_tokens, 4, nkv, d, 1)
+    q = torch.empty((pb.num_tokens, 4, d), dtype=torch.bfloat16, device=DEV)
+    ops.qk_norm_rope_kv(q, pb.k8, pb.v8, qkv, None, None, None, 0, 1e-6, pb.positions, pb.row_of_token, pb.page_indptr, pb.page_indices, page, pb.status)
+    out = torch.empty_like(q)
+    ops.attention(out, q, pb.k8, pb.v8, ku.make_context(pb), 0, 0.1, None)
+    _close(pb, q, out, 0.1)
+    ops.attention(out, q, pb.k8, pb.v8, ku.make_context(pb), 0, 0.1, 10)
+    _close(pb, q, out, 0.1, 10)
