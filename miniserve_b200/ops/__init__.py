@@ -12,8 +12,10 @@ from dataclasses import dataclass
 
 import torch
 
-from . import attention_bf16, blas, cache8, experts, native
+from . import adapters, attention_bf16, blas, cache8, experts, native
+from .adapters import AdapterRows, LowRank
 from .cache8 import Pool8, read_cache
+from .filtered import sample_filtered
 from .mixers import (act_mul, add_dyt, add_layernorm, add_normed_rmsnorm, add_rmsnorm_scaled, add_row_vector, axpby, channel_decay, channel_gate,  # noqa: F401
                      chunk_scan, chunk_scan_ok, clamped_glu, conv_bias, conv_silu_unit, conv_state_update, decay_scan, embed_sum, gate_relu_squared, gated_group_norm,
                      gelu_tanh, head_gate, head_norm_gate, latent_prepare, latent_rope_prepare, mlstm_gates, mlstm_output, qkv_prepare,
@@ -25,6 +27,7 @@ __all__ = [
     "NativeError", "OutOfBlocks", "dtype_code", "embed_gather", "add_rmsnorm", "silu_mul", "linear", "linear_silu_mul",
     "silu_mul_is_fused", "qkv_fused_ok", "qkv_norm_rope_kv", "linear_tc", "device_status", "qk_norm_rope_kv", "rope_table", "rope_table_tiled",
     "attention", "attention_rowwise", "sample", "to_float", "require_cuda_kernels", "Pool8", "read_cache",
+    "LowRank", "AdapterRows", "sample_filtered",
 ]
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
@@ -259,7 +262,8 @@ def _tc_decode_ok(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | Non
     return m >= 9 and n * k * 2 <= (16 << 20)
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = None, stream=None, low_rank: LowRank | None = None,
+           adapter_rows: AdapterRows | None = None) -> torch.Tensor:
     """x [M, K] times weight[N, K]^T -> [M, N].
 
     float32: this package's FFMA kernel (true 32-bit, fixed summation order per element).
@@ -268,7 +272,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
     bfloat16 otherwise: this package's tcgen05 kernel where it is the faster choice
     (``tc_gemm_ok``), else the vendor library's matrix product with float32 accumulation.
     ``out`` may be float32 (logits) or bfloat16.
+    ``low_rank`` and ``adapter_rows`` (both or neither): the tokens' adapters beside the product (``ops/adapters.py``).
     """
+    if low_rank is not None or adapter_rows is not None:
+        return adapters.linear(x, weight, out, _stream(stream), low_rank, adapter_rows)
     _check_dev(x, weight, out)
     m, kdim = x.shape
     n = weight.shape[0]
@@ -382,12 +389,15 @@ def silu_mul_is_fused(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) 
     return _skinny_ok(x, weight) or (x.shape[0] > SKINNY_MAX_M and tc_gemm_ok(x, weight, out, "silu_mul"))
 
 
-def linear_silu_mul(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scratch=None, stream=None) -> torch.Tensor:
+def linear_silu_mul(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scratch=None, stream=None, low_rank: LowRank | None = None,
+                    adapter_rows: AdapterRows | None = None) -> torch.Tensor:
     """out [M, I] = silu(x Wg^T) * (x Wu^T) for the stacked weight [2I, K] (gate rows, then up rows;
     miniserve/model/qwen3.py:128-131). bfloat16 with at most 16 rows: one weight-streaming kernel
     whose CTAs hold a gate row and its up row together. More rows: the 2-CTA tcgen05 kernel with
     the activation in its epilogue where that is the faster choice (``tc_gemm_ok``); otherwise the
-    product into ``scratch`` ([M, 2I], allocated if None) and the activation kernel."""
+    product into ``scratch`` ([M, 2I], allocated if None) and the activation kernel. ``low_rank`` and ``adapter_rows``: as ``linear``'s."""
+    if low_rank is not None or adapter_rows is not None:
+        return adapters.linear_silu_mul(x, weight, out, scratch, _stream(stream), low_rank, adapter_rows)
     m, kdim = x.shape
     inter = out.shape[1]
     assert weight.shape == (2 * inter, kdim) and out.shape[0] == m and out.dtype == x.dtype
