@@ -8,6 +8,8 @@
 // Masses are integers: exp(z - max) in 64-bit floating point, times 2^bits, rounded to the nearest (bits: as many as leave room for the sum of the whole row, at most
 // 45). Sums of integers do not depend on their order, so the same row gives the same token whatever adds it up, and borders fall where 64 bits put them: a
 // mass is off by 2^-46 of the likeliest token's at most, and tokens below that have none.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace ms {
@@ -20,194 +22,442 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-struct RowFilter {
-  float zmax;      // the largest logit
-  double t;
-  double unit;     // 2^bits
-  double min_p;
-  uint32_t key;    // kept: places above `key`, and those at it up to index `last`
-  int last;
-};
+typedef unsigned long long u64;
+namespace cg = cooperative_groups;
 
-// exp(z - max) of a logit, 0 .. 1
-__device__ __forceinline__ double likeness(float x, const RowFilter& f) {
+// A token's place in a row: its logit's, then (of equals) the earlier one first. Larger is likelier, and no two are the same.
+constexpr int INDEX_BITS = 20;
+__device__ __forceinline__ u64 place_of(float x, int v) { return ((u64)order_of(x) << INDEX_BITS) | (u64)((1 << INDEX_BITS) - 1 - v); }
+__device__ __forceinline__ int index_of(u64 place) { return (1 << INDEX_BITS) - 1 - (int)(place & ((1 << INDEX_BITS) - 1)); }
+__device__ __forceinline__ float logit_of(u64 place) {
+  const uint32_t key = (uint32_t)(place >> INDEX_BITS);
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+// What makes a mass of a logit.
+struct Scale {
+  float zmax;   // the row's largest logit
+  double t;
+  double unit;  // 2^bits
+};
+// exp(z - max), 0 .. 1
+__device__ __forceinline__ double likeness(float x, const Scale& f) {
   if (x == f.zmax) return 1.0;
-  if (x == -INFINITY) return 0.0;
+  if (x == -INFINITY || f.zmax == INFINITY) return 0.0;
   return exp(((double)x - (double)f.zmax) / f.t);
 }
-__device__ __forceinline__ unsigned long long mass_of(float x, const RowFilter& f) { return (unsigned long long)__double2ll_rn(likeness(x, f) * f.unit); }
+__device__ __forceinline__ u64 to_mass(double like, const Scale& f) { return (u64)__double2ll_rn(like * f.unit); }
 
-constexpr int SF_THREADS = 1024;
-struct Sums {
-  unsigned long long mass;
-  int count;
+// A row belongs to a cluster of CTAs, each of which keeps its stretch of the logits in shared memory. A filter's cut is a place, found by a histogram over the fall below the
+// largest logit (BINS bins up to where masses end), then the places of the one bin that the cut falls into, sorted. top-k alone, or ahead of the
+// other filters, leaves a short list, on which one CTA does all that is left. Everything that is added up is whole numbers.
+constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32, SF_CTAS = 8, BINS = 1024, LIST = 1024, LIMB = 15;
+
+struct SfShared {
+  u64 xchg[2][SF_CTAS][2];  // two numbers of every CTA of the cluster, two turns
+  u64 red[SF_WARPS][2];
+  u64 said[4];              // what one CTA tells all
+  union {
+    u64 list[LIST];               // (the first CTA's) places of one bin, or of all that is left
+    uint32_t merged_count[BINS];  // counts of this CTA's share of the bins, over the cluster
+  };
+  union {
+    u64 sums[LIST];
+    u64 merged[BINS];  // their masses
+  };
+  uint32_t count[BINS], limb[3][BINS];
+  int listed;
 };
-__device__ __forceinline__ Sums block_sums(Sums s, Sums* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s.mass += __shfl_xor_sync(0xffffffffu, s.mass, o);
-    s.count += __shfl_xor_sync(0xffffffffu, s.count, o);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = s;
-  __syncthreads();
-  Sums all{0, 0};
-  for (int w = 0; w < SF_THREADS / 32; ++w) {
-    all.mass += scratch[w].mass;
-    all.count += scratch[w].count;
-  }
-  return all;
-}
 
-// A block per row; every search looks at the whole row again.
-__global__ void __launch_bounds__(SF_THREADS)
-sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logits, const float* __restrict__ temperature, const void* __restrict__ uniform,
-                       const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, int vocab, int bits, int uniform64) {
-  __shared__ Sums scratch[SF_THREADS / 32];
-  __shared__ unsigned long long before_warp[SF_THREADS / 32 + 1];
-  __shared__ int found;
-  pdl_prologue(tokens, logits, temperature, uniform, top_k, top_p, min_p);
-  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const double u = uniform64 ? reinterpret_cast<const double*>(uniform)[r] : (double)reinterpret_cast<const float*>(uniform)[r];
-  if (!(u >= 0.0 && u < 1.0)) return;
-  const float* lg = logits + (size_t)r * vocab;
-  const float t = temperature[r];
-  RowFilter f;
-  // the largest, by its place in the order
-  uint32_t best = 0;
-  for (int v = threadIdx.x; v < vocab; v += SF_THREADS) best = max(best, order_of(clean(lg[v])));
-  best = __reduce_max_sync(0xffffffffu, best);
-  __syncthreads();
-  if (lane == 0) scratch[warp].count = (int)best;
-  if (threadIdx.x == 0) found = 0x7fffffff;
-  __syncthreads();
-  for (int w = 0; w < SF_THREADS / 32; ++w) best = max(best, (uint32_t)scratch[w].count);
-  __syncthreads();
-  if (best <= order_of(-INFINITY) || !(t > 0.f)) {
-    // nothing but -inf, or the likeliest token: the first at the largest
-    for (int v = threadIdx.x; v < vocab; v += SF_THREADS)
-      if (order_of(clean(lg[v])) == best) {
-        atomicMin(&found, v);
-        break;
-      }
+struct Cluster {
+  cg::cluster_group group;
+  SfShared& sh;
+  int rank, ctas, turn;
+
+  // a and b added up (or the largest taken) over all threads of all CTAs; the same in every thread
+  template <bool MAX>
+  __device__ __forceinline__ void reduce(u64& a, u64& b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto join = [](u64 x, u64 y) { return MAX ? (x > y ? x : y) : x + y; };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
+      b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+    if (lane == 0) {
+      sh.red[warp][0] = a;
+      sh.red[warp][1] = b;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) tokens[r] = best <= order_of(-INFINITY) ? 0 : found;
-    return;
+    if (warp == 0) {
+      a = lane < SF_WARPS ? sh.red[lane][0] : 0;
+      b = lane < SF_WARPS ? sh.red[lane][1] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
+        b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
+      }
+      if (lane < ctas) {
+        u64* to = group.map_shared_rank(&sh.xchg[turn][rank][0], lane);
+        to[0] = a;
+        to[1] = b;
+      }
+    }
+    group.sync();
+    a = sh.xchg[turn][0][0];
+    b = sh.xchg[turn][0][1];
+    for (int c = 1; c < ctas; ++c) {
+      a = join(a, sh.xchg[turn][c][0]);
+      b = join(b, sh.xchg[turn][c][1]);
+    }
+    turn ^= 1;
   }
-  f.zmax = __uint_as_float((best & 0x80000000u) ? best & 0x7fffffffu : ~best);
-  f.t = (double)t;
-  f.unit = (double)(1ull << bits);
-  f.key = 0;
-  f.last = 0x7fffffff;
-  const float mp = min_p ? min_p[r] : 0.f;
-  f.min_p = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-  auto kept_key = [&](uint32_t key, int v) { return key > f.key || (key == f.key && v <= f.last); };
-  // The cut of a filter: the largest key at which `enough` holds of the (mass, count) of what is kept and at or above it; of the tokens at the key itself the first `ties(above)`.
-  auto cut = [&](auto enough, auto ties) {
-    uint32_t lo = 0, hi = best;  // enough(lo) holds
-    while (lo < hi) {
-      const uint32_t mid = lo + ((hi - lo + 1) >> 1);
-      Sums s{0, 0};
-      for (int v = threadIdx.x; v < vocab; v += SF_THREADS) {
-        const float x = clean(lg[v]);
-        const uint32_t key = order_of(x);
-        if (key >= mid && kept_key(key, v)) {
-          s.mass += mass_of(x, f);
-          ++s.count;
+  // `said` of the CTA that has something to say (its first thread, before), in all of them
+  __device__ __forceinline__ void tell(const u64 (&what)[4]) {
+    for (int c = 0; c < ctas; ++c) {
+      u64* to = group.map_shared_rank(&sh.said[0], c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = what[i];
+    }
+  }
+};
+
+// sh.list[0 .. n) sorted, the largest first; n <= LIST.
+__device__ __forceinline__ void sort_list(u64* list, int n) {
+  int size = 32;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += SF_THREADS) list[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const int p = threadIdx.x;
+      if (p < size / 2) {
+        const int i = 2 * p - (p & (j - 1)), other = i + j;
+        const u64 x = list[i], y = list[other];
+        if (((i & k) == 0) ? x < y : x > y) {
+          list[i] = y;
+          list[other] = x;
         }
       }
-      s = block_sums(s, scratch);
-      if (enough(s)) lo = mid; else hi = mid - 1;
+      __syncthreads();
     }
-    Sums above{0, 0};
-    for (int v = threadIdx.x; v < vocab; v += SF_THREADS) {
-      const float x = clean(lg[v]);
-      const uint32_t key = order_of(x);
-      if (key > lo && kept_key(key, v)) {
-        above.mass += mass_of(x, f);
-        ++above.count;
-      }
-    }
-    above = block_sums(above, scratch);
-    const float at = __uint_as_float((lo & 0x80000000u) ? lo & 0x7fffffffu : ~lo);
-    const long long keep = ties(above, mass_of(at, f));
-    // the index of the keep-th token at the key, by bisection over indices
-    int first = 0, last = vocab - 1;
-    while (first < last) {
-      const int mid = (first + last) >> 1;
-      Sums s{0, 0};
-      for (int v = threadIdx.x; v <= mid; v += SF_THREADS)
-        if (order_of(clean(lg[v])) == lo && kept_key(lo, v)) ++s.count;
-      s = block_sums(s, scratch);
-      if (s.count >= keep) last = mid; else first = mid + 1;
-    }
-    f.last = (f.key == lo) ? min(f.last, first) : first;
-    f.key = lo;
-  };
-  const int k = top_k ? top_k[r] : 0;
-  if (k > 0 && k < vocab) cut([&](const Sums& s) { return s.count >= k; }, [&](const Sums& above, unsigned long long) { return (long long)k - above.count; });
-  const float p = top_p ? top_p[r] : 1.f;
-  auto total = [&]() {
-    Sums s{0, 0};
-    for (int v = threadIdx.x; v < vocab; v += SF_THREADS) {
-      const float x = clean(lg[v]);
-      if (kept_key(order_of(x), v)) {
-        const double like = likeness(x, f);
-        if (like >= f.min_p) s.mass += (unsigned long long)__double2ll_rn(like * f.unit);
-      }
-    }
-    return block_sums(s, scratch).mass;
-  };
-  if (p < 1.f) {
-    const double held = f.min_p;
-    f.min_p = 0.0;
-    // kept while the mass before is below the target, the likeliest in any case
-    const double target = fmax((double)p * (double)total(), 0.5);
-    f.min_p = held;
-    cut([&](const Sums& s) { return (double)s.mass >= target; },
-        [&](const Sums& above, unsigned long long each) {
-          const double n = ceil((target - (double)above.mass) / (double)each);
-          return n < 2147483647.0 ? (long long)n : 2147483647ll;
-        });
-  }
-  const unsigned long long all = total();
-  unsigned long long target = (unsigned long long)(u * (double)all);
-  if (target >= all) target = all - 1;
-  // the token whose mass takes the sum beyond the target: a stretch of the row a warp
-  const int per_warp = (vocab + SF_THREADS - 1) / SF_THREADS * 32, begin = min(vocab, warp * per_warp), end = min(vocab, begin + per_warp);
-  auto kept_mass = [&](int v) -> unsigned long long {
-    if (v >= end) return 0;
-    const float x = clean(lg[v]);
-    if (!kept_key(order_of(x), v)) return 0;
-    const double like = likeness(x, f);
-    return like >= f.min_p ? (unsigned long long)__double2ll_rn(like * f.unit) : 0;
-  };
-  unsigned long long mine = 0;
-  for (int v = begin + lane; v < end; v += 32) mine += kept_mass(v);
+}
+// the sums up to and with each of the n numbers in `sums` (n <= 2 SF_THREADS); returns nothing, all threads call it
+__device__ __forceinline__ void running_sums(u64* sums, int n, u64 (&red)[SF_WARPS][2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
+  u64 a = i < n ? sums[i] : 0, b = i + 1 < n ? sums[i + 1] : 0, s = a + b;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) before_warp[warp + 1] = mine;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    before_warp[0] = 0;
-    for (int w = 0; w < SF_THREADS / 32; ++w) before_warp[w + 1] += before_warp[w];
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += x;
   }
   __syncthreads();
-  if (before_warp[warp] <= target && target < before_warp[warp + 1]) {
-    unsigned long long before = before_warp[warp];
-    for (int v0 = begin; v0 < end; v0 += 32) {
-      unsigned long long sum = kept_mass(v0 + lane);
+  if (lane == 31) red[warp][0] = s;
+  __syncthreads();
+  u64 before = s - a - b;
+  for (int w = 0; w < warp; ++w) before += red[w][0];
+  if (i < n) sums[i] = before + a;
+  if (i + 1 < n) sums[i + 1] = before + a + b;
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(SF_THREADS)
+sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logits, const float* __restrict__ temperature, const void* __restrict__ uniform,
+                       const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, int vocab, int slice, int staged, int bits,
+                       int uniform64) {
+  extern __shared__ __align__(16) float sf_logits[];
+  __shared__ SfShared sh;
+  cg::cluster_group group = cg::this_cluster();
+  Cluster cl{group, sh, (int)group.block_rank(), (int)group.num_blocks(), 0};
+  pdl_prologue(tokens, logits, temperature, uniform, top_k, top_p, min_p);
+  const int ctas = cl.ctas, rank = cl.rank, r = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const double u = uniform64 ? reinterpret_cast<const double*>(uniform)[r] : (double)reinterpret_cast<const float*>(uniform)[r];
+  if (!(u >= 0.0 && u < 1.0)) return;  // (the whole cluster)
+  const float t = temperature[r];
+  const int k = top_k ? top_k[r] : 0;
+  const float p = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
+  const double least = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
+  const int begin = min(rank * slice, vocab), n = min(slice, vocab - begin);
+  const float* xs = logits + (size_t)r * vocab + begin;
+
+  // the likeliest token, and the smallest finite logit
+  u64 best = 0, lowest = 0;
+  auto meet = [&](float x, int i) {
+    x = clean(x);
+    const u64 place = place_of(x, begin + i);
+    best = place > best ? place : best;
+    const u64 low = x > -INFINITY ? (u64)~order_of(x) : 0;
+    lowest = low > lowest ? low : lowest;
+    return x;
+  };
+  if (staged && (reinterpret_cast<uintptr_t>(xs) & 15) == 0) {
+    for (int i = 4 * tid; i + 3 < n; i += 4 * SF_THREADS) {
+      float4 x = *reinterpret_cast<const float4*>(xs + i);
+      x.x = meet(x.x, i);
+      x.y = meet(x.y, i + 1);
+      x.z = meet(x.z, i + 2);
+      x.w = meet(x.w, i + 3);
+      *reinterpret_cast<float4*>(sf_logits + i) = x;
+    }
+    for (int i = (n & ~3) + tid; i < n; i += SF_THREADS) sf_logits[i] = meet(xs[i], i);
+  } else {
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const float x = meet(xs[i], i);
+      if (staged) sf_logits[i] = x;
+    }
+  }
+  for (int i = tid; i < BINS; i += SF_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0;
+  if (tid == 0) sh.listed = 0;
+  cl.reduce<true>(best, lowest);
+  const float zmax = logit_of(best);
+  if (!(t > 0.f) || zmax == -INFINITY) {
+    if (rank == 0 && tid == 0) tokens[r] = zmax == -INFINITY ? 0 : index_of(best);
+    return;
+  }
+  const float* mine = staged ? sf_logits : xs;
+  const Scale f{zmax, (double)t, (double)(1ull << bits)};
+  // Bins by the fall below the largest: up to the least finite logit, and no further than masses go (2^-46 is 31.9 falls of T).
+  const float floor_ = logit_of(((u64)~(uint32_t)lowest) << INDEX_BITS);
+  const float width = fminf((float)BINS / fmaxf(fminf(zmax - floor_, 32.f * t), 1e-35f), 1e37f);
+  auto bin_of = [&](float x) { return x == zmax ? 0 : (int)fminf((zmax - x) * width, (float)(BINS - 1)); };
+
+  u64 cut = 0;  // kept: places from here on
+  auto counted = [&](float x, int v) { return x > -INFINITY && place_of(x, v) >= cut; };
+  // Where the running sum over the bins, likeliest first, is `enough` for the first time: said[0] the bin, [1] the count and [2] the mass before it, [3] its count.
+  auto crossing = [&](auto enough) {
+    const int per = BINS / ctas;
+    u64 count = 0, mass = 0;
+    for (int i = tid; i < per; i += SF_THREADS) {
+      const int bin = rank * per + i;
+      u64 c = 0, m = 0;
+      for (int q = 0; q < ctas; ++q) {
+        const SfShared* other = group.map_shared_rank(&sh, q);
+        c += other->count[bin];
+        m += (u64)other->limb[0][bin] + ((u64)other->limb[1][bin] << LIMB) + ((u64)other->limb[2][bin] << (2 * LIMB));
+      }
+      sh.merged_count[i] = (uint32_t)c;
+      sh.merged[i] = m;
+      count += c;
+      mass += m;
+    }
+    const int turn = cl.turn;
+    cl.reduce<false>(count, mass);  // (every CTA's sums are in xchg[turn]; the totals in count and mass)
+    u64 cb = 0, mb = 0;
+    for (int q = 0; q < rank; ++q) {
+      cb += sh.xchg[turn][q][0];
+      mb += sh.xchg[turn][q][1];
+    }
+    if (warp == 0 && !(rank > 0 && enough(cb, mb, count, mass)) && (enough(cb + sh.xchg[turn][rank][0], mb + sh.xchg[turn][rank][1], count, mass) || rank == ctas - 1)) {
+      // this CTA's: lanes take runs of its bins
+      const int each = per / 32;
+      u64 c = 0, m = 0;
+      for (int i = 0; i < each; ++i) {
+        c += sh.merged_count[lane * each + i];
+        m += sh.merged[lane * each + i];
+      }
+      u64 ci = c, mi = m;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long other = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += other;
+        const u64 x = __shfl_up_sync(0xffffffffu, ci, o), y = __shfl_up_sync(0xffffffffu, mi, o);
+        if (lane >= o) {
+          ci += x;
+          mi += y;
+        }
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + sum > target);
+      const unsigned hit = __ballot_sync(0xffffffffu, enough(cb + ci, mb + mi, count, mass));
+      if (lane == (hit ? __ffs(hit) - 1 : 31)) {
+        u64 c1 = cb + ci - c, m1 = mb + mi - m;
+        int i = 0;
+        for (; i + 1 < each; ++i) {
+          const u64 c2 = c1 + sh.merged_count[lane * each + i], m2 = m1 + sh.merged[lane * each + i];
+          if (enough(c2, m2, count, mass)) break;
+          c1 = c2;
+          m1 = m2;
+        }
+        const u64 what[4] = {(u64)(rank * per + lane * each + i), c1, m1, sh.merged_count[lane * each + i]};
+        cl.tell(what);
+      }
+    }
+    group.sync();
+    return mass;
+  };
+  // The cut itself, the place at which `enough` comes true, within bin said[0]: by its places sorted in the first CTA; of more than those hold, by halving the range.
+  auto settle = [&](auto enough, u64 all_count, u64 all_mass) {
+    const int bin = (int)sh.said[0];
+    const u64 cb = sh.said[1], mb = sh.said[2], members = sh.said[3];
+    if (members == 0) return;  // (fewer tokens than top-k would keep)
+    if (members <= LIST) {
+      SfShared* first = group.map_shared_rank(&sh, 0);
+      for (int i = tid; i < n; i += SF_THREADS) {
+        const float x = clean(mine[i]);
+        if (!counted(x, begin + i) || bin_of(x) != bin) continue;
+        const int at = atomicAdd(&first->listed, 1);
+        if (at < LIST) first->list[at] = place_of(x, begin + i);
+      }
+      group.sync();
+      if (rank == 0) {
+        const int have = min(sh.listed, LIST);
+        sort_list(sh.list, have);
+        for (int i = tid; i < have; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of(sh.list[i]), f), f);
+        __syncthreads();
+        running_sums(sh.sums, have, sh.red);
+        for (int i = tid; i < have; i += SF_THREADS) {
+          const bool now = enough(cb + i + 1, mb + sh.sums[i], all_count, all_mass);
+          const bool then = i > 0 && enough(cb + i, mb + sh.sums[i - 1], all_count, all_mass);
+          if ((now && !then) || (i == have - 1 && !now)) {
+            const u64 what[4] = {sh.list[i], 0, 0, 0};
+            cl.tell(what);
+          }
+        }
+        __syncthreads();
+        if (tid == 0) sh.listed = 0;
+      }
+      group.sync();
+      cut = sh.said[0];
+    } else {
+      u64 hi = 0, lo = 0;  // the bin's largest place, and its smallest
+      for (int i = tid; i < n; i += SF_THREADS) {
+        const float x = clean(mine[i]);
+        if (!counted(x, begin + i) || bin_of(x) != bin) continue;
+        const u64 place = place_of(x, begin + i);
+        hi = place > hi ? place : hi;
+        lo = ~place > lo ? ~place : lo;
+      }
+      cl.reduce<true>(hi, lo);
+      lo = ~lo;
+      while (lo < hi) {  // the largest place that is enough
+        const u64 mid = lo + ((hi - lo + 1) >> 1);
+        u64 count = 0, mass = 0;
+        for (int i = tid; i < n; i += SF_THREADS) {
+          const float x = clean(mine[i]);
+          const u64 place = place_of(x, begin + i);
+          if (place < mid || !counted(x, begin + i) || bin_of(x) != bin) continue;
+          ++count;
+          mass += to_mass(likeness(x, f), f);
+        }
+        cl.reduce<false>(count, mass);
+        if (enough(cb + count, mb + mass, all_count, all_mass)) lo = mid; else hi = mid - 1;
+      }
+      cut = lo;
+    }
+  };
+  auto histogram = [&](bool masses) {
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const float x = clean(mine[i]);
+      if (!counted(x, begin + i)) continue;
+      const int bin = bin_of(x);
+      atomicAdd(&sh.count[bin], 1u);
+      if (masses) {
+        const u64 m = to_mass(likeness(x, f), f);
+        atomicAdd(&sh.limb[0][bin], (uint32_t)m & ((1u << LIMB) - 1));
+        atomicAdd(&sh.limb[1][bin], (uint32_t)(m >> LIMB) & ((1u << LIMB) - 1));
+        atomicAdd(&sh.limb[2][bin], (uint32_t)(m >> (2 * LIMB)));
+      }
+    }
+    group.sync();
+  };
+
+  if (k > 0 && k < vocab) {
+    histogram(false);
+    auto enough = [k](u64 count, u64, u64, u64) { return count >= (u64)k; };
+    crossing(enough);
+    const u64 listed = sh.said[1] + sh.said[3];
+    if (listed <= LIST) {
+      // all that top-k can leave is a short list: the first CTA finishes the row
+      SfShared* first = group.map_shared_rank(&sh, 0);
+      const int bin = (int)sh.said[0];
+      for (int i = tid; i < n; i += SF_THREADS) {
+        const float x = clean(mine[i]);
+        if (!counted(x, begin + i) || bin_of(x) > bin) continue;
+        const int at = atomicAdd(&first->listed, 1);
+        if (at < LIST) first->list[at] = place_of(x, begin + i);
+      }
+      group.sync();
+      if (rank) return;
+      const int have = min(sh.listed, LIST), kept_k = min(have, k);
+      sort_list(sh.list, have);
+      for (int i = tid; i < kept_k; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of(sh.list[i]), f), f);
+      __syncthreads();
+      running_sums(sh.sums, kept_k, sh.red);
+      // what is kept is a run from the likeliest on
+      const double target = p < 1.f ? fmax((double)p * (double)sh.sums[kept_k - 1], 0.5) : INFINITY;
+      int kept = 0;
+      for (int i = tid; i < kept_k; i += SF_THREADS)
+        if ((i == 0 || (double)sh.sums[i - 1] < target) && likeness(logit_of(sh.list[i]), f) >= least) ++kept;
+      kept = __reduce_add_sync(0xffffffffu, kept);
+      __syncthreads();
+      if (lane == 0) sh.red[warp][0] = kept;
+      __syncthreads();
+      kept = 0;
+      for (int w = 0; w < SF_WARPS; ++w) kept += (int)sh.red[w][0];
+      const u64 all = sh.sums[kept - 1];
+      u64 aim = (u64)(u * (double)all);
+      if (aim >= all) aim = all - 1;
+      // in the order of the vocabulary: places by what they have of the index, which falls with it
+      u64 held[LIST / SF_THREADS];
+#pragma unroll
+      for (int q = 0; q < LIST / SF_THREADS; ++q) {
+        const int i = tid + q * SF_THREADS;
+        if (i < kept) held[q] = sh.list[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < LIST / SF_THREADS; ++q) {
+        const int i = tid + q * SF_THREADS;
+        if (i < kept) sh.list[i] = (held[q] << 44) | (held[q] >> INDEX_BITS);  // the index in front, its complement: earlier tokens are larger
+      }
+      __syncthreads();
+      sort_list(sh.list, kept);
+      for (int i = tid; i < kept; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of((sh.list[i] & 0xffffffffull) << INDEX_BITS), f), f);
+      __syncthreads();
+      running_sums(sh.sums, kept, sh.red);
+      for (int i = tid; i < kept; i += SF_THREADS)
+        if (sh.sums[i] > aim && (i == 0 || sh.sums[i - 1] <= aim)) tokens[r] = (1 << INDEX_BITS) - 1 - (int)(sh.list[i] >> 44);
+      return;
+    }
+    settle(enough, 0, 0);
+    for (int i = tid; i < BINS; i += SF_THREADS) sh.count[i] = 0;
+    __syncthreads();
+  }
+  if (p < 1.f) {
+    histogram(true);
+    const double part = (double)p;
+    auto enough = [part](u64, u64 mass, u64, u64 all) { return (double)mass >= fmax(part * (double)all, 0.5); };
+    const u64 all = crossing(enough);
+    settle(enough, 0, all);
+  }
+  // the token whose mass takes the sum beyond u of all: a stretch of the CTA's tokens a warp
+  const int per_warp = ((n + SF_WARPS - 1) / SF_WARPS + 31) / 32 * 32, wb = min(warp * per_warp, n), we = min(wb + per_warp, n);
+  auto mass_at = [&](int i) -> u64 {
+    if (i >= we) return 0;
+    const float x = clean(mine[i]);
+    if (!counted(x, begin + i)) return 0;
+    const double like = likeness(x, f);
+    return like >= least ? to_mass(like, f) : 0;
+  };
+  u64 sum = 0, none = 0;
+  for (int i = wb + lane; i < we; i += 32) sum += mass_at(i);
+  const int turn = cl.turn;
+  cl.reduce<false>(sum, none);  // (a warp's sums are left in red)
+  u64 aim = (u64)(u * (double)sum);
+  if (aim >= sum) aim = sum - 1;
+  u64 before = 0;
+  for (int q = 0; q < rank; ++q) before += sh.xchg[turn][q][0];
+  for (int w = 0; w < warp; ++w) before += sh.red[w][0];
+  if (before <= aim && aim < before + sh.red[warp][0]) {
+    for (int i0 = wb; i0 < we; i0 += 32) {
+      u64 s = mass_at(i0 + lane);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + s > aim);
       if (hit) {
-        if (lane == 0) tokens[r] = v0 + __ffs(hit) - 1;
+        if (lane == 0) tokens[r] = begin + i0 + __ffs(hit) - 1;
         break;
       }
-      before += __shfl_sync(0xffffffffu, sum, 31);
+      before += __shfl_sync(0xffffffffu, s, 31);
     }
   }
 }
@@ -222,12 +472,21 @@ MS_DEFINE_PDL_SWITCH(ms_filters_set_pdl)
 // top_k, top_p, min_p: a number per row, or null. uniform: float64 (uniform64 = 1) or float32.
 MS_EXPORT int ms_sample_filtered(int* tokens, const float* logits, const float* temperature, const void* uniform, const int* top_k, const float* top_p,
                                  const float* min_p, int rows, int vocab, int uniform64, cudaStream_t stream) {
-  MS_CHECK_ARG(rows >= 0 && vocab > 0, "sample_filtered: bad sizes rows=%d vocab=%d", rows, vocab);
+  MS_CHECK_ARG(rows >= 0 && vocab > 0 && vocab <= (1 << INDEX_BITS), "sample_filtered: bad sizes rows=%d vocab=%d", rows, vocab);
   MS_CHECK_ARG(tokens && logits && temperature && uniform, "sample_filtered: null pointer");
   if (rows == 0) return 0;
   int bits = 62;  // a row's sum stays within 2^62
   while ((1ll << (62 - bits)) < vocab) --bits;
-  if (bits > 45) bits = 45;
-  MS_LAUNCH(sample_filtered_kernel, rows, SF_THREADS, 0, stream, tokens, logits, temperature, uniform, top_k, top_p, min_p, vocab, bits, uniform64);
+  if (bits > 3 * LIMB) bits = 3 * LIMB;
+  const int ctas = vocab >= 16384 ? SF_CTAS : 1, slice = ceil_div(ceil_div(vocab, ctas), 32) * 32;
+  MS_CHECK_ARG((long long)rows * ctas <= 0x7fffffffLL, "sample_filtered: %d rows are too many for one launch", rows);
+  const size_t smem = (size_t)slice * sizeof(float);
+  const int staged = smem <= 160 * 1024;  // (longer rows are read again for each search)
+  if (staged) {
+    static std::atomic<unsigned long long> allowed{0};
+    MS_CHECK_CUDA(allow_shared_memory((const void*)sample_filtered_kernel, 160 * 1024, allowed));
+  }
+  MS_LAUNCH_CLUSTERED(sample_filtered_kernel, rows * ctas, SF_THREADS, staged ? smem : 0, stream, ctas, tokens, logits, temperature, uniform, top_k, top_p, min_p,
+                      vocab, slice, staged, bits, uniform64);
   return 0;
 }
