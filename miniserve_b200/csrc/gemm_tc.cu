@@ -16,6 +16,9 @@
 // the fused epilogue, flashinfer.silu_and_mul after the gate_up product (miniserve/model/fused.py:195).
 
 
+#include <type_traits>
+
+#include "adapters.cuh"
 #include "common.cuh"
 #include "tensor_map.cuh"
 
@@ -666,6 +669,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
       ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(c0), "r"(c1) : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
 __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
   const uint32_t acc = accumulate ? 1u : 0u;
   asm volatile(
@@ -860,13 +868,27 @@ constexpr int PAIR_OUT_BYTES = TC_BM * 64 * 2;  // one [128][64] bfloat16 tile o
 // per CTA and stage: 128 rows of A and half of the tile's BN rows of W, 64 k each
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return (TC_BM + bn / 2) * TC_BK * 2; }
 
+// ADAPTED: low-rank adapters of the tokens' requests are a few k-blocks more of the tiles that have such tokens. The plan (adapters.cuh) lists for a row tile
+// the adapters in it; for each, A's block is V, the numbers that the adapter made of those tokens (zeros in the other rows), and W's is the adapter's B. A
+// stacked projection has these for each part that the tile's columns belong to: B's map of a part has that part's rows alone, so a copy reads zeros beyond it, as it
+// does beyond the rank. One k-block of 64 holds a rank of 64, so an adapter costs a tile 1/64 of its products at K = 4,096, and the sum is rounded once.
+struct AdaptedTiles {
+  CUtensorMap map_v;                // [blocks * 256, parts * rank]
+  CUtensorMap map_b[MAX_PARTS];     // [slots][the part's rows][rank]
+  const int* tile_first;            // the first block of each row tile, and where the last one's end
+  const int* block_slot;
+  int parts, rank, ends[MAX_PARTS];
+};
+struct NoAdapters {};
+
 // GROUPED: the row tiles are the plan's (256 sorted rows of one matrix each); a tile's rows beyond its run are computed with the run's matrix and not
 // stored. Row tiles change fastest here too: a run has two or three of them, which then take a tile of W from L2 together.
-template <int BN, int STAGES, int EPI, bool GROUPED = false>
+template <int BN, int STAGES, int EPI, bool GROUPED = false, bool ADAPTED = false>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_out, void* __restrict__ out,
-                    int M, int N_out, int K, int up_row_offset, int* __restrict__ status, const QkvEpilogue qe, const TcGroups grp) {
+                    int M, int N_out, int K, int up_row_offset, int* __restrict__ status, const QkvEpilogue qe, const TcGroups grp,
+                    const __grid_constant__ std::conditional_t<ADAPTED, AdaptedTiles, NoAdapters> ad) {
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
@@ -925,6 +947,23 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   // a tile's first row for this CTA, the matrix it belongs to and the end of that matrix's rows
   auto first_row = [&](int tile) { return (GROUPED ? grp.tiles[2 * tile_m(tile) + 1] : tile_m(tile) * 2 * TC_BM) + (int)rank * TC_BM; };
   auto matrix_of = [&](int tile) { return GROUPED ? grp.tiles[2 * tile_m(tile)] : 0; };
+  // ADAPTED: whether part p has rows of W in the tile, and how many k-blocks the tile's adapters are
+  auto meets = [&](int p, int n0) {
+    if constexpr (ADAPTED) {
+      const int from = p ? ad.ends[p - 1] : 0, to = ad.ends[p];
+      return (n0 < to && n0 + COLS > from) || (tc_gated(EPI) && up_row_offset + n0 < to && up_row_offset + n0 + COLS > from);
+    }
+    return false;
+  };
+  auto adapter_blocks = [&](int tile) {
+    int more = 0;
+    if constexpr (ADAPTED) {
+      const int n0 = tile_n(tile) * COLS, m = tile_m(tile);
+      for (int p = 0; p < ad.parts; ++p) more += meets(p, n0);
+      more *= (ad.tile_first[m + 1] - ad.tile_first[m]) * ((ad.rank + TC_BK - 1) / TC_BK);
+    }
+    return more;
+  };
 
   if (warp == 0) {
     if (elect_one()) {
@@ -947,6 +986,25 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
           tma_load_2d_pair(a_tile, &map_a, &full_bar[s], it * TC_BK, m0);
           tma_load_2d_pair(a_tile + A_BYTES, &map_w, &full_bar[s], it * TC_BK, w_row);
         }
+        if constexpr (ADAPTED) {
+          const int last = ad.tile_first[tile_m(tile) + 1];
+          for (int b = ad.tile_first[tile_m(tile)]; b < last && ok; ++b)
+            for (int p = 0; p < ad.parts && ok; ++p) {
+              if (!meets(p, n0)) continue;
+              for (int c = 0; c < ad.rank; c += TC_BK, ++kb) {
+                const int s = kb % STAGES;
+                if (kb >= STAGES && !mbar_wait(&empty_bar[s], ((kb / STAGES) - 1) & 1)) {
+                  atomicExch(status, 11);
+                  ok = false;
+                  break;
+                }
+                unsigned char* a_tile = smem + (size_t)s * STAGE_BYTES;
+                if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * STAGE_BYTES);  // (what a copy fills with zeros counts too)
+                tma_load_2d_pair(a_tile, &ad.map_v, &full_bar[s], p * ad.rank + c, b * 2 * TC_BM + (int)rank * TC_BM);
+                tma_load_3d_pair(a_tile + A_BYTES, &ad.map_b[p], &full_bar[s], c, w_row - (p ? ad.ends[p - 1] : 0), ad.block_slot[b]);
+              }
+            }
+        }
         if (!ok) break;
       }
     }
@@ -964,7 +1022,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const uint32_t tmem_acc = tmem_base + (uint32_t)buf * BN;
-        for (int it = 0; it < k_iters; ++it, ++kb) {
+        const int iters = k_iters + (ADAPTED ? adapter_blocks(tile) : 0);
+        for (int it = 0; it < iters; ++it, ++kb) {
           const int s = kb % STAGES;
           if (!mbar_wait(&full_bar[s], (kb / STAGES) & 1)) {
             atomicExch(status, 12);
@@ -1413,7 +1472,61 @@ static int launch_tc_pair(void* out, const void* A, const void* W, int M, int N_
   MS_CHECK_ARG(tiles < (1LL << 30), "gemm_tc: too many tiles (%lld)", tiles);
   const long long pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
   MS_LAUNCH_CLUSTERED(kernel, (unsigned)(2 * pairs), PAIR_THREADS, smem, stream, 2, map_a, map_w, map_out, out, M, N_out, K,
-                      up_row_offset, status, qe, TcGroups{});
+                      up_row_offset, status, qe, TcGroups{}, NoAdapters{});
+  return 0;
+}
+
+// The maps of an adapted product: V as the plan's blocks lay it out, B by its parts.
+static int make_adapted(AdaptedTiles* tiles, const AdaptedProduct& ap) {
+  const Adapters& ad = ap.ad;
+  if (int rc = make_map(&tiles->map_v, ap.v, (long long)ap.max_blocks * 2 * TC_BM, (long long)ad.parts * ad.rank, TC_BM)) return rc;
+  TensorMapEncodeFn encode;
+  if (int rc = tensor_map_encoder(&encode)) return rc;
+  const int n = ad.ends[ad.parts - 1];
+  for (int p = 0; p < MAX_PARTS; ++p) {
+    const int q = p < ad.parts ? p : 0, from = q ? ad.ends[q - 1] : 0;
+    const cuuint64_t dims[3] = {(cuuint64_t)ad.rank, (cuuint64_t)(ad.ends[q] - from), (cuuint64_t)ad.slots};
+    const cuuint64_t strides[2] = {(cuuint64_t)ad.rank * 2, (cuuint64_t)n * ad.rank * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)TC_BK, (cuuint32_t)TC_BM, 1}, elem[3] = {1, 1, 1};
+    const CUresult res = encode(&tiles->map_b[p], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (__nv_bfloat16*)ad.b + (size_t)from * ad.rank, dims, strides, box, elem,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    MS_CHECK_ARG(res == CUDA_SUCCESS, "gemm_tc: cuTensorMapEncodeTiled failed with code %d (%d adapters of rank %d)", (int)res, ad.slots, ad.rank);
+    tiles->ends[p] = ad.ends[q];
+  }
+  tiles->tile_first = ap.tile_first;
+  tiles->block_slot = ap.block_slot;
+  tiles->parts = ad.parts;
+  tiles->rank = ad.rank;
+  return 0;
+}
+
+// The product with the tokens' adapters beside it (256-column tiles; EPI as launch_tc_pair's).
+template <int STAGES, int EPI>
+static int launch_tc_pair_adapted(void* out, const void* A, const void* W, int M, int N_out, int w_rows, int K, int up_row_offset, const AdaptedProduct& ap,
+                                  int* status, cudaStream_t stream, const QkvEpilogue& qe = QkvEpilogue{}) {
+  constexpr int BN = PAIR_BN, COLS = tc_gated(EPI) ? BN / 2 : BN;
+  CUtensorMap map_a, map_w, map_out;
+  AdaptedTiles tiles;
+  if (int rc = make_map(&map_a, A, M, K, TC_BM)) return rc;
+  if (int rc = make_map(&map_w, W, w_rows, K, BN / 2)) return rc;
+  if (int rc = make_adapted(&tiles, ap)) return rc;
+  map_out = map_a;
+  if (EPI == TC_QKV_ROPE) {
+    if (int rc = make_map(&map_out, out, M, (long long)qe.nq * 128, TC_BM)) return rc;
+  } else if (N_out % 8 == 0 && (uintptr_t)out % 16 == 0) {
+    if (int rc = make_map(&map_out, out, M, N_out, TC_BM)) return rc;
+  }
+  constexpr size_t smem = (size_t)STAGES * pair_stage_bytes(BN) + 4 * PAIR_OUT_BYTES + (EPI == TC_QKV_ROPE ? CS_RING_BYTES : 0) + 1024;
+  static_assert(smem <= 227 * 1024, "the ring does not fit shared memory");
+  auto kernel = gemm_tc_pair_kernel<BN, STAGES, EPI, false, true>;
+  static std::atomic<unsigned long long> allowed{0};
+  MS_CHECK_CUDA(allow_shared_memory((const void*)kernel, (int)smem, allowed));
+  const long long tile_count = (long long)ceil_div(N_out, COLS) * ceil_div(M, 2 * TC_BM), sms = sm_count();
+  MS_CHECK_ARG(tile_count < (1LL << 30) && sms >= 2, "gemm_tc: too many tiles (%lld)", tile_count);
+  const long long pairs = tile_count < sms / 2 ? tile_count : sms / 2;
+  MS_LAUNCH_CLUSTERED(kernel, (unsigned)(2 * pairs), PAIR_THREADS, smem, stream, 2, map_a, map_w, map_out, out, M, N_out, K, up_row_offset, status, qe,
+                      TcGroups{}, tiles);
   return 0;
 }
 
@@ -1438,7 +1551,7 @@ static int launch_tc_pair_grouped(void* out, const void* A, const void* W, int r
   MS_CHECK_ARG(tiles < (1LL << 30) && sms >= 2, "gemm_tc: too many tiles (%lld)", tiles);
   const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
   MS_LAUNCH_CLUSTERED(kernel, (unsigned)(2 * pairs), PAIR_THREADS, smem, stream, 2, map_a, map_w, map_out, out, rows, N_out, K, up_row_offset, status,
-                      QkvEpilogue{}, grp);
+                      QkvEpilogue{}, grp, NoAdapters{});
   return 0;
 }
 
@@ -1530,11 +1643,11 @@ MS_EXPORT int ms_gemm_tc_prefers(int M, int N, int K, int epilogue) {
 
 // q_out [M, nq, 128], k_pool / v_pool [pages + 1, nkv, page_size, 128] from x [M, K] and the stacked
 // weight [(nq + 2 nkv) * 128, K]: the q|k|v product with the per-head norm, the rotation and the cache
-// write in its epilogue (the 2-CTA kernel). nq and nkv even, head size 128, the whole head rotated.
+// write in its epilogue (the 2-CTA kernel). nq and nkv even, head size 128, the whole head rotated. ap: the tokens' adapters beside the product, or null.
 MS_EXPORT int ms_gemm_tc_qkv_bf16(void* q_out, const void* x, const void* w_qkv, int M, int K, int nq, int nkv, void* k_pool,
                                   void* v_pool, const void* q_norm_w, const void* k_norm_w, const float* cos_sin,
                                   const int* positions, const int* row_of_token, const int* page_indptr,
-                                  const int* page_indices, int page_size, float eps, int* status, cudaStream_t stream) {
+                                  const int* page_indices, int page_size, float eps, int* status, cudaStream_t stream, const AdaptedProduct* ap) {
   if (M == 0) return 0;
   MS_CHECK_ARG(M > 0 && K > 0 && K % 8 == 0, "gemm_tc: bad sizes M=%d K=%d", M, K);
   MS_CHECK_ARG(nq > 0 && nkv > 0 && nq % 2 == 0 && nkv % 2 == 0, "gemm_tc: the q|k|v epilogue takes even head counts, not %d and %d", nq, nkv);
@@ -1550,7 +1663,27 @@ MS_EXPORT int ms_gemm_tc_qkv_bf16(void* q_out, const void* x, const void* w_qkv,
   const QkvEpilogue qe = {(__nv_bfloat16*)k_pool, (__nv_bfloat16*)v_pool, (const __nv_bfloat16*)q_norm_w, (const __nv_bfloat16*)k_norm_w,
                           cos_sin, positions, row_of_token, page_indptr, page_indices, nq, nkv, shift, eps};
   const int n_total = (nq + 2 * nkv) * 128;
+  if (ap != nullptr) {
+    MS_CHECK_ARG(ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 && ap->ad.ends[ap->ad.parts - 1] == n_total,
+                 "gemm_tc: an adapted product needs a plan of its outputs");
+    return launch_tc_pair_adapted<4, TC_QKV_ROPE>(q_out, x, w_qkv, M, n_total, n_total, K, 0, *ap, status, stream, qe);
+  }
   return launch_tc_pair<256, 4, TC_QKV_ROPE>(q_out, x, w_qkv, M, n_total, n_total, K, 0, status, stream, qe);
+}
+
+// out [M, N] bfloat16 = A W^T beside the adapters of A's rows (epilogue 0), or silu(gate) * up of the stacked W [2 N, K] beside them (epilogue 2). V and the plan
+// are the launches' before this one (ms_adapter_plan, ms_adapter_shrink_blocks).
+MS_EXPORT int ms_gemm_tc_adapted_bf16(void* out, const void* A, const void* W, int M, int N, int K, int epilogue, const AdaptedProduct* ap, int* status,
+                                      cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  MS_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 8 == 0, "gemm_tc: bad sizes M=%d N=%d K=%d", M, N, K);
+  MS_CHECK_ARG(((uintptr_t)A % 16 == 0) && ((uintptr_t)W % 16 == 0), "gemm_tc: operands must be 16-byte aligned");
+  MS_CHECK_ARG(status != nullptr && ap != nullptr && ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 &&
+                   ap->ad.ends[ap->ad.parts - 1] == (epilogue == TC_SILU_MUL ? 2 * N : N),
+               "gemm_tc: an adapted product needs a status word and a plan of its outputs");
+  if (epilogue == TC_OUT_BF16) return launch_tc_pair_adapted<5, TC_OUT_BF16>(out, A, W, M, N, N, K, 0, *ap, status, stream);
+  if (epilogue == TC_SILU_MUL) return launch_tc_pair_adapted<5, TC_SILU_MUL>(out, A, W, M, N, 2 * N, K, N, *ap, status, stream);
+  return fail("gemm_tc: unknown epilogue %d of an adapted product", epilogue);
 }
 
 MS_EXPORT int ms_gemm_tc_bf16(void* out, const void* A, const void* W, int M, int N, int K, int epilogue, int* status,

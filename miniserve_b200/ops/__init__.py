@@ -275,7 +275,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
     ``low_rank`` and ``adapter_rows`` (both or neither): the tokens' adapters beside the product (``ops/adapters.py``).
     """
     if low_rank is not None or adapter_rows is not None:
-        return adapters.linear(x, weight, out, _stream(stream), low_rank, adapter_rows)
+        return adapters.linear(x, weight, out, stream, low_rank, adapter_rows)
     _check_dev(x, weight, out)
     m, kdim = x.shape
     n = weight.shape[0]
@@ -397,7 +397,7 @@ def linear_silu_mul(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, sc
     the activation in its epilogue where that is the faster choice (``tc_gemm_ok``); otherwise the
     product into ``scratch`` ([M, 2I], allocated if None) and the activation kernel. ``low_rank`` and ``adapter_rows``: as ``linear``'s."""
     if low_rank is not None or adapter_rows is not None:
-        return adapters.linear_silu_mul(x, weight, out, scratch, _stream(stream), low_rank, adapter_rows)
+        return adapters.linear_silu_mul(x, weight, out, stream, low_rank, adapter_rows)
     m, kdim = x.shape
     inter = out.shape[1]
     assert weight.shape == (2 * inter, kdim) and out.shape[0] == m and out.dtype == x.dtype
@@ -466,11 +466,13 @@ def qkv_fused_ok(x: torch.Tensor, w_qkv: torch.Tensor, nq: int, nkv: int, d: int
 def qkv_norm_rope_kv(q_out: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, x: torch.Tensor, w_qkv: torch.Tensor,
                      q_norm_w: torch.Tensor | None, k_norm_w: torch.Tensor | None, cos_sin: torch.Tensor | None, eps: float,
                      positions: torch.Tensor, row_of_token: torch.Tensor, page_indptr: torch.Tensor,
-                     page_indices: torch.Tensor, page_size: int, stream=None) -> None:
+                     page_indices: torch.Tensor, page_size: int, stream=None, low_rank: LowRank | None = None,
+                     adapter_rows: AdapterRows | None = None) -> None:
     """The q|k|v projection of x [T, K] with what follows it in its epilogue: per-head norm of q and
     k, rotation by position (``cos_sin``: the step's float32 table as ``rope_table_tiled`` lays it out, None for no rotation),
     q to ``q_out`` [T, nq, 128] and the new k, v into their pages. The same arithmetic as
-    ``linear`` followed by ``qk_norm_rope_kv``, without the [T, (nq + 2 nkv) * 128] tensor in between."""
+    ``linear`` followed by ``qk_norm_rope_kv``, without the [T, (nq + 2 nkv) * 128] tensor in between.
+    ``low_rank`` and ``adapter_rows``: as ``linear``'s."""
     _check_dev(q_out, k_pool, v_pool, x, w_qkv, q_norm_w, k_norm_w, cos_sin, positions, row_of_token, page_indptr, page_indices)
     t, nq, d = q_out.shape
     nkv = k_pool.shape[1]
@@ -478,10 +480,16 @@ def qkv_norm_rope_kv(q_out: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     assert x.dtype == torch.bfloat16 and w_qkv.shape == ((nq + 2 * nkv) * d, x.shape[1]) and x.shape[0] == t
     assert cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.shape == (2 * -(-t // 256), 8, 2, 128, 8))
     lib = native.gemm_tc()
+    product = v = None  # (v: what the product points to)
+    if low_rank is not None or adapter_rows is not None:
+        adapters.check(x, w_qkv, None, low_rank, adapter_rows, False)
+        if t == 0:
+            return
+        product, v = adapters.product(x, low_rank, adapter_rows, _stream(stream))
     native.kernel_check(lib.ms_gemm_tc_qkv_bf16(
         _ptr(q_out), _ptr(x), _ptr(w_qkv), t, x.shape[1], nq, nkv, _ptr(k_pool), _ptr(v_pool), _ptr(q_norm_w), _ptr(k_norm_w),
         _ptr(cos_sin), _ptr(positions), _ptr(row_of_token), _ptr(page_indptr), _ptr(page_indices), page_size, float(eps),
-        _ptr(device_status(x.device)), _stream(stream)), lib=lib, errfn="ms_gemm_tc_last_error")
+        _ptr(device_status(x.device)), _stream(stream), None if product is None else ctypes.addressof(product)), lib=lib, errfn="ms_gemm_tc_last_error")
 
 
 def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, num_tokens: int, rotary_dim: int, stream=None) -> torch.Tensor:

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 ONE = [(1, 2)]
 EIGHT = [(1, 0), (1, 3), (1, 3), (1, 1), (1, -1), (1, 0), (1, 2), (1, 1)]
-DECODE64 = [(1, (5 * i) % 5 - 1) for i in range(64)]
+DECODE64 = [(1, (7 * i) % 5 - 1) for i in range(64)]
 MIXED = [(1, i % 4) for i in range(20)] + [(0, 1), (157, 2), (1, -1), (33, 0)]
 PROMPTS = [(300, 1), (7, -1), (255, 3), (1, 0), (513, 1)]
 LONG = [(1531, 3), (517, 1)]
@@ -205,3 +205,43 @@ def test_refusals_on_the_device():
     with pytest.raises(ValueError, match="16 bytes"):
         shifted = torch.empty(8 * 256 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(8, 256)
         ops.linear(shifted, w, low_rank=low, adapter_rows=ar)
+
+
+@pytest.mark.parametrize("rows,rank,full", [(LONG[:1], 16, False), (LONG, 16, True), (PROMPTS, 72, True), (DECODE64 + PROMPTS, 8, True), ([(40, 1)], 24, False)])
+def test_qkv_with_norm_rotation_and_cache_write_behind(rows, rank, full):
+    """The q|k|v product's epilogue works on the adapted product: against the formula in 64 bits, carried through norm and rotation. The tolerance follows
+    the product's through them: a norm's factor moves with the mean of squares, a rotated number with both of its pair (first order, 5 % for the rest)."""
+    from miniserve_b200 import ops
+
+    from .kernel_util import PagedBatch
+
+    nq, nkv, d, page, hidden, eps = 4, 2, 128, 16, 1024, 1e-6
+    pb = PagedBatch([(3 * i, n) for i, (n, _) in enumerate(rows)], page, nkv, d, torch.bfloat16, seed=3)
+    x, w, low, ar = au.made(rows, hidden, (nq * d, nkv * d, nkv * d), rank, 4, torch.bfloat16, seed=rank)
+    t = x.shape[0]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    qw, kw = ((1 + 0.1 * torch.randn((d,), generator=gen, device="cuda")).bfloat16() for _ in range(2)) if full else (None, None)
+    inv_freq = (1.0 / (1e6 ** (torch.arange(0, d, 2, dtype=torch.float64) / d))).float().cuda()
+    table = ops.rope_table(pb.positions, inv_freq, t, d) if full else None
+    q = torch.full((t, nq, d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ops.qkv_norm_rope_kv(q, pb.k_pool, pb.v_pool, x, w, qw, kw, ops.rope_table_tiled(table) if full else None, eps, pb.positions, pb.row_of_token, pb.page_indptr,
+                         pb.page_indices, page, low_rank=low, adapter_rows=ar)
+    y, tol = (z.view(t, nq + 2 * nkv, d) for z in au.formula(x, w, low, ar))
+    want, off = [y[:, :nq], y[:, nq:nq + nkv], y[:, nq + nkv:]], [tol[:, :nq], tol[:, nq:nq + nkv], tol[:, nq + nkv:]]
+    if full:
+        cos, sin = table[:, None, :d // 2].double(), table[:, None, d // 2:].double()
+        for i, weight in enumerate((qw, kw)):
+            v, dv, g = want[i], off[i], weight.double()
+            inv = (v * v).mean(-1, keepdim=True).add(eps).rsqrt()
+            v, dv = v * inv * g, 1.05 * g.abs() * (inv * dv + v.abs() * inv ** 3 * (v.abs() * dv).mean(-1, keepdim=True))
+            (lo, hi), (dlo, dhi) = v.chunk(2, -1), dv.chunk(2, -1)
+            want[i] = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], -1)
+            off[i] = torch.cat([dlo * cos.abs() + dhi * sin.abs(), dhi * cos.abs() + dlo * sin.abs()], -1) + (2.0 ** -8 + 2.0 ** -18) * v.abs().amax(-1, keepdim=True) * 1.42
+    au.close(q, want[0], off[0])
+    at = 0
+    for r, (start, n) in enumerate(pb.rows):
+        for pool, i in ((pb.k_pool, 1), (pb.v_pool, 2)):
+            got = pb.read(r, pool, start + n)[start:]
+            au.close(got, want[i][at:at + n], off[i][at:at + n])
+        at += n
+    assert int(ops.device_status("cuda")) == 0
