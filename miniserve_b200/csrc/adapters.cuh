@@ -17,10 +17,10 @@ struct Adapters {
   const int* slot_of_row;
   const int* row_of_token;
   int* status;            // raised (6) by a slot that is not there
-  int slots, rank, parts, ends[MAX_PARTS];  // ends[p]: the first column behind part p
+  int slots, rank, parts, ends[MAX_PARTS];  // ends[p]: the first column behind part p (of parts that there are not, N)
 };
 
-// An adapted product of many tokens: what ms_adapter_plan and ms_adapter_shrink_blocks have written for it. A block is the tokens of one row tile that have
+// An adapted product of many tokens: what launches before it have written for it (ms_adapter_plan, ms_gemm_tc_adapter_v). A block is the tokens of one row tile that have
 // one adapter: 256 rows of V, zeros in those of other tokens.
 struct AdaptedProduct {
   Adapters ad;
@@ -30,9 +30,16 @@ struct AdaptedProduct {
   int max_blocks;
 };
 
-// The adapter's term of a product of few tokens, for its epilogue: sum_j B_s[n, j] v[t, p(n) rank + j].
-struct AdapterTerm {
-  const float* v;  // [T, parts * rank], null: no adapters
+// What a block is: its adapter, its row tile, and which of the tile's tokens have it, a bit each.
+struct AdapterBlock {
+  int slot, tile, pad[2];
+  unsigned members[ADAPTER_ROWS / 32];
+};
+static_assert(sizeof(AdapterBlock) == 48, "what the host allots");
+
+// An adapted product of few tokens: v float32 [T, parts * rank] (ms_adapter_shrink); rows of tokens without an adapter are not read.
+struct AdapterTerms {
+  const float* v;
   Adapters ad;
 };
 
@@ -45,9 +52,17 @@ __device__ __forceinline__ int adapter_of(const Adapters& ad, int t) {
 __device__ __forceinline__ int part_of(const Adapters& ad, int n) {
   int p = 0;
 #pragma unroll
-  for (int i = 0; i + 1 < MAX_PARTS; ++i)
-    if (i + 1 < ad.parts && n >= ad.ends[i]) p = i + 1;
+  for (int i = 0; i + 1 < MAX_PARTS; ++i) p += n >= ad.ends[i];
   return p;
+}
+
+// (host) Whether the sizes are ones that the kernels take.
+inline bool adapters_ok(const Adapters& ad, int N, int K) {
+  if (ad.slots < 1 || ad.rank < 8 || ad.rank % 8 || ad.parts < 1 || ad.parts > MAX_PARTS || K < 8 || K % 8) return false;
+  if ((uintptr_t)ad.a % 16 || (uintptr_t)ad.b % 16 || !ad.scale || !ad.slot_of_row || !ad.row_of_token || !ad.status) return false;
+  for (int p = 0; p < MAX_PARTS; ++p)
+    if (p + 1 < ad.parts ? ad.ends[p] <= (p ? ad.ends[p - 1] : 0) || ad.ends[p] >= N : ad.ends[p] != N) return false;
+  return true;
 }
 
 // 16 bytes as float32

@@ -693,6 +693,22 @@ __device__ __forceinline__ void mbar_arrive_first_cta(uint64_t* bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
 }
 
+// ADAPTED: low-rank adapters of the tokens' requests are a few k-blocks more of the tiles that have such tokens. The plan (adapters.cuh) lists for a row tile
+// the adapters in it; for each, A's block is V, the numbers that the adapter made of those tokens (zeros in the other rows), and W's is the adapter's B. A
+// stacked projection has these for each part that the tile's columns belong to: B's map of a part has that part's rows alone, so a copy reads zeros beyond it, as it
+// does beyond the rank. One k-block of 64 holds a rank of 64, so an adapter costs a tile 1/64 of its products at K = 4,096, and the sum is rounded once.
+struct AdaptedTiles {
+  CUtensorMap map_v;                // [blocks * 256, parts * rank]
+  CUtensorMap map_b[MAX_PARTS];     // [slots][the part's rows][rank]
+  const int* tile_first;            // the first block of each row tile, and where the last one's end
+  const int* block_slot;
+  int parts, rank, ends[MAX_PARTS];
+};
+struct NoAdapters {};
+
+// the plain barrier (hardware barrier `id`) of 128 epilogue threads
+__device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+
 // ---------------------------------------------------------------- decode products with a long k
 // out[M, N] = X[M, K] W[N, K]^T for a handful of tokens (M <= 64), with the operands swapped: 128 rows
 // of W are the instruction's M, the tokens its N (16, 32 or 64 columns of tensor memory). Such a
@@ -703,11 +719,18 @@ __device__ __forceinline__ void mbar_arrive_first_cta(uint64_t* bar) {
 // every CTA of the cluster adding up the tokens that fall to it, in the order of the slices.
 // The weights of the first stages are asked for before the wait on the kernels launched earlier
 // (they do not depend on them), the activations after it.
-template <int BT, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+// ADAPTED: beside the product the terms of the tokens' low-rank adapters, sum_j B_s[n, j] v[t, j] with v an earlier kernel's (rounded to bfloat16 here). The warps that
+// store the outputs have nothing to do while the weights stream, and work out terms then: tokens in the order of their adapters, eight of one adapter at most times the
+// warp's 32 rows of B an instruction; a cluster's CTAs share the adapters out, and a term enters the sum over the slices with the CTA that made it. One rounding.
+// (Terms as k-blocks of the tensor cores, as in the 2-CTA kernel, cost a copy of 128 short rows for each adapter of the step: 42.9 us at 64 tokens of 16 adapters, rank 32,
+// 4096 -> 6144; row by row with multiply-adds 63.7.)
+// GATED: W is [2 N, K], gate rows, then up rows; a tile is 64 of each, out = silu(gate) * up.
+constexpr bool decode_twice(int bt, bool adapted) { return adapted && bt <= 16; }  // two CTAs an SM: a tile more than there are SMs does not wait for a whole one
+template <int BT, int STAGES, bool ADAPTED = false, bool GATED = false>
+__global__ void __launch_bounds__(TC_THREADS, decode_twice(BT, ADAPTED) ? 2 : 1)
 gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                       __nv_bfloat16* __restrict__ out, int M, int N, int K, int slices, int iters_per_slice,
-                      int* __restrict__ status) {
+                      int* __restrict__ status, const std::conditional_t<ADAPTED, AdapterTerms, NoAdapters> term) {
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], accum_bar;
@@ -715,11 +738,18 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   constexpr int W_BYTES = TC_BM * TC_BK * 2, X_BYTES = BT * TC_BK * 2, STAGE_BYTES = W_BYTES + X_BYTES;
   constexpr uint32_t TMEM_COLS = BT <= 32 ? 32 : 64;
   float* part = reinterpret_cast<float*>(smem + (size_t)STAGES * STAGE_BYTES);  // [BT tokens][128 rows of W]: this slice's sums
+  __shared__ int tok_slot[ADAPTED ? BT : 1], order[ADAPTED ? BT : 1], group_at[ADAPTED ? BT : 1], group_count;
+  __shared__ bool begins[ADAPTED ? BT : 1];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
-  const int n0 = ((int)blockIdx.x / slices) * TC_BM;
+  constexpr int ROWS = GATED ? TC_BM / 2 : TC_BM;  // outputs of a tile
+  const int n0 = ((int)blockIdx.x / slices) * ROWS;
   const int k_iters = (K + TC_BK - 1) / TC_BK;
+  auto load_w = [&](unsigned char* to, uint64_t* bar, int k) {
+    tma_load_2d(to, &map_w, bar, k, n0);
+    if (GATED) tma_load_2d(to + W_BYTES / 2, &map_w, bar, k, N + n0);
+  };
   const int it0 = min(k_iters, rank * iters_per_slice), n_it = min(k_iters, it0 + iters_per_slice) - it0;
 
   // Thread 0 is the producer. It sets the barriers up and asks for the weights of the first stages at
@@ -735,7 +765,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     for (int i = 0; i < ahead; ++i) {
       mbar_expect_tx(&full_bar[i], STAGE_BYTES);
-      tma_load_2d(smem + (size_t)i * STAGE_BYTES, &map_w, &full_bar[i], (it0 + i) * TC_BK, n0);
+      load_w(smem + (size_t)i * STAGE_BYTES, &full_bar[i], (it0 + i) * TC_BK);
     }
   }
   if (warp == 1) {
@@ -759,7 +789,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
           break;
         }
         mbar_expect_tx(&full_bar[s], STAGE_BYTES);
-        tma_load_2d(smem + (size_t)s * STAGE_BYTES, &map_w, &full_bar[s], (it0 + i) * TC_BK, n0);
+        load_w(smem + (size_t)s * STAGE_BYTES, &full_bar[s], (it0 + i) * TC_BK);
         tma_load_2d(smem + (size_t)s * STAGE_BYTES + W_BYTES, &map_x, &full_bar[s], (it0 + i) * TC_BK, 0);
       }
     }
@@ -785,6 +815,110 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     // warps 2..5: warp w may touch tensor-memory lanes 32 * (w % 4) .. + 31, i.e. rows of W
     pdl_wait();
     const int quad = warp & 3, l = quad * 32 + lane;
+    if constexpr (ADAPTED) {
+      const Adapters& ad = term.ad;
+      const int e = threadIdx.x - 64, numbers = ad.parts * ad.rank, rows = ad.ends[MAX_PARTS - 1], g = lane >> 2, t4 = lane & 3;
+      constexpr int NONE = 0x7fffffff;
+      // tokens in the order of their slots, and where runs of up to eight of one slot begin
+      if (e < M) {
+        const int s = adapter_of(ad, e);
+        tok_slot[e] = s < 0 ? NONE : s;
+      }
+      for (int i = e; i < M * TC_BM; i += 128) part[i] = 0.f;
+      epilogue_sync(1);
+      if (e < M) {
+        const int s = tok_slot[e];
+        int before = 0, same = 0;
+        for (int j = 0; j < M; ++j) {
+          before += tok_slot[j] < s;
+          same += tok_slot[j] == s && j < e;
+        }
+        order[before + same] = e;
+        begins[before + same] = s != NONE && same % 8 == 0;
+      }
+      epilogue_sync(1);
+      int groups = 0;
+      if (e < M) {
+        int at = 0;
+        for (int j = 0; j < M; ++j) {
+          at += j < e && begins[j];
+          groups += begins[j];
+        }
+        if (begins[e]) group_at[at] = e;
+        if (e == 0) group_count = groups;
+      }
+      epilogue_sync(1);
+      groups = group_count;
+      // this lane's four rows of B: 16 m + g and 8 further
+      int n[4];
+      bool has[4];
+      int first_part = MAX_PARTS, last_part = -1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = quad * 32 + 8 * i + g;
+        has[i] = n0 + (GATED ? row & (ROWS - 1) : row) < N;
+        n[i] = GATED && row >= ROWS ? N + n0 + row - ROWS : n0 + row;
+        if (has[i]) {
+          first_part = min(first_part, part_of(ad, n[i]));
+          last_part = max(last_part, part_of(ad, n[i]));
+        }
+      }
+      first_part = __reduce_min_sync(0xffffffffu, first_part);
+      last_part = __reduce_max_sync(0xffffffffu, last_part);
+      const int chunks = (ad.rank + 31) / 32, items = groups > rank ? (groups - rank + slices - 1) / slices * chunks : 0;
+      for (int p = first_part; p <= last_part; ++p) {
+        // an item: a group and 32 of the rank's numbers; the next one's are asked for ahead of this one's instructions
+        uint32_t b_regs[2][2][2][4];
+        float2 v_regs[2][2][2];
+        auto load = [&](int item, uint32_t (&br)[2][2][4], float2 (&vr)[2][2]) {
+          const int at = group_at[rank + slices * (item / chunks)], c0 = (item % chunks) * 32, s = tok_slot[order[at]];
+          const int tok = at + g < M && tok_slot[order[at + g]] == s ? order[at + g] : -1;
+          const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(ad.b) + (size_t)s * rows * ad.rank;
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + 16 * k + 8 * h + 2 * t4;
+              const bool in = c < ad.rank;
+              vr[k][h] = in && tok >= 0 ? *reinterpret_cast<const float2*>(term.v + (size_t)tok * numbers + p * ad.rank + c) : make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)  // rows 16 m + g (i = 2 m) and 8 further (i = 2 m + 1)
+                br[k][i >> 1][2 * h + (i & 1)] = in && has[i] && part_of(ad, n[i]) == p ? *reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank + c) : 0u;
+            }
+        };
+        auto add = [&](int item, const uint32_t (&br)[2][2][4], const float2 (&vr)[2][2]) {
+          float acc[2][4] = {};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(vr[k][0].x, vr[k][0].y), hi = __floats2bfloat162_rn(vr[k][1].x, vr[k][1].y);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                           : "+f"(acc[m][0]), "+f"(acc[m][1]), "+f"(acc[m][2]), "+f"(acc[m][3])
+                           : "r"(br[k][m][0]), "r"(br[k][m][1]), "r"(br[k][m][2]), "r"(br[k][m][3]), "r"(*reinterpret_cast<const uint32_t*>(&lo)),
+                             "r"(*reinterpret_cast<const uint32_t*>(&hi)));
+          }
+          const int at = group_at[rank + slices * (item / chunks)], s = tok_slot[order[at]];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int pos = at + 2 * t4 + q;
+            if (pos >= M || tok_slot[order[pos]] != s) continue;
+            float* to = part + order[pos] * TC_BM + quad * 32 + g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[8 * i] += acc[i >> 1][2 * (i & 1) + q];
+          }
+        };
+        if (items > 0) load(0, b_regs[0], v_regs[0]);
+        for (int item = 0; item < items; item += 2) {
+          if (item + 1 < items) load(item + 1, b_regs[1], v_regs[1]);
+          add(item, b_regs[0], v_regs[0]);
+          if (item + 1 >= items) break;
+          if (item + 2 < items) load(item + 2, b_regs[0], v_regs[0]);
+          add(item + 1, b_regs[1], v_regs[1]);
+        }
+      }
+      __syncwarp();
+    }
     bool ok = true;
     if (n_it > 0) {
       ok = mbar_wait(&accum_bar, 0);
@@ -804,13 +938,44 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (c + j < BT) part[(c + j) * TC_BM + l] = __uint_as_float(acc[j]);
+        if (c + j < BT) {
+          float* to = part + (c + j) * TC_BM + l;
+          if (ADAPTED) {
+            if (c + j < M) *to += __uint_as_float(acc[j]);
+          } else {
+            *to = __uint_as_float(acc[j]);
+          }
+        }
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
   cluster_sync_all();  // every slice's sums are in its shared memory
-  if (warp >= 2) {
+  if (GATED && warp >= 2) {
+    // every second of the CTA's tokens, the other half of the threads has the rest
+    const int l = (warp & 3) * 32 + lane, row = l & (ROWS - 1);
+    if (n0 + row < N) {
+      uint32_t peer[8];
+#pragma unroll
+      for (int sl = 0; sl < 8; ++sl)
+        asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(peer[sl]) : "r"(smem_u32(part + row)), "r"((uint32_t)(sl < slices ? sl : 0)));
+      for (int tok = rank + slices * (l / ROWS); tok < M; tok += 2 * slices) {
+        float v[2][8], sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int sl = 0; sl < 8; ++sl) {
+            v[h][sl] = 0.f;
+            if (sl < slices) asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v[h][sl]) : "r"(peer[sl] + (uint32_t)((tok * TC_BM + h * ROWS) * 4)));
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int sl = 0; sl < 8; ++sl) sum[h] += v[h][sl];
+        out[(size_t)tok * N + n0 + row] = __float2bfloat16_rn(sum[0] / (1.0f + expf(-sum[0])) * sum[1]);
+      }
+    }
+  } else if (warp >= 2) {
     const int l = (warp & 3) * 32 + lane;
     if (n0 + l < N) {
       // the tokens rank, rank + slices, ...: all slices' sums of a token are asked for together (eight
@@ -839,7 +1004,175 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   }
 }
 
-// AND of a flag over the 128 threads of a group of epilogue warps (hardware barrier `id`), and their plain barrier
+// ---------------------------------------------------------------- what the adapters' A make of many tokens
+// V = c_s x A_s^T by the blocks of a plan (adapters.cuh), N = BT numbers at a time: a stream of x (A is a few hundred KB), so K is cut into the CTAs of a
+// cluster and everything that a CTA reads of an item is asked for at once. An item: 128 rows of a block and BT numbers. Clusters stay and walk the items; those whose rows have no token
+// of the adapter are zeros. The slices' sums meet in shared memory, eight numbers of a row a thread.
+// COMPACT: float32 v [T, numbers] of the adapters' own tokens, else bfloat16 V [blocks * 256, numbers] with zeros elsewhere: rounded to 8 bits, as the tensor cores take it (2^-8 of
+// an adapter's share of an output, where the output itself is rounded so). 2,048 tokens of 4,096, 48 numbers: see the launcher.
+template <int BT, int STAGES, bool COMPACT>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+adapter_v_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, void* v, const Adapters ad, const int* tile_first, const AdapterBlock* blocks,
+                 int T, int K, int slices, int iters_per_slice, int chunks, int* status) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], accum_bar;
+  __shared__ uint32_t tmem_base_slot;
+  constexpr int X_BYTES = TC_BM * TC_BK * 2, A_BYTES = BT * TC_BK * 2, STAGE_BYTES = X_BYTES + A_BYTES;
+  constexpr uint32_t TMEM_COLS = BT <= 32 ? 32 : BT <= 64 ? 64 : 128;
+  float* part = reinterpret_cast<float*>(smem + (size_t)STAGES * STAGE_BYTES);  // [BT numbers][128 rows]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_ctarank();
+  const int k_iters = (K + TC_BK - 1) / TC_BK, it0 = min(k_iters, rank * iters_per_slice), n_it = min(k_iters, it0 + iters_per_slice) - it0;
+  const int numbers = ad.parts * ad.rank, cluster = (int)blockIdx.x / slices, clusters = (int)gridDim.x / slices;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&accum_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem_base = tmem_base_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int items = tile_first[(T + ADAPTER_ROWS - 1) / ADAPTER_ROWS] * 2 * chunks;
+  int kb = 0, done = 0, issued = 0;  // k-blocks and items so far that had products; (the producer's) blocks asked for
+  bool ok = true;
+  for (int item = cluster; item < items; item += clusters) {
+    const int b = item / (2 * chunks), half = item / chunks & 1, j0 = (item % chunks) * BT;
+    const int2 which = *reinterpret_cast<const int2*>(&blocks[b].slot);
+    const uint4 members = *reinterpret_cast<const uint4*>(&blocks[b].members[4 * half]);
+    const int s = which.x, tok0 = which.y * ADAPTER_ROWS + half * TC_BM;
+    const bool any = (members.x | members.y | members.z | members.w) != 0;
+    if (any) {
+      if (warp == 0) {
+        if (elect_one()) {
+          for (int i = 0; i < n_it && ok; ++i, ++issued) {
+            const int at = kb + i, st = at % STAGES;
+            if (at >= STAGES && !mbar_wait(&empty_bar[st], ((at / STAGES) - 1) & 1)) {
+              atomicExch(status, 16);
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(&full_bar[st], STAGE_BYTES);
+            tma_load_2d(smem + (size_t)st * STAGE_BYTES, &map_x, &full_bar[st], (it0 + i) * TC_BK, tok0);
+            tma_load_2d(smem + (size_t)st * STAGE_BYTES + X_BYTES, &map_a, &full_bar[st], (it0 + i) * TC_BK, s * numbers + j0);
+          }
+        }
+      } else if (warp == 1) {
+        if (elect_one()) {
+          constexpr uint32_t idesc = make_idesc(TC_BM, BT);
+          for (int i = 0; i < n_it && ok; ++i) {
+            const int at = kb + i, st = at % STAGES;
+            if (!mbar_wait(&full_bar[st], (at / STAGES) & 1)) {
+              atomicExch(status, 17);
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const unsigned char* x_tile = smem + (size_t)st * STAGE_BYTES;
+            const uint64_t da = make_smem_desc(x_tile), db = make_smem_desc(x_tile + X_BYTES);
+#pragma unroll
+            for (int k = 0; k < TC_BK / 16; ++k) umma_bf16(tmem_base, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (i | k) != 0);
+            umma_commit(&empty_bar[st]);
+          }
+          if (ok) umma_commit(&accum_bar);
+        }
+      } else {
+        const int quad = warp & 3, l = quad * 32 + lane;
+        const bool have = ok && n_it > 0 && mbar_wait(&accum_bar, done & 1);
+        if (n_it > 0 && !have) {
+          if (ok) atomicExch(status, 18);
+          ok = false;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < BT; c += 32) {
+          uint32_t acc[32];
+          if (have) {
+            tmem_ld32(lane_addr + (uint32_t)c, acc);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < BT) part[(c + j) * TC_BM + l] = __uint_as_float(acc[j]);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      }
+      if (n_it > 0) {
+        kb += n_it;
+        ++done;
+      }
+      __syncwarp();
+      cluster_sync_all();  // every slice's sums are in its shared memory
+    }
+    if (warp >= 2) {
+      const int l = (warp & 3) * 32 + lane;
+      const unsigned word = (warp & 3) == 0 ? members.x : (warp & 3) == 1 ? members.y : (warp & 3) == 2 ? members.z : members.w;
+      const bool mine = (word >> lane) & 1;
+      const float c = mine ? ad.scale[s] : 0.f;
+      uint32_t peer[8];
+#pragma unroll
+      for (int sl = 0; sl < 8; ++sl)
+        asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(peer[sl]) : "r"(smem_u32(part + l)), "r"((uint32_t)(sl < slices ? sl : 0)));
+      for (int j = 8 * rank; j < BT && j0 + j < numbers; j += 8 * slices) {  // (numbers are a multiple of 8)
+        float sum[8], x[8][8];  // all 64 asked for before the first is used
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int sl = 0; sl < 8; ++sl) {
+            x[i][sl] = 0.f;
+            if (any && sl < slices) asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(x[i][sl]) : "r"(peer[sl] + (uint32_t)((j + i) * TC_BM * 4)));
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sum[i] = 0.f;
+#pragma unroll
+          for (int sl = 0; sl < 8; ++sl) sum[i] += x[i][sl];
+          sum[i] = mine ? sum[i] * c : 0.f;
+        }
+        if (COMPACT) {
+          if (mine) {
+            float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(v) + (size_t)(tok0 + l) * numbers + j0 + j);
+            to[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+            to[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+          }
+        } else {
+          *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(v) + ((size_t)b * ADAPTER_ROWS + half * TC_BM + l) * numbers + j0 + j) = float_to_bf16x8(sum);
+        }
+      }
+    }
+    if (any) {
+      __syncwarp();
+      cluster_sync_all();  // everyone has read the sums; the next item's may take their place
+    }
+  }
+  // arrivals that nobody waits for must not outlive the CTA
+  if (warp == 1 && elect_one())
+    for (int i = max(0, kb - STAGES); i < kb && ok; ++i) ok = mbar_wait(&empty_bar[i % STAGES], (i / STAGES) & 1);
+  // (after a wait that gave up) copies in flight end before the CTA does
+  if (warp == 0 && !ok)
+    for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait_bounded(smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1, MS_WAIT_NS / 64);
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// AND of a flag over the 128 threads of a group of epilogue warps (hardware barrier `id`)
 __device__ __forceinline__ bool epilogue_all(int id, bool flag) {
   uint32_t res;
   asm volatile(
@@ -848,7 +1181,6 @@ __device__ __forceinline__ bool epilogue_all(int id, bool flag) {
       : "=r"(res) : "r"(id), "r"((uint32_t)flag) : "memory");
   return res != 0;
 }
-__device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
 
 // The q|k|v epilogue's ring for the rotation table: four slots of [128 tokens][8 cosines] then
 // [128 tokens][8 sines] (float32), one quarter of a half head each, read by both groups of epilogue warps
@@ -867,19 +1199,6 @@ constexpr int PAIR_BN = 256;                    // the wide tile; outputs too na
 constexpr int PAIR_OUT_BYTES = TC_BM * 64 * 2;  // one [128][64] bfloat16 tile of the epilogue's four
 // per CTA and stage: 128 rows of A and half of the tile's BN rows of W, 64 k each
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return (TC_BM + bn / 2) * TC_BK * 2; }
-
-// ADAPTED: low-rank adapters of the tokens' requests are a few k-blocks more of the tiles that have such tokens. The plan (adapters.cuh) lists for a row tile
-// the adapters in it; for each, A's block is V, the numbers that the adapter made of those tokens (zeros in the other rows), and W's is the adapter's B. A
-// stacked projection has these for each part that the tile's columns belong to: B's map of a part has that part's rows alone, so a copy reads zeros beyond it, as it
-// does beyond the rank. One k-block of 64 holds a rank of 64, so an adapter costs a tile 1/64 of its products at K = 4,096, and the sum is rounded once.
-struct AdaptedTiles {
-  CUtensorMap map_v;                // [blocks * 256, parts * rank]
-  CUtensorMap map_b[MAX_PARTS];     // [slots][the part's rows][rank]
-  const int* tile_first;            // the first block of each row tile, and where the last one's end
-  const int* block_slot;
-  int parts, rank, ends[MAX_PARTS];
-};
-struct NoAdapters {};
 
 // GROUPED: the row tiles are the plan's (256 sorted rows of one matrix each); a tile's rows beyond its run are computed with the run's matrix and not
 // stored. Row tiles change fastest here too: a run has two or three of them, which then take a tile of W from L2 together.
@@ -959,7 +1278,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     int more = 0;
     if constexpr (ADAPTED) {
       const int n0 = tile_n(tile) * COLS, m = tile_m(tile);
-      for (int p = 0; p < ad.parts; ++p) more += meets(p, n0);
+#pragma unroll
+      for (int p = 0; p < MAX_PARTS; ++p) more += p < ad.parts && meets(p, n0);
       more *= (ad.tile_first[m + 1] - ad.tile_first[m]) * ((ad.rank + TC_BK - 1) / TC_BK);
     }
     return more;
@@ -989,8 +1309,9 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if constexpr (ADAPTED) {
           const int last = ad.tile_first[tile_m(tile) + 1];
           for (int b = ad.tile_first[tile_m(tile)]; b < last && ok; ++b)
-            for (int p = 0; p < ad.parts && ok; ++p) {
-              if (!meets(p, n0)) continue;
+#pragma unroll
+            for (int p = 0; p < MAX_PARTS; ++p) {
+              if (p >= ad.parts || !ok || !meets(p, n0)) continue;
               for (int c = 0; c < ad.rank; c += TC_BK, ++kb) {
                 const int s = kb % STAGES;
                 if (kb >= STAGES && !mbar_wait(&empty_bar[s], ((kb / STAGES) - 1) & 1)) {
@@ -1479,10 +1800,10 @@ static int launch_tc_pair(void* out, const void* A, const void* W, int M, int N_
 // The maps of an adapted product: V as the plan's blocks lay it out, B by its parts.
 static int make_adapted(AdaptedTiles* tiles, const AdaptedProduct& ap) {
   const Adapters& ad = ap.ad;
-  if (int rc = make_map(&tiles->map_v, ap.v, (long long)ap.max_blocks * 2 * TC_BM, (long long)ad.parts * ad.rank, TC_BM)) return rc;
+  if (int rc = make_map(&tiles->map_v, ap.v, (long long)ap.max_blocks * ADAPTER_ROWS, (long long)ad.parts * ad.rank, TC_BM)) return rc;
   TensorMapEncodeFn encode;
   if (int rc = tensor_map_encoder(&encode)) return rc;
-  const int n = ad.ends[ad.parts - 1];
+  const int n = ad.ends[MAX_PARTS - 1];
   for (int p = 0; p < MAX_PARTS; ++p) {
     const int q = p < ad.parts ? p : 0, from = q ? ad.ends[q - 1] : 0;
     const cuuint64_t dims[3] = {(cuuint64_t)ad.rank, (cuuint64_t)(ad.ends[q] - from), (cuuint64_t)ad.slots};
@@ -1555,14 +1876,15 @@ static int launch_tc_pair_grouped(void* out, const void* A, const void* W, int r
   return 0;
 }
 
-template <int BT, int STAGES>
-static int launch_tc_decode(void* out, const void* X, const void* W, int M, int N, int K, int* status, cudaStream_t stream) {
+template <int BT, int STAGES, bool ADAPTED = false, bool GATED = false>
+static int launch_tc_decode(void* out, const void* X, const void* W, int M, int N, int K, int* status, cudaStream_t stream,
+                            const std::conditional_t<ADAPTED, AdapterTerms, NoAdapters>& term = {}) {
   CUtensorMap map_w, map_x;
-  if (int rc = make_map(&map_w, W, N, K, TC_BM)) return rc;
+  if (int rc = make_map(&map_w, W, GATED ? 2LL * N : N, K, GATED ? TC_BM / 2 : TC_BM)) return rc;
   if (int rc = make_map(&map_x, X, M, K, BT)) return rc;
   constexpr size_t smem = (size_t)STAGES * (TC_BM + BT) * TC_BK * 2 + (size_t)BT * TC_BM * 4 + 1024;
-  static_assert(smem <= 227 * 1024, "the ring does not fit shared memory");
-  auto kernel = gemm_tc_decode_kernel<BT, STAGES>;
+  static_assert((decode_twice(BT, ADAPTED) ? 2 : 1) * (smem + 1024) <= 227 * 1024, "the ring does not fit shared memory");
+  auto kernel = gemm_tc_decode_kernel<BT, STAGES, ADAPTED, GATED>;
   static bool configured = false;
   static int sm_count = 0;
   if (!configured) {
@@ -1592,13 +1914,37 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
       fit[size] = n;
     }
   }
-  const int tiles = ceil_div(N, TC_BM), k_iters = ceil_div(K, TC_BK);
+  const int tiles = ceil_div(N, GATED ? TC_BM / 2 : TC_BM), k_iters = ceil_div(K, TC_BK);
   int slices = 1;
   for (int size = 2; size <= 8 && size <= k_iters / 4; ++size)
     if (fit[size] >= tiles) slices = size;
   const int iters_per_slice = ceil_div(k_iters, slices);
   MS_LAUNCH_CLUSTERED(kernel, (unsigned)(tiles * slices), TC_THREADS, smem, stream, slices, map_w, map_x, (__nv_bfloat16*)out, M, N, K, slices,
-                      iters_per_slice, status);
+                      iters_per_slice, status, term);
+  return 0;
+}
+
+
+template <int BT, int STAGES, bool COMPACT>
+static int launch_adapter_v(void* v, const void* X, const Adapters& ad, const int* tile_first, const AdapterBlock* blocks, int T, int K, int max_blocks,
+                            int* status, cudaStream_t stream) {
+  const int numbers = ad.parts * ad.rank, chunks = ceil_div(numbers, BT), k_iters = ceil_div(K, TC_BK);
+  CUtensorMap map_x, map_a;
+  if (int rc = make_map(&map_x, X, T, K, TC_BM)) return rc;
+  if (int rc = make_map(&map_a, ad.a, (long long)ad.slots * numbers, K, BT)) return rc;
+  constexpr size_t smem = (size_t)STAGES * (TC_BM + BT) * TC_BK * 2 + (size_t)BT * TC_BM * 4 + 1024;
+  static_assert(smem <= 227 * 1024, "the ring does not fit shared memory");
+  auto kernel = adapter_v_kernel<BT, STAGES, COMPACT>;
+  static std::atomic<unsigned long long> allowed{0};
+  MS_CHECK_CUDA(allow_shared_memory((const void*)kernel, (int)smem, allowed));
+  // Slices of k: as many as give the items of a step with an adapter a row tile a cluster each, eight at most, of four k-blocks at least.
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  const long long likely = (long long)ceil_div(T, TC_BM) * chunks, most = 2LL * max_blocks * chunks;
+  int slices = 1;
+  while (slices < 8 && (slices + 1) * likely <= sms && slices + 1 <= k_iters / 4) ++slices;
+  const long long fit = sms / slices > 1 ? sms / slices : 1, clusters = most < fit ? most : fit;
+  MS_LAUNCH_CLUSTERED(kernel, (unsigned)(clusters * slices), TC_THREADS, smem, stream, slices, map_x, map_a, v, ad, tile_first, blocks, T, K, slices,
+                      ceil_div(k_iters, slices), chunks, status);
   return 0;
 }
 
@@ -1664,7 +2010,7 @@ MS_EXPORT int ms_gemm_tc_qkv_bf16(void* q_out, const void* x, const void* w_qkv,
                           cos_sin, positions, row_of_token, page_indptr, page_indices, nq, nkv, shift, eps};
   const int n_total = (nq + 2 * nkv) * 128;
   if (ap != nullptr) {
-    MS_CHECK_ARG(ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 && ap->ad.ends[ap->ad.parts - 1] == n_total,
+    MS_CHECK_ARG(ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 && adapters_ok(ap->ad, n_total, K),
                  "gemm_tc: an adapted product needs a plan of its outputs");
     return launch_tc_pair_adapted<4, TC_QKV_ROPE>(q_out, x, w_qkv, M, n_total, n_total, K, 0, *ap, status, stream, qe);
   }
@@ -1679,7 +2025,7 @@ MS_EXPORT int ms_gemm_tc_adapted_bf16(void* out, const void* A, const void* W, i
   MS_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 8 == 0, "gemm_tc: bad sizes M=%d N=%d K=%d", M, N, K);
   MS_CHECK_ARG(((uintptr_t)A % 16 == 0) && ((uintptr_t)W % 16 == 0), "gemm_tc: operands must be 16-byte aligned");
   MS_CHECK_ARG(status != nullptr && ap != nullptr && ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 &&
-                   ap->ad.ends[ap->ad.parts - 1] == (epilogue == TC_SILU_MUL ? 2 * N : N),
+                   adapters_ok(ap->ad, epilogue == TC_SILU_MUL ? 2 * N : N, K),
                "gemm_tc: an adapted product needs a status word and a plan of its outputs");
   if (epilogue == TC_OUT_BF16) return launch_tc_pair_adapted<5, TC_OUT_BF16>(out, A, W, M, N, N, K, 0, *ap, status, stream);
   if (epilogue == TC_SILU_MUL) return launch_tc_pair_adapted<5, TC_SILU_MUL>(out, A, W, M, N, 2 * N, K, N, *ap, status, stream);
@@ -1785,6 +2131,43 @@ MS_EXPORT int ms_gemm_tc_experts_bf16(void* out, const void* A, const void* W, i
   const TcGroups grp{tiles, meta, offsets, N, {}};
   if (gated == 2) return launch_grouped_plain<TC_RELU2>(out, A, W, rows, N, experts, K, grp, tile_rows, max_tiles, status, stream);
   return launch_grouped_plain<TC_OUT_F32>(out, A, W, rows, N, experts, K, grp, tile_rows, max_tiles, status, stream);
+}
+
+// What the adapters' A make of X [T, K] by a plan (ms_adapter_plan): compact = 0: v bfloat16 [max_blocks * 256, parts * rank]; 1: float32 [T, parts * rank], rows of tokens without
+// an adapter left as they were.
+MS_EXPORT int ms_gemm_tc_adapter_v(void* v, const void* X, const Adapters* ad, const int* tile_first, const void* blocks, int T, int K, int max_blocks,
+                                   int compact, int* status, cudaStream_t stream) {
+  if (T == 0) return 0;
+  MS_CHECK_ARG(T > 0 && ad != nullptr && adapters_ok(*ad, ad->ends[MAX_PARTS - 1], K) && max_blocks > 0, "gemm_tc: bad sizes T=%d K=%d", T, K);
+  MS_CHECK_ARG((uintptr_t)X % 16 == 0 && (uintptr_t)ad->a % 16 == 0 && (uintptr_t)v % 16 == 0, "gemm_tc: operands must be 16-byte aligned");
+  MS_CHECK_ARG(status != nullptr && tile_first && blocks && (uintptr_t)blocks % 16 == 0, "gemm_tc: needs a plan and a status word");
+  const int numbers = ad->parts * ad->rank;
+#define MS_V(BT, STAGES) \
+  return compact ? launch_adapter_v<BT, STAGES, true>(v, X, *ad, tile_first, (const AdapterBlock*)blocks, T, K, max_blocks, status, stream) \
+                 : launch_adapter_v<BT, STAGES, false>(v, X, *ad, tile_first, (const AdapterBlock*)blocks, T, K, max_blocks, status, stream)
+  if (numbers <= 16) MS_V(16, 10);
+  if (numbers <= 32) MS_V(32, 9);
+  if (numbers <= 48) MS_V(48, 8);
+  if (numbers <= 64) MS_V(64, 7);
+  MS_V(128, 4);
+#undef MS_V
+}
+
+// out [M, N] bfloat16 = X W^T beside the adapters of X's rows, or (gated) silu(gate) * up of the stacked W [2 N, K] beside them, M <= 64 tokens; term->v is an earlier launch's.
+MS_EXPORT int ms_gemm_tc_decode_adapted_bf16(void* out, const void* X, const void* W, int M, int N, int K, int gated, const AdapterTerms* term, int* status, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  MS_CHECK_ARG(M > 0 && M <= 64 && N > 0 && K > 0, "gemm_tc: a decode product takes 1..64 rows, not M=%d (N=%d K=%d)", M, N, K);
+  MS_CHECK_ARG(K % 8 == 0, "gemm_tc: K=%d must be a multiple of 8 (rows must be 16-byte multiples for TMA)", K);
+  MS_CHECK_ARG(((uintptr_t)X % 16 == 0) && ((uintptr_t)W % 16 == 0), "gemm_tc: operands must be 16-byte aligned");
+  MS_CHECK_ARG(status != nullptr && term != nullptr && term->v != nullptr && (uintptr_t)term->v % 16 == 0 && adapters_ok(term->ad, gated ? 2 * N : N, K),
+               "gemm_tc: an adapted product needs a status word and its adapters' numbers");
+#define MS_DECODE(BT, STAGES)                                                                                     \
+  return gated ? launch_tc_decode<BT, STAGES, true, true>(out, X, W, M, N, K, status, stream, *term)              \
+               : launch_tc_decode<BT, STAGES, true, false>(out, X, W, M, N, K, status, stream, *term)
+  if (M <= 16) MS_DECODE(16, 5);
+  if (M <= 32) MS_DECODE(32, 10);
+  MS_DECODE(64, 8);
+#undef MS_DECODE
 }
 
 // out [M, N] bfloat16 = X [M, K] W [N, K]^T for M <= 64 tokens (decode steps), see gemm_tc_decode_kernel.

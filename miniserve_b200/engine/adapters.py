@@ -1,0 +1,157 @@
+"""The low-rank adapters that an engine holds beside its model's projections, a slot each (``AdapterStore``).
+
+An adapter comes as a folder with ``adapter_config.json`` (``r``, ``lora_alpha``) and safetensors, or as its tensors: for each adapted matrix ``<matrix>.lora_A.weight``
+[r, inputs] and ``<matrix>.lora_B.weight`` [outputs, r], ``<matrix>.weight`` being the model's tensor, with or without ``base_model.model.`` in front. It adds
+alpha / r B A x to the matrix's product. Which matrices may have one is the parts' to say (``Part.adapted_products``); others are refused, all that is wrong in one error.
+"""
+
+from __future__ import annotations
+
+import json
+import math
+from pathlib import Path
+from typing import Mapping
+
+import torch
+
+from .. import ops
+
+_PREFIX = "base_model.model."
+_ENDS = {".lora_A.weight": 0, ".lora_B.weight": 1}
+
+
+class AdapterStore:
+    def __init__(self, model, slots: int, rank: int):
+        """Room for ``slots`` adapters of a rank up to ``rank`` (made up to a multiple of 8) beside every projection of ``model`` that takes them."""
+        if slots < 1 or not 1 <= rank <= ops.adapters.MAX_RANK:
+            raise ValueError(f"max_adapters={slots} and max_adapter_rank={rank}: at least one adapter, a rank of 1 to {ops.adapters.MAX_RANK}")
+        self.slots, self.rank = slots, rank
+        self.names: dict[str, int] = {}
+        # matrix -> (the LowRank of its product, its part there, the part's first row and the row behind)
+        self.places: dict[str, tuple] = {}
+        held = -(-rank // 8) * 8
+        self.products: dict[tuple, ops.LowRank] = {}  # (part, product) -> its adapters
+
+        def walk(part, prefix):
+            decls = part.weights()
+            for product, matrices in part.adapted_products().items():
+                ends, at = [], 0
+                for m in matrices:
+                    at += decls[m].shape[0]
+                    ends.append(at)
+                inputs = decls[matrices[0]].shape[1]
+                if inputs % 8:
+                    continue  # (no kernel takes it; an adapter that names it is refused)
+                low = self.products[part, product] = ops.LowRank.zeros(slots, inputs, tuple(ends), held, model.dtype, model.device)
+                for p, m in enumerate(matrices):
+                    self.places[prefix + m] = (low, p, ends[p - 1] if p else 0, ends[p])
+            for sub, child in part.sub_parts().items():
+                walk(child, prefix + sub)
+
+        for prefix, layer in zip(model.prefixes, model.layers):
+            walk(layer, prefix)
+        if not self.places:
+            raise ValueError(f"no projection of a {model.spec.architecture} model takes adapters")
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for low in self.products.values() for t in (low.a, low.b, low.scale))
+
+    # ------------------------------------------------------------------ loading
+    def load(self, name: str, source: "str | Path | Mapping[str, torch.Tensor]", alpha: float | None = None) -> int:
+        """Put an adapter into a free slot; returns the slot. ``source``: a folder, or the tensors by name (then ``alpha`` says lora_alpha; left out, the rank:
+        a factor of 1). Nothing is changed where anything is wrong with it."""
+        if name in self.names:
+            raise ValueError(f"there is an adapter {name!r} already")
+        free = [s for s in range(self.slots) if s not in self.names.values()]
+        if not free:
+            raise ValueError(f"all {self.slots} adapters' places are taken ({', '.join(sorted(self.names))}): unload one, or ask for more (max_adapters)")
+        factor = None
+        if isinstance(source, (str, Path)):
+            tensors, factor = self._read(Path(source))
+            if alpha is not None:
+                raise ValueError("alpha is what the adapter's folder says")
+        else:
+            tensors = dict(source)
+        pairs = self._pairs(name, tensors)
+        slot = free[0]
+        for low in self.products.values():
+            low.scale[slot] = 0.0
+        used: dict[int, tuple] = {}
+        for matrix, (a, b) in pairs.items():
+            low, part, first, behind = self.places[matrix]
+            r = a.shape[0]
+            if id(low) not in used:
+                low.a[slot].zero_()
+                low.b[slot].zero_()
+                used[id(low)] = (low, r)
+            low.a[slot, part * low.rank:part * low.rank + r] = a.to(low.a.dtype)
+            low.b[slot, first:behind, :r] = b.to(low.b.dtype)
+        for low, r in used.values():
+            low.scale[slot] = factor if factor is not None else (1.0 if alpha is None else float(alpha) / r)
+        self.names[name] = slot
+        return slot
+
+    def unload(self, name: str) -> None:
+        """Free the adapter's slot (no request that still runs may have it: the engine sees to that)."""
+        self.slot(name)
+        del self.names[name]
+
+    def slot(self, name: str) -> int:
+        try:
+            return self.names[name]
+        except KeyError:
+            raise ValueError(f"no adapter named {name!r}; there are {sorted(self.names)}") from None
+
+    def _read(self, folder: Path) -> tuple[dict, float]:
+        from safetensors.torch import load_file
+
+        try:
+            cfg = json.loads((folder / "adapter_config.json").read_text())
+        except FileNotFoundError:
+            raise FileNotFoundError(f"no adapter_config.json in {folder}") from None
+        odd = [k for k in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "fan_in_fan_out") if cfg.get(k)]
+        if cfg.get("bias", "none") not in ("none", None):
+            odd.append(f"bias={cfg['bias']}")
+        if odd:
+            raise ValueError(f"the adapter in {folder} has what there is nothing for here: {', '.join(odd)}")
+        r = int(cfg["r"])
+        files = sorted(folder.glob("*.safetensors"))
+        if not files:
+            raise FileNotFoundError(f"no .safetensors files in {folder}")
+        tensors: dict = {}
+        for f in files:
+            tensors.update(load_file(str(f)))
+        alpha = float(cfg.get("lora_alpha", r))
+        return tensors, alpha / (math.sqrt(r) if cfg.get("use_rslora") else r)
+
+    def _pairs(self, name: str, tensors: Mapping[str, torch.Tensor]) -> dict[str, tuple]:
+        """(A, B) by the model's matrix, or one error about all that does not fit."""
+        halves: dict[str, list] = {}
+        wrong: list[str] = []
+        for key, t in tensors.items():
+            at = key[len(_PREFIX):] if key.startswith(_PREFIX) else key
+            end = next((e for e in _ENDS if at.endswith(e)), None)
+            matrix = at[:-len(end)] + ".weight" if end else None
+            if matrix not in self.places:
+                wrong.append(f"{key}: no projection here that takes an adapter")
+                continue
+            halves.setdefault(matrix, [None, None])[_ENDS[end]] = t
+        ranks = set()
+        for matrix, (a, b) in halves.items():
+            low, _, first, behind = self.places[matrix]
+            if a is None or b is None:
+                wrong.append(f"{matrix}: lora_{'A' if a is None else 'B'} is missing")
+            elif a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[1] != low.inputs or b.shape[0] != behind - first:
+                wrong.append(f"{matrix}: A {tuple(a.shape)} and B {tuple(b.shape)} beside a matrix of {behind - first} x {low.inputs}")
+            else:
+                ranks.add(a.shape[0])
+                if not 1 <= a.shape[0] <= self.rank:
+                    wrong.append(f"{matrix}: rank {a.shape[0]}, there is room for 1 to {self.rank} (max_adapter_rank)")
+        if len(ranks) > 1:
+            wrong.append(f"ranks {sorted(ranks)}: all of an adapter's are one")
+        if not halves and not wrong:
+            wrong.append("it has no tensors")
+        if wrong:
+            more = f" ... and {len(wrong) - 12} more" if len(wrong) > 12 else ""
+            raise ValueError(f"adapter {name!r} does not fit: {'; '.join(wrong[:12])}{more}")
+        return {m: (a, b) for m, (a, b) in halves.items()}

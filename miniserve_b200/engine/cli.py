@@ -33,6 +33,8 @@ def add_engine_args(parser: argparse.ArgumentParser) -> None:
                    help="bfloat16: the serving kernels; float32: the whole model in true 32-bit")
     g.add_argument("--kv-cache-dtype", choices=["auto", "fp8"], default="auto",
                    help="auto: keys and values in the model's type; fp8: in 8 bits, half the memory a token")
+    g.add_argument("--max-adapters", type=int, default=0, help="room for so many low-rank adapters beside the model's projections")
+    g.add_argument("--max-adapter-rank", type=int, default=16, help="the largest rank that they may have")
     g.add_argument("--disable-overlap", action="store_true",
                    help="wait for a step's tokens before planning the next one (the host then idles while the GPU works)")
     g.add_argument("--poison-on-free", action="store_true",
@@ -66,6 +68,8 @@ def engine_kwargs(args: argparse.Namespace) -> dict:
         poison_on_free=args.poison_on_free,
         schedule_policy=args.schedule_policy,
         kv_cache_dtype=args.kv_cache_dtype,
+        max_adapters=args.max_adapters,
+        max_adapter_rank=args.max_adapter_rank,
     )
 
 

@@ -53,6 +53,8 @@ class StepContext:
     # Who makes the context says so: the tables above, and the cache of all tokens before this step's, are in place before the step's first kernel starts (behind
     # a copy, say, which kernels do not start ahead of). A kernel may then read them while the kernels before it in the step still run.
     tables_ahead: bool = False
+    adapter_rows: object | None = None  # which adapter each token has (ops.AdapterRows); None: no request of the step has one
+    low_rank: dict = field(default_factory=dict)  # (part, product) -> ops.LowRank: the adapters beside the parts' products
     layout: tuple = ()  # where each field starts in the arena (a replayed graph checks it has not moved)
 
     def buffer(self, role: str, shape: tuple, dtype: torch.dtype, device) -> torch.Tensor:

@@ -28,6 +28,7 @@ from ..cache.manager import KV_DTYPES, CacheManager, group_needs, vector_bytes, 
 from ..ops.cache8 import UNPACKED_BYTES
 from ..parts.decoder import DecoderModel
 from ..sampling.sampler import Sampler
+from .adapters import AdapterStore
 from .request import PLACEHOLDER, Request, RequestState, SamplingParams
 from .scheduler import Plan, Scheduler
 from .step import StepError, StepFunction, StepRow
@@ -78,7 +79,8 @@ class Engine:
                  max_running: int = 64, max_prefill_tokens: int = 8192, chunked_prefill_size: int | None = None,
                  seed: int = 0, cuda_graph: bool = True, cuda_graph_max_bs: int | None = None,
                  kv_mem_fraction: float = 0.9, overlap: bool = True, cache: CacheManager | None = None, step_fn=None,
-                 sampler=None, poison_on_free: bool = False, step_graphs: bool = True, schedule_policy: str = "fcfs", kv_cache_dtype: str = "auto"):
+                 sampler=None, poison_on_free: bool = False, step_graphs: bool = True, schedule_policy: str = "fcfs", kv_cache_dtype: str = "auto",
+                 max_adapters: int = 0, max_adapter_rank: int = 16):
         """``kv_pool_tokens``: exact size of the cache pool in tokens, rounded down to whole pages
         (default: ``kv_mem_fraction`` of the memory the device has free after the weights, less a
         reserve for activations). ``chunked_prefill_size``: tokens per step, decode tokens included,
@@ -91,6 +93,8 @@ class Engine:
         ``schedule_policy``: "fcfs" or "sjf" (``Scheduler``). ``kv_cache_dtype``: "auto" keeps keys and values in the
         model's type, "fp8" in 8 bits with a power of two per token and head (``ops.Pool8``): half the bytes a token, for
         bfloat16 models whose attention layers are plain grouped-query ones (windows and a sink of score 0 allowed).
+        ``max_adapters``: room for so many low-rank adapters of a rank up to ``max_adapter_rank`` beside the model's projections
+        (``load_adapter``; ``add_request(..., adapter=NAME)``): requests of one step may have different ones, or none.
         Names and meanings follow miniserve/engine/engine.py:42-77. ``cache``, ``step_fn`` and
         ``sampler`` replace the ones the engine would build (a test can run the whole loop on the
         host against a stand-in step function this way). ``poison_on_free``: a debugging aid, see
@@ -101,6 +105,7 @@ class Engine:
         step_tokens = chunked_prefill_size if chunked_prefill_size else max_prefill_tokens
         if kv_cache_dtype not in KV_DTYPES:
             raise ValueError(f"kv_cache_dtype is one of {KV_DTYPES}, not {kv_cache_dtype!r}")
+        self.adapters: AdapterStore | None = AdapterStore(model, max_adapters, max_adapter_rank) if max_adapters else None
         if cache is None:
             if kv_cache_dtype == "fp8":
                 model.check_cache8(page_size)
@@ -115,8 +120,12 @@ class Engine:
         self.settings = dict(kv_pool_tokens=kv_pool_tokens, page_size=page_size, max_running=max_running,
                              max_prefill_tokens=max_prefill_tokens, chunked_prefill_size=chunked_prefill_size, seed=seed,
                              cuda_graph=cuda_graph, cuda_graph_max_bs=cuda_graph_max_bs or max_running, overlap=overlap,
-                             schedule_policy=schedule_policy, kv_cache_dtype=getattr(cache, "kv_dtype", "auto"))
+                             schedule_policy=schedule_policy, kv_cache_dtype=getattr(cache, "kv_dtype", "auto"),
+                             max_adapters=max_adapters, max_adapter_rank=max_adapter_rank)
         self.step_fn = step_fn if step_fn is not None else StepFunction(model, self.cache)
+        if self.adapters is not None and step_fn is None:
+            self.step_fn.low_rank = self.adapters.products
+            self.step_fn.reserve_adapter_slots(max_running + 8)
         self.scheduler = Scheduler(self.cache, max_running, max_prefill_tokens, chunked_prefill_size, schedule_policy)
         self.sampler = sampler if sampler is not None else Sampler(model.device, model.spec.vocab_size, max_running)
         self.requests: dict[int, Request] = {}
@@ -197,7 +206,7 @@ class Engine:
     def capture_graphs(self, modes=("greedy",), context_lengths=(0,), prompt_tokens: int = 0) -> int:
         """Capture the decode graphs of every batch bucket now (while the engine is idle) instead
         of at their first use; returns how many were captured. ``modes``: of "greedy",
-        "temperature", "top_p". ``context_lengths``: lengths that requests will reach; the graphs of
+        "temperature", "top_p", "filtered" (top_k or min_p). ``context_lengths``: lengths that requests will reach; the graphs of
         every class of context length from the shortest's to the longest's are captured (those for short
         contexts by default). ``prompt_tokens``: also capture the step graphs that lone prompts of up to so
         many tokens meet (no more than a step's token budget), so that the first requests replay them."""
@@ -214,8 +223,28 @@ class Engine:
             count += step_graphs.capture_prompt_shapes(min(prompt_tokens, self.scheduler.chunked_prefill_size or prompt_tokens))
         return count
 
-    def add_request(self, prompt_ids: Sequence[int], params: SamplingParams) -> Request:
-        req = Request(next(self._rids), list(prompt_ids), params)
+    def load_adapter(self, name: str, source, alpha: float | None = None) -> None:
+        """Take a low-rank adapter in (``AdapterStore.load``: a folder, or tensors by name); requests may have it from then on."""
+        if self.adapters is None:
+            raise ValueError("this engine was made without room for adapters (max_adapters)")
+        self.adapters.load(name, source, alpha)
+
+    def unload_adapter(self, name: str) -> None:
+        """Give an adapter's place back. Refused while a request that is not done has it."""
+        if self.adapters is None:
+            raise ValueError("this engine was made without room for adapters (max_adapters)")
+        slot = self.adapters.slot(name)
+        users = [r.rid for r in self.requests.values() if r.adapter == slot]
+        if users:
+            raise RuntimeError(f"requests {users} still run with adapter {name!r}")
+        self.adapters.unload(name)
+
+    def add_request(self, prompt_ids: Sequence[int], params: SamplingParams, adapter: str | None = None) -> Request:
+        """``adapter``: the name of a loaded low-rank adapter, for this request's tokens alone."""
+        if adapter is not None and self.adapters is None:
+            raise ValueError("this engine was made without room for adapters (max_adapters)")
+        slot = -1 if adapter is None else self.adapters.slot(adapter)
+        req = Request(next(self._rids), list(prompt_ids), params, adapter=slot)
         req.seed = params.seed if params.seed is not None else self._seeds.randrange(2 ** 32)
         self.scheduler.add(req)
         self.requests[req.rid] = req
@@ -267,6 +296,8 @@ class Engine:
         args = None if greedy else dict(
             temperatures=[r.params.temperature for r in reqs], top_ps=[r.params.top_p for r in reqs],
             seeds=[r.seed for r in reqs], counters=[r.seq_len for r in reqs])
+        if any(r.params.is_filtered for r in reqs):
+            args.update(top_ks=[r.params.top_k for r in reqs], min_ps=[r.params.min_p for r in reqs])
         rows = []
         prev_tokens = None
         for r in plan.rows:
@@ -278,7 +309,7 @@ class Engine:
                 if r.count != 1 or prev is None or req.rid not in prev.row_of:
                     raise RuntimeError("a placeholder token outside a decode row, or without the step that sampled it")
                 fill_from, prev_tokens, tokens = prev.row_of[req.rid], prev.tokens, [0]
-            rows.append(StepRow(req.cache, tokens, (r.count - 1,) if r.completes else (), fill_from))
+            rows.append(StepRow(req.cache, tokens, (r.count - 1,) if r.completes else (), fill_from, req.adapter))
         if self.graphs is not None and self.logits_hook is None and plan.phase == "decode" and self.graphs.takes(len(rows)):
             tokens = self.graphs.run(rows, args, prev_tokens=prev_tokens)
         else:
@@ -335,18 +366,23 @@ class Engine:
                 self._retire(req)
 
     def generate(self, prompts: Sequence[Sequence[int]], params: SamplingParams | Sequence[SamplingParams],
-                 on_step=None, max_steps: int | None = None) -> list[list[int]]:
+                 on_step=None, max_steps: int | None = None, adapters: Sequence[str | None] | str | None = None) -> list[list[int]]:
         """Submit all prompts (token ids) at once and run to completion; output token ids per prompt.
         ``on_step(engine, plan)`` is called after every step with the plan that step launched (None if it
-        launched nothing): a place to count, time or check. ``max_steps``: raise if not done by then."""
+        launched nothing): a place to count, time or check. ``max_steps``: raise if not done by then.
+        ``adapters``: the name of each prompt's low-rank adapter (None: none), or one for all."""
         if isinstance(params, SamplingParams):
             params = [params] * len(prompts)
         if len(params) != len(prompts):
             raise ValueError(f"{len(prompts)} prompts but {len(params)} sampling parameters")
+        if adapters is None or isinstance(adapters, str):
+            adapters = [adapters] * len(prompts)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(prompts)} prompts but {len(adapters)} adapters")
         reqs: list[Request] = []
         try:
-            for p, sp in zip(prompts, params):
-                reqs.append(self.add_request(p, sp))
+            for p, sp, name in zip(prompts, params, adapters):
+                reqs.append(self.add_request(p, sp, name) if name is not None else self.add_request(p, sp))
         except Exception:
             # a prompt was refused: none of this call's requests stays behind in the queues
             for r in reqs:

@@ -25,6 +25,7 @@ from typing import Sequence
 
 import torch
 
+from ..sampling.sampler import draw, settings
 from .step import StepFunction, StepRow
 
 
@@ -47,10 +48,11 @@ def graph_buckets(max_bs: int) -> list[int]:
 
 
 class _Captured:
-    __slots__ = ("graph", "tokens", "logits", "f32", "i64", "launches", "sampler_scratch")
+    __slots__ = ("graph", "tokens", "logits", "settings", "launches", "sampler_scratch")
 
-    def __init__(self, graph, tokens, logits, f32, i64, launches, sampler_scratch):
-        self.graph, self.tokens, self.logits, self.f32, self.i64 = graph, tokens, logits, f32, i64
+    def __init__(self, graph, tokens, logits, settings, launches, sampler_scratch):
+        self.graph, self.tokens, self.logits = graph, tokens, logits
+        self.settings = settings  # device tensors that the sampling kernels inside read: f32, i64, top_k, uniform
         self.launches = launches  # launches of this package's kernels inside the graph
         self.sampler_scratch = sampler_scratch  # the sampler's scratch tensor whose address the graph holds (None: none)
 
@@ -96,30 +98,24 @@ class DecodeGraphs:
         n = len(rows)
         bucket = self._bucket(n)
         pad = bucket - n
-        mode = "greedy"
-        if sampling is not None:
-            mode = "top_p" if any(p < 1 for p in sampling["top_ps"]) else "temperature"
+        drawn = settings(**sampling, rows=bucket) if sampling is not None else None
+        mode = drawn.mode if drawn is not None else "greedy"
         ctx = sf.prepare(rows, pad_rows=pad, indices_cap=self.indices_cap, want_pad_rows=True, prev_tokens=prev_tokens)
         if sf.arena_generation != self._generation:  # the arena moved while preparing
             self._drop_all()
         if klass is None:
             klass = length_class(ctx.max_kv_len)
-        cap = self._graphs.get((bucket, mode, klass))
+        # a step with adapters runs other kernels: its graphs are its own
+        key = (bucket, mode if ctx.adapter_rows is None else mode + "+adapters", klass)
+        cap = self._graphs.get(key)
         if cap is not None and cap.sampler_scratch is not None and cap.sampler_scratch is not self.sampler._scratch:
             cap = None  # the sampler has moved to a larger scratch since: the graph's address is stale
         if cap is None:
             cap = self._capture(ctx, bucket, mode, klass)
-            self._graphs[(bucket, mode, klass)] = cap
-        if sampling is not None:
-            f32 = torch.ones((2, bucket), dtype=torch.float32)
-            i64 = torch.zeros((2, bucket), dtype=torch.int64)
-            f32[0, :n] = torch.tensor(sampling["temperatures"], dtype=torch.float32)
-            f32[0, n:] = 0.0
-            f32[1, :n] = torch.tensor(sampling["top_ps"], dtype=torch.float32)
-            i64[0, :n] = torch.tensor(sampling["seeds"], dtype=torch.int64)
-            i64[1, :n] = torch.tensor(sampling["counters"], dtype=torch.int64)
-            cap.f32.copy_(f32.pin_memory(), non_blocking=True)
-            cap.i64.copy_(i64.pin_memory(), non_blocking=True)
+            self._graphs[key] = cap
+        if mode != "greedy":
+            for dst, src in zip(cap.settings, (drawn.f32, drawn.i64) + ((drawn.top_k, drawn.uniform) if drawn.filtered else ())):
+                dst.copy_(src.pin_memory(), non_blocking=True)
         cap.graph.replay()
         self.replayed_launches += cap.launches
         for r in rows:
@@ -136,6 +132,7 @@ class DecodeGraphs:
             "greedy": lambda n: None,
             "temperature": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n),
             "top_p": lambda n: dict(temperatures=[1.0] * n, top_ps=[0.5] * n, seeds=[0] * n, counters=[0] * n),
+            "filtered": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n, top_ks=[2] * n),
         }
         before = len(self._graphs)
         for mode, klass in ((m, k) for m in modes for k in classes):
@@ -149,28 +146,22 @@ class DecodeGraphs:
         torch.cuda.current_stream(sf.device).synchronize()
         return len(self._graphs) - before
 
-    def _forward(self, ctx, bucket: int, mode: str, klass: int, f32, i64):
+    def _forward(self, ctx, bucket: int, mode: str, klass: int, held):
         sf = self.step_fn
         ctx.stream = torch.cuda.current_stream(sf.device).cuda_stream
         ctx.graph_bucket = bucket
         ctx.graph_kv_len = klass
         logits = sf.model.forward(ctx, sf.cache.entry_views)
         tokens = torch.empty(bucket, dtype=torch.int32, device=sf.device)
-        from .. import ops
-
-        if mode == "greedy":
-            ops.sample(tokens, logits, stream=ctx.stream)
-        else:
-            ops.sample(tokens, logits, temperature=f32[0], top_p=f32[1] if mode == "top_p" else None, seed=i64[0],
-                       counter=i64[1], scratch=self.sampler._scratch if mode == "top_p" else None,
-                       stream=ctx.stream)
+        draw(tokens, logits, mode, *held, self.sampler._scratch, ctx.stream)
         return logits, tokens
 
     def _capture(self, ctx, bucket: int, mode: str, klass: int) -> _Captured:
         sf = self.step_fn
-        f32 = torch.zeros((2, bucket), dtype=torch.float32, device=sf.device)
-        f32[1] = 1.0
-        i64 = torch.zeros((2, bucket), dtype=torch.int64, device=sf.device)
+        f32 = torch.zeros((5, bucket), dtype=torch.float32, device=sf.device)
+        f32[1] = f32[3] = 1.0
+        held = (f32, torch.zeros((2, bucket), dtype=torch.int64, device=sf.device), torch.zeros(bucket, dtype=torch.int32, device=sf.device),
+                torch.zeros(bucket, dtype=torch.float64, device=sf.device))
         self.sampler._ensure(bucket)
         torch.cuda.current_stream(sf.device).synchronize()
         s = self.capture_stream
@@ -182,7 +173,7 @@ class DecodeGraphs:
         kept = [(st, st[slots].clone()) for st in sf.cache.state_tensors()]
         with torch.cuda.stream(s):
             s.wait_stream(torch.cuda.current_stream(sf.device))
-            self._forward(ctx, bucket, mode, klass, f32, i64)
+            self._forward(ctx, bucket, mode, klass, held)
         s.synchronize()
         for st, value in kept:
             st[slots] = value
@@ -197,7 +188,7 @@ class DecodeGraphs:
         try:
             with torch.cuda.graph(graph, pool=self._pool, stream=s):
                 gc.disable()
-                logits, tokens = self._forward(ctx, bucket, mode, klass, f32, i64)
+                logits, tokens = self._forward(ctx, bucket, mode, klass, held)
         finally:
             if collecting:
                 gc.enable()
@@ -205,7 +196,7 @@ class DecodeGraphs:
         native.LAUNCHES[0] = before  # a capture launches nothing
         if self._pool is None:
             self._pool = graph.pool()
-        return _Captured(graph, tokens, logits, f32, i64, launches, self.sampler._scratch if mode == "top_p" else None)
+        return _Captured(graph, tokens, logits, held, launches, self.sampler._scratch if mode.startswith("top_p") else None)
 
 
 class _Recorder:
@@ -341,7 +332,9 @@ class StepGraphs:
         # decoding rows come first in a mixed step; how many there are decides which attention kernels run on what
         single = next((i for i, r in enumerate(rows) if len(r.tokens) != 1), len(rows))
         # (tokens run, rows with the padding row, wanted logits, decoding rows at the front)
-        return run_with, len(rows) + (run_with != tokens), sum(len(r.want) for r in rows), single
+        key = run_with, len(rows) + (run_with != tokens), sum(len(r.want) for r in rows), single
+        # a step with adapters runs other kernels
+        return key + ("adapters",) if any(r.adapter >= 0 for r in rows) else key
 
     def run(self, rows: Sequence[StepRow], prev_tokens: torch.Tensor | None = None) -> torch.Tensor | None:
         """The step's logits, or None if this step is left to the eager path (nothing was touched then)."""

@@ -66,7 +66,9 @@ class SamplingParams:
     ``max_new_tokens``: the most tokens to produce (at least one). ``stop_token_ids``: producing
     any of these ends the request; the token stays in the output. ``temperature``: 0 picks the most
     likely token, larger values sample from the softened distribution. ``top_p``: sample only among
-    the most likely tokens whose probabilities add up to this much. ``seed``: makes sampling
+    the most likely tokens whose probabilities add up to this much. ``top_k``: sample only among so many of the most likely
+    tokens (0: all). ``min_p``: only among tokens at least this much as likely as the most likely one (0: all). top_k comes first, top_p is of
+    what it leaves. A request with top_k or min_p is sampled by ``ops.sample_filtered`` from one random number a token, others as ever. ``seed``: makes sampling
     repeatable; left None, the engine draws one per request from its own seed.
     """
 
@@ -75,6 +77,8 @@ class SamplingParams:
     temperature: float = 0.0
     top_p: float = 1.0
     seed: int | None = None
+    top_k: int = 0
+    min_p: float = 0.0
 
     def __post_init__(self):
         object.__setattr__(self, "stop_token_ids", frozenset(self.stop_token_ids))
@@ -82,6 +86,8 @@ class SamplingParams:
             (self.max_new_tokens >= 1, f"max_new_tokens={self.max_new_tokens}: a request produces at least one token"),
             (self.temperature >= 0, f"temperature={self.temperature}: cannot be negative (0 is greedy)"),  # NaN fails too
             (0 < self.top_p <= 1, f"top_p={self.top_p}: a probability mass in (0, 1]"),
+            (self.top_k >= 0 and self.top_k == int(self.top_k) and self.top_k < 1 << 31, f"top_k={self.top_k}: a number of tokens (0: all)"),
+            (0 <= self.min_p <= 1, f"min_p={self.min_p}: a share of the most likely token's probability in [0, 1]"),
             (self.seed is None or 0 <= self.seed < 1 << 32, f"seed={self.seed}: an unsigned 32-bit number, or None"),
         ]
         for ok, message in problems:
@@ -91,6 +97,11 @@ class SamplingParams:
     @property
     def is_greedy(self) -> bool:
         return self.temperature == 0
+
+    @property
+    def is_filtered(self) -> bool:
+        """Whether it samples through ``ops.sample_filtered``."""
+        return not self.is_greedy and (self.top_k > 0 or self.min_p > 0)
 
 
 @dataclass(eq=False)
@@ -103,6 +114,7 @@ class Request:
     cache: RequestCache | None = None  # its pages and state slot, from admission until it ends or is preempted
     seed: int = 0
     num_preemptions: int = 0
+    adapter: int = -1  # the slot of its low-rank adapter, below 0: none
     num_pending: int = 0  # how many entries at the end of output_ids are still PLACEHOLDER
 
     def __post_init__(self):

@@ -16,6 +16,7 @@ from typing import Sequence
 import numpy as np
 import torch
 
+from .. import ops
 from ..cache.manager import CacheManager, RequestCache
 from ..ops import native
 from ..parts.decoder import DecoderModel
@@ -33,6 +34,7 @@ class StepRow:
     # If set, the row brings one token that the host does not know yet: it is entry ``fill_from``
     # of the previous step's sampled tokens, still on the device (``tokens`` then holds any valid id).
     fill_from: int | None = None
+    adapter: int = -1  # the slot of the request's low-rank adapter (engine/adapters.py); below 0: none
 
 
 def _leading_ones(q_len: np.ndarray, pad_rows: int, pad_len: int = 1) -> int:
@@ -66,12 +68,13 @@ class StepFunction:
         self._turn = 0
         self.arena_generation = 0  # bumped when the device arena moves (captured graphs become stale)
         self._grow(arena_ints)
-        from .. import ops
-
         self.status = ops.device_status(self.device)  # shared by every kernel launched on this device
         props = torch.cuda.get_device_properties(self.device)
         self.sm_count = props.multi_processor_count
         self.persistent_scratch: dict = {}
+        self.low_rank: dict = {}  # (part, product) -> ops.LowRank (``AdapterStore.products``) where requests may have adapters
+        self._adapter_slots: torch.Tensor | None = None  # int32 [rows]: a step's, where a request of it has an adapter
+        self._adapter_pinned: list[torch.Tensor] = []
         self.h2d_bytes = 0  # bytes of step metadata copied to the device so far
         # StepGraphs (engine/graphs.py) when the engine replays recurring step shapes from CUDA graphs; its
         # run() returns None for a step it does not take, which then runs eagerly
@@ -91,6 +94,15 @@ class StepFunction:
         if ints > self._arena_ints:
             torch.cuda.current_stream(self.device).synchronize()
             self._grow(ints)
+
+    def reserve_adapter_slots(self, rows: int) -> None:
+        """Room for the adapters of steps of so many rows; made once, it does not move under captured graphs unless a larger step comes."""
+        if self._adapter_slots is None or rows > self._adapter_slots.numel():
+            torch.cuda.current_stream(self.device).synchronize()
+            rows = max(rows, 256)
+            self._adapter_slots = torch.full((rows,), -1, dtype=torch.int32, device=self.device)
+            self._adapter_pinned = [torch.empty(rows, dtype=torch.int32, pin_memory=True) for _ in range(_NUM_BUFFERS)]
+            self.arena_generation += 1  # (graphs hold its address as they do the arena's)
 
     def _arena_need(self, rows: Sequence[StepRow], pad_rows: int, indices_cap: int = 0, pad_len: int = 1) -> int:
         t = sum(len(r.tokens) for r in rows) + pad_rows * pad_len
@@ -146,6 +158,11 @@ class StepFunction:
         if fills:
             if prev_tokens is None or any(len(rows[i].tokens) != 1 for i, _ in fills):
                 raise ValueError("a row filled from the previous step brings exactly one token and needs that step's tokens")
+        adapted = any(r.adapter >= 0 for r in rows)
+        if adapted:
+            if not self.low_rank:
+                raise ValueError("a row with an adapter needs the adapters (StepFunction.low_rank)")
+            self.reserve_adapter_slots(len(rows) + pad_rows)
         need = self._arena_need(rows, pad_rows, indices_cap, pad_len) + 2 * len(fills) + 8
         if need > self._arena_ints:
             torch.cuda.current_stream(self.device).synchronize()
@@ -192,6 +209,11 @@ class StepFunction:
             native.kernel_check(k.ms_fill_tokens(dev[int(offsets[0]):].data_ptr(), dev[packed:].data_ptr(), prev_tokens.data_ptr(),
                                                  dev[packed + len(fills):].data_ptr(), len(fills), stream.cuda_stream))
             total = packed
+        if adapted:
+            of_row = self._adapter_pinned[turn][:len(rows) + pad_rows]
+            of_row.copy_(torch.tensor([r.adapter for r in rows] + [-1] * pad_rows, dtype=torch.int32))
+            self._adapter_slots[:len(rows) + pad_rows].copy_(of_row, non_blocking=True)
+            self.h2d_bytes += 4 * (len(rows) + pad_rows)
         ev = torch.cuda.Event()
         ev.record(stream)
         self._events[turn] = ev
@@ -222,7 +244,8 @@ class StepFunction:
             max_q_len=max(int(q_len.max()), pad_len if pad_rows else 1), max_kv_len=max(int(kv_end.max()), pad_len if pad_rows else 1),
             decode_only=bool((q_len == 1).all()),
             leading_single_rows=_leading_ones(q_len, pad_rows, pad_len), sm_count=self.sm_count, scratch=self.persistent_scratch,
-            tables_ahead=True, layout=tuple(o))
+            adapter_rows=ops.AdapterRows(self._adapter_slots[:r_all], view(o[2], t_all)) if adapted else None,
+            low_rank=self.low_rank if adapted else {}, tables_ahead=True, layout=tuple(o))
 
     def reset_after_fault(self) -> None:
         """After a kernel raised the status word: wait for what is in flight, then zero the word and

@@ -489,7 +489,7 @@ def qkv_norm_rope_kv(q_out: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     native.kernel_check(lib.ms_gemm_tc_qkv_bf16(
         _ptr(q_out), _ptr(x), _ptr(w_qkv), t, x.shape[1], nq, nkv, _ptr(k_pool), _ptr(v_pool), _ptr(q_norm_w), _ptr(k_norm_w),
         _ptr(cos_sin), _ptr(positions), _ptr(row_of_token), _ptr(page_indptr), _ptr(page_indices), page_size, float(eps),
-        _ptr(device_status(x.device)), _stream(stream), None if product is None else ctypes.addressof(product)), lib=lib, errfn="ms_gemm_tc_last_error")
+        _ptr(device_status(x.device)), _stream(stream), product), lib=lib, errfn="ms_gemm_tc_last_error")
 
 
 def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, num_tokens: int, rotary_dim: int, stream=None) -> torch.Tensor:

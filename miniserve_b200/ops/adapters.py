@@ -5,6 +5,7 @@ adapters (``LowRank``), which adapter each of a step's tokens has (``AdapterRows
 from __future__ import annotations
 
 import ctypes
+import struct
 from contextlib import nullcontext
 from ctypes import c_char_p, c_int, c_ulonglong, c_void_p
 from dataclasses import dataclass
@@ -16,6 +17,7 @@ from . import build, native
 
 _p, _i = c_void_p, c_int
 MAX_PARTS, MAX_RANK, TILE = 4, 256, 256  # TILE: tokens of a row tile of the plan
+BLOCK_BYTES = 48  # of an ``AdapterBlock`` (csrc/adapters.cuh)
 ADAPTERS = build.Module("adapters", ("adapters.cu",))
 _TYPES = (torch.bfloat16, torch.float32)
 
@@ -47,7 +49,10 @@ class LowRank:
             raise ValueError(f"the parts of {n} outputs end at {ends}")
         if not (a.device == b.device == c.device) or any(not t.is_contiguous() for t in (a, b, c)) or a.data_ptr() % 16 or b.data_ptr() % 16:
             raise ValueError("an adapter's tensors lie on one device, contiguous, the matrices on 16 bytes")
-        for name, value in (("ends", ends), ("slots", slots), ("rank", rank), ("parts", len(ends)), ("outputs", n), ("inputs", a.shape[2]), ("index", a.get_device())):
+        # what every call asks for: sizes, the device's index (-1: the host), the two ends of the kernels' ``Adapters``
+        for name, value in (("ends", ends), ("slots", slots), ("rank", rank), ("parts", len(ends)), ("outputs", n), ("inputs", a.shape[2]), ("index", a.get_device()),
+                            ("dtype", a.dtype), ("numbers", len(ends) * rank), ("head", struct.pack("3Q", a.data_ptr(), b.data_ptr(), c.data_ptr())),
+                            ("tail", struct.pack("7i4x", slots, rank, len(ends), *ends, *[n] * (MAX_PARTS - len(ends))))):
             object.__setattr__(self, name, value)
 
     @classmethod
@@ -72,6 +77,10 @@ class AdapterRows:
         self.slot_of_row, self.row_of_token = slot_of_row, row_of_token
         self.rows, self.tokens, self.index = slot_of_row.shape[0], row_of_token.shape[0], slot_of_row.get_device()
         self._plans: dict = {}
+        if self.index >= 0:
+            from . import device_status
+
+            self.middle = struct.pack("3Q", slot_of_row.data_ptr(), row_of_token.data_ptr(), device_status(slot_of_row.device).data_ptr())
 
     def plan(self, slots: int, stream: int) -> "_Plan":
         """The adapters of each row tile, for projections with ``slots`` of them."""
@@ -82,34 +91,19 @@ class AdapterRows:
         return held
 
 
-class _Adapters(ctypes.Structure):
-    """``Adapters`` of csrc/adapters.cuh."""
-
-    _fields_ = [(n, _p) for n in ("a", "b", "scale", "slot_of_row", "row_of_token", "status")] + [("slots", _i), ("rank", _i), ("parts", _i), ("ends", _i * MAX_PARTS)]
-
-
-class _Product(ctypes.Structure):
-    """``AdaptedProduct`` of csrc/adapters.cuh."""
-
-    _fields_ = [("ad", _Adapters), ("v", _p), ("tile_first", _p), ("block_slot", _p), ("max_blocks", _i)]
-
-
 class _Plan:
     def __init__(self, rows: AdapterRows, slots: int, stream: int):
-        from . import device_status
-
         device, t = rows.slot_of_row.device, rows.tokens
         tiles = -(-t // TILE)
         # a request of several tiles has a block in each, and each request behind the first may add one to a tile that it shares
         self.max_blocks = max(1, min(tiles * min(slots, TILE), tiles + rows.rows - 1))
         with on_stream(stream, device):
-            self.ints = torch.empty(tiles + 1 + 2 * self.max_blocks + t, dtype=torch.int32, device=device)
-        at = self.ints.data_ptr()
-        self.tile_first, self.block_slot = at, at + 4 * (tiles + 1)
-        self.block_tile = self.block_slot + 4 * self.max_blocks
-        self.token_slot = self.block_tile + 4 * self.max_blocks
-        ad = _Adapters(None, None, None, rows.slot_of_row.data_ptr(), rows.row_of_token.data_ptr(), device_status(device).data_ptr(), slots, 0, 0)
-        _check(_lib().ms_adapter_plan(self.tile_first, self.block_slot, self.block_tile, self.token_slot, ctypes.addressof(ad), t, self.max_blocks, stream))
+            self.ints = torch.empty((BLOCK_BYTES // 4 + 1) * self.max_blocks + tiles + 1, dtype=torch.int32, device=device)
+        self.blocks = self.ints.data_ptr()
+        self.block_slot = self.blocks + BLOCK_BYTES * self.max_blocks
+        self.tile_first = self.block_slot + 4 * self.max_blocks
+        ad = bytes(24) + rows.middle + struct.pack("7i4x", slots, 0, 0, 0, 0, 0, 0)
+        _check(_lib().ms_adapter_plan(self.tile_first, self.block_slot, self.blocks, ad, t, self.max_blocks, stream))
 
 
 @lru_cache(maxsize=None)
@@ -118,10 +112,9 @@ def _lib():
     native._declare(lib, "ms_adapters_last_error", [], c_char_p)
     native._declare(lib, "ms_adapters_set_pdl", [_i], None)
     native._declare(lib, "ms_adapter_capture_id", [_p], c_ulonglong)
-    native._declare(lib, "ms_adapter_plan", [_p] * 5 + [_i, _i, _p])
-    native._declare(lib, "ms_adapter_shrink", [_p, _p, _p, _i, _i, _i, _i, _p])
-    native._declare(lib, "ms_adapter_shrink_blocks", [_p] * 7 + [_i] * 5 + [_p])
-    native._declare(lib, "ms_adapter_expand", [_p] * 4 + [_i] * 6 + [_p])
+    native._declare(lib, "ms_adapter_plan", [_p] * 3 + [c_char_p, _i, _i, _p])
+    native._declare(lib, "ms_adapter_shrink", [_p, _p, c_char_p, _i, _i, _i, _i, _p])
+    native._declare(lib, "ms_adapter_expand", [_p, _p, _p, c_char_p] + [_i] * 6 + [_p])
     lib.ms_adapters_set_pdl(int(native.pdl_enabled()))
     return lib
 
@@ -140,102 +133,102 @@ def on_stream(stream: int, device: torch.device):
 def check(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
     if not isinstance(low_rank, LowRank) or not isinstance(rows, AdapterRows):
         raise TypeError("an adapted product takes low_rank (ops.LowRank) and adapter_rows (ops.AdapterRows), both")
-    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != low_rank.inputs or tuple(weight.shape) != (low_rank.outputs, low_rank.inputs):
-        raise ValueError(f"x is {tuple(x.shape)}, the weight {tuple(weight.shape)}, its adapters take {low_rank.inputs} and give {low_rank.outputs}")
-    if x.shape[0] != rows.tokens:
-        raise ValueError(f"x has {x.shape[0]} tokens, adapter_rows {rows.tokens}")
-    if x.dtype is not low_rank.a.dtype or weight.dtype is not x.dtype:
-        raise TypeError(f"x, the weight and its adapters are of one type, not {x.dtype}, {weight.dtype} and {low_rank.a.dtype}")
-    if not (x.get_device() == weight.get_device() == low_rank.index == rows.index >= 0) or not x.is_contiguous() or not weight.is_contiguous() or x.data_ptr() % 16:
+    shape, dtype, index = x.shape, x.dtype, low_rank.index
+    if len(shape) != 2 or shape[1] != low_rank.inputs or weight.shape != (low_rank.outputs, low_rank.inputs):
+        raise ValueError(f"x is {tuple(shape)}, the weight {tuple(weight.shape)}, its adapters take {low_rank.inputs} and give {low_rank.outputs}")
+    if shape[0] != rows.tokens:
+        raise ValueError(f"x has {shape[0]} tokens, adapter_rows {rows.tokens}")
+    if dtype is not low_rank.dtype or weight.dtype is not dtype:
+        raise TypeError(f"x, the weight and its adapters are of one type, not {dtype}, {weight.dtype} and {low_rank.dtype}")
+    if not (x.get_device() == weight.get_device() == index == rows.index >= 0) or not x.is_contiguous() or not weight.is_contiguous() or x.data_ptr() % 16:
         raise ValueError("kernel operands must be contiguous CUDA tensors on one device, x on 16 bytes")
-    out_columns = low_rank.outputs // 2 if gated else low_rank.outputs
-    if gated and (low_rank.outputs % 2 or out.dtype is not x.dtype):
-        raise ValueError(f"a gate|up projection of {low_rank.outputs} rows, out {out.dtype} for x {x.dtype}")
-    if out is not None and (tuple(out.shape) != (x.shape[0], out_columns) or out.get_device() != low_rank.index or not out.is_contiguous()
-                            or out.dtype not in ((torch.float32,) if x.dtype is torch.float32 else _TYPES)):
-        raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, not a contiguous [{x.shape[0]}, {out_columns}]")
-
-
-def _struct(low_rank: LowRank, rows: AdapterRows) -> _Adapters:
-    from . import device_status
-
-    return _Adapters(low_rank.a.data_ptr(), low_rank.b.data_ptr(), low_rank.scale.data_ptr(), rows.slot_of_row.data_ptr(), rows.row_of_token.data_ptr(),
-                     device_status(low_rank.a.device).data_ptr(), low_rank.slots, low_rank.rank, low_rank.parts,
-                     (_i * MAX_PARTS)(*low_rank.ends, *[low_rank.outputs] * (MAX_PARTS - low_rank.parts)))
+    if gated and (low_rank.outputs % 2 or out.dtype is not dtype):
+        raise ValueError(f"a gate|up projection of {low_rank.outputs} rows, out {out.dtype} for x {dtype}")
+    if out is not None and (out.shape != (shape[0], low_rank.outputs // 2 if gated else low_rank.outputs) or out.get_device() != index or not out.is_contiguous()
+                            or (out.dtype is not dtype and out.dtype is not torch.float32)):
+        raise ValueError(f"out is {out.dtype} {tuple(out.shape)} for {shape[0]} tokens and {low_rank.outputs} outputs{' (gate and up)' if gated else ''}: a contiguous tensor on the "
+                         "adapters' device, of x's type or float32")
 
 
 def _code(dtype: torch.dtype) -> int:
     return 0 if dtype is torch.float32 else 1
 
 
-FEW_TOKENS = 48  # up to so many, v is made token by token
+FEW_TOKENS = 64  # up to so many, v is made token by token, and the products are the decode steps' tcgen05 kernel
 
 
-def _v(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: _Adapters, stream: int) -> torch.Tensor:
+def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, stream: int) -> torch.Tensor:
     """What the adapters' A make of x, float32 [T, parts * rank]."""
+    from . import tc_gemm_enabled
+
     t, k = x.shape
     with on_stream(stream, x.device):
-        v = torch.empty((t, low_rank.parts * low_rank.rank), dtype=torch.float32, device=x.device)
-    if x.dtype is torch.float32 or t <= FEW_TOKENS:
-        _check(_lib().ms_adapter_shrink(v.data_ptr(), x.data_ptr(), ctypes.addressof(ad), t, low_rank.outputs, k, _code(x.dtype), stream))
+        v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=x.device)
+    if t <= FEW_TOKENS or x.dtype is torch.float32 or not tc_gemm_enabled():
+        _check(_lib().ms_adapter_shrink(v.data_ptr(), x.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), stream))
     else:
-        plan = rows.plan(low_rank.slots, stream)
-        _check(_lib().ms_adapter_shrink_blocks(v.data_ptr(), x.data_ptr(), ctypes.addressof(ad), plan.tile_first, plan.block_slot, plan.block_tile, plan.token_slot, t,
-                                               low_rank.outputs, k, plan.max_blocks, 1, stream))
+        _blocks(v, x, rows.plan(low_rank.slots, stream), ad, True, stream)
     return v
 
 
+def _blocks(v: torch.Tensor, x: torch.Tensor, plan: _Plan, ad: bytes, compact: bool, stream: int) -> None:
+    from . import device_status
+
+    lib = native.gemm_tc()
+    rc = lib.ms_gemm_tc_adapter_v(v.data_ptr(), x.data_ptr(), ad, plan.tile_first, plan.blocks, x.shape[0], x.shape[1], plan.max_blocks, int(compact), device_status(x.device).data_ptr(), stream)
+    native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
+
+
 def product(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, stream: int) -> tuple:
-    """What a product on the 2-CTA tcgen05 kernel takes of the adapters, and the V it points to."""
-    t, k = x.shape
-    ad, plan = _struct(low_rank, rows), rows.plan(low_rank.slots, stream)
+    """What a product on the 2-CTA tcgen05 kernel takes of the adapters (``AdaptedProduct``), and the V it points to."""
+    ad, plan = low_rank.head + rows.middle + low_rank.tail, rows.plan(low_rank.slots, stream)
     with on_stream(stream, x.device):
-        v = torch.empty((plan.max_blocks * TILE, low_rank.parts * low_rank.rank), dtype=torch.bfloat16, device=x.device)
-    _check(_lib().ms_adapter_shrink_blocks(v.data_ptr(), x.data_ptr(), ctypes.addressof(ad), plan.tile_first, plan.block_slot, plan.block_tile, plan.token_slot, t,
-                                           low_rank.outputs, k, plan.max_blocks, 0, stream))
-    return _Product(ad, v.data_ptr(), plan.tile_first, plan.block_slot, plan.max_blocks), v
+        v = torch.empty((plan.max_blocks * TILE, low_rank.numbers), dtype=torch.bfloat16, device=x.device)
+    _blocks(v, x, plan, ad, False, stream)
+    return ad + struct.pack("3Qi4x", v.data_ptr(), plan.tile_first, plan.block_slot, plan.max_blocks), v
 
 
-def _in_its_sums(x, weight, out, epilogue: str) -> bool:
-    """Whether the product runs on the 2-CTA tcgen05 kernel, which takes the adapters in its own sums."""
-    from . import tc_gemm_ok
-
-    return x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and x.shape[0] > FEW_TOKENS and tc_gemm_ok(x, weight, out, epilogue)
+def in_its_sums(tokens: int, outputs: int, gated: bool, sms: int) -> bool:
+    """Whether a product of many tokens runs on the 2-CTA tcgen05 kernel, which takes the adapters in its own sums, rather than in float32 wherever ``linear`` sends it, with
+    the adapters' terms added behind."""
+    tiles = -(-tokens // TILE) * -(-outputs // (128 if gated else 256))
+    return tiles >= sms // 8
 
 
 def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
-    from . import TC_EPILOGUE, device_status
+    from . import _sm_count, device_status, tc_gemm_enabled
     from . import linear as shared
 
     t, k = x.shape
-    epilogue = "silu_mul" if gated else "bf16"
-    if _in_its_sums(x, weight, out, epilogue):
-        held, v = product(x, low_rank, rows, stream)
-        lib = native.gemm_tc()
-        native.kernel_check(lib.ms_gemm_tc_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, out.shape[1], k, TC_EPILOGUE[epilogue], ctypes.addressof(held),
-                                                        device_status(x.device).data_ptr(), stream), lib=lib, errfn="ms_gemm_tc_last_error")
-        return
+    n, ad = out.shape[1], low_rank.head + rows.middle + low_rank.tail
+    if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and weight.data_ptr() % 16 == 0 and tc_gemm_enabled():
+        few = t <= FEW_TOKENS
+        if few or in_its_sums(t, n, gated, _sm_count(x.device)):
+            lib, status = native.gemm_tc(), device_status(x.device).data_ptr()
+            if few:
+                v = _terms(x, low_rank, rows, ad, stream)
+                rc = lib.ms_gemm_tc_decode_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated), struct.pack("Q", v.data_ptr()) + ad, status, stream)
+            else:
+                held, v = product(x, low_rank, rows, stream)
+                rc = lib.ms_gemm_tc_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, 2 if gated else 0, held, status, stream)
+            native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
+            return
     # the shared product in float32, so that the sum is rounded once
-    ad = _struct(low_rank, rows)
-    if out.dtype is torch.float32 and not gated:
-        y = out
-    else:
+    y = out
+    if out.dtype is not torch.float32 or gated:
         with on_stream(stream, x.device):
             y = torch.empty((t, low_rank.outputs), dtype=torch.float32, device=x.device)
     shared(x, weight, out=y, stream=stream)
-    v = _v(x, low_rank, rows, ad, stream)
-    _check(_lib().ms_adapter_expand(out.data_ptr(), y.data_ptr(), v.data_ptr(), ctypes.addressof(ad), t, low_rank.outputs, k, _code(x.dtype), _code(out.dtype), int(gated), stream))
+    v = _terms(x, low_rank, rows, ad, stream)
+    _check(_lib().ms_adapter_expand(out.data_ptr(), y.data_ptr(), v.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), _code(out.dtype), int(gated), stream))
 
 
 def _here(call, x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
     """The call on its tensors' device, and its stream (None: that device's current one)."""
-    device = low_rank.a.device
-    if stream is None:
-        stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == low_rank.index:
-        return call(x, weight, out, stream, low_rank, rows)
-    with torch.cuda.device(device):
-        return call(x, weight, out, stream, low_rank, rows)
+        return call(x, weight, out, torch.cuda.current_stream().cuda_stream if stream is None else stream, low_rank, rows)
+    with torch.cuda.device(low_rank.index):
+        return call(x, weight, out, torch.cuda.current_stream().cuda_stream if stream is None else stream, low_rank, rows)
 
 
 def linear(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:

@@ -249,8 +249,10 @@ def gemm_tc():
     _declare(lib, "ms_gemm_tc_set_config", [_i], None)
     _declare(lib, "ms_gemm_tc_set_grouped", [_i], None)
     _declare(lib, "ms_gemm_tc_prefers", [_i, _i, _i, _i])
-    _declare(lib, "ms_gemm_tc_qkv_bf16", [_p, _p, _p, _i, _i, _i, _i] + [_p] * 9 + [_i, _f, _p, _p, _p])
-    _declare(lib, "ms_gemm_tc_adapted_bf16", [_p, _p, _p, _i, _i, _i, _i, _p, _p, _p])
+    _declare(lib, "ms_gemm_tc_qkv_bf16", [_p, _p, _p, _i, _i, _i, _i] + [_p] * 9 + [_i, _f, _p, _p, c_char_p])
+    _declare(lib, "ms_gemm_tc_adapted_bf16", [_p, _p, _p, _i, _i, _i, _i, c_char_p, _p, _p])
+    _declare(lib, "ms_gemm_tc_decode_adapted_bf16", [_p, _p, _p, _i, _i, _i, _i, c_char_p, _p, _p])
+    _declare(lib, "ms_gemm_tc_adapter_v", [_p, _p, c_char_p, _p, _p, _i, _i, _i, _i, _p, _p])
     lib.ms_gemm_tc_set_pdl(int(pdl_enabled()))
     return lib
 

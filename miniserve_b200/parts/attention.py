@@ -182,6 +182,11 @@ class GQAttention(Part):
         # one product makes q, k and v (miniserve/model/fused.py:41-95 joins the same rows), and the gate
         return dict([self._stack()]) if self.owns_cache or self.out_gate else {}
 
+    def adapted_products(self):
+        if self.general:  # (its products are also made by callers, joined with others)
+            return {}
+        return {"qkv": self._stack()[1], "o": (self.names["o"],)}
+
     def bind(self, tensors):
         n = self.names
         if self.owns_cache or self.out_gate:
@@ -281,9 +286,9 @@ class GQAttention(Part):
                 if tiled is None:  # once per step; every layer with the same table shares it
                     tiled = ctx.step_cache[key] = ops.rope_table_tiled(table, stream=ctx.stream)
             ops.qkv_norm_rope_kv(q, cache.k, cache.v, x, self.w_qkv, self.w_q_norm, self.w_k_norm, tiled, self.qk_norm_eps,
-                                 ctx.positions, ctx.row_of_token, indptr, indices, cache.page_size, stream=ctx.stream)
+                                 ctx.positions, ctx.row_of_token, indptr, indices, cache.page_size, stream=ctx.stream, **self.beside(ctx, "qkv"))
         else:
-            qkv = ops.linear(x, self.w_qkv, stream=ctx.stream, out=ctx.buffer("attn.qkv", (t, self.w_qkv.shape[0]), dt, dev))
+            qkv = ops.linear(x, self.w_qkv, stream=ctx.stream, out=ctx.buffer("attn.qkv", (t, self.w_qkv.shape[0]), dt, dev), **self.beside(ctx, "qkv"))
             ops.qk_norm_rope_kv(
                 q, cache.k if self.owns_cache else None, cache.v if self.owns_cache else None, qkv,
                 self.w_q_norm, self.w_k_norm, inv_freq, rotary_dim, self.qk_norm_eps, ctx.positions,
@@ -292,4 +297,4 @@ class GQAttention(Part):
         out = ctx.buffer("attn.out", (t, self.heads, self.head_dim), dt, dev)
         ops.attention(out, q, cache.k, cache.v, ctx, cache.group, self.scale, self.window, self.sink)
         return ops.linear(out.view(t, self.heads * self.head_dim), self.w_o, stream=ctx.stream,
-                          out=ctx.buffer("attn.proj", (t, self.w_o.shape[0]), dt, dev))
+                          out=ctx.buffer("attn.proj", (t, self.w_o.shape[0]), dt, dev), **self.beside(ctx, "o"))

@@ -139,6 +139,19 @@ class Part:
         place in one buffer; a part that declares a stack accepts either."""
         return {}
 
+    def adapted_products(self) -> dict[str, tuple[str, ...]]:
+        """Products that requests may have low-rank adapters beside: ``{product: (declared names of the matrices that are stacked in it, in order)}``. A step
+        that has adapters carries an ``ops.LowRank`` for each (``ctx.low_rank``); the part hands it on (``beside``)."""
+        return {}
+
+    def beside(self, ctx, product: str) -> dict:
+        """What a product of this part takes of the step's adapters: nothing where the step's requests have none, or none beside it."""
+        rows = getattr(ctx, "adapter_rows", None)
+        if rows is None:
+            return {}
+        low = ctx.low_rank.get((self, product))
+        return {} if low is None else dict(low_rank=low, adapter_rows=rows)
+
     def bind(self, tensors: Mapping[str, torch.Tensor]) -> None:
         for name in self.weights():
             setattr(self, "w_" + name.replace(".", "_"), tensors[name])

@@ -43,6 +43,9 @@ class SwiGLU(Part):
     def stacks(self):
         return dict([self._stack()])
 
+    def adapted_products(self):
+        return {"gate_up": self._stack()[1], "down": (self.names["down"],)} if self.activation == "silu" else {}
+
     def bind(self, tensors):
         self.w_gate_up = self.joined(tensors, *self._stack())
         self.w_down = tensors[self.names["down"]].contiguous()
@@ -50,7 +53,10 @@ class SwiGLU(Part):
     def forward(self, x, ctx) -> torch.Tensor:
         t, dt, dev = x.shape[0], self.env.dtype, self.w_down.device
         act = ctx.buffer("mlp.act", (t, self.inter), dt, dev)
-        if dt == torch.bfloat16 and self.activation == "silu":
+        adapted = self.beside(ctx, "gate_up")
+        if adapted:
+            ops.linear_silu_mul(x, self.w_gate_up, act, stream=ctx.stream, **adapted)
+        elif dt == torch.bfloat16 and self.activation == "silu":
             # one kernel with the activation in its epilogue where there is one (decode steps, wide prompt steps)
             fused = ops.silu_mul_is_fused(x, self.w_gate_up, act)
             scratch = None if fused else ctx.buffer("mlp.gate_up", (t, 2 * self.inter), dt, dev)
@@ -61,7 +67,7 @@ class SwiGLU(Part):
                 ops.silu_mul(act, gate_up, stream=ctx.stream)
             else:
                 ops.act_mul(act, gate_up, self.activation, stream=ctx.stream)
-        return ops.linear(act, self.w_down, stream=ctx.stream, out=ctx.buffer("mlp.down", (t, self.hidden), dt, dev))
+        return ops.linear(act, self.w_down, stream=ctx.stream, out=ctx.buffer("mlp.down", (t, self.hidden), dt, dev), **self.beside(ctx, "down"))
 
 
 @register_part("feed_forward", "clamped_glu")
