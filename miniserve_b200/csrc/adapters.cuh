@@ -37,10 +37,12 @@ struct AdapterBlock {
 };
 static_assert(sizeof(AdapterBlock) == 48, "what the host allots");
 
-// An adapted product of few tokens: v float32 [T, parts * rank] (ms_adapter_shrink); rows of tokens without an adapter are not read.
+// An adapted product of few tokens: v float32 [T, parts * rank]; rows of tokens without an adapter are not read. tickets null: an earlier launch made v (ms_adapter_shrink);
+// else the product's own CTAs make it, and tickets are two zeros that no other launch has.
 struct AdapterTerms {
-  const float* v;
+  float* v;
   Adapters ad;
+  int* tickets;
 };
 
 __device__ __forceinline__ int adapter_of(const Adapters& ad, int t) {

@@ -724,13 +724,16 @@ __device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %
 // warp's 32 rows of B an instruction; a cluster's CTAs share the adapters out, and a term enters the sum over the slices with the CTA that made it. One rounding.
 // (Terms as k-blocks of the tensor cores, as in the 2-CTA kernel, cost a copy of 128 short rows for each adapter of the step: 42.9 us at 64 tokens of 16 adapters, rank 32,
 // 4096 -> 6144; row by row with multiply-adds 63.7.)
+// v may be this kernel's own work (tickets): the same warps of all CTAs take (token, number) after (token, number) from a counter, a dot product of x's row and A's each,
+// and a second counter says when all are done. What is taken is being worked on by a warp that runs, so the wait for the rest ends whether or not all CTAs are on
+// the GPU at once. That leaves one launch, and x's part of the product does not wait for v.
 // GATED: W is [2 N, K], gate rows, then up rows; a tile is 64 of each, out = silu(gate) * up.
 constexpr bool decode_twice(int bt, bool adapted) { return adapted && bt <= 16; }  // two CTAs an SM: a tile more than there are SMs does not wait for a whole one
 template <int BT, int STAGES, bool ADAPTED = false, bool GATED = false>
 __global__ void __launch_bounds__(TC_THREADS, decode_twice(BT, ADAPTED) ? 2 : 1)
 gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                       __nv_bfloat16* __restrict__ out, int M, int N, int K, int slices, int iters_per_slice,
-                      int* __restrict__ status, const std::conditional_t<ADAPTED, AdapterTerms, NoAdapters> term) {
+                      int* __restrict__ status, const std::conditional_t<ADAPTED, AdapterTerms, NoAdapters> term, const __nv_bfloat16* x) {
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], accum_bar;
@@ -825,7 +828,43 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         tok_slot[e] = s < 0 ? NONE : s;
       }
       for (int i = e; i < M * TC_BM; i += 128) part[i] = 0.f;
+      const int units = M * numbers;
+      int unit = 0;
+      if (term.tickets != nullptr && lane == 0) unit = atomicAdd(term.tickets, 1);
       epilogue_sync(1);
+      if (term.tickets != nullptr) {
+        for (unit = __shfl_sync(0xffffffffu, unit, 0); unit < units;) {
+          const int tok = unit / numbers, j = unit - tok * numbers, s = tok_slot[tok];
+          int next = 0;
+          if (lane == 0) next = atomicAdd(term.tickets, 1);
+          if (s != NONE) {
+            const uint4* a_row = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(ad.a) + ((size_t)s * numbers + j) * K);
+            const uint4* x_row = reinterpret_cast<const uint4*>(x + (size_t)tok * K);
+            float sum = 0.f;
+            for (int c = lane; c < K / 8; c += 32 * 8) {
+              uint4 av[8], xv[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const bool in = c + 32 * i < K / 8;
+                av[i] = in ? a_row[c + 32 * i] : make_uint4(0u, 0u, 0u, 0u);
+                xv[i] = in ? x_row[c + 32 * i] : make_uint4(0u, 0u, 0u, 0u);
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float fa[8], fx[8];
+                bf16x8_to_float(av[i], fa);
+                bf16x8_to_float(xv[i], fx);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) sum = fmaf(fa[q], fx[q], sum);
+              }
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) term.v[unit] = sum * ad.scale[s];
+          }
+          if (lane == 0) asm volatile("red.release.gpu.global.add.s32 [%0], 1;\n" ::"l"(term.tickets + 1) : "memory");
+          unit = __shfl_sync(0xffffffffu, next, 0);
+        }
+      }
       if (e < M) {
         const int s = tok_slot[e];
         int before = 0, same = 0;
@@ -880,7 +919,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             for (int h = 0; h < 2; ++h) {
               const int c = c0 + 16 * k + 8 * h + 2 * t4;
               const bool in = c < ad.rank;
-              vr[k][h] = in && tok >= 0 ? *reinterpret_cast<const float2*>(term.v + (size_t)tok * numbers + p * ad.rank + c) : make_float2(0.f, 0.f);
+              vr[k][h] = in && tok >= 0 ? __ldcg(reinterpret_cast<const float2*>(term.v + (size_t)tok * numbers + p * ad.rank + c)) : make_float2(0.f, 0.f);
 #pragma unroll
               for (int i = 0; i < 4; ++i)  // rows 16 m + g (i = 2 m) and 8 further (i = 2 m + 1)
                 br[k][i >> 1][2 * h + (i & 1)] = in && has[i] && part_of(ad, n[i]) == p ? *reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank + c) : 0u;
@@ -908,6 +947,23 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             for (int i = 0; i < 4; ++i) to[8 * i] += acc[i >> 1][2 * (i & 1) + q];
           }
         };
+        if (items > 0 && p == first_part && term.tickets != nullptr) {
+          // all of v is there
+          unsigned long long began = 0;
+          for (int polls = 1;; ++polls) {
+            int done;
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];\n" : "=r"(done) : "l"(term.tickets + 1) : "memory");
+            if (__all_sync(0xffffffffu, done >= units)) break;
+            if (polls % 64) continue;
+            unsigned long long now;
+            asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
+            if (began == 0) began = now;
+            if (__any_sync(0xffffffffu, now - began > MS_WAIT_NS)) {
+              if (lane == 0) atomicExch(status, 19);
+              break;
+            }
+          }
+        }
         if (items > 0) load(0, b_regs[0], v_regs[0]);
         for (int item = 0; item < items; item += 2) {
           if (item + 1 < items) load(item + 1, b_regs[1], v_regs[1]);
@@ -1920,7 +1976,7 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
     if (fit[size] >= tiles) slices = size;
   const int iters_per_slice = ceil_div(k_iters, slices);
   MS_LAUNCH_CLUSTERED(kernel, (unsigned)(tiles * slices), TC_THREADS, smem, stream, slices, map_w, map_x, (__nv_bfloat16*)out, M, N, K, slices,
-                      iters_per_slice, status, term);
+                      iters_per_slice, status, term, (const __nv_bfloat16*)X);
   return 0;
 }
 

@@ -35,17 +35,33 @@ __device__ __forceinline__ float logit_of(u64 place) {
 }
 
 // What makes a mass of a logit.
+constexpr int STEPS = 64;  // of 2^x between two powers of two
 struct Scale {
-  float zmax;   // the row's largest logit
-  double t;
-  double unit;  // 2^bits
+  float zmax;           // the row's largest logit
+  double per;           // log2(e) / T
+  double unit;          // 2^bits
+  int bits;
+  const double* powers; // 2^(i / STEPS)
 };
-// exp(z - max), 0 .. 1
+// exp(z - max), 0 .. 1: a power of two, a step of the table, and the exponential series of what is left (at most 1 / 128 of a doubling, so five terms are good to 2^-54).
+// A dozen operations of 64 bits where exp() behind a division takes several times that (a row's masses were half of the kernel's time).
 __device__ __forceinline__ double likeness(float x, const Scale& f) {
   if (x == f.zmax) return 1.0;
   if (x == -INFINITY || f.zmax == INFINITY) return 0.0;
-  return exp(((double)x - (double)f.zmax) / f.t);
+  const double t = ((double)x - (double)f.zmax) * f.per;  // doublings: 0 or below
+  if (t < -(double)(f.bits + 2)) return 0.0;              // (rounds to no mass)
+  const double n = rint(t * STEPS), r = fma(n, -1.0 / STEPS, t);
+  constexpr double L = 0.69314718055994530942;  // ln 2
+  double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
+  p = fma(r, p, L * L * L / 6);
+  p = fma(r, p, L * L / 2);
+  p = fma(r, p, L);
+  p = fma(r, p, 1.0);
+  const int i = (int)n;
+  const double m = f.powers[i & (STEPS - 1)] * p;
+  return __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));  // (2^-47 at the least: the exponent stays a normal number's)
 }
+static_assert(STEPS == 1 << 6, "the step's index");
 __device__ __forceinline__ u64 to_mass(double like, const Scale& f) { return (u64)__double2ll_rn(like * f.unit); }
 
 // A row belongs to a cluster of CTAs, each of which keeps its stretch of the logits in shared memory. A filter's cut is a place, found by a histogram over the fall below the
@@ -66,6 +82,7 @@ struct SfShared {
     u64 merged[BINS];  // their masses
   };
   uint32_t count[BINS], limb[3][BINS];
+  double powers[STEPS];
   int listed;
 };
 
@@ -122,15 +139,37 @@ struct Cluster {
   }
 };
 
-// sh.list[0 .. n) sorted, the largest first; n <= LIST.
+// list[0 .. n) sorted, the largest first; n <= LIST. Up to a number a thread: partners of the same warp by shuffles, others through the list.
 __device__ __forceinline__ void sort_list(u64* list, int n) {
   int size = 32;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += SF_THREADS) list[i] = 0;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (size <= SF_THREADS) {
+    u64 v = tid < n ? list[tid] : 0;
+    if (size == 32 && tid >= 32) v = 0;
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        u64 other;
+        if (j >= 32) {
+          if (tid < size) list[tid] = v;
+          __syncthreads();
+          other = tid < size ? list[tid ^ j] : 0;
+          __syncthreads();
+        } else {
+          other = __shfl_xor_sync(0xffffffffu, v, j);
+        }
+        v = (((tid & k) == 0) == ((tid & j) == 0)) == (v > other) ? v : other;
+      }
+    if (tid < size) list[tid] = v;
+    __syncthreads();
+    return;
+  }
+  for (int i = n + tid; i < size; i += SF_THREADS) list[i] = 0;
   __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      const int p = threadIdx.x;
+      const int p = tid;
       if (p < size / 2) {
         const int i = 2 * p - (p & (j - 1)), other = i + j;
         const u64 x = list[i], y = list[other];
@@ -180,65 +219,90 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   const int begin = min(rank * slice, vocab), n = min(slice, vocab - begin);
   const float* xs = logits + (size_t)r * vocab + begin;
 
-  // the likeliest token, and the smallest finite logit
-  u64 best = 0, lowest = 0;
-  auto meet = [&](float x, int i) {
-    x = clean(x);
-    const u64 place = place_of(x, begin + i);
-    best = place > best ? place : best;
-    const u64 low = x > -INFINITY ? (u64)~order_of(x) : 0;
-    lowest = low > lowest ? low : lowest;
-    return x;
+  // the largest logit and the least finite one (NaN is neither)
+  float top = -INFINITY, low = INFINITY;
+  auto meet = [&](float x) {
+    top = fmaxf(top, x);
+    low = fminf(low, x > -INFINITY ? x : INFINITY);
+    return clean(x);
   };
+  if (tid < STEPS) sh.powers[tid] = exp2((double)tid / STEPS);
   if (staged && (reinterpret_cast<uintptr_t>(xs) & 15) == 0) {
-    for (int i = 4 * tid; i + 3 < n; i += 4 * SF_THREADS) {
-      float4 x = *reinterpret_cast<const float4*>(xs + i);
-      x.x = meet(x.x, i);
-      x.y = meet(x.y, i + 1);
-      x.z = meet(x.z, i + 2);
-      x.w = meet(x.w, i + 3);
-      *reinterpret_cast<float4*>(sf_logits + i) = x;
+    constexpr int AHEAD = 5;
+    for (int i0 = 4 * tid; i0 + 3 < n; i0 += 4 * SF_THREADS * AHEAD) {
+      float4 x[AHEAD];
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        const int i = i0 + q * 4 * SF_THREADS;
+        if (i + 3 < n) x[q] = behind_loadf4(xs + i);
+      }
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        const int i = i0 + q * 4 * SF_THREADS;
+        if (i + 3 < n) *reinterpret_cast<float4*>(sf_logits + i) = make_float4(meet(x[q].x), meet(x[q].y), meet(x[q].z), meet(x[q].w));
+      }
     }
-    for (int i = (n & ~3) + tid; i < n; i += SF_THREADS) sf_logits[i] = meet(xs[i], i);
+    for (int i = (n & ~3) + tid; i < n; i += SF_THREADS) sf_logits[i] = meet(xs[i]);
   } else {
     for (int i = tid; i < n; i += SF_THREADS) {
-      const float x = meet(xs[i], i);
+      const float x = meet(xs[i]);
       if (staged) sf_logits[i] = x;
     }
   }
   for (int i = tid; i < BINS; i += SF_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0;
   if (tid == 0) sh.listed = 0;
+  u64 best = order_of(top), lowest = low < INFINITY ? (u64)~order_of(low) : 0;
   cl.reduce<true>(best, lowest);
-  const float zmax = logit_of(best);
+  const float zmax = logit_of(best << INDEX_BITS);
+  const float* mine = staged ? sf_logits : xs;
   if (!(t > 0.f) || zmax == -INFINITY) {
-    if (rank == 0 && tid == 0) tokens[r] = zmax == -INFINITY ? 0 : index_of(best);
+    // the first of the largest (of nothing but -inf: 0)
+    u64 first = 0, none = 0;
+    if (zmax > -INFINITY)
+      for (int i = tid; i < n; i += SF_THREADS)
+        if (mine[i] == zmax) {
+          first = (u64)(vocab - begin - i);
+          break;
+        }
+    cl.reduce<true>(first, none);
+    if (rank == 0 && tid == 0) tokens[r] = zmax == -INFINITY ? 0 : vocab - (int)first;
     return;
   }
-  const float* mine = staged ? sf_logits : xs;
-  const Scale f{zmax, (double)t, (double)(1ull << bits)};
+  const Scale f{zmax, 1.4426950408889634074 / (double)t, (double)(1ull << bits), bits, sh.powers};
   // Bins by the fall below the largest: up to the least finite logit, and no further than masses go (2^-46 is 31.9 falls of T).
   const float floor_ = logit_of(((u64)~(uint32_t)lowest) << INDEX_BITS);
   const float width = fminf((float)BINS / fmaxf(fminf(zmax - floor_, 32.f * t), 1e-35f), 1e37f);
   auto bin_of = [&](float x) { return x == zmax ? 0 : (int)fminf((zmax - x) * width, (float)(BINS - 1)); };
 
   u64 cut = 0;  // kept: places from here on
-  auto counted = [&](float x, int v) { return x > -INFINITY && place_of(x, v) >= cut; };
+  auto counted = [&](float x, int v) { return x > -INFINITY && (cut == 0 || place_of(x, v) >= cut); };
+  auto at = [&](int i) { return staged ? sf_logits[i] : clean(xs[i]); };
   // Where the running sum over the bins, likeliest first, is `enough` for the first time: said[0] the bin, [1] the count and [2] the mass before it, [3] its count.
-  auto crossing = [&](auto enough) {
+  auto crossing = [&](auto enough, bool masses) {
     const int per = BINS / ctas;
     u64 count = 0, mass = 0;
-    for (int i = tid; i < per; i += SF_THREADS) {
-      const int bin = rank * per + i;
+    // lanes side by side have a bin, and half of the cluster's CTAs each
+    for (int i0 = 0; i0 < per; i0 += SF_THREADS / 2) {
+      const int i = i0 + tid / 2;
       u64 c = 0, m = 0;
-      for (int q = 0; q < ctas; ++q) {
-        const SfShared* other = group.map_shared_rank(&sh, q);
-        c += other->count[bin];
-        m += (u64)other->limb[0][bin] + ((u64)other->limb[1][bin] << LIMB) + ((u64)other->limb[2][bin] << (2 * LIMB));
+      if (i < per) {
+        const int bin = rank * per + i;
+#pragma unroll
+        for (int q = 0; q < SF_CTAS / 2; ++q) {
+          if (2 * q + (tid & 1) >= ctas) break;
+          const SfShared* other = group.map_shared_rank(&sh, 2 * q + (tid & 1));
+          c += other->count[bin];
+          if (masses) m += (u64)other->limb[0][bin] + ((u64)other->limb[1][bin] << LIMB) + ((u64)other->limb[2][bin] << (2 * LIMB));
+        }
       }
-      sh.merged_count[i] = (uint32_t)c;
-      sh.merged[i] = m;
       count += c;
       mass += m;
+      c += __shfl_xor_sync(0xffffffffu, c, 1);
+      m += __shfl_xor_sync(0xffffffffu, m, 1);
+      if (i < per && (tid & 1) == 0) {
+        sh.merged_count[i] = (uint32_t)c;
+        sh.merged[i] = m;
+      }
     }
     const int turn = cl.turn;
     cl.reduce<false>(count, mass);  // (every CTA's sums are in xchg[turn]; the totals in count and mass)
@@ -289,10 +353,10 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     if (members <= LIST) {
       SfShared* first = group.map_shared_rank(&sh, 0);
       for (int i = tid; i < n; i += SF_THREADS) {
-        const float x = clean(mine[i]);
-        if (!counted(x, begin + i) || bin_of(x) != bin) continue;
-        const int at = atomicAdd(&first->listed, 1);
-        if (at < LIST) first->list[at] = place_of(x, begin + i);
+        const float x = at(i);
+        if (bin_of(x) != bin || !counted(x, begin + i)) continue;
+        const int slot = atomicAdd(&first->listed, 1);
+        if (slot < LIST) first->list[slot] = place_of(x, begin + i);
       }
       group.sync();
       if (rank == 0) {
@@ -317,8 +381,8 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     } else {
       u64 hi = 0, lo = 0;  // the bin's largest place, and its smallest
       for (int i = tid; i < n; i += SF_THREADS) {
-        const float x = clean(mine[i]);
-        if (!counted(x, begin + i) || bin_of(x) != bin) continue;
+        const float x = at(i);
+        if (bin_of(x) != bin || !counted(x, begin + i)) continue;
         const u64 place = place_of(x, begin + i);
         hi = place > hi ? place : hi;
         lo = ~place > lo ? ~place : lo;
@@ -329,9 +393,9 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
         const u64 mid = lo + ((hi - lo + 1) >> 1);
         u64 count = 0, mass = 0;
         for (int i = tid; i < n; i += SF_THREADS) {
-          const float x = clean(mine[i]);
+          const float x = at(i);
           const u64 place = place_of(x, begin + i);
-          if (place < mid || !counted(x, begin + i) || bin_of(x) != bin) continue;
+          if (place < mid || bin_of(x) != bin || !counted(x, begin + i)) continue;
           ++count;
           mass += to_mass(likeness(x, f), f);
         }
@@ -343,7 +407,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   };
   auto histogram = [&](bool masses) {
     for (int i = tid; i < n; i += SF_THREADS) {
-      const float x = clean(mine[i]);
+      const float x = at(i);
       if (!counted(x, begin + i)) continue;
       const int bin = bin_of(x);
       atomicAdd(&sh.count[bin], 1u);
@@ -360,17 +424,17 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   if (k > 0 && k < vocab) {
     histogram(false);
     auto enough = [k](u64 count, u64, u64, u64) { return count >= (u64)k; };
-    crossing(enough);
+    crossing(enough, false);
     const u64 listed = sh.said[1] + sh.said[3];
     if (listed <= LIST) {
       // all that top-k can leave is a short list: the first CTA finishes the row
       SfShared* first = group.map_shared_rank(&sh, 0);
       const int bin = (int)sh.said[0];
       for (int i = tid; i < n; i += SF_THREADS) {
-        const float x = clean(mine[i]);
-        if (!counted(x, begin + i) || bin_of(x) > bin) continue;
-        const int at = atomicAdd(&first->listed, 1);
-        if (at < LIST) first->list[at] = place_of(x, begin + i);
+        const float x = at(i);
+        if (bin_of(x) > bin || !counted(x, begin + i)) continue;
+        const int slot = atomicAdd(&first->listed, 1);
+        if (slot < LIST) first->list[slot] = place_of(x, begin + i);
       }
       group.sync();
       if (rank) return;
@@ -423,14 +487,14 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     histogram(true);
     const double part = (double)p;
     auto enough = [part](u64, u64 mass, u64, u64 all) { return (double)mass >= fmax(part * (double)all, 0.5); };
-    const u64 all = crossing(enough);
+    const u64 all = crossing(enough, true);
     settle(enough, 0, all);
   }
   // the token whose mass takes the sum beyond u of all: a stretch of the CTA's tokens a warp
   const int per_warp = ((n + SF_WARPS - 1) / SF_WARPS + 31) / 32 * 32, wb = min(warp * per_warp, n), we = min(wb + per_warp, n);
   auto mass_at = [&](int i) -> u64 {
     if (i >= we) return 0;
-    const float x = clean(mine[i]);
+    const float x = at(i);
     if (!counted(x, begin + i)) return 0;
     const double like = likeness(x, f);
     return like >= least ? to_mass(like, f) : 0;

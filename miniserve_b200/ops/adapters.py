@@ -17,9 +17,11 @@ from . import build, native
 
 _p, _i = c_void_p, c_int
 MAX_PARTS, MAX_RANK, TILE = 4, 256, 256  # TILE: tokens of a row tile of the plan
+TICKETS = 256  # pairs of counters that a step makes at a time
 BLOCK_BYTES = 48  # of an ``AdapterBlock`` (csrc/adapters.cuh)
 ADAPTERS = build.Module("adapters", ("adapters.cu",))
 _TYPES = (torch.bfloat16, torch.float32)
+_Q = struct.Struct("Q").pack
 
 
 @dataclass(frozen=True, eq=False)
@@ -51,7 +53,7 @@ class LowRank:
             raise ValueError("an adapter's tensors lie on one device, contiguous, the matrices on 16 bytes")
         # what every call asks for: sizes, the device's index (-1: the host), the two ends of the kernels' ``Adapters``
         for name, value in (("ends", ends), ("slots", slots), ("rank", rank), ("parts", len(ends)), ("outputs", n), ("inputs", a.shape[2]), ("index", a.get_device()),
-                            ("dtype", a.dtype), ("numbers", len(ends) * rank), ("head", struct.pack("3Q", a.data_ptr(), b.data_ptr(), c.data_ptr())),
+                            ("dtype", a.dtype), ("numbers", len(ends) * rank), ("weight_shape", (n, a.shape[2])), ("head", struct.pack("3Q", a.data_ptr(), b.data_ptr(), c.data_ptr())),
                             ("tail", struct.pack("7i4x", slots, rank, len(ends), *ends, *[n] * (MAX_PARTS - len(ends))))):
             object.__setattr__(self, name, value)
 
@@ -77,10 +79,13 @@ class AdapterRows:
         self.slot_of_row, self.row_of_token = slot_of_row, row_of_token
         self.rows, self.tokens, self.index = slot_of_row.shape[0], row_of_token.shape[0], slot_of_row.get_device()
         self._plans: dict = {}
+        self._tickets: dict = {}
         if self.index >= 0:
-            from . import device_status
+            from . import _sm_count, device_status
 
-            self.middle = struct.pack("3Q", slot_of_row.data_ptr(), row_of_token.data_ptr(), device_status(slot_of_row.device).data_ptr())
+            self.status = device_status(slot_of_row.device).data_ptr()
+            self.middle = struct.pack("3Q", slot_of_row.data_ptr(), row_of_token.data_ptr(), self.status)
+            self.sms = _sm_count(slot_of_row.device)
 
     def plan(self, slots: int, stream: int) -> "_Plan":
         """The adapters of each row tile, for projections with ``slots`` of them."""
@@ -89,6 +94,18 @@ class AdapterRows:
         if held is None:
             held = self._plans[key] = _Plan(self, slots, stream)
         return held
+
+
+    def tickets(self, stream: int) -> int:
+        """The address of two zeros on the device that no launch has had: a launch leaves its counts in them."""
+        key = (stream, _lib().ms_adapter_capture_id(stream))
+        held = self._tickets.get(key)
+        if held is None or held[1] == held[2]:
+            with on_stream(stream, self.slot_of_row.device):
+                zeros = torch.zeros(2 * TICKETS, dtype=torch.int32, device=self.slot_of_row.device)
+            held = self._tickets[key] = [zeros, zeros.data_ptr(), zeros.data_ptr() + 8 * TICKETS]
+        held[1] += 8
+        return held[1] - 8
 
 
 class _Plan:
@@ -102,6 +119,7 @@ class _Plan:
         self.blocks = self.ints.data_ptr()
         self.block_slot = self.blocks + BLOCK_BYTES * self.max_blocks
         self.tile_first = self.block_slot + 4 * self.max_blocks
+        self.status = rows.status
         ad = bytes(24) + rows.middle + struct.pack("7i4x", slots, 0, 0, 0, 0, 0, 0)
         _check(_lib().ms_adapter_plan(self.tile_first, self.block_slot, self.blocks, ad, t, self.max_blocks, stream))
 
@@ -134,7 +152,7 @@ def check(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None, low_r
     if not isinstance(low_rank, LowRank) or not isinstance(rows, AdapterRows):
         raise TypeError("an adapted product takes low_rank (ops.LowRank) and adapter_rows (ops.AdapterRows), both")
     shape, dtype, index = x.shape, x.dtype, low_rank.index
-    if len(shape) != 2 or shape[1] != low_rank.inputs or weight.shape != (low_rank.outputs, low_rank.inputs):
+    if len(shape) != 2 or shape[1] != low_rank.inputs or weight.shape != low_rank.weight_shape:
         raise ValueError(f"x is {tuple(shape)}, the weight {tuple(weight.shape)}, its adapters take {low_rank.inputs} and give {low_rank.outputs}")
     if shape[0] != rows.tokens:
         raise ValueError(f"x has {shape[0]} tokens, adapter_rows {rows.tokens}")
@@ -155,6 +173,10 @@ def _code(dtype: torch.dtype) -> int:
 
 
 FEW_TOKENS = 64  # up to so many, v is made token by token, and the products are the decode steps' tcgen05 kernel
+# That kernel makes v itself where the tokens are at most OWN_TOKENS, the numbers at most OWN_NUMBERS and the weight at least OWN_WEIGHT bytes: v is then ready before the
+# weights have come. In a launch ahead of it / its own work, us: 1 token of rank 16, 4096 -> 6144 17.9 / 12.8, 8 tokens of one adapter 17.8 / 14.1, 16 18.7 / 15.0, 8 of
+# rank 64 18.4 / 18.9, 16 of rank 64 21.3 / 23.8; 8 tokens, 2048 -> 4096 8.4 / 9.0, 1024 -> 4096 7.7 / 8.7.
+OWN_TOKENS, OWN_NUMBERS, OWN_WEIGHT = 16, 384, 24 << 20
 
 
 def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, stream: int) -> torch.Tensor:
@@ -172,10 +194,8 @@ def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, str
 
 
 def _blocks(v: torch.Tensor, x: torch.Tensor, plan: _Plan, ad: bytes, compact: bool, stream: int) -> None:
-    from . import device_status
-
     lib = native.gemm_tc()
-    rc = lib.ms_gemm_tc_adapter_v(v.data_ptr(), x.data_ptr(), ad, plan.tile_first, plan.blocks, x.shape[0], x.shape[1], plan.max_blocks, int(compact), device_status(x.device).data_ptr(), stream)
+    rc = lib.ms_gemm_tc_adapter_v(v.data_ptr(), x.data_ptr(), ad, plan.tile_first, plan.blocks, x.shape[0], x.shape[1], plan.max_blocks, int(compact), plan.status, stream)
     native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
 
 
@@ -195,62 +215,60 @@ def in_its_sums(tokens: int, outputs: int, gated: bool, sms: int) -> bool:
     return tiles >= sms // 8
 
 
-def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
-    from . import _sm_count, device_status, tc_gemm_enabled
+def _run(x, weight, out, stream: int, current: bool, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
     from . import linear as shared
+    from . import tc_gemm_enabled
 
     t, k = x.shape
-    n, ad = out.shape[1], low_rank.head + rows.middle + low_rank.tail
+    n, ad, device = out.shape[1], low_rank.head + rows.middle + low_rank.tail, x.device
     if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and weight.data_ptr() % 16 == 0 and tc_gemm_enabled():
-        few = t <= FEW_TOKENS
-        if few or in_its_sums(t, n, gated, _sm_count(x.device)):
-            lib, status = native.gemm_tc(), device_status(x.device).data_ptr()
-            if few:
-                v = _terms(x, low_rank, rows, ad, stream)
-                rc = lib.ms_gemm_tc_decode_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated), struct.pack("Q", v.data_ptr()) + ad, status, stream)
+        lib = native.gemm_tc()
+        if t <= FEW_TOKENS:
+            if t <= OWN_TOKENS and t * low_rank.numbers <= OWN_NUMBERS and 2 * k * low_rank.outputs >= OWN_WEIGHT:
+                tickets = rows.tickets(stream)
+                with nullcontext() if current else on_stream(stream, device):
+                    v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=device)
             else:
-                held, v = product(x, low_rank, rows, stream)
-                rc = lib.ms_gemm_tc_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, 2 if gated else 0, held, status, stream)
+                v, tickets = _terms(x, low_rank, rows, ad, stream), 0
+            term = b"".join((_Q(v.data_ptr()), ad, _Q(tickets)))
+            rc = lib.ms_gemm_tc_decode_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated), term, rows.status, stream)
+            native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
+            return
+        if in_its_sums(t, n, gated, rows.sms):
+            held, v = product(x, low_rank, rows, stream)
+            rc = lib.ms_gemm_tc_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, 2 if gated else 0, held, rows.status, stream)
             native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
             return
     # the shared product in float32, so that the sum is rounded once
     y = out
     if out.dtype is not torch.float32 or gated:
-        with on_stream(stream, x.device):
-            y = torch.empty((t, low_rank.outputs), dtype=torch.float32, device=x.device)
+        with on_stream(stream, device):
+            y = torch.empty((t, low_rank.outputs), dtype=torch.float32, device=device)
     shared(x, weight, out=y, stream=stream)
     v = _terms(x, low_rank, rows, ad, stream)
     _check(_lib().ms_adapter_expand(out.data_ptr(), y.data_ptr(), v.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), _code(out.dtype), int(gated), stream))
 
 
-def _here(call, x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
+def _call(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows, gated: bool) -> torch.Tensor:
     """The call on its tensors' device, and its stream (None: that device's current one)."""
-    if torch.cuda.current_device() == low_rank.index:
-        return call(x, weight, out, torch.cuda.current_stream().cuda_stream if stream is None else stream, low_rank, rows)
-    with torch.cuda.device(low_rank.index):
-        return call(x, weight, out, torch.cuda.current_stream().cuda_stream if stream is None else stream, low_rank, rows)
-
-
-def linear(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
-    check(x, weight, out, low_rank, rows, False)
-    return _here(_linear, x, weight, out, stream, low_rank, rows)
-
-
-def linear_silu_mul(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
-    check(x, weight, out, low_rank, rows, True)
-    return _here(_linear_silu_mul, x, weight, out, stream, low_rank, rows)
-
-
-def _linear(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
+    if torch.cuda.current_device() != low_rank.index:
+        with torch.cuda.device(low_rank.index):
+            return _call(x, weight, out, stream, low_rank, rows, gated)
+    now = torch.cuda.current_stream().cuda_stream
+    stream = now if stream is None else stream
     if out is None:
         with on_stream(stream, x.device):
             out = torch.empty((x.shape[0], low_rank.outputs), dtype=x.dtype, device=x.device)
     if x.shape[0]:
-        _run(x, weight, out, stream, low_rank, rows, False)
+        _run(x, weight, out, stream, stream == now, low_rank, rows, gated)
     return out
 
 
-def _linear_silu_mul(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
-    if x.shape[0]:
-        _run(x, weight, out, stream, low_rank, rows, True)
-    return out
+def linear(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
+    check(x, weight, out, low_rank, rows, False)
+    return _call(x, weight, out, stream, low_rank, rows, False)
+
+
+def linear_silu_mul(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows) -> torch.Tensor:
+    check(x, weight, out, low_rank, rows, True)
+    return _call(x, weight, out, stream, low_rank, rows, True)
