@@ -8,6 +8,8 @@
 // Masses are integers: exp(z - max) in 64-bit floating point, times 2^bits, rounded to the nearest (bits: as many as leave room for the sum of the whole row, at most
 // 45). Sums of integers do not depend on their order, so the same row gives the same token whatever adds it up, and borders fall where 64 bits put them: a
 // mass is off by 2^-46 of the likeliest token's at most, and tokens below that have none.
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -37,37 +39,41 @@ __device__ __forceinline__ float logit_of(u64 place) {
 // What makes a mass of a logit.
 constexpr int STEPS = 64;  // of 2^x between two powers of two
 struct Scale {
-  float zmax;           // the row's largest logit
-  double per;           // log2(e) / T
-  double unit;          // 2^bits
+  float zmax;            // the row's largest logit
+  float least;           // logits below round to no mass (-inf among them)
+  double ref;            // zmax, or 0 where that is infinite (then it alone has a mass)
+  double per;            // steps a unit of logit: STEPS log2(e) / T
   int bits;
-  const double* powers; // 2^(i / STEPS)
+  const double* powers;  // 2^(i / STEPS)
 };
-// exp(z - max), 0 .. 1: a power of two, a step of the table, and the exponential series of what is left (at most 1 / 128 of a doubling, so five terms are good to 2^-54).
-// A dozen operations of 64 bits where exp() behind a division takes several times that (a row's masses were half of the kernel's time).
-__device__ __forceinline__ double likeness(float x, const Scale& f) {
-  if (x == f.zmax) return 1.0;
-  if (x == -INFINITY || f.zmax == INFINITY) return 0.0;
-  const double t = ((double)x - (double)f.zmax) * f.per;  // doublings: 0 or below
-  if (t < -(double)(f.bits + 2)) return 0.0;              // (rounds to no mass)
-  const double n = rint(t * STEPS), r = fma(n, -1.0 / STEPS, t);
-  constexpr double L = 0.69314718055994530942;  // ln 2
+// exp(z - max) 2^bits, not rounded: a power of two, a step of the table, and the exponential series of what is left (half a step at most, so five terms are good to
+// 2^-54). Rounding to whole numbers is adding a number whose last place is one. Eleven operations of 64 bits and no conversions but x's, where exp() behind a
+// division takes several times that (masses were half of the kernel's time); no branches, so that several tokens' chains run beside each other.
+__device__ __forceinline__ double weight_of(float x, const Scale& f) {
+  constexpr double ROUND = 6755399441055744.0, L = 0.69314718055994530942 / STEPS;  // 1.5 * 2^52; ln 2 / STEPS
+  const double d = x == f.zmax ? 0.0 : (double)fmaxf(x, f.least) - f.ref;
+  const double shifted = fma(d, f.per, ROUND), r = fma(d, f.per, ROUND - shifted);
+  const int n = __double2loint(shifted);  // steps: 0 or below
   double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
   p = fma(r, p, L * L * L / 6);
   p = fma(r, p, L * L / 2);
   p = fma(r, p, L);
   p = fma(r, p, 1.0);
-  const int i = (int)n;
-  const double m = f.powers[i & (STEPS - 1)] * p;
-  return __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));  // (2^-47 at the least: the exponent stays a normal number's)
+  const double m = f.powers[n & (STEPS - 1)] * p;
+  const double w = __hiloint2double(__double2hiint(m) + (((n >> 6) + f.bits) << 20), __double2loint(m));  // (2^-4 at the least: a normal number)
+  return x >= f.least ? w : 0.0;
 }
 static_assert(STEPS == 1 << 6, "the step's index");
-__device__ __forceinline__ u64 to_mass(double like, const Scale& f) { return (u64)__double2ll_rn(like * f.unit); }
+// the nearest whole number, below 2^51
+__device__ __forceinline__ u64 to_mass(double w) {
+  constexpr double ONES = 4503599627370496.0;  // 2^52
+  return (u64)(__double_as_longlong(w + ONES) - __double_as_longlong(ONES));
+}
 
 // A row belongs to a cluster of CTAs, each of which keeps its stretch of the logits in shared memory. A filter's cut is a place, found by a histogram over the fall below the
 // largest logit (BINS bins up to where masses end), then the places of the one bin that the cut falls into, sorted. top-k alone, or ahead of the
 // other filters, leaves a short list, on which one CTA does all that is left. Everything that is added up is whole numbers.
-constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32, SF_CTAS = 8, BINS = 1024, LIST = 1024, LIMB = 15;
+constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32, SF_CTAS = 16, BINS = 1024, LIST = 1024, LIMB = 15;
 
 struct SfShared {
   u64 xchg[2][SF_CTAS][2];  // two numbers of every CTA of the cluster, two turns
@@ -215,7 +221,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   const float t = temperature[r];
   const int k = top_k ? top_k[r] : 0;
   const float p = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
-  const double least = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
+  const double least = mp > 0.f ? fmin((double)mp, 1.0) * (double)(1ull << bits) : 0.0;
   const int begin = min(rank * slice, vocab), n = min(slice, vocab - begin);
   const float* xs = logits + (size_t)r * vocab + begin;
 
@@ -268,15 +274,44 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     if (rank == 0 && tid == 0) tokens[r] = zmax == -INFINITY ? 0 : vocab - (int)first;
     return;
   }
-  const Scale f{zmax, 1.4426950408889634074 / (double)t, (double)(1ull << bits), bits, sh.powers};
+  const double steps = STEPS * 1.4426950408889634074 / (double)t;
+  // the least logit that is not below 2^-3 of a mass (rounded up, so that no logit from it on is either)
+  const float from = zmax < INFINITY ? __double2float_ru((double)zmax - (double)(bits + 3) * STEPS / steps) : INFINITY;
+  const Scale f{zmax, fmaxf(from, -FLT_MAX), zmax < INFINITY ? (double)zmax : 0.0, steps, bits, sh.powers};
   // Bins by the fall below the largest: up to the least finite logit, and no further than masses go (2^-46 is 31.9 falls of T).
   const float floor_ = logit_of(((u64)~(uint32_t)lowest) << INDEX_BITS);
   const float width = fminf((float)BINS / fmaxf(fminf(zmax - floor_, 32.f * t), 1e-35f), 1e37f);
   auto bin_of = [&](float x) { return x == zmax ? 0 : (int)fminf((zmax - x) * width, (float)(BINS - 1)); };
 
   u64 cut = 0;  // kept: places from here on
-  auto counted = [&](float x, int v) { return x > -INFINITY && (cut == 0 || place_of(x, v) >= cut); };
   auto at = [&](int i) { return staged ? sf_logits[i] : clean(xs[i]); };
+  auto counted = [&](float x, int v) { return x > -INFINITY && (cut == 0 || place_of(x, v) >= cut); };
+  // f(i, x) of the CTA's tokens i of [from, to), `step` threads side by side, four of a thread's at a time
+  auto each = [&](int from, int to, int step, auto f4) {
+    for (int i0 = from; i0 < to; i0 += 4 * step) {
+      float x[4];
+      bool in[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        in[q] = i0 + q * step < to;
+        x[q] = in[q] ? at(i0 + q * step) : -INFINITY;
+      }
+      f4(i0, x, in);
+    }
+  };
+  // the places of the counted tokens of bins [low, high] in the first CTA's list
+  auto gather = [&](int low, int high) {
+    SfShared* first = group.map_shared_rank(&sh, 0);
+    each(tid, n, SF_THREADS, [&](int i0, const float (&x)[4], const bool (&in)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int bin = bin_of(x[q]), v = begin + i0 + q * SF_THREADS;
+        if (bin < low || bin > high || !in[q] || !counted(x[q], v)) continue;
+        const int slot = atomicAdd(&first->listed, 1);
+        if (slot < LIST) first->list[slot] = place_of(x[q], v);
+      }
+    });
+  };
   // Where the running sum over the bins, likeliest first, is `enough` for the first time: said[0] the bin, [1] the count and [2] the mass before it, [3] its count.
   auto crossing = [&](auto enough, bool masses) {
     const int per = BINS / ctas;
@@ -351,18 +386,12 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     const u64 cb = sh.said[1], mb = sh.said[2], members = sh.said[3];
     if (members == 0) return;  // (fewer tokens than top-k would keep)
     if (members <= LIST) {
-      SfShared* first = group.map_shared_rank(&sh, 0);
-      for (int i = tid; i < n; i += SF_THREADS) {
-        const float x = at(i);
-        if (bin_of(x) != bin || !counted(x, begin + i)) continue;
-        const int slot = atomicAdd(&first->listed, 1);
-        if (slot < LIST) first->list[slot] = place_of(x, begin + i);
-      }
+      gather(bin, bin);
       group.sync();
       if (rank == 0) {
         const int have = min(sh.listed, LIST);
         sort_list(sh.list, have);
-        for (int i = tid; i < have; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of(sh.list[i]), f), f);
+        for (int i = tid; i < have; i += SF_THREADS) sh.sums[i] = to_mass(weight_of(logit_of(sh.list[i]), f));
         __syncthreads();
         running_sums(sh.sums, have, sh.red);
         for (int i = tid; i < have; i += SF_THREADS) {
@@ -397,7 +426,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
           const u64 place = place_of(x, begin + i);
           if (place < mid || bin_of(x) != bin || !counted(x, begin + i)) continue;
           ++count;
-          mass += to_mass(likeness(x, f), f);
+          mass += to_mass(weight_of(x, f));
         }
         cl.reduce<false>(count, mass);
         if (enough(cb + count, mb + mass, all_count, all_mass)) lo = mid; else hi = mid - 1;
@@ -406,18 +435,22 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     }
   };
   auto histogram = [&](bool masses) {
-    for (int i = tid; i < n; i += SF_THREADS) {
-      const float x = at(i);
-      if (!counted(x, begin + i)) continue;
-      const int bin = bin_of(x);
-      atomicAdd(&sh.count[bin], 1u);
-      if (masses) {
-        const u64 m = to_mass(likeness(x, f), f);
-        atomicAdd(&sh.limb[0][bin], (uint32_t)m & ((1u << LIMB) - 1));
-        atomicAdd(&sh.limb[1][bin], (uint32_t)(m >> LIMB) & ((1u << LIMB) - 1));
-        atomicAdd(&sh.limb[2][bin], (uint32_t)(m >> (2 * LIMB)));
+    each(tid, n, SF_THREADS, [&](int i0, const float (&x)[4], const bool (&in)[4]) {
+      u64 m[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m[q] = masses ? to_mass(weight_of(x[q], f)) : 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (!in[q] || !counted(x[q], begin + i0 + q * SF_THREADS)) continue;
+        const int bin = bin_of(x[q]);
+        atomicAdd(&sh.count[bin], 1u);
+        if (masses) {
+          atomicAdd(&sh.limb[0][bin], (uint32_t)m[q] & ((1u << LIMB) - 1));
+          atomicAdd(&sh.limb[1][bin], (uint32_t)(m[q] >> LIMB) & ((1u << LIMB) - 1));
+          atomicAdd(&sh.limb[2][bin], (uint32_t)(m[q] >> (2 * LIMB)));
+        }
       }
-    }
+    });
     group.sync();
   };
 
@@ -428,26 +461,19 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     const u64 listed = sh.said[1] + sh.said[3];
     if (listed <= LIST) {
       // all that top-k can leave is a short list: the first CTA finishes the row
-      SfShared* first = group.map_shared_rank(&sh, 0);
-      const int bin = (int)sh.said[0];
-      for (int i = tid; i < n; i += SF_THREADS) {
-        const float x = at(i);
-        if (bin_of(x) > bin || !counted(x, begin + i)) continue;
-        const int slot = atomicAdd(&first->listed, 1);
-        if (slot < LIST) first->list[slot] = place_of(x, begin + i);
-      }
+      gather(0, (int)sh.said[0]);
       group.sync();
       if (rank) return;
       const int have = min(sh.listed, LIST), kept_k = min(have, k);
       sort_list(sh.list, have);
-      for (int i = tid; i < kept_k; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of(sh.list[i]), f), f);
+      for (int i = tid; i < kept_k; i += SF_THREADS) sh.sums[i] = to_mass(weight_of(logit_of(sh.list[i]), f));
       __syncthreads();
       running_sums(sh.sums, kept_k, sh.red);
       // what is kept is a run from the likeliest on
       const double target = p < 1.f ? fmax((double)p * (double)sh.sums[kept_k - 1], 0.5) : INFINITY;
       int kept = 0;
       for (int i = tid; i < kept_k; i += SF_THREADS)
-        if ((i == 0 || (double)sh.sums[i - 1] < target) && likeness(logit_of(sh.list[i]), f) >= least) ++kept;
+        if ((i == 0 || (double)sh.sums[i - 1] < target) && weight_of(logit_of(sh.list[i]), f) >= least) ++kept;
       kept = __reduce_add_sync(0xffffffffu, kept);
       __syncthreads();
       if (lane == 0) sh.red[warp][0] = kept;
@@ -472,7 +498,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
       }
       __syncthreads();
       sort_list(sh.list, kept);
-      for (int i = tid; i < kept; i += SF_THREADS) sh.sums[i] = to_mass(likeness(logit_of((sh.list[i] & 0xffffffffull) << INDEX_BITS), f), f);
+      for (int i = tid; i < kept; i += SF_THREADS) sh.sums[i] = to_mass(weight_of(logit_of((sh.list[i] & 0xffffffffull) << INDEX_BITS), f));
       __syncthreads();
       running_sums(sh.sums, kept, sh.red);
       for (int i = tid; i < kept; i += SF_THREADS)
@@ -492,15 +518,21 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   }
   // the token whose mass takes the sum beyond u of all: a stretch of the CTA's tokens a warp
   const int per_warp = ((n + SF_WARPS - 1) / SF_WARPS + 31) / 32 * 32, wb = min(warp * per_warp, n), we = min(wb + per_warp, n);
-  auto mass_at = [&](int i) -> u64 {
-    if (i >= we) return 0;
-    const float x = at(i);
-    if (!counted(x, begin + i)) return 0;
-    const double like = likeness(x, f);
-    return like >= least ? to_mass(like, f) : 0;
+  const float edge = cut ? logit_of(cut) : -INFINITY;  // the cut's logit
+  auto mass_of = [&](float x, int i) -> u64 {
+    const double w = weight_of(x, f);
+    return w >= least && (x > edge || (x == edge && place_of(x, begin + i) >= cut)) ? to_mass(w) : 0;
   };
   u64 sum = 0, none = 0;
-  for (int i = wb + lane; i < we; i += 32) sum += mass_at(i);
+  each(wb + lane, we, 32, [&](int i0, const float (&x)[4], const bool (&in)[4]) {
+    u64 m[4];
+    // (a warp whose tokens are all below the cut has nothing to work out: all but a few of them where a row has a few likely tokens)
+    if (!__any_sync(__activemask(), fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= edge)) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) m[q] = mass_of(x[q], i0 + 32 * q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += in[q] ? m[q] : 0;
+  });
   const int turn = cl.turn;
   cl.reduce<false>(sum, none);  // (a warp's sums are left in red)
   u64 aim = (u64)(u * (double)sum);
@@ -510,7 +542,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   for (int w = 0; w < warp; ++w) before += sh.red[w][0];
   if (before <= aim && aim < before + sh.red[warp][0]) {
     for (int i0 = wb; i0 < we; i0 += 32) {
-      u64 s = mass_at(i0 + lane);
+      u64 s = i0 + lane < we ? mass_of(at(i0 + lane), i0 + lane) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const u64 x = __shfl_up_sync(0xffffffffu, s, o);
@@ -542,10 +574,20 @@ MS_EXPORT int ms_sample_filtered(int* tokens, const float* logits, const float* 
   int bits = 62;  // a row's sum stays within 2^62
   while ((1ll << (62 - bits)) < vocab) --bits;
   if (bits > 3 * LIMB) bits = 3 * LIMB;
-  const int ctas = vocab >= 16384 ? SF_CTAS : 1, slice = ceil_div(ceil_div(vocab, ctas), 32) * 32;
+  // Sixteen CTAs a row while that leaves each an SM of its own, else eight (8 rows of 151,936 tokens by top-p alone 38.9 us, 55.7 with eight; one row by top-k 15.0 and 16.8).
+  const int ctas = vocab < 16384 ? 1 : rows * SF_CTAS <= (sm_count() > 0 ? sm_count() : 148) ? SF_CTAS : SF_CTAS / 2, slice = ceil_div(ceil_div(vocab, ctas), 32) * 32;
   MS_CHECK_ARG((long long)rows * ctas <= 0x7fffffffLL, "sample_filtered: %d rows are too many for one launch", rows);
   const size_t smem = (size_t)slice * sizeof(float);
   const int staged = smem <= 160 * 1024;  // (longer rows are read again for each search)
+  if (ctas == SF_CTAS) {
+    static std::atomic<unsigned long long> wide{0};
+    int dev = 0;
+    MS_CHECK_CUDA(cudaGetDevice(&dev));
+    if (dev >= KNOWN_DEVICES || !((wide.load(std::memory_order_relaxed) >> dev) & 1ull)) {
+      MS_CHECK_CUDA(cudaFuncSetAttribute((const void*)sample_filtered_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      if (dev < KNOWN_DEVICES) wide.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+  }
   if (staged) {
     static std::atomic<unsigned long long> allowed{0};
     MS_CHECK_CUDA(allow_shared_memory((const void*)sample_filtered_kernel, 160 * 1024, allowed));

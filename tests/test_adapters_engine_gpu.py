@@ -82,20 +82,27 @@ NAMES = ["a", None, "b", "a", "c", "b"]
 
 
 @pytest.mark.parametrize("dtype, kw", [("float32", dict(cuda_graph=False)), ("float32", dict()), ("bfloat16", dict(cuda_graph=False)), ("bfloat16", dict()),
-                                       ("bfloat16", dict(chunked_prefill_size=24)), ("bfloat16", dict(overlap=False)), ("bfloat16", dict(kv_pool_tokens=112))])
+                                       ("bfloat16", dict(chunked_prefill_size=24)), ("bfloat16", dict(overlap=False))])
 def test_requests_of_one_batch_have_their_own_adapters(held, dtype, kw):
     prompts = prompts_of(held, [5, 17, 33, 1, 9, 40], 1)
     llm = engine(held, dtype, **kw)
     outs = llm.generate(prompts, SamplingParams(max_new_tokens=12), adapters=NAMES)
     assert llm.engine.cache.is_idle()
-    if "kv_pool_tokens" in kw:
-        assert llm.engine.scheduler.num_preemptions > 0
     for p, o, n in zip(prompts, outs, NAMES):
         assert len(o) == 12
         margins(held, p, o, n, dtype)
     again = llm.generate(prompts, SamplingParams(max_new_tokens=12), adapters=NAMES)
     if dtype == "float32":
         assert again == outs
+
+
+def test_requests_that_are_preempted_keep_their_adapters(held):
+    prompts = prompts_of(held, [30, 12, 25, 7, 40, 18], 3)
+    roomy = engine(held, "float32", chunked_prefill_size=16).generate(prompts, SamplingParams(max_new_tokens=20), adapters=NAMES)
+    tight = engine(held, "float32", chunked_prefill_size=16, kv_pool_tokens=128, page_size=8)
+    assert tight.generate(prompts, SamplingParams(max_new_tokens=20), adapters=NAMES) == roomy
+    assert tight.engine.scheduler.num_preemptions > 0, "the pool was meant to run out"
+    assert tight.engine.cache.is_idle()
 
 
 def test_prompts_of_many_tokens(held):
