@@ -213,6 +213,15 @@ class _Recorder:
         # rows, which attention sends to another kernel than the rest)
         self.single_rows = single_rows
         self._open: torch.cuda.CUDAGraph | None = None
+        self._ahead, self._taken = torch.empty(1024, dtype=torch.int32, device=stream.device), 0
+
+    def ahead(self, ints: int) -> torch.Tensor:
+        """int32 [ints] for what a hook writes before every replay. It is not of the captured memory: there a tensor may lie where an earlier one of the same pass was, and a
+        replay would write that one over what the hook wrote."""
+        if self._taken + ints > self._ahead.numel():
+            raise RuntimeError("a captured pass wants more than 1,024 numbers written ahead of its replays")
+        self._taken += ints
+        return self._ahead[self._taken - ints:self._taken]
 
     def begin(self) -> None:
         self._open = torch.cuda.CUDAGraph()
