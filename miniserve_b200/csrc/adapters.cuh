@@ -26,7 +26,7 @@ struct AdaptedProduct {
   Adapters ad;
   const void* v;          // bfloat16 [max_blocks * 256, parts * rank]
   const int* tile_first;  // [row tiles + 1]
-  const int* block_slot;  // [max_blocks]
+  const void* blocks;     // AdapterBlock [max_blocks]
   int max_blocks;
 };
 
@@ -101,6 +101,145 @@ __device__ __forceinline__ float adapter_dot(const T* row, const float* v, int r
     }
   }
   return sum;
+}
+
+// ---- terms of few tokens on the tensor cores: sum_j B_s[n, j] v[t, j], v rounded to bfloat16 (2^-8 of an adapter's share of an output, where the output itself is rounded so)
+constexpr int NO_SLOT = 0x7fffffff;
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Waits until other CTAs of the launch have counted up to `all`, for at most MS_WAIT_NS: false then. What they wrote before is visible behind it.
+__device__ __forceinline__ bool tickets_reach(const int* counter, int all) {
+  unsigned long long began = 0;
+  for (unsigned polls = 1;; ++polls) {
+    int done;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];\n" : "=r"(done) : "l"(counter) : "memory");
+    if (done >= all) return true;
+    if (polls % 64) continue;
+    unsigned long long now;
+    asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
+    if (began == 0) began = now;
+    else if (now - began > MS_WAIT_NS) return false;
+  }
+}
+__device__ __forceinline__ int adapter_slot(const Adapters& ad, int t) {
+  const int s = adapter_of(ad, t);
+  return s < 0 ? NO_SLOT : s;
+}
+// Tokens in the order of their slots, and where runs of up to eight of one slot begin.
+template <int MOST>
+struct TokenGroups {
+  int slot[MOST], order[MOST], at[MOST], count;
+  bool begins[MOST];
+};
+// From g.slot [M], written by the calling threads (e = 0 .., at least M of them); sync: their barrier.
+template <int MOST, typename Sync>
+__device__ __forceinline__ void group_tokens(TokenGroups<MOST>& g, int M, int e, Sync sync) {
+  sync();
+  if (e < M) {
+    const int s = g.slot[e];
+    int before = 0, same = 0;
+    for (int j = 0; j < M; ++j) {
+      before += g.slot[j] < s;
+      same += g.slot[j] == s && j < e;
+    }
+    g.order[before + same] = e;
+    g.begins[before + same] = s != NO_SLOT && same % 8 == 0;
+  }
+  sync();
+  if (e < M) {
+    int at = 0, all = 0;
+    for (int j = 0; j < M; ++j) {
+      at += j < e && g.begins[j];
+      all += g.begins[j];
+    }
+    if (g.begins[e]) g.at[at] = e;
+    if (e == 0) g.count = all;
+  }
+  sync();
+}
+// A warp's 32 rows of B (n[i] is this lane's row 8 i + lane / 4 of them, has[i] whether there is one) times the tokens of the groups first, first + step, ..: add(token,
+// i, term) for the lane's rows. An instruction is 16 rows and the eight tokens of a group; a group and 32 of the rank's numbers are an item, the next one's asked for ahead of
+// this one's instructions. ready: called before the first of v is read. v: float32 [.., parts * rank], by the tokens of g.
+template <int MOST, typename Ready, typename Add>
+__device__ __forceinline__ void warp_terms(const Adapters& ad, const float* v, const TokenGroups<MOST>& g, int M, int first, int step, const int (&n)[4], const bool (&has)[4],
+                                           Ready ready, Add add) {
+  const int lane = threadIdx.x & 31, col = lane >> 2, t4 = lane & 3, numbers = ad.parts * ad.rank, rows = ad.ends[MAX_PARTS - 1];
+  int low = MAX_PARTS, high = -1;  // the parts that the rows belong to: one, but where two meet
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (has[i]) {
+      low = min(low, part_of(ad, n[i]));
+      high = max(high, part_of(ad, n[i]));
+    }
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  const int chunks = (ad.rank + 31) / 32, items = g.count > first ? (g.count - first + step - 1) / step * chunks : 0;
+  if (items == 0) return;
+  for (int p = low; p <= high; ++p) {
+    uint32_t b_regs[2][2][2][4];
+    float2 v_regs[2][2][2];
+    auto load_b = [&](int item, uint32_t (&br)[2][2][4]) {
+      const int c0 = (item % chunks) * 32, s = g.slot[g.order[g.at[first + step * (item / chunks)]]];
+      const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(ad.b) + (size_t)s * rows * ad.rank;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = c0 + 16 * k + 8 * h + 2 * t4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            br[k][i >> 1][2 * h + (i & 1)] = c < ad.rank && has[i] && part_of(ad, n[i]) == p ? *reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank + c) : 0u;
+        }
+    };
+    auto load_v = [&](int item, float2 (&vr)[2][2]) {
+      const int at = g.at[first + step * (item / chunks)], c0 = (item % chunks) * 32, s = g.slot[g.order[at]];
+      const int tok = at + col < M && g.slot[g.order[at + col]] == s ? g.order[at + col] : -1;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = c0 + 16 * k + 8 * h + 2 * t4;
+          vr[k][h] = c < ad.rank && tok >= 0 ? __ldcg(reinterpret_cast<const float2*>(v + (size_t)tok * numbers + p * ad.rank + c)) : make_float2(0.f, 0.f);
+        }
+    };
+    auto multiply = [&](int item, const uint32_t (&br)[2][2][4], const float2 (&vr)[2][2]) {
+      float acc[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(vr[k][0].x, vr[k][0].y), hi = __floats2bfloat162_rn(vr[k][1].x, vr[k][1].y);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          mma_16816(acc[m], br[k][m][0], br[k][m][1], br[k][m][2], br[k][m][3], *reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+      const int at = g.at[first + step * (item / chunks)], s = g.slot[g.order[at]];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int pos = at + 2 * t4 + q;
+        if (pos >= M || g.slot[g.order[pos]] != s) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(g.order[pos], i, acc[i >> 1][2 * (i & 1) + q]);
+      }
+    };
+    load_b(0, b_regs[0]);
+    if (p == low) ready();
+    load_v(0, v_regs[0]);
+    for (int item = 0; item < items; item += 2) {
+      if (item + 1 < items) {
+        load_b(item + 1, b_regs[1]);
+        load_v(item + 1, v_regs[1]);
+      }
+      multiply(item, b_regs[0], v_regs[0]);
+      if (item + 1 >= items) break;
+      if (item + 2 < items) {
+        load_b(item + 2, b_regs[0]);
+        load_v(item + 2, v_regs[0]);
+      }
+      multiply(item + 1, b_regs[1], v_regs[1]);
+    }
+  }
 }
 
 }  // namespace ms

@@ -701,7 +701,7 @@ struct AdaptedTiles {
   CUtensorMap map_v;                // [blocks * 256, parts * rank]
   CUtensorMap map_b[MAX_PARTS];     // [slots][the part's rows][rank]
   const int* tile_first;            // the first block of each row tile, and where the last one's end
-  const int* block_slot;
+  const AdapterBlock* blocks;
   int parts, rank, ends[MAX_PARTS];
 };
 struct NoAdapters {};
@@ -741,8 +741,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   constexpr int W_BYTES = TC_BM * TC_BK * 2, X_BYTES = BT * TC_BK * 2, STAGE_BYTES = W_BYTES + X_BYTES;
   constexpr uint32_t TMEM_COLS = BT <= 32 ? 32 : 64;
   float* part = reinterpret_cast<float*>(smem + (size_t)STAGES * STAGE_BYTES);  // [BT tokens][128 rows of W]: this slice's sums
-  __shared__ int tok_slot[ADAPTED ? BT : 1], order[ADAPTED ? BT : 1], group_at[ADAPTED ? BT : 1], group_count;
-  __shared__ bool begins[ADAPTED ? BT : 1];
+  __shared__ TokenGroups<ADAPTED ? BT : 1> tokens;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
@@ -820,13 +819,9 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const int quad = warp & 3, l = quad * 32 + lane;
     if constexpr (ADAPTED) {
       const Adapters& ad = term.ad;
-      const int e = threadIdx.x - 64, numbers = ad.parts * ad.rank, rows = ad.ends[MAX_PARTS - 1], g = lane >> 2, t4 = lane & 3;
-      constexpr int NONE = 0x7fffffff;
-      // tokens in the order of their slots, and where runs of up to eight of one slot begin
-      if (e < M) {
-        const int s = adapter_of(ad, e);
-        tok_slot[e] = s < 0 ? NONE : s;
-      }
+      const int e = threadIdx.x - 64, numbers = ad.parts * ad.rank;
+      auto sync = [] { epilogue_sync(1); };
+      if (e < M) tokens.slot[e] = adapter_slot(ad, e);
       for (int i = e; i < M * TC_BM; i += 128) part[i] = 0.f;
       const int units = M * numbers;
       int unit = 0;
@@ -834,10 +829,10 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       epilogue_sync(1);
       if (term.tickets != nullptr) {
         for (unit = __shfl_sync(0xffffffffu, unit, 0); unit < units;) {
-          const int tok = unit / numbers, j = unit - tok * numbers, s = tok_slot[tok];
+          const int tok = unit / numbers, j = unit - tok * numbers, s = tokens.slot[tok];
           int next = 0;
           if (lane == 0) next = atomicAdd(term.tickets, 1);
-          if (s != NONE) {
+          if (s != NO_SLOT) {
             const uint4* a_row = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(ad.a) + ((size_t)s * numbers + j) * K);
             const uint4* x_row = reinterpret_cast<const uint4*>(x + (size_t)tok * K);
             float sum = 0.f;
@@ -865,114 +860,20 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
           unit = __shfl_sync(0xffffffffu, next, 0);
         }
       }
-      if (e < M) {
-        const int s = tok_slot[e];
-        int before = 0, same = 0;
-        for (int j = 0; j < M; ++j) {
-          before += tok_slot[j] < s;
-          same += tok_slot[j] == s && j < e;
-        }
-        order[before + same] = e;
-        begins[before + same] = s != NONE && same % 8 == 0;
-      }
-      epilogue_sync(1);
-      int groups = 0;
-      if (e < M) {
-        int at = 0;
-        for (int j = 0; j < M; ++j) {
-          at += j < e && begins[j];
-          groups += begins[j];
-        }
-        if (begins[e]) group_at[at] = e;
-        if (e == 0) group_count = groups;
-      }
-      epilogue_sync(1);
-      groups = group_count;
-      // this lane's four rows of B: 16 m + g and 8 further
+      group_tokens(tokens, M, e, sync);
+      // this lane's four rows of B: 16 m + (lane / 4) and 8 further
       int n[4];
       bool has[4];
-      int first_part = MAX_PARTS, last_part = -1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = quad * 32 + 8 * i + g;
+        const int row = quad * 32 + 8 * i + (lane >> 2);
         has[i] = n0 + (GATED ? row & (ROWS - 1) : row) < N;
         n[i] = GATED && row >= ROWS ? N + n0 + row - ROWS : n0 + row;
-        if (has[i]) {
-          first_part = min(first_part, part_of(ad, n[i]));
-          last_part = max(last_part, part_of(ad, n[i]));
-        }
       }
-      first_part = __reduce_min_sync(0xffffffffu, first_part);
-      last_part = __reduce_max_sync(0xffffffffu, last_part);
-      const int chunks = (ad.rank + 31) / 32, items = groups > rank ? (groups - rank + slices - 1) / slices * chunks : 0;
-      for (int p = first_part; p <= last_part; ++p) {
-        // an item: a group and 32 of the rank's numbers; the next one's are asked for ahead of this one's instructions
-        uint32_t b_regs[2][2][2][4];
-        float2 v_regs[2][2][2];
-        auto load = [&](int item, uint32_t (&br)[2][2][4], float2 (&vr)[2][2]) {
-          const int at = group_at[rank + slices * (item / chunks)], c0 = (item % chunks) * 32, s = tok_slot[order[at]];
-          const int tok = at + g < M && tok_slot[order[at + g]] == s ? order[at + g] : -1;
-          const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(ad.b) + (size_t)s * rows * ad.rank;
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = c0 + 16 * k + 8 * h + 2 * t4;
-              const bool in = c < ad.rank;
-              vr[k][h] = in && tok >= 0 ? __ldcg(reinterpret_cast<const float2*>(term.v + (size_t)tok * numbers + p * ad.rank + c)) : make_float2(0.f, 0.f);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)  // rows 16 m + g (i = 2 m) and 8 further (i = 2 m + 1)
-                br[k][i >> 1][2 * h + (i & 1)] = in && has[i] && part_of(ad, n[i]) == p ? *reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank + c) : 0u;
-            }
-        };
-        auto add = [&](int item, const uint32_t (&br)[2][2][4], const float2 (&vr)[2][2]) {
-          float acc[2][4] = {};
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(vr[k][0].x, vr[k][0].y), hi = __floats2bfloat162_rn(vr[k][1].x, vr[k][1].y);
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-              asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                           : "+f"(acc[m][0]), "+f"(acc[m][1]), "+f"(acc[m][2]), "+f"(acc[m][3])
-                           : "r"(br[k][m][0]), "r"(br[k][m][1]), "r"(br[k][m][2]), "r"(br[k][m][3]), "r"(*reinterpret_cast<const uint32_t*>(&lo)),
-                             "r"(*reinterpret_cast<const uint32_t*>(&hi)));
-          }
-          const int at = group_at[rank + slices * (item / chunks)], s = tok_slot[order[at]];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int pos = at + 2 * t4 + q;
-            if (pos >= M || tok_slot[order[pos]] != s) continue;
-            float* to = part + order[pos] * TC_BM + quad * 32 + g;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[8 * i] += acc[i >> 1][2 * (i & 1) + q];
-          }
-        };
-        if (items > 0 && p == first_part && term.tickets != nullptr) {
-          // all of v is there
-          unsigned long long began = 0;
-          for (int polls = 1;; ++polls) {
-            int done;
-            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];\n" : "=r"(done) : "l"(term.tickets + 1) : "memory");
-            if (__all_sync(0xffffffffu, done >= units)) break;
-            if (polls % 64) continue;
-            unsigned long long now;
-            asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(now));
-            if (began == 0) began = now;
-            if (__any_sync(0xffffffffu, now - began > MS_WAIT_NS)) {
-              if (lane == 0) atomicExch(status, 19);
-              break;
-            }
-          }
-        }
-        if (items > 0) load(0, b_regs[0], v_regs[0]);
-        for (int item = 0; item < items; item += 2) {
-          if (item + 1 < items) load(item + 1, b_regs[1], v_regs[1]);
-          add(item, b_regs[0], v_regs[0]);
-          if (item + 1 >= items) break;
-          if (item + 2 < items) load(item + 2, b_regs[0], v_regs[0]);
-          add(item + 1, b_regs[1], v_regs[1]);
-        }
-      }
+      auto ready = [&] {
+        if (term.tickets != nullptr && !__all_sync(0xffffffffu, tickets_reach(term.tickets + 1, units)) && lane == 0) atomicExch(status, 19);
+      };
+      warp_terms(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i, float x) { part[tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i] += x; });
       __syncwarp();
     }
     bool ok = true;
@@ -1378,7 +1279,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 unsigned char* a_tile = smem + (size_t)s * STAGE_BYTES;
                 if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * STAGE_BYTES);  // (what a copy fills with zeros counts too)
                 tma_load_2d_pair(a_tile, &ad.map_v, &full_bar[s], p * ad.rank + c, b * 2 * TC_BM + (int)rank * TC_BM);
-                tma_load_3d_pair(a_tile + A_BYTES, &ad.map_b[p], &full_bar[s], c, w_row - (p ? ad.ends[p - 1] : 0), ad.block_slot[b]);
+                tma_load_3d_pair(a_tile + A_BYTES, &ad.map_b[p], &full_bar[s], c, w_row - (p ? ad.ends[p - 1] : 0), ad.blocks[b].slot);
               }
             }
         }
@@ -1872,7 +1773,7 @@ static int make_adapted(AdaptedTiles* tiles, const AdaptedProduct& ap) {
     tiles->ends[p] = ad.ends[q];
   }
   tiles->tile_first = ap.tile_first;
-  tiles->block_slot = ap.block_slot;
+  tiles->blocks = (const AdapterBlock*)ap.blocks;
   tiles->parts = ad.parts;
   tiles->rank = ad.rank;
   return 0;
@@ -2066,7 +1967,7 @@ MS_EXPORT int ms_gemm_tc_qkv_bf16(void* q_out, const void* x, const void* w_qkv,
                           cos_sin, positions, row_of_token, page_indptr, page_indices, nq, nkv, shift, eps};
   const int n_total = (nq + 2 * nkv) * 128;
   if (ap != nullptr) {
-    MS_CHECK_ARG(ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 && adapters_ok(ap->ad, n_total, K),
+    MS_CHECK_ARG(ap->v != nullptr && ap->tile_first != nullptr && ap->blocks != nullptr && ap->max_blocks > 0 && adapters_ok(ap->ad, n_total, K),
                  "gemm_tc: an adapted product needs a plan of its outputs");
     return launch_tc_pair_adapted<4, TC_QKV_ROPE>(q_out, x, w_qkv, M, n_total, n_total, K, 0, *ap, status, stream, qe);
   }
@@ -2074,13 +1975,13 @@ MS_EXPORT int ms_gemm_tc_qkv_bf16(void* q_out, const void* x, const void* w_qkv,
 }
 
 // out [M, N] bfloat16 = A W^T beside the adapters of A's rows (epilogue 0), or silu(gate) * up of the stacked W [2 N, K] beside them (epilogue 2). V and the plan
-// are the launches' before this one (ms_adapter_plan, ms_adapter_shrink_blocks).
+// are the launches' before this one (ms_adapter_plan, ms_gemm_tc_adapter_v).
 MS_EXPORT int ms_gemm_tc_adapted_bf16(void* out, const void* A, const void* W, int M, int N, int K, int epilogue, const AdaptedProduct* ap, int* status,
                                       cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
   MS_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 8 == 0, "gemm_tc: bad sizes M=%d N=%d K=%d", M, N, K);
   MS_CHECK_ARG(((uintptr_t)A % 16 == 0) && ((uintptr_t)W % 16 == 0), "gemm_tc: operands must be 16-byte aligned");
-  MS_CHECK_ARG(status != nullptr && ap != nullptr && ap->v != nullptr && ap->tile_first != nullptr && ap->block_slot != nullptr && ap->max_blocks > 0 &&
+  MS_CHECK_ARG(status != nullptr && ap != nullptr && ap->v != nullptr && ap->tile_first != nullptr && ap->blocks != nullptr && ap->max_blocks > 0 &&
                    adapters_ok(ap->ad, epilogue == TC_SILU_MUL ? 2 * N : N, K),
                "gemm_tc: an adapted product needs a status word and a plan of its outputs");
   if (epilogue == TC_OUT_BF16) return launch_tc_pair_adapted<5, TC_OUT_BF16>(out, A, W, M, N, N, K, 0, *ap, status, stream);

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import sys
 from contextlib import nullcontext
 from ctypes import c_char_p, c_int, c_ulonglong, c_void_p
 from dataclasses import dataclass
@@ -22,6 +23,11 @@ BLOCK_BYTES = 48  # of an ``AdapterBlock`` (csrc/adapters.cuh)
 ADAPTERS = build.Module("adapters", ("adapters.cu",))
 _TYPES = (torch.bfloat16, torch.float32)
 _Q = struct.Struct("Q").pack
+
+
+def _ops():
+    """The package that imports this module."""
+    return sys.modules[__package__]
 
 
 @dataclass(frozen=True, eq=False)
@@ -81,11 +87,9 @@ class AdapterRows:
         self._plans: dict = {}
         self._tickets: dict = {}
         if self.index >= 0:
-            from . import _sm_count, device_status
-
-            self.status = device_status(slot_of_row.device).data_ptr()
+            self.status = _ops().device_status(slot_of_row.device).data_ptr()
             self.middle = struct.pack("3Q", slot_of_row.data_ptr(), row_of_token.data_ptr(), self.status)
-            self.sms = _sm_count(slot_of_row.device)
+            self.sms = _ops()._sm_count(slot_of_row.device)
 
     def plan(self, slots: int, stream: int) -> "_Plan":
         """The adapters of each row tile, for projections with ``slots`` of them."""
@@ -94,7 +98,6 @@ class AdapterRows:
         if held is None:
             held = self._plans[key] = _Plan(self, slots, stream)
         return held
-
 
     def tickets(self, stream: int) -> int:
         """The address of two zeros on the device that no launch has had: a launch leaves its counts in them."""
@@ -115,13 +118,11 @@ class _Plan:
         # a request of several tiles has a block in each, and each request behind the first may add one to a tile that it shares
         self.max_blocks = max(1, min(tiles * min(slots, TILE), tiles + rows.rows - 1))
         with on_stream(stream, device):
-            self.ints = torch.empty((BLOCK_BYTES // 4 + 1) * self.max_blocks + tiles + 1, dtype=torch.int32, device=device)
+            self.ints = torch.empty(BLOCK_BYTES // 4 * self.max_blocks + tiles + 1, dtype=torch.int32, device=device)
         self.blocks = self.ints.data_ptr()
-        self.block_slot = self.blocks + BLOCK_BYTES * self.max_blocks
-        self.tile_first = self.block_slot + 4 * self.max_blocks
-        self.status = rows.status
+        self.tile_first = self.blocks + BLOCK_BYTES * self.max_blocks
         ad = bytes(24) + rows.middle + struct.pack("7i4x", slots, 0, 0, 0, 0, 0, 0)
-        _check(_lib().ms_adapter_plan(self.tile_first, self.block_slot, self.blocks, ad, t, self.max_blocks, stream))
+        _check(_lib().ms_adapter_plan(self.tile_first, self.blocks, ad, t, self.max_blocks, stream))
 
 
 @lru_cache(maxsize=None)
@@ -130,7 +131,7 @@ def _lib():
     native._declare(lib, "ms_adapters_last_error", [], c_char_p)
     native._declare(lib, "ms_adapters_set_pdl", [_i], None)
     native._declare(lib, "ms_adapter_capture_id", [_p], c_ulonglong)
-    native._declare(lib, "ms_adapter_plan", [_p] * 3 + [c_char_p, _i, _i, _p])
+    native._declare(lib, "ms_adapter_plan", [_p] * 2 + [c_char_p, _i, _i, _p])
     native._declare(lib, "ms_adapter_shrink", [_p, _p, c_char_p, _i, _i, _i, _i, _p])
     native._declare(lib, "ms_adapter_expand", [_p, _p, _p, c_char_p] + [_i] * 6 + [_p])
     lib.ms_adapters_set_pdl(int(native.pdl_enabled()))
@@ -141,10 +142,14 @@ def _check(rc: int) -> None:
     native.kernel_check(rc, lib=_lib() if rc else None, errfn="ms_adapters_last_error")
 
 
+_now = torch._C._cuda_getCurrentRawStream  # the handle of a device's current stream (what torch.cuda.current_stream(index).cuda_stream is, in a tenth of its time)
+_HERE = nullcontext()
+
+
 def on_stream(stream: int, device: torch.device):
     """Allocations in the order of ``stream`` (a handle), where that is not the current one."""
-    if stream == torch.cuda.current_stream(device).cuda_stream:
-        return nullcontext()
+    if stream == _now(device.index):
+        return _HERE
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device))
 
 
@@ -172,61 +177,73 @@ def _code(dtype: torch.dtype) -> int:
     return 0 if dtype is torch.float32 else 1
 
 
-FEW_TOKENS = 64  # up to so many, v is made token by token, and the products are the decode steps' tcgen05 kernel
+WAY: str | None = None  # tests and measurements: "decode", "pair" or "apart" instead of the rules'
+# Up to so many products (tokens x numbers x k) v is made token by token, beyond by a plan on the tensor cores. Token by token / by a plan, us, of one adapter and of 16: 64 tokens, 96
+# numbers, k 4,096 7.6 / 8.4 and 7.6 / 15.8; 48 numbers, k 12,288 8.6 / 10.2 and 10.7 / 19.6; 96 numbers, k 12,288 14.2 / 11.9 and 17.8 / 27.8.
+TOKEN_WISE = 48 << 20
+FEW_TOKENS = 32  # up to so many (in some cases half or twice so many), the products are the decode steps' tcgen05 kernel
 # That kernel makes v itself where the tokens are at most OWN_TOKENS, the numbers at most OWN_NUMBERS and the weight at least OWN_WEIGHT bytes: v is then ready before the
-# weights have come. In a launch ahead of it / its own work, us: 1 token of rank 16, 4096 -> 6144 17.9 / 12.8, 8 tokens of one adapter 17.8 / 14.1, 16 18.7 / 15.0, 8 of
-# rank 64 18.4 / 18.9, 16 of rank 64 21.3 / 23.8; 8 tokens, 2048 -> 4096 8.4 / 9.0, 1024 -> 4096 7.7 / 8.7.
-OWN_TOKENS, OWN_NUMBERS, OWN_WEIGHT = 16, 384, 24 << 20
+# weights have come. In a launch ahead of it / its own work, us, rank 16: 1 token of 4096 -> 6144 15.4 / 12.7, 8 of one adapter 15.8 / 14.2, of eight 16.3 / 17.3, 8 of 12288 -> 4096 25.0 / 22.5
+# and 25.4 / 25.2, 16 of sixteen 26.4 / 28.2, 8 of rank 64 28.2 / 29.4, 8 gated of 4096 -> 2 x 12288 37.3 / 34.5 and 38.0 / 35.5; 8 of 2048 -> 4096 8.1 / 9.1.
+OWN_TOKENS, OWN_NUMBERS, OWN_WEIGHT = 16, 128, 24 << 20
 
 
 def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, stream: int) -> torch.Tensor:
     """What the adapters' A make of x, float32 [T, parts * rank]."""
-    from . import tc_gemm_enabled
-
     t, k = x.shape
     with on_stream(stream, x.device):
         v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=x.device)
-    if t <= FEW_TOKENS or x.dtype is torch.float32 or not tc_gemm_enabled():
+    if t * low_rank.numbers * k <= TOKEN_WISE or x.dtype is torch.float32 or not _ops().tc_gemm_enabled():
         _check(_lib().ms_adapter_shrink(v.data_ptr(), x.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), stream))
     else:
-        _blocks(v, x, rows.plan(low_rank.slots, stream), ad, True, stream)
+        _by_plan(v, x, rows.plan(low_rank.slots, stream), ad, rows, True, stream)
     return v
 
 
-def _blocks(v: torch.Tensor, x: torch.Tensor, plan: _Plan, ad: bytes, compact: bool, stream: int) -> None:
+def _by_plan(v: torch.Tensor, x: torch.Tensor, plan: _Plan, ad: bytes, rows: AdapterRows, compact: bool, stream: int) -> None:
     lib = native.gemm_tc()
-    rc = lib.ms_gemm_tc_adapter_v(v.data_ptr(), x.data_ptr(), ad, plan.tile_first, plan.blocks, x.shape[0], x.shape[1], plan.max_blocks, int(compact), plan.status, stream)
-    native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
+    native.kernel_check(lib.ms_gemm_tc_adapter_v(v.data_ptr(), x.data_ptr(), ad, plan.tile_first, plan.blocks, x.shape[0], x.shape[1], plan.max_blocks, int(compact), rows.status,
+                                                 stream), lib=lib, errfn="ms_gemm_tc_last_error")
 
 
 def product(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, stream: int) -> tuple:
-    """What a product on the 2-CTA tcgen05 kernel takes of the adapters (``AdaptedProduct``), and the V it points to."""
+    """What a product on the 2-CTA tcgen05 kernel takes of the adapters (``AdaptedProduct``), and the V that it points to."""
     ad, plan = low_rank.head + rows.middle + low_rank.tail, rows.plan(low_rank.slots, stream)
     with on_stream(stream, x.device):
         v = torch.empty((plan.max_blocks * TILE, low_rank.numbers), dtype=torch.bfloat16, device=x.device)
-    _blocks(v, x, plan, ad, False, stream)
-    return ad + struct.pack("3Qi4x", v.data_ptr(), plan.tile_first, plan.block_slot, plan.max_blocks), v
+    _by_plan(v, x, plan, ad, rows, False, stream)
+    return ad + struct.pack("3Qi4x", v.data_ptr(), plan.tile_first, plan.blocks, plan.max_blocks), v
 
 
-def in_its_sums(tokens: int, outputs: int, gated: bool, sms: int) -> bool:
-    """Whether a product of many tokens runs on the 2-CTA tcgen05 kernel, which takes the adapters in its own sums, rather than in float32 wherever ``linear`` sends it, with
-    the adapters' terms added behind."""
-    tiles = -(-tokens // TILE) * -(-outputs // (128 if gated else 256))
-    return tiles >= sms // 8
+def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: int) -> str:
+    """The way of a bfloat16 product with adapters. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
+    takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it, the terms added behind.
+
+    Up to 32 tokens decode (16 where the row tiles of gate and up are more than the SMs: 32 tokens of 4096 -> 2 x 12288 55 / 50, of 16 adapters 67 / 55); up to 64 too where it is not
+    gated and k is 4,096 or more. decode / apart, us, one adapter of rank 16: 32 tokens of 4096 -> 6144 17.8 / 22.2, of 2048 -> 4096 11.1 /
+    13.0, of 12288 -> 4096 25.6 / 34.3, gated 2048 -> 2 x 6144 19.7 / 23.5; 64 tokens of 4096 -> 4096 17.8 / 18.7 (rank 64: 23.4 / 27.9), of 12288 -> 4096
+    30.2 / 34.3, of 2048 -> 4096 15.9 / 14.1.
+
+    Beyond, by what both take (us, fitted to a B200): a round of tiles of 256 x 256 on pairs of SMs goes with k; apart is the weights or the operations, three launches, and the outputs
+    read and written again. pair / apart: 4096 -> 4096 at 100 tokens 31 / 20, at 512 32 / 33 (rank 64: 33 / 48), at 700 32 / 46; 4096 -> 6144 at 200 32 / 33, at 512 33 / 44; 12288 ->
+    4096 at 512 73 / 61, at 700 76 / 83; 1024 -> 4096 at 100 14 / 13, at 1,100 21 / 36; gated 4096 -> 2 x 12288 at 64 59 / 59, at 200 60 / 90."""
+    if tokens <= (FEW_TOKENS // 2 if gated and outputs > 64 * sms else FEW_TOKENS) or (tokens <= 2 * FEW_TOKENS and inputs >= 4096 and not gated):
+        return "decode"
+    tiles, rows = -(-tokens // TILE) * -(-outputs // (128 if gated else 256)), outputs * (2 if gated else 1)
+    apart = max(2.4 * inputs * rows / 6.3e6, 2 * tokens * inputs * rows / 1.2e9) + 12 + (2 + 0.15 * rank) * 1e-6 * tokens * rows
+    return "pair" if 7 + -(-tiles // (sms // 2)) * inputs * 0.006 <= apart else "apart"
 
 
-def _run(x, weight, out, stream: int, current: bool, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
-    from . import linear as shared
-    from . import tc_gemm_enabled
-
+def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
     t, k = x.shape
     n, ad, device = out.shape[1], low_rank.head + rows.middle + low_rank.tail, x.device
-    if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and weight.data_ptr() % 16 == 0 and tc_gemm_enabled():
+    if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and weight.data_ptr() % 16 == 0 and _ops().tc_gemm_enabled():
         lib = native.gemm_tc()
-        if t <= FEW_TOKENS:
+        way = WAY or way_of(t, n, k, low_rank.rank, gated, rows.sms)
+        if way == "decode":
             if t <= OWN_TOKENS and t * low_rank.numbers <= OWN_NUMBERS and 2 * k * low_rank.outputs >= OWN_WEIGHT:
                 tickets = rows.tickets(stream)
-                with nullcontext() if current else on_stream(stream, device):
+                with on_stream(stream, device):
                     v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=device)
             else:
                 v, tickets = _terms(x, low_rank, rows, ad, stream), 0
@@ -234,7 +251,7 @@ def _run(x, weight, out, stream: int, current: bool, low_rank: LowRank, rows: Ad
             rc = lib.ms_gemm_tc_decode_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated), term, rows.status, stream)
             native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
             return
-        if in_its_sums(t, n, gated, rows.sms):
+        if way == "pair":
             held, v = product(x, low_rank, rows, stream)
             rc = lib.ms_gemm_tc_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, 2 if gated else 0, held, rows.status, stream)
             native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
@@ -244,7 +261,7 @@ def _run(x, weight, out, stream: int, current: bool, low_rank: LowRank, rows: Ad
     if out.dtype is not torch.float32 or gated:
         with on_stream(stream, device):
             y = torch.empty((t, low_rank.outputs), dtype=torch.float32, device=device)
-    shared(x, weight, out=y, stream=stream)
+    _ops().linear(x, weight, out=y, stream=stream)
     v = _terms(x, low_rank, rows, ad, stream)
     _check(_lib().ms_adapter_expand(out.data_ptr(), y.data_ptr(), v.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), _code(out.dtype), int(gated), stream))
 
@@ -254,13 +271,13 @@ def _call(x, weight, out, stream, low_rank: LowRank, rows: AdapterRows, gated: b
     if torch.cuda.current_device() != low_rank.index:
         with torch.cuda.device(low_rank.index):
             return _call(x, weight, out, stream, low_rank, rows, gated)
-    now = torch.cuda.current_stream().cuda_stream
-    stream = now if stream is None else stream
+    if stream is None:
+        stream = _now(low_rank.index)
     if out is None:
         with on_stream(stream, x.device):
             out = torch.empty((x.shape[0], low_rank.outputs), dtype=x.dtype, device=x.device)
     if x.shape[0]:
-        _run(x, weight, out, stream, stream == now, low_rank, rows, gated)
+        _run(x, weight, out, stream, low_rank, rows, gated)
     return out
 
 

@@ -39,17 +39,21 @@ def sample_filtered(tokens: torch.Tensor, logits: torch.Tensor, temperature: tor
         raise ValueError(f"logits are a contiguous float32 CUDA tensor, not {logits.dtype} on {logits.device}")
     if not 1 <= vocab <= MAX_VOCAB:
         raise ValueError(f"a vocabulary of 1 to {MAX_VOCAB} tokens, not {vocab}")
-    for name, t, dtypes in (("tokens", tokens, (torch.int32,)), ("temperature", temperature, (torch.float32,)), ("uniform", uniform, (torch.float32, torch.float64)),
-                            ("top_k", top_k, (torch.int32,)), ("top_p", top_p, (torch.float32,)), ("min_p", min_p, (torch.float32,))):
-        if t is None and name.startswith(("top", "min")):
-            continue
-        if t.dtype not in dtypes or t.dim() != 1 or t.shape[0] < rows or t.get_device() != dev or not t.is_contiguous():
-            raise ValueError(f"{name} is a contiguous {' or '.join(map(str, dtypes))} tensor of {rows} rows on the logits' device, not {t.dtype} {tuple(t.shape)}")
+    wide = uniform.dtype is torch.float64
+    ptr = [_row("tokens", tokens, torch.int32, rows, dev), logits.data_ptr(), _row("temperature", temperature, torch.float32, rows, dev),
+           _row("uniform", uniform, torch.float64 if wide else torch.float32, rows, dev), None if top_k is None else _row("top_k", top_k, torch.int32, rows, dev),
+           None if top_p is None else _row("top_p", top_p, torch.float32, rows, dev), None if min_p is None else _row("min_p", min_p, torch.float32, rows, dev)]
     if not rows:
         return
     if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
-            return sample_filtered(tokens, logits, temperature, uniform, top_k, top_p, min_p, torch.cuda.current_stream(dev).cuda_stream if stream is None else stream)
-    ptr = [None if t is None else t.data_ptr() for t in (tokens, logits, temperature, uniform, top_k, top_p, min_p)]
-    rc = _lib().ms_sample_filtered(*ptr, rows, vocab, int(uniform.dtype is torch.float64), torch.cuda.current_stream(dev).cuda_stream if stream is None else stream)
+            return sample_filtered(tokens, logits, temperature, uniform, top_k, top_p, min_p, stream)
+    rc = _lib().ms_sample_filtered(*ptr, rows, vocab, int(wide), torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     native.kernel_check(rc, lib=_lib() if rc else None, errfn="ms_filters_last_error")
+
+
+def _row(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, dev: int) -> int:
+    """The address of a number per row."""
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] < rows or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous {dtype} tensor of {rows} rows on the logits' device, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
