@@ -1842,22 +1842,16 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
   constexpr size_t smem = (size_t)STAGES * (TC_BM + BT) * TC_BK * 2 + (size_t)BT * TC_BM * 4 + 1024;
   static_assert((decode_twice(BT, ADAPTED) ? 2 : 1) * (smem + 1024) <= 227 * 1024, "the ring does not fit shared memory");
   auto kernel = gemm_tc_decode_kernel<BT, STAGES, ADAPTED, GATED>;
-  static bool configured = false;
-  static int sm_count = 0;
-  if (!configured) {
-    MS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    int dev = 0;
-    MS_CHECK_CUDA(cudaGetDevice(&dev));
-    MS_CHECK_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev));
-    configured = true;
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  MS_CHECK_CUDA(allow_shared_memory((const void*)kernel, (int)smem, allowed));
+  const int sms = sm_count() > 0 ? sm_count() : 148;
   // Slices of k: as many as still let every cluster be resident at once (clusters are placed within a
   // group of SMs, so fewer fit than SMs / size), each of at least four k-blocks, at most eight.
   static int fit[9] = {0};  // how many clusters of each size the device holds at once
   if (fit[1] == 0) {
     for (int size = 1; size <= 8; ++size) {
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)(size * sm_count));
+      cfg.gridDim = dim3((unsigned)(size * sms));
       cfg.blockDim = dim3(TC_THREADS);
       cfg.dynamicSmemBytes = smem;
       cudaLaunchAttribute attr;
@@ -1867,7 +1861,7 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) n = sm_count / size / 2;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) n = sms / size / 2;
       fit[size] = n;
     }
   }
