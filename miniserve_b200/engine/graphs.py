@@ -125,7 +125,7 @@ class DecodeGraphs:
     def capture_all(self, modes: Sequence[str] = ("greedy",), classes: Sequence[int] = (0,)) -> int:
         """Capture the graphs of every batch bucket now instead of at their first use (the reference
         captures at start-up, miniserve/engine/cuda_graph.py), for the given classes of context length.
-        Needs an idle cache: it steps ``max_batch`` one-token requests that it creates and releases.
+        Needs an idle cache: it steps ``max_batch`` one-token requests that it creates and releases. Where requests may have adapters, those of steps that have some too.
         Returns how many it captured."""
         sf = self.step_fn
         sampling_for = {
@@ -135,11 +135,11 @@ class DecodeGraphs:
             "filtered": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n, top_ks=[2] * n),
         }
         before = len(self._graphs)
-        for mode, klass in ((m, k) for m in modes for k in classes):
+        for mode, klass, adapter in ((m, k, a) for m in modes for k in classes for a in ((-1, 0) if sf.low_rank else (-1,))):
             for bucket in self.buckets:
                 caches = [sf.cache.new_request() for _ in range(bucket)]
                 try:
-                    self.run([StepRow(c, [0], (0,)) for c in caches], sampling_for[mode](bucket), klass=klass)
+                    self.run([StepRow(c, [0], (0,), adapter=adapter) for c in caches], sampling_for[mode](bucket), klass=klass)
                 finally:
                     for c in caches:
                         sf.cache.release(c)
@@ -398,7 +398,7 @@ class StepGraphs:
         """Capture now, on an idle cache, the shapes that lone prompts of up to ``max_tokens`` tokens meet
         (every padded size up to there), instead of at their second sighting: each size is first run
         once as it is (what a kernel or the library sets up at its first use must not happen inside a
-        capture), then captured from a prompt one token shorter. Returns how many were captured."""
+        capture), then captured from a prompt one token shorter. Where requests may have adapters, those of prompts that have one too. Returns how many were captured."""
         if not self.enabled or not self.pad:
             return 0
         sf = self.step_fn
@@ -407,11 +407,12 @@ class StepGraphs:
         sizes = [n for n in sizes if n <= min(max_tokens, room) and n * self.flops_per_token <= self.max_step_flops]
         before = self.captures
         kept = self.sightings, self.capture_every, self.max_shapes
-        self.max_shapes = max(self.max_shapes, len(self._shapes) + len(sizes))
+        adapters = (-1, 0) if sf.low_rank else (-1,)
+        self.max_shapes = max(self.max_shapes, len(self._shapes) + len(sizes) * len(adapters))
         try:
-            for n in sizes:
+            for n, adapter in ((n, a) for n in sizes for a in adapters):
                 for tokens, sightings in ((n, 1 << 30), (n - 1, 1)):
-                    rows = [StepRow(sf.cache.new_request(), [0] * tokens, (tokens - 1,))]
+                    rows = [StepRow(sf.cache.new_request(), [0] * tokens, (tokens - 1,), adapter=adapter)]
                     self.sightings, self.capture_every, self._since_capture = sightings, 0, 1
                     try:
                         if self._key(rows) not in self._shapes:

@@ -265,4 +265,5 @@ class StepFunction:
         if code:
             self.reset_after_fault()
             raise StepError(f"a kernel reported a fault it caught itself (code {code}: 2-3 inconsistent cache "
-                            f"metadata; 11-13, 21-24, 31-34, 41-42 a bounded wait in a tensor-core pipeline ran out)")
+                            f"metadata; 6 an adapter's slot that is not there, or tokens that are not in the order of their rows; 11-13, 16-19, 21-24, 31-34, 41-42 a bounded wait in a "
+                            f"tensor-core pipeline ran out)")

@@ -7,6 +7,8 @@ Each *module* is one shared library made from a few source files under ``csrc/``
 - ``mixers``: pointwise kernels of parts that only some models have, compiled when one of them is first used;
 - ``recurrence``: the linear-attention recurrences and what surrounds them, compiled when a model has such a layer;
 - ``experts``: the kernels of a routed feed-forward, compiled when a model has one;
+- ``adapters``: what low-rank adapters of many requests need beside the products of ``gemm_tc``, compiled when a step has one;
+- ``filters``: sampling with top-k, top-p and min-p from given random numbers, compiled when a request asks for it;
 - further modules are compiled only when a model needs them (for instance the bfloat16
   attention kernels for one head size), so a first call compiles what that model uses.
 

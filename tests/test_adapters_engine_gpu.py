@@ -193,6 +193,24 @@ def test_the_random_numbers_are_the_ones_of_seed_and_counter(held):
 def test_graphs_of_filtered_steps_are_captured_ahead(held):
     llm = engine(held, "bfloat16", max_running=2)
     n = llm.engine.capture_graphs(("greedy", "filtered"))
-    assert n == len(llm.engine.graphs._graphs) == 4
-    llm.generate(prompts_of(held, [5], 1), SamplingParams(max_new_tokens=4, temperature=0.5, top_k=3, seed=1))
-    assert len(llm.engine.graphs._graphs) == 4
+    assert n == len(llm.engine.graphs._graphs) == 8  # (of one request and of two, steps with adapters and without)
+    for name in (None, "b"):
+        llm.generate(prompts_of(held, [5], 1), SamplingParams(max_new_tokens=4, temperature=0.5, top_k=3, seed=1), adapters=name)
+        llm.generate(prompts_of(held, [5, 7], 1), SamplingParams(max_new_tokens=4), adapters=[name, None])
+    assert len(llm.engine.graphs._graphs) == 8
+
+
+def test_graphs_of_prompts_with_adapters_are_captured_ahead(held):
+    prompt = prompts_of(held, [200], 2)
+    plain_engine = engine(held, "bfloat16", step_graphs=False)
+    llm = engine(held, "bfloat16")
+    shapes = llm.engine.step_fn.graphs
+    n = llm.engine.capture_graphs(("greedy",), prompt_tokens=300)
+    captured = shapes.captures
+    assert n > captured > 0
+    for name in ("a", None, "c"):
+        before = shapes.replayed_launches
+        tokens = llm.generate(prompt, SamplingParams(max_new_tokens=4), adapters=name)[0]
+        assert shapes.replayed_launches > before and shapes.captures == captured
+        margins(held, prompt[0], tokens, name, "bfloat16")
+        margins(held, prompt[0], plain_engine.generate(prompt, SamplingParams(max_new_tokens=4), adapters=name)[0], name, "bfloat16")
