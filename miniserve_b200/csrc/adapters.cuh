@@ -16,7 +16,8 @@ struct Adapters {
   const float* scale;     // [slots]
   const int* slot_of_row;
   const int* row_of_token;
-  int* status;            // raised (6) by a slot that is not there
+  int* status;            // raised (6) by a slot or a row that is not there
+  int rows, unused;       // of slot_of_row
   int slots, rank, parts, ends[MAX_PARTS];  // ends[p]: the first column behind part p (of parts that there are not, N)
 };
 
@@ -46,8 +47,11 @@ struct AdapterTerms {
 };
 
 __device__ __forceinline__ int adapter_of(const Adapters& ad, int t) {
-  const int s = behind_load(ad.slot_of_row + behind_load(ad.row_of_token + t));
-  if (s < ad.slots) return s < 0 ? -1 : s;
+  const int row = behind_load(ad.row_of_token + t);
+  if ((unsigned)row < (unsigned)ad.rows) {
+    const int s = behind_load(ad.slot_of_row + row);
+    if (s < ad.slots) return s < 0 ? -1 : s;
+  }
   atomicExch(ad.status, 6);
   return -1;
 }

@@ -72,6 +72,8 @@ class AdapterStore:
                 raise ValueError("alpha is what the adapter's folder says")
         else:
             tensors = dict(source)
+        if not math.isfinite(factor if factor is not None else 1.0 if alpha is None else alpha):
+            raise ValueError(f"adapter {name!r} has a factor that is not finite")
         pairs = self._pairs(name, tensors)
         slot = free[0]
         for low in self.products.values():
@@ -145,6 +147,8 @@ class AdapterStore:
                 wrong.append(f"{matrix}: A {tuple(a.shape)} and B {tuple(b.shape)} beside a matrix of {behind - first} x {low.inputs}")
             else:
                 ranks.add(a.shape[0])
+                if not all(bool(torch.isfinite(t.to(low.a.dtype)).all()) for t in (a, b)):
+                    wrong.append(f"{matrix}: numbers that are not finite (other requests' tokens would meet them)")
                 if not 1 <= a.shape[0] <= self.rank:
                     wrong.append(f"{matrix}: rank {a.shape[0]}, there is room for 1 to {self.rank} (max_adapter_rank)")
         if len(ranks) > 1:

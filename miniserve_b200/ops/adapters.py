@@ -34,7 +34,8 @@ def _ops():
 class LowRank:
     """The adapters of one projection, W [N, K]: slot s adds ``scale[s]`` B_s A_s x to W x. ``a`` [slots, parts * rank, K] and ``b`` [slots, N, rank] in the
     weight's type, ``scale`` float32 [slots]. A stacked projection (q|k|v, gate|up) has ``parts``: ``ends[p]`` is the first of W's rows behind part p (the
-    last is N), a's rows [p * rank, (p + 1) * rank) and part p's rows of b belong together. An adapter of a smaller rank fills its place up with zeros."""
+    last is N), a's rows [p * rank, (p + 1) * rank) and part p's rows of b belong together. An adapter of a smaller rank fills its place up with zeros.
+    All are finite: in a step of many tokens other requests' tokens meet an adapter with zeros for v."""
 
     a: torch.Tensor
     b: torch.Tensor
@@ -73,8 +74,8 @@ class LowRank:
 class AdapterRows:
     """Which adapter each token of a step has: ``slot_of_row`` int32 [rows], the slot of each request (below 0: none), and ``row_of_token`` int32
     [tokens], the request of each token, tokens in the order of the requests. Made once per step and used by all its layers: steps of many tokens have a plan, which the
-    first product of a stream (or of a capture) makes of what the tensors hold then. A slot that the adapters do not have raises the status word, and the
-    token counts as one without an adapter."""
+    first product of a stream (or of a capture) makes of what the tensors hold then. A slot that the adapters do not have, or a row
+    that there is not, raises the status word, and the token counts as one without an adapter."""
 
     def __init__(self, slot_of_row: torch.Tensor, row_of_token: torch.Tensor):
         for t in (slot_of_row, row_of_token):
@@ -88,7 +89,7 @@ class AdapterRows:
         self._tickets: dict = {}
         if self.index >= 0:
             self.status = _ops().device_status(slot_of_row.device).data_ptr()
-            self.middle = struct.pack("3Q", slot_of_row.data_ptr(), row_of_token.data_ptr(), self.status)
+            self.middle = struct.pack("3Q2i", slot_of_row.data_ptr(), row_of_token.data_ptr(), self.status, self.rows, 0)
             self.sms = _ops()._sm_count(slot_of_row.device)
 
     def plan(self, slots: int, stream: int) -> "_Plan":
@@ -163,14 +164,15 @@ def check(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None, low_r
         raise ValueError(f"x has {shape[0]} tokens, adapter_rows {rows.tokens}")
     if dtype is not low_rank.dtype or weight.dtype is not dtype:
         raise TypeError(f"x, the weight and its adapters are of one type, not {dtype}, {weight.dtype} and {low_rank.dtype}")
-    if not (x.get_device() == weight.get_device() == index == rows.index >= 0) or not x.is_contiguous() or not weight.is_contiguous() or x.data_ptr() % 16:
-        raise ValueError("kernel operands must be contiguous CUDA tensors on one device, x on 16 bytes")
+    if (not (x.get_device() == weight.get_device() == index == rows.index >= 0) or not x.is_contiguous() or not weight.is_contiguous() or x.data_ptr() % 16
+            or weight.data_ptr() % 16):
+        raise ValueError("kernel operands must be contiguous CUDA tensors on one device, x and the weight on 16 bytes")
     if gated and (low_rank.outputs % 2 or out.dtype is not dtype):
         raise ValueError(f"a gate|up projection of {low_rank.outputs} rows, out {out.dtype} for x {dtype}")
     if out is not None and (out.shape != (shape[0], low_rank.outputs // 2 if gated else low_rank.outputs) or out.get_device() != index or not out.is_contiguous()
-                            or (out.dtype is not dtype and out.dtype is not torch.float32)):
+                            or (out.dtype is not dtype and out.dtype is not torch.float32) or out.data_ptr() % 16):
         raise ValueError(f"out is {out.dtype} {tuple(out.shape)} for {shape[0]} tokens and {low_rank.outputs} outputs{' (gate and up)' if gated else ''}: a contiguous tensor on the "
-                         "adapters' device, of x's type or float32")
+                         "adapters' device, of x's type or float32, on 16 bytes")
 
 
 def _code(dtype: torch.dtype) -> int:
@@ -237,7 +239,7 @@ def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: 
 def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gated: bool) -> None:
     t, k = x.shape
     n, ad, device = out.shape[1], low_rank.head + rows.middle + low_rank.tail, x.device
-    if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and weight.data_ptr() % 16 == 0 and _ops().tc_gemm_enabled():
+    if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and _ops().tc_gemm_enabled():
         lib = native.gemm_tc()
         way = WAY or way_of(t, n, k, low_rank.rank, gated, rows.sms)
         if way == "decode":

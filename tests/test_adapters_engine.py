@@ -105,6 +105,19 @@ def test_all_that_does_not_fit_is_one_error_and_changes_nothing():
         store.unload("another")
 
 
+def test_numbers_that_are_not_finite_are_refused():
+    m = model(dtype=torch.bfloat16)
+    store = AdapterStore(m, 1, 8)
+    for value in (float("nan"), float("inf"), 3.4e38):  # (the last is finite in 32 bits alone)
+        given = tensors(m, 4)
+        next(iter(given.values()))[1, 2] = value
+        with pytest.raises(ValueError, match="not finite"):
+            store.load("bad", given)
+    with pytest.raises(ValueError, match="factor"):
+        store.load("bad", tensors(m, 4), alpha=float("inf"))
+    assert not store.names and not any(bool(low.a.any()) for low in store.products.values())
+
+
 def test_a_folder_says_rank_and_factor(tmp_path):
     from safetensors.torch import save_file
 

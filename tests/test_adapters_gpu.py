@@ -172,6 +172,93 @@ def test_a_captured_call_follows_its_inputs(rows):
             au.close(out, *au.formula(x, w, low, ar))
 
 
+# 8 and 16 tokens beside a weight of 32 MiB: the product's own warps make v (counters that a launch has to itself)
+@pytest.mark.parametrize("tokens", [8, 16])
+def test_own_terms_on_two_streams_at_once(tokens):
+    """Calls of two streams with the same AdapterRows, more than a stretch of counters holds, against the same calls one after the other."""
+    from miniserve_b200 import ops
+
+    a = ops.adapters
+    k, n = 4096, 4096
+    assert tokens <= a.OWN_TOKENS and 8 * tokens <= a.OWN_NUMBERS and 2 * k * n >= a.OWN_WEIGHT
+    x, w, low, ar = au.made([(1, i % 3 - (i == 5)) for i in range(tokens)], k, (n,), 8, 3, torch.bfloat16)
+    want, tol = au.formula(x, w, low, ar)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[torch.full((tokens, n), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(150)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(150):
+        for s, out in zip(streams, outs):
+            ops.linear(x, w, out=out[i], low_rank=low, adapter_rows=ar, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    au.close(outs[0][0], want, tol)
+    first = outs[0][0]
+    assert all(torch.equal(o, first) for out in outs for o in out) and int(ops.device_status("cuda")) == 0
+
+
+def test_own_terms_of_many_captured_calls():
+    """More calls in one graph than a stretch of counters holds, replayed; another graph of the same AdapterRows in between."""
+    from miniserve_b200 import ops
+
+    x, w, low, ar = au.made(EIGHT, 4096, (4096,), 8, 4, torch.bfloat16)
+    side = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(side):
+        ops.linear(x, w, low_rank=low, adapter_rows=ar)
+    side.synchronize()
+    for calls in (ops.adapters.TICKETS + 20, 3):
+        outs = [torch.empty((8, 4096), dtype=torch.bfloat16, device="cuda") for _ in range(calls)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            for out in outs:
+                ops.linear(x, w, out=out, low_rank=low, adapter_rows=ar)
+        graphs.append((graph, outs))
+    for turn in range(4):
+        x.copy_(torch.randn_like(x))
+        graph, outs = graphs[turn % 2]
+        for out in outs:
+            out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        au.close(outs[0], *au.formula(x, w, low, ar))
+        assert all(torch.equal(out, outs[0]) for out in outs)
+    assert int(ops.device_status("cuda")) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_tokens_than_a_grid_has_rows(dtype):
+    """70,000 tokens (beyond 65,535) of a few requests; the formula at some of them."""
+    rows = [(1, 2), (65535, 1), (1, -1), (4000, 0), (463, 3)]
+    x, w, low, ar = au.made(rows, 64, (128,), 8, 4, dtype)
+    got = run_linear(x, w, low, ar)
+    at = torch.tensor([0, 1, 2, 255, 256, 32767, 65535, 65536, 65537, 65538, 69536, 69537, 69999], device="cuda")
+    from miniserve_b200 import ops
+
+    want, tol = au.formula(x[at], w, low, ops.AdapterRows(ar.slot_of_row, ar.row_of_token[at].contiguous()))
+    au.close(got[at], want, tol)
+    plain = x.double() @ w.double().T
+    none = torch.nonzero(ar.slot_of_row[ar.row_of_token.long()] < 0)[:, 0]
+    assert none.tolist() == [65536] and bool(((got - plain).abs().amax(1) > 0.05).sum() > 69000)
+
+
+@pytest.mark.parametrize("rows", [EIGHT, DECODE64, MIXED, LONG])
+def test_a_row_that_is_not_there_raises_the_status_word(rows):
+    from miniserve_b200 import ops
+
+    x, w, low, ar = au.made(rows, 256, (4096,), 8, 4, torch.bfloat16)
+    status, last = ops.device_status("cuda"), ar.rows
+    of_token = ar.row_of_token.clone()
+    of_token[0], of_token[-1] = -3, last
+    try:
+        got = run_linear(x, w, low, ops.AdapterRows(ar.slot_of_row, of_token))
+        assert int(status) == 6
+    finally:
+        status.zero_()
+    slots = torch.cat([ar.slot_of_row, torch.full((1,), -1, dtype=torch.int32, device="cuda")])
+    of_token[0] = last
+    au.close(got, *au.formula(x, w, low, ops.AdapterRows(slots, of_token)))
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 numbers of B: the last slot's."""
     from miniserve_b200 import ops
@@ -205,6 +292,10 @@ def test_refusals_on_the_device():
     with pytest.raises(ValueError, match="16 bytes"):
         shifted = torch.empty(8 * 256 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(8, 256)
         ops.linear(shifted, w, low_rank=low, adapter_rows=ar)
+    with pytest.raises(ValueError, match="weight on 16 bytes"):
+        ops.linear(x, torch.empty(128 * 256 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(128, 256), low_rank=low, adapter_rows=ar)
+    with pytest.raises(ValueError, match="on 16 bytes"):
+        ops.linear(x, w, out=torch.empty(8 * 128 + 1, dtype=torch.float32, device="cuda")[1:].view(8, 128), low_rank=low, adapter_rows=ar)
 
 
 @pytest.mark.parametrize("rows,rank,full", [(LONG[:1], 16, False), (LONG, 16, True), (PROMPTS, 72, True), (DECODE64 + PROMPTS, 8, True), ([(40, 1)], 24, False)])

@@ -63,7 +63,7 @@ SETTINGS = [dict(), dict(k=1), dict(k=3), dict(k=40), dict(k=100000), dict(p=0.9
             dict(k=50, p=0.9, m=0.05), dict(p=0.95, m=0.02), dict(k=5, m=0.2)]
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 1000, 4097, 50000, 151936, 400003])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 1000, 4097, 50000, 151936, 400003, 1 << 20])
 @pytest.mark.parametrize("t", [0.7, 1.0, 3.0])
 def test_tokens(vocab, t):
     rows = len(SETTINGS)
