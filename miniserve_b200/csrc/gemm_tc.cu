@@ -997,8 +997,9 @@ adapter_v_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem_base = tmem_base_slot;
-  pdl_launch_dependents();
+  // The wait comes first: the product behind starts on what earlier kernels have left, before this one has ended.
   pdl_wait();
+  pdl_launch_dependents();
   const int items = tile_first[(T + ADAPTER_ROWS - 1) / ADAPTER_ROWS] * 2 * chunks;
   int kb = 0, done = 0, issued = 0;  // k-blocks and items so far that had products; (the producer's) blocks asked for
   bool ok = true;
@@ -1217,7 +1218,9 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   const uint32_t tmem_base = tmem_base_slot;
 
   pdl_launch_dependents();
-  pdl_wait();
+  // ADAPTED: the kernel before is adapter_v_kernel, whose CTAs have waited for all that ran before it by the time this one starts. Of its own work only V is read, by the thread
+  // that asks for it, which waits then (once, whether or not its tiles have adapters: this kernel ends behind that one).
+  if (!ADAPTED) pdl_wait();
   if (GROUPED) m_tiles = grp.meta[0];  // (the plan is an earlier kernel's)
   const int num_tiles = n_tiles * m_tiles;
   // a tile's first row for this CTA, the matrix it belongs to and the end of that matrix's rows
@@ -1245,6 +1248,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   if (warp == 0) {
     if (elect_one()) {
       int kb = 0;
+      bool waited = !ADAPTED;
       for (int tile = pair; tile < num_tiles; tile += num_pairs) {
         const int n0 = tile_n(tile) * COLS, m0 = first_row(tile);
         // this CTA's 128 of the tile's 256 rows of W: for SiLU * up the first CTA brings the gate rows, the second the up rows
@@ -1265,6 +1269,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         if constexpr (ADAPTED) {
           const int last = ad.tile_first[tile_m(tile) + 1];
+          if (!waited) pdl_wait();
+          waited = true;
           for (int b = ad.tile_first[tile_m(tile)]; b < last && ok; ++b)
 #pragma unroll
             for (int p = 0; p < MAX_PARTS; ++p) {
@@ -1285,6 +1291,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         if (!ok) break;
       }
+      if (!waited) pdl_wait();
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
