@@ -95,7 +95,9 @@ __global__ void __launch_bounds__(SHRINK_WARPS * 32, EACH == 1 ? 3 : 4)
 adapter_shrink_kernel(float* v, const T* x, const Adapters ad, int K, int split) {
   constexpr int W = Wide<T>::N;
   __shared__ float sums[SHRINK_WARPS][EACH];
-  pdl_prologue(v, x);
+  // The wait comes first: a product behind may start on what earlier kernels have left, before this one has ended.
+  pdl_wait(v, x);
+  pdl_launch_dependents();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int s = adapter_of(ad, t), numbers = ad.parts * ad.rank;
   if (s < 0) return;

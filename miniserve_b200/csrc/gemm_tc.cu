@@ -724,6 +724,8 @@ __device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %
 // warp's 32 rows of B an instruction; a cluster's CTAs share the adapters out, and a term enters the sum over the slices with the CTA that made it. One rounding.
 // (Terms as k-blocks of the tensor cores, as in the 2-CTA kernel, cost a copy of 128 short rows for each adapter of the step: 42.9 us at 64 tokens of 16 adapters, rank 32,
 // 4096 -> 6144; row by row with multiply-adds 63.7.)
+// The kernel that made v has waited, in all its CTAs, for what ran before it by the time this one starts, so x and the weights are asked for at once and only the first reading of v
+// waits for that kernel's end (8 tokens of 12288 -> 4096: 22.2 us instead of 24.6).
 // v may be this kernel's own work (tickets): the same warps of all CTAs take (token, number) after (token, number) from a counter, a dot product of x's row and A's each,
 // and a second counter says when all are done. What is taken is being worked on by a warp that runs, so the wait for the rest ends whether or not all CTAs are on
 // the GPU at once. That leaves one launch, and x's part of the product does not wait for v.
@@ -782,7 +784,11 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
   if (warp == 0) {
     if (threadIdx.x == 0) {
-      pdl_wait();
+      if constexpr (ADAPTED) {
+        if (term.tickets != nullptr) pdl_wait();
+      } else {
+        pdl_wait();
+      }
       for (int i = 0; i < ahead; ++i) tma_load_2d(smem + (size_t)i * STAGE_BYTES + W_BYTES, &map_x, &full_bar[i], (it0 + i) * TC_BK, 0);
       for (int i = ahead; i < n_it; ++i) {
         const int s = i % STAGES;
@@ -815,7 +821,11 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
   } else {
     // warps 2..5: warp w may touch tensor-memory lanes 32 * (w % 4) .. + 31, i.e. rows of W
-    pdl_wait();
+    if constexpr (ADAPTED) {
+      if (term.tickets != nullptr) pdl_wait();
+    } else {
+      pdl_wait();
+    }
     const int quad = warp & 3, l = quad * 32 + lane;
     if constexpr (ADAPTED) {
       const Adapters& ad = term.ad;
@@ -871,9 +881,11 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         n[i] = GATED && row >= ROWS ? N + n0 + row - ROWS : n0 + row;
       }
       auto ready = [&] {
+        if (term.tickets == nullptr) pdl_wait();
         if (term.tickets != nullptr && !__all_sync(0xffffffffu, tickets_reach(term.tickets + 1, units)) && lane == 0) atomicExch(status, 19);
       };
       warp_terms(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i, float x) { part[tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i] += x; });
+      if (term.tickets == nullptr) pdl_wait();
       __syncwarp();
     }
     bool ok = true;

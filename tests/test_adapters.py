@@ -74,6 +74,11 @@ def test_which_way_a_product_goes():
         assert ways == sorted(ways) and set(ways) <= {"apart", "pair"}, ways  # from some number of tokens on, the 2-CTA kernel
 
 
+def test_whose_work_the_numbers_are():
+    own = ops.adapters.makes_its_own
+    assert own(16, 48) and not own(19, 48) and own(256, 192) and not own(512, 192) and not own(8, 47) and not own(128, 96)
+
+
 def test_sampling_on_the_host_or_of_other_types_is_refused():
     logits, f, i = torch.zeros((2, 8)), torch.zeros(2), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):

@@ -172,15 +172,14 @@ def test_a_captured_call_follows_its_inputs(rows):
             au.close(out, *au.formula(x, w, low, ar))
 
 
-# 8 and 16 tokens beside a weight of 32 MiB: the product's own warps make v (counters that a launch has to itself)
+# 8 and 16 tokens beside a weight of 128 MiB: the product's own warps make v (counters that a launch has to itself)
 @pytest.mark.parametrize("tokens", [8, 16])
 def test_own_terms_on_two_streams_at_once(tokens):
     """Calls of two streams with the same AdapterRows, more than a stretch of counters holds, against the same calls one after the other."""
     from miniserve_b200 import ops
 
-    a = ops.adapters
-    k, n = 4096, 4096
-    assert tokens <= a.OWN_TOKENS and 8 * tokens <= a.OWN_NUMBERS and 2 * k * n >= a.OWN_WEIGHT
+    k, n = 4096, 16384
+    assert ops.adapters.makes_its_own(8 * tokens, 2 * k * n >> 20)
     x, w, low, ar = au.made([(1, i % 3 - (i == 5)) for i in range(tokens)], k, (n,), 8, 3, torch.bfloat16)
     want, tol = au.formula(x, w, low, ar)
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -200,14 +199,15 @@ def test_own_terms_of_many_captured_calls():
     """More calls in one graph than a stretch of counters holds, replayed; another graph of the same AdapterRows in between."""
     from miniserve_b200 import ops
 
-    x, w, low, ar = au.made(EIGHT, 4096, (4096,), 8, 4, torch.bfloat16)
+    x, w, low, ar = au.made(EIGHT, 4096, (16384,), 8, 4, torch.bfloat16)
+    assert ops.adapters.makes_its_own(64, 128)
     side = torch.cuda.Stream()
     graphs = []
     with torch.cuda.stream(side):
         ops.linear(x, w, low_rank=low, adapter_rows=ar)
     side.synchronize()
     for calls in (ops.adapters.TICKETS + 20, 3):
-        outs = [torch.empty((8, 4096), dtype=torch.bfloat16, device="cuda") for _ in range(calls)]
+        outs = [torch.empty((8, 16384), dtype=torch.bfloat16, device="cuda") for _ in range(calls)]
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             for out in outs:
