@@ -183,7 +183,7 @@ WAY: str | None = None  # tests and measurements: "decode", "pair" or "apart" in
 # Up to so many products (tokens x numbers x k) v is made token by token, beyond by a plan on the tensor cores. Token by token / by a plan, us, of one adapter and of 16: 64 tokens, 96
 # numbers, k 4,096 7.6 / 8.4 and 7.6 / 15.8; 48 numbers, k 12,288 8.6 / 10.2 and 10.7 / 19.6; 96 numbers, k 12,288 14.2 / 11.9 and 17.8 / 27.8.
 TOKEN_WISE = 48 << 20
-FEW_TOKENS = 32  # up to so many (in some cases half or twice so many), the products are the decode steps' tcgen05 kernel
+FEW_TOKENS = 32  # up to so many (in some cases twice so many), the products are the decode steps' tcgen05 kernel
 # That kernel makes v itself where the weight is at least OWN_WEIGHT MiB and the numbers (tokens x rank x parts) are few beside it (the square of the MiB over 128: 18 beside 48
 # MiB, 288 beside 192): it then fetches the weights while the kernels before it still run, and v is ready before they have come; in a launch ahead v comes sooner where it is much. In a launch ahead / its own work, us, behind a norm, rank
 # 16: 1 token of 4096 -> 6144 17.1 / 15.7, gated 2048 -> 2 x 6144 16.0 / 13.5, 4096 -> 2 x 12288 39.2 / 35.6 and 8 of eight adapters 41.2 / 38.1; but 8 of 12288 -> 4096 22.4 / 24.9, 8 of 4096 -> 6144 18.2 / 20.6, of 2048 -> 2 x
@@ -226,14 +226,15 @@ def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: 
     """The way of a bfloat16 product with adapters. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
     takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it, the terms added behind.
 
-    Up to 32 tokens decode (16 where the row tiles of gate and up are more than the SMs: 32 tokens of 4096 -> 2 x 12288 54 / 48 apart, of 16 adapters 65 / 55); up to 64 too where it is not
-    gated and k is 4,096 or more, or no fewer than the outputs. decode / apart, us, one adapter of rank 16: 32 tokens of 4096 -> 6144 16.3 / 22.3, of 2048 -> 4096 10.0 / 12.9, of 12288 ->
-    4096 22.7 / 34.3, gated 2048 -> 2 x 6144 19.2 / 23.6; 64 tokens of 4096 -> 4096 18.0 / 18.8 (rank 64: 23.6 / 28.1), of 12288 -> 4096 29.0 / 34.4, of 2048 -> 4096 16.1 / 14.2.
+    Up to 32 tokens decode; up to 64 too where it is not gated and k is 4,096 or more, or no fewer than the outputs, and where it is gated, its row tiles more than the SMs and the rank no
+    more than 32. decode / apart, us, one adapter of rank 16: 32 tokens of 4096 -> 6144 16.3 / 22.3, of 2048 -> 4096 10.0 / 12.9, of 12288 -> 4096 22.7 / 34.3, gated 2048 -> 2 x 6144 19.2 /
+    23.6, 4096 -> 2 x 12288 43.5 / 48.4; 64 tokens of 4096 -> 4096 16.3 / 18.7 (rank 64: 20.0 / 28.4), of 12288 -> 4096 29.9 / 34.6, of 1024 -> 4096 13.8 / 12.9; gated 4096 -> 2 x 12288 51.7
+    / 57.8, pair 55.2 (rank 64: 59.1 / 75.5 / 55.2).
 
     Beyond, by what both take (us, fitted to a B200): a round of tiles of 256 x 256 on pairs of SMs goes with k; apart is the weights or the operations, three launches, and the outputs
     read and written again. pair / apart: 4096 -> 4096 at 64 tokens 27 / 19, at 512 28 / 33 (rank 64: 29 / 48); 4096 -> 6144 at 200 28 / 33; 12288 -> 4096 at 200 66 / 50, at 700 68 / 79;
     1024 -> 4096 at 64 11 / 13, at 1,100 19 / 36; gated 4096 -> 2 x 12288 at 64 55 / 58, at 200 56 / 90. (Over a hundred such cases the rule's way takes 0.7 % longer than the best one's.)"""
-    if tokens <= (FEW_TOKENS // 2 if gated and outputs > 64 * sms else FEW_TOKENS) or (tokens <= 2 * FEW_TOKENS and not gated and (inputs >= 4096 or outputs <= inputs)):
+    if tokens <= FEW_TOKENS or (tokens <= 2 * FEW_TOKENS and (outputs > 64 * sms and rank <= 32 if gated else inputs >= 4096 or outputs <= inputs)):
         return "decode"
     tiles, rows = -(-tokens // TILE) * -(-outputs // (128 if gated else 256)), outputs * (2 if gated else 1)
     apart = max(2.4 * inputs * rows / 6.3e6, 2 * tokens * inputs * rows / 1.2e9) + 10 + (2 + 0.2 * rank) * 1e-6 * tokens * rows

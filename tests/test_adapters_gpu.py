@@ -51,6 +51,7 @@ def test_linear_of_whole_prompts(rows, k, parts, rank):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,k,inter,rank,parts", [
+    (DECODE64[:25], 256, 9728, 24, 2), (DECODE64[:60], 128, 9500, 8, 2),
     (ONE, 1024, 512, 16, 2), (EIGHT, 1024, 264, 16, 2), (EIGHT, 4096, 1024, 64, 2), (EIGHT, 2048, 96, 8, 1), (DECODE64[:17], 512, 1024, 16, 2), (DECODE64, 1024, 1000, 32, 2),
     (MIXED, 512, 136, 16, 2), (PROMPTS, 256, 1024, 24, 2)])
 def test_silu_mul(dtype, rows, k, inter, rank, parts):
