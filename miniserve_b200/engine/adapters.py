@@ -76,6 +76,7 @@ class AdapterStore:
             raise ValueError(f"adapter {name!r} has a factor that is not finite")
         pairs = self._pairs(name, tensors)
         slot = free[0]
+        self._settle()  # (a step in flight may still read what the place held)
         for low in self.products.values():
             low.scale[slot] = 0.0
         used: dict[int, tuple] = {}
@@ -90,8 +91,14 @@ class AdapterStore:
             low.b[slot, first:behind, :r] = b.to(low.b.dtype)
         for low, r in used.values():
             low.scale[slot] = factor if factor is not None else (1.0 if alpha is None else float(alpha) / r)
+        self._settle()  # (steps may run on another stream)
         self.names[name] = slot
         return slot
+
+    def _settle(self) -> None:
+        device = next(iter(self.products.values())).a.device
+        if device.type == "cuda":
+            torch.cuda.synchronize(device)
 
     def unload(self, name: str) -> None:
         """Free the adapter's slot (no request that still runs may have it: the engine sees to that)."""
