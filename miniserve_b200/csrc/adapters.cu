@@ -215,7 +215,7 @@ adapter_expand_mma_kernel(O* out, const float* y, const float* v, const Adapters
       n[i] = GATED && r >= ROWS ? cols + n0 + r - ROWS : n0 + r;
     }
     warp_terms(ad, v + (size_t)t0 * ad.parts * ad.rank, tokens, M, warp >> 2, EXPAND_SETS, n, has, [] {},
-               [&](int tok, int i, float x) { sums[tok][quad * 32 + (lane >> 2) + 8 * i] += x; });
+               [&](int tok, int i) { return &sums[tok][quad * 32 + (lane >> 2) + 8 * i]; });
     __syncthreads();
     constexpr int SIDE = EXPAND_THREADS / ROWS;  // tokens side by side
     const int col = e & (ROWS - 1);

@@ -132,10 +132,13 @@ __device__ __forceinline__ int adapter_slot(const Adapters& ad, int t) {
   const int s = adapter_of(ad, t);
   return s < 0 ? NO_SLOT : s;
 }
-// Tokens in the order of their slots, and where runs of up to eight of one slot begin.
+// Tokens in the order of their slots, and the groups: runs of up to eight of one slot.
 template <int MOST>
 struct TokenGroups {
-  int slot[MOST], order[MOST], at[MOST], count;
+  int slot[MOST];
+  int2 token[MOST];  // in order: the token, its slot
+  int2 group[MOST];  // where the group begins among them, its slot
+  int count;
   bool begins[MOST];
 };
 // From g.slot [M], written by the calling threads (e = 0 .., at least M of them); sync: their barrier.
@@ -149,7 +152,7 @@ __device__ __forceinline__ void group_tokens(TokenGroups<MOST>& g, int M, int e,
       before += g.slot[j] < s;
       same += g.slot[j] == s && j < e;
     }
-    g.order[before + same] = e;
+    g.token[before + same] = make_int2(e, s);
     g.begins[before + same] = s != NO_SLOT && same % 8 == 0;
   }
   sync();
@@ -159,89 +162,115 @@ __device__ __forceinline__ void group_tokens(TokenGroups<MOST>& g, int M, int e,
       at += j < e && g.begins[j];
       all += g.begins[j];
     }
-    if (g.begins[e]) g.at[at] = e;
+    if (g.begins[e]) g.group[at] = make_int2(e, g.token[e].y);
     if (e == 0) g.count = all;
   }
   sync();
 }
-// A warp's 32 rows of B (n[i] is this lane's row 8 i + lane / 4 of them, has[i] whether there is one) times the tokens of the groups first, first + step, ..: add(token,
-// i, term) for the lane's rows. An instruction is 16 rows and the eight tokens of a group; a group and 32 of the rank's numbers are an item, the next one's asked for ahead of
-// this one's instructions. ready: called before the first of v is read. v: float32 [.., parts * rank], by the tokens of g.
-template <int MOST, typename Ready, typename Add>
+// A warp's 32 rows of B (n[i] is this lane's row 8 i + lane / 4 of them, has[i] whether there is one) times the tokens of the groups first, first + step, ..: the terms are
+// added to *cell(token, i) for the lane's rows. An instruction is 16 rows and the eight tokens of a group; a group and 32 of the rank's numbers are an item, the next one's asked
+// for ahead of this one's instructions. ready: called before the first of v is read. v: float32 [.., parts * rank], by the tokens of g. One warp a scheduler has nothing to hide its
+// trips to shared memory behind, so an item makes few: its tokens, then all of its cells at once.
+template <int MOST, typename Ready, typename Cell>
 __device__ __forceinline__ void warp_terms(const Adapters& ad, const float* v, const TokenGroups<MOST>& g, int M, int first, int step, const int (&n)[4], const bool (&has)[4],
-                                           Ready ready, Add add) {
+                                           Ready ready, Cell cell) {
   const int lane = threadIdx.x & 31, col = lane >> 2, t4 = lane & 3, numbers = ad.parts * ad.rank, rows = ad.ends[MAX_PARTS - 1];
-  int low = MAX_PARTS, high = -1;  // the parts that the rows belong to: one, but where two meet
+  int part[4], low = MAX_PARTS, high = -1;  // the parts that the rows belong to: one, but where two meet
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    part[i] = has[i] ? part_of(ad, n[i]) : -1;
     if (has[i]) {
-      low = min(low, part_of(ad, n[i]));
-      high = max(high, part_of(ad, n[i]));
+      low = min(low, part[i]);
+      high = max(high, part[i]);
     }
+  }
   low = __reduce_min_sync(0xffffffffu, low);
   high = __reduce_max_sync(0xffffffffu, high);
-  const int chunks = (ad.rank + 31) / 32, items = g.count > first ? (g.count - first + step - 1) / step * chunks : 0;
-  if (items == 0) return;
+  struct Item {
+    int at, slot, c0;  // the group's first token in order, its slot, the first of 32 numbers of the rank
+    uint32_t b[2][2][4];
+    float2 v[2][2];
+  };
+  const __nv_bfloat16* b_all = reinterpret_cast<const __nv_bfloat16*>(ad.b);
   for (int p = low; p <= high; ++p) {
-    uint32_t b_regs[2][2][2][4];
-    float2 v_regs[2][2][2];
-    auto load_b = [&](int item, uint32_t (&br)[2][2][4]) {
-      const int c0 = (item % chunks) * 32, s = g.slot[g.order[g.at[first + step * (item / chunks)]]];
-      const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(ad.b) + (size_t)s * rows * ad.rank;
+    int next = first, c_next = 0;  // the group and the numbers that are asked for next
+    auto load_b = [&](Item& it) {
+      const int2 where = g.group[next];
+      it.at = where.x;
+      it.slot = where.y;
+      it.c0 = c_next;
+      c_next += 32;
+      if (c_next >= ad.rank) {
+        c_next = 0;
+        next += step;
+      }
+      const __nv_bfloat16* b = b_all + (size_t)it.slot * rows * ad.rank + it.c0 + 2 * t4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            it.b[k][i >> 1][2 * h + (i & 1)] = part[i] == p && it.c0 + 16 * k + 8 * h < ad.rank ? row[8 * k + 4 * h] : 0u;  // (the rank is a multiple of 8)
+      }
+    };
+    auto load_v = [&](Item& it) {
+      const int2 who = it.at + col < M ? g.token[it.at + col] : make_int2(0, NO_SLOT);
+      const float2* row = reinterpret_cast<const float2*>(v + (size_t)who.x * numbers + p * ad.rank + it.c0 + 2 * t4);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = c0 + 16 * k + 8 * h + 2 * t4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            br[k][i >> 1][2 * h + (i & 1)] = c < ad.rank && has[i] && part_of(ad, n[i]) == p ? *reinterpret_cast<const uint32_t*>(b + (size_t)n[i] * ad.rank + c) : 0u;
-        }
+        for (int h = 0; h < 2; ++h) it.v[k][h] = who.y == it.slot && it.c0 + 16 * k + 8 * h < ad.rank ? __ldcg(row + 8 * k + 4 * h) : make_float2(0.f, 0.f);
     };
-    auto load_v = [&](int item, float2 (&vr)[2][2]) {
-      const int at = g.at[first + step * (item / chunks)], c0 = (item % chunks) * 32, s = g.slot[g.order[at]];
-      const int tok = at + col < M && g.slot[g.order[at + col]] == s ? g.order[at + col] : -1;
+    auto multiply = [&](const Item& it) {
+      int2 who[2];
+      float* to[2][4];
+      float sum[2][4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int q = 0; q < 2; ++q) who[q] = it.at + 2 * t4 + q < M ? g.token[it.at + 2 * t4 + q] : make_int2(0, NO_SLOT);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = c0 + 16 * k + 8 * h + 2 * t4;
-          vr[k][h] = c < ad.rank && tok >= 0 ? __ldcg(reinterpret_cast<const float2*>(v + (size_t)tok * numbers + p * ad.rank + c)) : make_float2(0.f, 0.f);
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          to[q][i] = cell(who[q].x, i);
+          sum[q][i] = *to[q][i];
         }
-    };
-    auto multiply = [&](int item, const uint32_t (&br)[2][2][4], const float2 (&vr)[2][2]) {
       float acc[2][4] = {};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(vr[k][0].x, vr[k][0].y), hi = __floats2bfloat162_rn(vr[k][1].x, vr[k][1].y);
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(it.v[k][0].x, it.v[k][0].y), hi = __floats2bfloat162_rn(it.v[k][1].x, it.v[k][1].y);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
-          mma_16816(acc[m], br[k][m][0], br[k][m][1], br[k][m][2], br[k][m][3], *reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+          mma_16816(acc[m], it.b[k][m][0], it.b[k][m][1], it.b[k][m][2], it.b[k][m][3], *reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
       }
-      const int at = g.at[first + step * (item / chunks)], s = g.slot[g.order[at]];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int pos = at + 2 * t4 + q;
-        if (pos >= M || g.slot[g.order[pos]] != s) continue;
+      for (int q = 0; q < 2; ++q)
+        if (who[q].y == it.slot) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) add(g.order[pos], i, acc[i >> 1][2 * (i & 1) + q]);
-      }
+          for (int i = 0; i < 4; ++i) *to[q][i] = sum[q][i] + acc[i >> 1][2 * (i & 1) + q];
+        }
     };
-    load_b(0, b_regs[0]);
+    if (next >= g.count) return;
+    Item a, b;
+    load_b(a);
     if (p == low) ready();
-    load_v(0, v_regs[0]);
-    for (int item = 0; item < items; item += 2) {
-      if (item + 1 < items) {
-        load_b(item + 1, b_regs[1]);
-        load_v(item + 1, v_regs[1]);
+    load_v(a);
+    for (;;) {
+      const bool more = next < g.count;
+      if (more) {
+        load_b(b);
+        load_v(b);
       }
-      multiply(item, b_regs[0], v_regs[0]);
-      if (item + 1 >= items) break;
-      if (item + 2 < items) {
-        load_b(item + 2, b_regs[0]);
-        load_v(item + 2, v_regs[0]);
+      multiply(a);
+      if (!more) break;
+      const bool again = next < g.count;
+      if (again) {
+        load_b(a);
+        load_v(a);
       }
-      multiply(item + 1, b_regs[1], v_regs[1]);
+      multiply(b);
+      if (!again) break;
     }
   }
 }

@@ -886,7 +886,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         if (term.tickets == nullptr) pdl_wait();
         if (term.tickets != nullptr && !__all_sync(0xffffffffu, tickets_reach(term.tickets + 1, units)) && lane == 0) atomicExch(status, 19);
       };
-      warp_terms(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i, float x) { part[tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i] += x; });
+      warp_terms(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i) { return part + tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i; });
       if (term.tickets == nullptr) pdl_wait();
       __syncwarp();
     }
