@@ -8,7 +8,9 @@
 // activations from shared memory, and the warps' partial sums are added in shared memory in a
 // fixed order.
 // Stands where the reference's decode step calls F.linear (miniserve/model/qwen3.py:115-131,186).
-#include "common.cuh"
+#include <type_traits>
+
+#include "adapters.cuh"
 
 namespace ms {
 
@@ -37,6 +39,7 @@ __device__ __forceinline__ uint4 ldg_stream(const void* p) {
 // g sigmoid(alpha g) (u + shift) with g capped at limit and u held within +-limit (a negative limit: neither).
 // Several inputs: rows [i * x_rows, (i + 1) * x_rows) of W (a multiple of a CTA's rows) multiply the input at X + i * x_stride (the last input
 // takes all rows behind). MODE 5: out columns from tanh_from on become tanh of the product.
+struct NoTerms {};
 struct SkinnyExtras {
   int x_rows;            // 0: one input
   long long x_stride;
@@ -49,10 +52,12 @@ struct SkinnyExtras {
 // stated gave 86 and 94 (a replayed step at Qwen3-0.6B sizes, us, none / one: 4 requests of 2,048 keys 1,007 / 997, one of 8,192 1,168 / 1,162, one of
 // 2,048 900 / 897, 16 of 300 991 / 992). The step with two / three CTAs of the gated forms: 8 requests of 2,048 keys 1,159 / 1,102, 16 of 300 1,054 / 992,
 // one of 300 854 / 802.
-template <int MT, int MODE>
+// ADAPTED (MODE 0 and 3): beside the product the terms of the tokens' low-rank adapters, sum_j B_s[n, j] v[t, j], in float32, a thread an output, and one rounding behind both. v is the
+// kernel's before this one, which has waited for all that ran before it by the time this one starts: only v is waited for.
+template <int MT, int MODE, bool ADAPTED = false>
 __global__ void __launch_bounds__(SK_THREADS, MODE == 3 || MODE == 6 ? 3 : 1)
 gemm_skinny_kernel(void* __restrict__ out, const __nv_bfloat16* __restrict__ X, const __nv_bfloat16* __restrict__ W,
-                   int M, int N, int K, const SkinnyExtras ex) {
+                   int M, int N, int K, const SkinnyExtras ex, const std::conditional_t<ADAPTED, AdapterTerms, NoTerms> term) {
   constexpr bool GATED = MODE == 3 || MODE == 6;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -91,7 +96,18 @@ gemm_skinny_kernel(void* __restrict__ out, const __nv_bfloat16* __restrict__ X, 
       if (row_b) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(wb_ptr + kk));
     }
   }
-  pdl_wait();
+  // ADAPTED: this thread's output, its row of B and its adapter
+  const int cell_row = tid & (SK_ROWS - 1), cell_tok = tid / SK_ROWS;
+  int cell_n = GATED && cell_row >= 8 ? N + n0 + cell_row - 8 : n0 + cell_row, slot = -1;
+  if constexpr (ADAPTED) {
+    if (cell_tok < M && (GATED ? n0 + (cell_row & 7) < N : cell_n < N)) slot = adapter_of(term.ad, cell_tok);
+    if (slot >= 0) {
+      const int rows = term.ad.ends[MAX_PARTS - 1];
+      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(reinterpret_cast<const __nv_bfloat16*>(term.ad.b) + ((size_t)slot * rows + cell_n) * term.ad.rank));
+    }
+  } else {
+    pdl_wait();
+  }
 
   // activations of this K slice: [MT * 8][k_len], rows past M are zero
   const int chunks = k_len >> 3;
@@ -143,17 +159,44 @@ gemm_skinny_kernel(void* __restrict__ out, const __nv_bfloat16* __restrict__ X, 
     base[(g + 8) * TOK + 8 * j + 2 * t + 1] = acc[j][3];
   }
   __syncthreads();
+  constexpr int SUMS = ADAPTED ? 1 : SK_WARPS;  // what is left to add up
+  if constexpr (ADAPTED) {
+    pdl_wait();
+    if (tid < SK_ROWS * TOK) {
+      float* cell = red + cell_row * TOK + cell_tok;
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < SK_WARPS; ++w) s += cell[(size_t)w * SK_ROWS * TOK];
+      if (slot >= 0) {
+        const Adapters& ad = term.ad;
+        const uint4* b = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(ad.b) + ((size_t)slot * ad.ends[MAX_PARTS - 1] + cell_n) * ad.rank);
+        const float4* v = reinterpret_cast<const float4*>(term.v + ((size_t)cell_tok * ad.parts + part_of(ad, cell_n)) * ad.rank);
+        float terms = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < ad.rank / 8; ++c) {
+          float f[8];
+          bf16x8_to_float(b[c], f);
+          const float4 lo = __ldcg(v + 2 * c), hi = __ldcg(v + 2 * c + 1);
+          terms = fmaf(f[0], lo.x, fmaf(f[1], lo.y, fmaf(f[2], lo.z, fmaf(f[3], lo.w, terms))));
+          terms = fmaf(f[4], hi.x, fmaf(f[5], hi.y, fmaf(f[6], hi.z, fmaf(f[7], hi.w, terms))));
+        }
+        s += terms;
+      }
+      *cell = s;
+    }
+    __syncthreads();
+  }
   if (GATED) {
     for (int idx = tid; idx < 8 * TOK; idx += SK_THREADS) {
       const int tok = idx >> 3, row = idx & 7;
       if (tok >= M || n0 + row >= N) continue;
       float sg = 0.f, su = 0.f;
 #pragma unroll
-      for (int w = 0; w < SK_WARPS; ++w) {
+      for (int w = 0; w < SUMS; ++w) {
         sg += red[(size_t)w * SK_ROWS * TOK + row * TOK + tok];
         su += red[(size_t)w * SK_ROWS * TOK + (row + 8) * TOK + tok];
       }
-      float gt = __bfloat162float(__float2bfloat16_rn(sg)), up = __bfloat162float(__float2bfloat16_rn(su));
+      float gt = ADAPTED ? sg : __bfloat162float(__float2bfloat16_rn(sg)), up = ADAPTED ? su : __bfloat162float(__float2bfloat16_rn(su));
       if (MODE == 6) {
         if (ex.limit >= 0.f) {
           gt = fminf(gt, ex.limit);
@@ -170,7 +213,7 @@ gemm_skinny_kernel(void* __restrict__ out, const __nv_bfloat16* __restrict__ X, 
     if (tok >= M || n0 + row >= N) continue;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < SK_WARPS; ++w) s += red[(size_t)w * SK_ROWS * TOK + row * TOK + tok];
+    for (int w = 0; w < SUMS; ++w) s += red[(size_t)w * SK_ROWS * TOK + row * TOK + tok];
     const size_t o = (size_t)tok * N + n0 + row;
     if (MODE == 0) {
       reinterpret_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(s);
@@ -337,20 +380,21 @@ static int launch_skinny_stream(void* out, const void* X, const void* W, int M, 
   return 0;
 }
 
-template <int MT, int MODE>
-static int launch_skinny(void* out, const void* X, const void* W, int M, int N, int K, cudaStream_t stream, const SkinnyExtras& ex = SkinnyExtras{}) {
+template <int MT, int MODE, bool ADAPTED = false>
+static int launch_skinny(void* out, const void* X, const void* W, int M, int N, int K, cudaStream_t stream, const SkinnyExtras& ex = SkinnyExtras{},
+                         const std::conditional_t<ADAPTED, AdapterTerms, NoTerms>& term = {}) {
   const size_t smem_x = (size_t)MT * 8 * (K + 32) * 2;
   const size_t smem_red = (size_t)SK_WARPS * SK_ROWS * MT * 8 * 4;
   const size_t smem = smem_x > smem_red ? smem_x : smem_red;
   MS_CHECK_ARG(smem <= 200 * 1024, "gemm_skinny: K=%d needs %zu bytes of shared memory", K, smem);
-  auto kernel = gemm_skinny_kernel<MT, MODE>;
+  auto kernel = gemm_skinny_kernel<MT, MODE, ADAPTED>;
   static size_t configured = 0;
   if (smem > 48 * 1024 && smem > configured) {
     MS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured = smem;
   }
   dim3 grid(ceil_div(N, MODE == 3 || MODE == 6 ? 8 : SK_ROWS));
-  MS_LAUNCH(kernel, grid, SK_THREADS, smem, stream, out, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W, M, N, K, ex);
+  MS_LAUNCH(kernel, grid, SK_THREADS, smem, stream, out, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W, M, N, K, ex, term);
   return 0;
 }
 
@@ -438,4 +482,14 @@ MS_EXPORT int ms_gemm_skinny_inputs_bf16(void* out, const void* X, const void* W
                "gemm_skinny: %d inputs of %d rows each of %d", inputs, rows_each, N);
   const SkinnyExtras ex{rows_each, (long long)M * K, inputs - 1, tanh_from, 0.f, 0.f, 0.f};
   return M > 8 ? launch_skinny<2, 5>(out, X, W, M, N, K, stream, ex) : launch_skinny<1, 5>(out, X, W, M, N, K, stream, ex);
+}
+
+// out [M, N] bfloat16 = X W^T, or (gated) silu(X Wg^T) * (X Wu^T), with low-rank adapters beside the product (adapters.cuh); the launch before is the one that makes term->v.
+MS_EXPORT int ms_gemm_skinny_adapted_bf16(void* out, const void* X, const void* W, int M, int N, int K, int gated, const AdapterTerms* term, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  if (int rc = check_skinny(W, M, N, K, 0)) return rc;
+  MS_CHECK_ARG((uintptr_t)X % 16 == 0, "gemm_skinny: the activations must be 16-byte aligned");
+  MS_CHECK_ARG(term != nullptr && term->v != nullptr && (uintptr_t)term->v % 16 == 0 && adapters_ok(term->ad, gated ? 2 * N : N, K), "gemm_skinny: an adapted product needs its adapters' numbers");
+  if (gated) return M > 8 ? launch_skinny<2, 3, true>(out, X, W, M, N, K, stream, {}, *term) : launch_skinny<1, 3, true>(out, X, W, M, N, K, stream, {}, *term);
+  return M > 8 ? launch_skinny<2, 0, true>(out, X, W, M, N, K, stream, {}, *term) : launch_skinny<1, 0, true>(out, X, W, M, N, K, stream, {}, *term);
 }

@@ -179,7 +179,7 @@ def _code(dtype: torch.dtype) -> int:
     return 0 if dtype is torch.float32 else 1
 
 
-WAY: str | None = None  # tests and measurements: "decode", "pair" or "apart" instead of the rules'
+WAY: str | None = None  # tests and measurements: "stream", "decode", "pair" or "apart" instead of the rules'
 # Up to so many products (tokens x numbers x k) v is made token by token, beyond by a plan on the tensor cores. Token by token / by a plan, us, of one adapter and of 16: 64 tokens, 96
 # numbers, k 4,096 7.6 / 8.4 and 7.6 / 15.8; 48 numbers, k 12,288 8.6 / 10.2 and 10.7 / 19.6; 96 numbers, k 12,288 14.2 / 11.9 and 17.8 / 27.8.
 TOKEN_WISE = 48 << 20
@@ -223,10 +223,14 @@ def product(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, stream: int) 
 
 
 def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: int) -> str:
-    """The way of a bfloat16 product with adapters. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
+    """The way of a bfloat16 product with adapters. "stream": the weight-streaming kernel of decode steps, a thread's terms behind an output's sum. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
     takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it, the terms added behind.
 
-    Up to 32 tokens decode; up to 64 too where it is not gated and k is 4,096 or more, or no fewer than the outputs, and where it is gated, its row tiles more than the SMs and the rank no
+    Up to 16 tokens stream, where k is at most 2,048, the weight at most 12 MiB and tokens times rank at most 256. decode / stream, us, behind a norm: 8 tokens of rank 16, 1024 -> 4096 8.9 / 6.9,
+    1 token 7.2 / 5.8, 16 10.4 / 8.5, 8 of rank 32 9.3 / 8.5, gated 1024 -> 2 x 3 Ki 10.7 / 8.0, 2048 -> 1024 7.9 / 7.1; but 16 of rank 32, 1024 -> 4096 11.2 / 11.4, 8 of rank 64 10.9 / 12.1, 8 of rank
+    32, 2048 -> 4096 9.6 / 10.2, 1 of 4096 -> 1024 8.5 / 9.3, 8 gated of 2048 -> 2 x 4096 13.2 / 15.7.
+
+    Else up to 32 tokens decode; up to 64 too where it is not gated and k is 4,096 or more, or no fewer than the outputs, and where it is gated, its row tiles more than the SMs and the rank no
     more than 32. decode / apart, us, one adapter of rank 16: 32 tokens of 4096 -> 6144 16.3 / 22.3, of 2048 -> 4096 10.0 / 12.9, of 12288 -> 4096 22.7 / 34.3, gated 2048 -> 2 x 6144 19.2 /
     23.6, 4096 -> 2 x 12288 43.5 / 48.4; 64 tokens of 4096 -> 4096 16.3 / 18.7 (rank 64: 20.0 / 28.4), of 12288 -> 4096 29.9 / 34.6, of 1024 -> 4096 13.8 / 12.9; gated 4096 -> 2 x 12288 51.7
     / 57.8, pair 55.2 (rank 64: 59.1 / 75.5 / 55.2).
@@ -234,9 +238,12 @@ def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: 
     Beyond, by what both take (us, fitted to a B200): a round of tiles of 256 x 256 on pairs of SMs goes with k; apart is the weights or the operations, three launches, and the outputs
     read and written again. pair / apart: 4096 -> 4096 at 64 tokens 27 / 19, at 512 28 / 33 (rank 64: 29 / 48); 4096 -> 6144 at 200 28 / 33; 12288 -> 4096 at 200 66 / 50, at 700 68 / 79;
     1024 -> 4096 at 64 11 / 13, at 1,100 19 / 36; gated 4096 -> 2 x 12288 at 64 55 / 58, at 200 56 / 90. (Over a hundred such cases the rule's way takes 0.7 % longer than the best one's.)"""
+    rows = outputs * (2 if gated else 1)
+    if tokens <= 16 and inputs <= 2048 and inputs * rows <= 6 << 20 and tokens * rank <= 256:
+        return "stream"
     if tokens <= FEW_TOKENS or (tokens <= 2 * FEW_TOKENS and (outputs > 64 * sms and rank <= 32 if gated else inputs >= 4096 or outputs <= inputs)):
         return "decode"
-    tiles, rows = -(-tokens // TILE) * -(-outputs // (128 if gated else 256)), outputs * (2 if gated else 1)
+    tiles = -(-tokens // TILE) * -(-outputs // (128 if gated else 256))
     apart = max(2.4 * inputs * rows / 6.3e6, 2 * tokens * inputs * rows / 1.2e9) + 10 + (2 + 0.2 * rank) * 1e-6 * tokens * rows
     return "pair" if 6 + -(-tiles // (sms // 2)) * inputs * 0.0048 <= apart else "apart"
 
@@ -247,6 +254,11 @@ def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gate
     if x.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and _ops().tc_gemm_enabled():
         lib = native.gemm_tc()
         way = WAY or way_of(t, n, k, low_rank.rank, gated, rows.sms)
+        if way == "stream":
+            v = _terms(x, low_rank, rows, ad, stream)
+            native.kernel_check(native.kernels().ms_gemm_skinny_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated),
+                                                                             b"".join((_Q(v.data_ptr()), ad, _Q(0))), stream))
+            return
         if way == "decode":
             if makes_its_own(t * low_rank.numbers, 2 * k * low_rank.outputs >> 20):
                 tickets = rows.tickets(stream)

@@ -104,6 +104,7 @@ def kernels():
     _declare(lib, "ms_gemm_skinny_relu2_bf16", [_p, _p, _p, _i, _i, _i, _p])
     _declare(lib, "ms_gemm_skinny_clamped_glu_bf16", [_p, _p, _p, _i, _i, _i, _f, _f, _f, _p])
     _declare(lib, "ms_gemm_skinny_inputs_bf16", [_p, _p, _p, _i, _i, _i, _i, _i, _i, _p])
+    _declare(lib, "ms_gemm_skinny_adapted_bf16", [_p, _p, _p, _i, _i, _i, _i, c_char_p, _p])
     _declare(lib, "ms_gemm_skinny_set_stream", [_i], None)
     _declare(lib, "ms_silu_mul", [_p, _p, _i, _i, _i, _p])
     _declare(lib, "ms_to_float", [_p, _p, _ll, _i, _p])

@@ -29,7 +29,7 @@ def run_linear(x, w, low, rows, out_dtype=None, stream=None):
 @pytest.mark.parametrize("rows,k,parts,rank", [
     (ONE, 1024, (256, 128, 128), 16), (ONE, 12288, (512,), 8), (ONE, 8, (3,), 8), (ONE, 2048, (1001,), 256),
     (EIGHT, 1024, (256, 128, 128), 16), (EIGHT, 4096, (1024,), 64), (EIGHT, 6144, (264, 8), 24), (EIGHT, 40, (37,), 8),
-    (DECODE64, 512, (384, 64, 64), 32), (DECODE64[:17], 2048, (512,), 16), (DECODE64[:33], 4104, (200, 72, 24, 8), 40),
+    (DECODE64[:16], 1000, (700, 40, 40), 16), (EIGHT, 2048, (72, 24, 8, 1), 32), (DECODE64[:9], 4096, (512,), 8), (DECODE64[:13], 2504, (96, 40), 24), (DECODE64, 512, (384, 64, 64), 32), (DECODE64[:17], 2048, (512,), 16), (DECODE64[:33], 4104, (200, 72, 24, 8), 40),
     (MIXED, 1024, (512, 256, 256), 16), (MIXED, 520, (100, 28), 136), (MIXED, 64, (77,), 8),
     (PROMPTS, 256, (256, 128, 128), 8), (PROMPTS, 1024, (640, 24), 72),
 ])
@@ -51,7 +51,7 @@ def test_linear_of_whole_prompts(rows, k, parts, rank):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,k,inter,rank,parts", [
-    (DECODE64[:25], 256, 9728, 24, 2), (DECODE64[:60], 128, 9500, 8, 2),
+    (DECODE64[:16], 1024, 1500, 16, 2), (EIGHT, 2048, 200, 32, 2), (DECODE64[:9], 72, 5, 24, 1), (DECODE64[:25], 256, 9728, 24, 2), (DECODE64[:60], 128, 9500, 8, 2),
     (ONE, 1024, 512, 16, 2), (EIGHT, 1024, 264, 16, 2), (EIGHT, 4096, 1024, 64, 2), (EIGHT, 2048, 96, 8, 1), (DECODE64[:17], 512, 1024, 16, 2), (DECODE64, 1024, 1000, 32, 2),
     (MIXED, 512, 136, 16, 2), (PROMPTS, 256, 1024, 24, 2)])
 def test_silu_mul(dtype, rows, k, inter, rank, parts):
