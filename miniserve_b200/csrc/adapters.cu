@@ -89,12 +89,20 @@ adapter_plan_kernel(int* __restrict__ tile_first, AdapterBlock* __restrict__ blo
 // v[t, j] = c_s sum_k A_s[j, k] x[t, k]. A block: one token, SHRINK_WARPS / split sets of EACH numbers; `split` warps share their k, the sums added in
 // order. The order of a sum follows from K alone, so a token's numbers do not depend on the step around it. Bound by the trips to memory of a block (where an adapter is, its
 // rows, the sum): 64 tokens of 96 numbers, k 4,096 take 7.6 us with four numbers a warp, 16.3 with one; 8 tokens of 16 numbers 2.7.
-constexpr int SHRINK_WARPS = 8;
+constexpr int SHRINK_WARPS = 8, AHEAD_CHUNK = 16384;  // (bytes that a thread asks for at a time)
 template <typename T, int EACH>
 __global__ void __launch_bounds__(SHRINK_WARPS * 32, EACH == 1 ? 3 : 4)
-adapter_shrink_kernel(float* v, const T* x, const Adapters ad, int K, int split) {
+adapter_shrink_kernel(float* v, const T* x, const Adapters ad, int tokens, int K, int split, const unsigned char* ahead, long long ahead_bytes) {
   constexpr int W = Wide<T>::N;
   __shared__ float sums[SHRINK_WARPS][EACH];
+  // Blocks beyond the tokens' ask the weight of the product behind into L2 while the kernels before this one still run.
+  if ((int)blockIdx.x >= tokens) {
+    const long long first = (long long)(blockIdx.x - tokens) * gridDim.y + blockIdx.y, step = (long long)(gridDim.x - tokens) * gridDim.y;
+    if (threadIdx.x == 0)
+      for (long long at = first * AHEAD_CHUNK; at < ahead_bytes; at += step * AHEAD_CHUNK)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(ahead + at), "r"((uint32_t)(ahead_bytes - at < AHEAD_CHUNK ? ahead_bytes - at : AHEAD_CHUNK)) : "memory");
+    return;
+  }
   // The wait comes first: a product behind may start on what earlier kernels have left, before this one has ended.
   pdl_wait(v, x);
   pdl_launch_dependents();
@@ -261,24 +269,28 @@ MS_EXPORT int ms_adapter_plan(int* tile_first, void* blocks, const Adapters* ad,
 }
 
 template <typename T>
-static int launch_shrink(float* v, const void* x, const Adapters& ad, int tokens, int K, int numbers, int split, cudaStream_t stream) {
+static int launch_shrink(float* v, const void* x, const Adapters& ad, int tokens, int K, int numbers, int split, const void* ahead, long long ahead_bytes, cudaStream_t stream) {
   // four numbers a warp, which then reads x once for them, where that leaves warps enough
   const int each = (long long)tokens * numbers * split > 3 * 8 * 148 ? 4 : 1;
-  const dim3 grid(tokens, ceil_div(numbers, SHRINK_WARPS / split * each));
-  if (each == 4) MS_LAUNCH((adapter_shrink_kernel<T, 4>), grid, SHRINK_WARPS * 32, 0, stream, v, (const T*)x, ad, K, split);
-  else MS_LAUNCH((adapter_shrink_kernel<T, 1>), grid, SHRINK_WARPS * 32, 0, stream, v, (const T*)x, ad, K, split);
+  const int chunks = (int)((ahead_bytes + AHEAD_CHUNK - 1) / AHEAD_CHUNK), rows = ceil_div(numbers, SHRINK_WARPS / split * each);
+  const dim3 grid(tokens + ceil_div(chunks < 148 ? chunks : 148, rows), rows);
+  if (each == 4) MS_LAUNCH((adapter_shrink_kernel<T, 4>), grid, SHRINK_WARPS * 32, 0, stream, v, (const T*)x, ad, tokens, K, split, (const unsigned char*)ahead, ahead_bytes);
+  else MS_LAUNCH((adapter_shrink_kernel<T, 1>), grid, SHRINK_WARPS * 32, 0, stream, v, (const T*)x, ad, tokens, K, split, (const unsigned char*)ahead, ahead_bytes);
   return 0;
 }
 
 // v float32 [T, parts * rank]; rows of tokens without an adapter are left as they were.
-MS_EXPORT int ms_adapter_shrink(float* v, const void* x, const Adapters* ad, int T, int N, int K, int dtype, cudaStream_t stream) {
+// ahead: ahead_bytes (a multiple of 16; 0: none) that the launch behind will read and that no kernel that may still run writes.
+MS_EXPORT int ms_adapter_shrink(float* v, const void* x, const Adapters* ad, int T, int N, int K, int dtype, const void* ahead, long long ahead_bytes, cudaStream_t stream) {
   if (int rc = check_adapters(ad, T, N, K)) return rc;
-  MS_CHECK_ARG((uintptr_t)x % 16 == 0, "adapters: x must be 16-byte aligned");
+  MS_CHECK_ARG((uintptr_t)x % 16 == 0 && (uintptr_t)ahead % 16 == 0, "adapters: x and the weight must be 16-byte aligned");
+  MS_CHECK_ARG(ahead_bytes >= 0 && ahead_bytes % 16 == 0 && (ahead != nullptr || ahead_bytes == 0), "adapters: bad bytes ahead: %lld", ahead_bytes);
   if (T == 0) return 0;
   const int numbers = ad->parts * ad->rank;
   int split = 1;
   while (split < SHRINK_WARPS && K > 2048 * split) split *= 2;
-  return dtype == MS_F32 ? launch_shrink<float>(v, x, *ad, T, K, numbers, split, stream) : launch_shrink<__nv_bfloat16>(v, x, *ad, T, K, numbers, split, stream);
+  return dtype == MS_F32 ? launch_shrink<float>(v, x, *ad, T, K, numbers, split, ahead, ahead_bytes, stream)
+                         : launch_shrink<__nv_bfloat16>(v, x, *ad, T, K, numbers, split, ahead, ahead_bytes, stream);
 }
 
 static int launch_expand(float* out, const float* y, const float* v, const Adapters* ad, int T_all, int N, int gated, cudaStream_t stream) {

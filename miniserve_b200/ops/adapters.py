@@ -8,7 +8,7 @@ import ctypes
 import struct
 import sys
 from contextlib import nullcontext
-from ctypes import c_char_p, c_int, c_ulonglong, c_void_p
+from ctypes import c_char_p, c_int, c_longlong, c_ulonglong, c_void_p
 from dataclasses import dataclass
 from functools import lru_cache
 
@@ -133,7 +133,7 @@ def _lib():
     native._declare(lib, "ms_adapters_set_pdl", [_i], None)
     native._declare(lib, "ms_adapter_capture_id", [_p], c_ulonglong)
     native._declare(lib, "ms_adapter_plan", [_p] * 2 + [c_char_p, _i, _i, _p])
-    native._declare(lib, "ms_adapter_shrink", [_p, _p, c_char_p, _i, _i, _i, _i, _p])
+    native._declare(lib, "ms_adapter_shrink", [_p, _p, c_char_p, _i, _i, _i, _i, _p, c_longlong, _p])
     native._declare(lib, "ms_adapter_expand", [_p, _p, _p, c_char_p] + [_i] * 6 + [_p])
     lib.ms_adapters_set_pdl(int(native.pdl_enabled()))
     return lib
@@ -183,6 +183,9 @@ WAY: str | None = None  # tests and measurements: "stream", "decode", "pair" or 
 # Up to so many products (tokens x numbers x k) v is made token by token, beyond by a plan on the tensor cores. Token by token / by a plan, us, of one adapter and of 16: 64 tokens, 96
 # numbers, k 4,096 7.6 / 8.4 and 7.6 / 15.8; 48 numbers, k 12,288 8.6 / 10.2 and 10.7 / 19.6; 96 numbers, k 12,288 14.2 / 11.9 and 17.8 / 27.8.
 TOKEN_WISE = 48 << 20
+# A weight of up to so many bytes is asked into L2 by the launch that makes v, while the kernels before it still run. A decode step of 0.6b with adapters, ms, without / with: 1 request 1.157 /
+# 1.128, 8 on eight adapters 1.338 / 1.291; a product behind a short kernel loses 0.1 to 0.2 us. Beside larger weights it loses (12288 -> 4096 22.3 / 28.5 us: the product asks for them itself).
+AHEAD = 16 << 20
 FEW_TOKENS = 32  # up to so many (in some cases twice so many), the products are the decode steps' tcgen05 kernel
 # That kernel makes v itself where the weight is at least OWN_WEIGHT MiB and the numbers (tokens x rank x parts) are few beside it (the square of the MiB over 128: 18 beside 48
 # MiB, 288 beside 192): it then fetches the weights while the kernels before it still run, and v is ready before they have come; in a launch ahead v comes sooner where it is much. In a launch ahead / its own work, us, behind a norm, rank
@@ -195,13 +198,15 @@ def makes_its_own(numbers: int, weight: int) -> bool:
     return weight >= OWN_WEIGHT and 128 * numbers <= weight * weight
 
 
-def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, stream: int) -> torch.Tensor:
-    """What the adapters' A make of x, float32 [T, parts * rank]."""
+def _terms(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, ad: bytes, stream: int, weight: torch.Tensor | None = None) -> torch.Tensor:
+    """What the adapters' A make of x, float32 [T, parts * rank]. ``weight``: the one of the product behind, which the launch may ask into L2."""
     t, k = x.shape
+    size = 2 * k * low_rank.outputs
+    ahead = size if weight is not None and size <= AHEAD else 0
     with on_stream(stream, x.device):
         v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=x.device)
     if t * low_rank.numbers * k <= TOKEN_WISE or x.dtype is torch.float32 or not _ops().tc_gemm_enabled():
-        _check(_lib().ms_adapter_shrink(v.data_ptr(), x.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), stream))
+        _check(_lib().ms_adapter_shrink(v.data_ptr(), x.data_ptr(), ad, t, low_rank.outputs, k, _code(x.dtype), weight.data_ptr() if ahead else None, ahead, stream))
     else:
         _by_plan(v, x, rows.plan(low_rank.slots, stream), ad, rows, True, stream)
     return v
@@ -255,7 +260,7 @@ def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gate
         lib = native.gemm_tc()
         way = WAY or way_of(t, n, k, low_rank.rank, gated, rows.sms)
         if way == "stream":
-            v = _terms(x, low_rank, rows, ad, stream)
+            v = _terms(x, low_rank, rows, ad, stream, weight)
             native.kernel_check(native.kernels().ms_gemm_skinny_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated),
                                                                              b"".join((_Q(v.data_ptr()), ad, _Q(0))), stream))
             return
@@ -265,7 +270,7 @@ def _run(x, weight, out, stream: int, low_rank: LowRank, rows: AdapterRows, gate
                 with on_stream(stream, device):
                     v = torch.empty((t, low_rank.numbers), dtype=torch.float32, device=device)
             else:
-                v, tickets = _terms(x, low_rank, rows, ad, stream), 0
+                v, tickets = _terms(x, low_rank, rows, ad, stream, weight), 0
             term = b"".join((_Q(v.data_ptr()), ad, _Q(tickets)))
             rc = lib.ms_gemm_tc_decode_adapted_bf16(out.data_ptr(), x.data_ptr(), weight.data_ptr(), t, n, k, int(gated), term, rows.status, stream)
             native.kernel_check(rc, lib=lib, errfn="ms_gemm_tc_last_error")
