@@ -730,11 +730,12 @@ __device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %
 // and a second counter says when all are done. What is taken is being worked on by a warp that runs, so the wait for the rest ends whether or not all CTAs are on
 // the GPU at once. That leaves one launch, and x's part of the product does not wait for v.
 // GATED: W is [2 N, K], gate rows, then up rows; a tile is 64 of each, out = silu(gate) * up.
-// Two CTAs an SM where their rings fit: a tile more than there are SMs does not wait for a whole one, and a narrow output's k is cut into more slices.
+// ADAPTED: two CTAs an SM. The terms are work of the SM's other units, k is cut into more slices that share them out, and a tile more than there are SMs does not wait for a whole
+// one. One / two, us: 32 tokens of one adapter, 4096 -> 6144 16.5 / 14.9, of 16 adapters 19.0 / 16.1, gated 2048 -> 2 x 6144 26.5 / 20.0, 1024 -> 2 x 3 Ki 14.1 / 11.1; 64 of 16 adapters of rank
+// 32, 4096 -> 6144 33.7 / 24.9; but 16 adapters of rank 64, 1024 -> 4096 15.3 / 17.3.
 constexpr size_t decode_smem(int bt, int stages) { return (size_t)stages * (TC_BM + bt) * TC_BK * 2 + (size_t)bt * TC_BM * 4 + 1024; }
-constexpr bool decode_twice(int bt, int stages, bool adapted) { return adapted && 2 * (decode_smem(bt, stages) + 1024) <= 227 * 1024; }
 template <int BT, int STAGES, bool ADAPTED = false, bool GATED = false>
-__global__ void __launch_bounds__(TC_THREADS, decode_twice(BT, STAGES, ADAPTED) ? 2 : 1)
+__global__ void __launch_bounds__(TC_THREADS, ADAPTED ? 2 : 1)
 gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                       __nv_bfloat16* __restrict__ out, int M, int N, int K, int slices, int iters_per_slice,
                       int* __restrict__ status, const std::conditional_t<ADAPTED, AdapterTerms, NoAdapters> term, const __nv_bfloat16* x) {
@@ -1861,7 +1862,7 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
   if (int rc = make_map(&map_w, W, GATED ? 2LL * N : N, K, GATED ? TC_BM / 2 : TC_BM)) return rc;
   if (int rc = make_map(&map_x, X, M, K, BT)) return rc;
   constexpr size_t smem = decode_smem(BT, STAGES);
-  static_assert(smem + 1024 <= 227 * 1024, "the ring does not fit shared memory");
+  static_assert((ADAPTED ? 2 : 1) * (smem + 2048) <= 228 * 1024, "the ring does not fit shared memory");
   auto kernel = gemm_tc_decode_kernel<BT, STAGES, ADAPTED, GATED>;
   static std::atomic<unsigned long long> allowed{0};
   MS_CHECK_CUDA(allow_shared_memory((const void*)kernel, (int)smem, allowed));
@@ -1889,7 +1890,7 @@ static int launch_tc_decode(void* out, const void* X, const void* W, int M, int 
   const int tiles = ceil_div(N, GATED ? TC_BM / 2 : TC_BM), k_iters = ceil_div(K, TC_BK);
   int slices = 1;
   for (int size = 2; size <= 8 && size <= k_iters / 4; ++size)
-    if (fit[size] >= tiles) slices = size;
+    if ((ADAPTED ? 2 : 1) * fit[size] >= tiles) slices = size;  // (the query counts one CTA an SM for these kernels; two run)
   const int iters_per_slice = ceil_div(k_iters, slices);
   MS_LAUNCH_CLUSTERED(kernel, (unsigned)(tiles * slices), TC_THREADS, smem, stream, slices, map_w, map_x, (__nv_bfloat16*)out, M, N, K, slices,
                       iters_per_slice, status, term, (const __nv_bfloat16*)X);
@@ -2136,10 +2137,7 @@ MS_EXPORT int ms_gemm_tc_decode_adapted_bf16(void* out, const void* X, const voi
 #define MS_DECODE(BT, STAGES)                                                                                     \
   return gated ? launch_tc_decode<BT, STAGES, true, true>(out, X, W, M, N, K, status, stream, *term)              \
                : launch_tc_decode<BT, STAGES, true, false>(out, X, W, M, N, K, status, stream, *term)
-  // Up to 16 tokens and beyond 32 two CTAs an SM; in between where the tiles are more than the SMs. Two / one, us: 64 tokens of 16 adapters of rank 32, 4096 -> 6144 28.9 / 33.7,
-  // 64 of one of rank 16, 4096 -> 4096 16.3 / 18.0; 32, gated 4096 -> 2 x 12288 43.5 / 54.3; but 32 of 4096 -> 6144 19.0 / 16.3, of 12288 -> 4096 25.7 / 22.7.
   if (M <= 16) MS_DECODE(16, 5);
-  if (M <= 32 && ceil_div(N, gated ? TC_BM / 2 : TC_BM) <= sm_count()) MS_DECODE(32, 10);
   if (M <= 32) MS_DECODE(32, 4);
   MS_DECODE(64, 3);
 #undef MS_DECODE

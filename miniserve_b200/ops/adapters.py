@@ -231,22 +231,22 @@ def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: 
     """The way of a bfloat16 product with adapters. "stream": the weight-streaming kernel of decode steps, a thread's terms behind an output's sum. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
     takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it, the terms added behind.
 
-    Up to 16 tokens stream, where k is at most 2,048, the weight at most 12 MiB and tokens times rank at most 256. decode / stream, us, behind a norm: 8 tokens of rank 16, 1024 -> 4096 8.9 / 6.9,
-    1 token 7.2 / 5.8, 16 10.4 / 8.5, 8 of rank 32 9.3 / 8.5, gated 1024 -> 2 x 3 Ki 10.7 / 8.0, 2048 -> 1024 7.9 / 7.1; but 16 of rank 32, 1024 -> 4096 11.2 / 11.4, 8 of rank 64 10.9 / 12.1, 8 of rank
-    32, 2048 -> 4096 9.6 / 10.2, 1 of 4096 -> 1024 8.5 / 9.3, 8 gated of 2048 -> 2 x 4096 13.2 / 15.7.
+    Up to 16 tokens stream, where k is at most 2,048, the weight at most 12 MiB and tokens times rank at most 256. decode / stream, us, behind a norm: 8 tokens of rank 16, 1024 -> 4096 9.1 / 6.9,
+    1 token 7.4 / 6.2, 16 10.4 / 8.4, 8 of rank 32 9.3 / 8.9, gated 1024 -> 2 x 3 Ki 9.6 / 7.7 (rank 32: 9.9 / 11.0), 2048 -> 1024 8.1 / 7.3; but 16 tokens of 2048 -> 4096 10.6 / 11.1, 8 of
+    rank 32 9.7 / 10.5, 4 of rank 64 9.8 / 10.8.
 
-    Else up to 32 tokens decode; up to 64 too where it is not gated and k is 4,096 or more, or no fewer than the outputs, and where it is gated, its row tiles more than the SMs and the rank no
-    more than 32. decode / apart, us, one adapter of rank 16: 32 tokens of 4096 -> 6144 16.3 / 22.3, of 2048 -> 4096 10.0 / 12.9, of 12288 -> 4096 22.7 / 34.3, gated 2048 -> 2 x 6144 19.2 /
-    23.6, 4096 -> 2 x 12288 43.5 / 48.4; 64 tokens of 4096 -> 4096 16.3 / 18.7 (rank 64: 20.0 / 28.4), of 12288 -> 4096 29.9 / 34.6, of 1024 -> 4096 13.8 / 12.9; gated 4096 -> 2 x 12288 51.7
-    / 57.8, pair 55.2 (rank 64: 59.1 / 75.5 / 55.2).
+    Else up to 32 tokens decode; up to 64 too at ranks up to 32, and beyond that rank where it is not gated and the outputs are at most twice k. decode / apart / pair, us, one adapter of
+    rank 16: 32 tokens of 4096 -> 6144 14.9 / 21.7, of 2048 -> 4096 9.4 / 12.7, of 12288 -> 4096 22.9 / 33.8, gated 4096 -> 2 x 12288 43.2 / 48.7; 64 tokens of 4096 -> 4096 15.0 / 18.4 / 27
+    (of 16 adapters 16.7 / 25.6 / 37), of 12288 -> 4096 25.7 / 34.2 / 65, of 1024 -> 4096 13.0 / 12.5 / 11.1 (16 adapters 14.7 / 17.4 / 19.2), gated 4096 -> 2 x 12288 51.7 / 56.9 / 55.2; rank
+    64: 4096 -> 4096 18.6 / 28.0 / 27, 1024 -> 4096 16.1 / 19.0 / 11.1, gated 2048 -> 2 x 6144 29.7 / 35.0 / 20.6.
 
     Beyond, by what both take (us, fitted to a B200): a round of tiles of 256 x 256 on pairs of SMs goes with k; apart is the weights or the operations, three launches, and the outputs
     read and written again. pair / apart: 4096 -> 4096 at 64 tokens 27 / 19, at 512 28 / 33 (rank 64: 29 / 48); 4096 -> 6144 at 200 28 / 33; 12288 -> 4096 at 200 66 / 50, at 700 68 / 79;
-    1024 -> 4096 at 64 11 / 13, at 1,100 19 / 36; gated 4096 -> 2 x 12288 at 64 55 / 58, at 200 56 / 90. (Over a hundred such cases the rule's way takes 0.7 % longer than the best one's.)"""
+    1024 -> 4096 at 64 11 / 13, at 1,100 19 / 36; gated 4096 -> 2 x 12288 at 64 55 / 58, at 200 56 / 90. (Over a hundred such cases the rule's way takes 1 % longer than the best one's.)"""
     rows = outputs * (2 if gated else 1)
     if tokens <= 16 and inputs <= 2048 and inputs * rows <= 6 << 20 and tokens * rank <= 256:
         return "stream"
-    if tokens <= FEW_TOKENS or (tokens <= 2 * FEW_TOKENS and (outputs > 64 * sms and rank <= 32 if gated else inputs >= 4096 or outputs <= inputs)):
+    if tokens <= FEW_TOKENS or (tokens <= 2 * FEW_TOKENS and (rank <= 32 or (not gated and outputs <= 2 * inputs))):
         return "decode"
     tiles = -(-tokens // TILE) * -(-outputs // (128 if gated else 256))
     apart = max(2.4 * inputs * rows / 6.3e6, 2 * tokens * inputs * rows / 1.2e9) + 10 + (2 + 0.2 * rank) * 1e-6 * tokens * rows
