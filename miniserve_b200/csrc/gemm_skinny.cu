@@ -388,11 +388,8 @@ static int launch_skinny(void* out, const void* X, const void* W, int M, int N, 
   const size_t smem = smem_x > smem_red ? smem_x : smem_red;
   MS_CHECK_ARG(smem <= 200 * 1024, "gemm_skinny: K=%d needs %zu bytes of shared memory", K, smem);
   auto kernel = gemm_skinny_kernel<MT, MODE, ADAPTED>;
-  static size_t configured = 0;
-  if (smem > 48 * 1024 && smem > configured) {
-    MS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    configured = smem;
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  if (smem > 48 * 1024) MS_CHECK_CUDA(allow_shared_memory((const void*)kernel, 200 * 1024, allowed));
   dim3 grid(ceil_div(N, MODE == 3 || MODE == 6 ? 8 : SK_ROWS));
   MS_LAUNCH(kernel, grid, SK_THREADS, smem, stream, out, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W, M, N, K, ex, term);
   return 0;
