@@ -260,6 +260,23 @@ def test_a_row_that_is_not_there_raises_the_status_word(rows):
     au.close(got, *au.formula(x, w, low, ops.AdapterRows(slots, of_token)))
 
 
+@pytest.mark.parametrize("way,rows", [("stream", EIGHT), ("decode", EIGHT), ("decode", DECODE64), ("pair", DECODE64[:5]), ("pair", PROMPTS), ("apart", ONE), ("apart", PROMPTS)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_every_way_takes_sizes_that_the_rule_sends_elsewhere(way, rows, gated, monkeypatch):
+    from miniserve_b200 import ops
+
+    monkeypatch.setattr(ops.adapters, "WAY", way)
+    k, parts = (4096, (520, 520)) if gated else (4096, (264, 96, 72))
+    x, w, low, ar = au.made(rows, k, parts, 40, 4, torch.bfloat16, seed=3)
+    want, tol = au.formula(x, w, low, ar)
+    if gated:
+        out = torch.full((x.shape[0], 520), float("nan"), dtype=torch.bfloat16, device="cuda")
+        ops.linear_silu_mul(x, w, out, low_rank=low, adapter_rows=ar)
+        au.close(out, *au.gated(want, tol, torch.bfloat16))
+    else:
+        au.close(run_linear(x, w, low, ar), want, tol)
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 numbers of B: the last slot's."""
     from miniserve_b200 import ops
