@@ -272,7 +272,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
     bfloat16 otherwise: this package's tcgen05 kernel where it is the faster choice
     (``tc_gemm_ok``), else the vendor library's matrix product with float32 accumulation.
     ``out`` may be float32 (logits) or bfloat16.
-    ``low_rank`` and ``adapter_rows`` (both or neither): the tokens' adapters beside the product (``ops/adapters.py``).
+    ``low_rank`` and ``adapter_rows`` (both or neither): the tokens' adapters beside the product (``ops/adapters.py``), by what the rows' tensors hold at the
+    call; where they are written in a way that torch does not count, ``adapter_rows.refresh()`` comes before it.
     """
     if low_rank is not None or adapter_rows is not None:
         return adapters.linear(x, weight, out, stream, low_rank, adapter_rows)

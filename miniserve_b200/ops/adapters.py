@@ -73,9 +73,11 @@ class LowRank:
 
 class AdapterRows:
     """Which adapter each token of a step has: ``slot_of_row`` int32 [rows], the slot of each request (below 0: none), and ``row_of_token`` int32
-    [tokens], the request of each token, tokens in the order of the requests. Made once per step and used by all its layers: steps of many tokens have a plan, which the
-    first product of a stream (or of a capture) makes of what the tensors hold then. A slot that the adapters do not have, or a row
-    that there is not, raises the status word, and the token counts as one without an adapter."""
+    [tokens], the request of each token, tokens in the order of the requests. Made once per step and used by all its layers: products of many tokens work by a plan of the two,
+    which is written once for each stream (or capture, whose replays write it again) and kept. Writing to the tensors in place makes it anew, as far as torch counts what is
+    written (``Tensor._version``); behind writes that it does not count (a kernel of one's own, ``.data``, a replayed graph) call ``refresh``. Tensors of inference mode, whose
+    writes nobody counts, have no plan that is kept. A slot that the adapters do not have, or a row that there is not, raises the status word, and the token counts as one
+    without an adapter."""
 
     def __init__(self, slot_of_row: torch.Tensor, row_of_token: torch.Tensor):
         for t in (slot_of_row, row_of_token):
@@ -85,7 +87,7 @@ class AdapterRows:
             raise ValueError("slots and rows lie on one device")
         self.slot_of_row, self.row_of_token = slot_of_row, row_of_token
         self.rows, self.tokens, self.index = slot_of_row.shape[0], row_of_token.shape[0], slot_of_row.get_device()
-        self._plans: dict = {}
+        self._plans: dict = {}  # (slots, stream, capture) -> (what the tensors' versions were, the plan)
         self._tickets: dict = {}
         if self.index >= 0:
             self.status = _ops().device_status(slot_of_row.device).data_ptr()
@@ -93,12 +95,22 @@ class AdapterRows:
             self.sms = _ops()._sm_count(slot_of_row.device)
 
     def plan(self, slots: int, stream: int) -> "_Plan":
-        """The adapters of each row tile, for projections with ``slots`` of them."""
-        key = (slots, stream, _lib().ms_adapter_capture_id(stream))
+        """The adapters of each row tile, for projections with ``slots`` of them, of what the tensors hold now."""
+        key, version = (slots, stream, _lib().ms_adapter_capture_id(stream)), self._version()
         held = self._plans.get(key)
-        if held is None:
-            held = self._plans[key] = _Plan(self, slots, stream)
-        return held
+        if held is None or held[0] != version or version is None:
+            held = self._plans[key] = (version, _Plan(self, slots, stream))
+        return held[1]
+
+    def _version(self) -> tuple | None:
+        """How often torch has seen the tensors written (None: it does not count)."""
+        if self.slot_of_row.is_inference() or self.row_of_token.is_inference():
+            return None
+        return self.slot_of_row._version, self.row_of_token._version
+
+    def refresh(self) -> None:
+        """Forget the plans: the tensors were written in a way that torch does not count."""
+        self._plans.clear()
 
     def tickets(self, stream: int) -> int:
         """The address of two zeros on the device that no launch has had: a launch leaves its counts in them."""
