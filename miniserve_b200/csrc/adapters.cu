@@ -222,7 +222,7 @@ adapter_expand_mma_kernel(O* out, const float* y, const float* v, const Adapters
       has[i] = n0 + (GATED ? r & (ROWS - 1) : r) < cols;
       n[i] = GATED && r >= ROWS ? cols + n0 + r - ROWS : n0 + r;
     }
-    warp_terms(ad, v + (size_t)t0 * ad.parts * ad.rank, tokens, M, warp >> 2, EXPAND_SETS, n, has, [] {},
+    warp_terms<sizeof(O) == 4 ? 3 : TERM_PIECES>(ad, v + (size_t)t0 * ad.parts * ad.rank, tokens, M, warp >> 2, EXPAND_SETS, n, has, [] {},
                [&](int tok, int i) { return &sums[tok][quad * 32 + (lane >> 2) + 8 * i]; });
     __syncthreads();
     constexpr int SIDE = EXPAND_THREADS / ROWS;  // tokens side by side

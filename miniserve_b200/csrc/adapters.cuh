@@ -107,8 +107,10 @@ __device__ __forceinline__ float adapter_dot(const T* row, const float* v, int r
   return sum;
 }
 
-// ---- terms of few tokens on the tensor cores: sum_j B_s[n, j] v[t, j], v rounded to bfloat16 (2^-8 of an adapter's share of an output, where the output itself is rounded so)
-constexpr int NO_SLOT = 0x7fffffff;
+// ---- terms of few tokens on the tensor cores: sum_j B_s[n, j] v[t, j], v as the sum of PIECES bfloat16 numbers: three hold all of its 24 bits, for outputs in
+// 32 bits; two hold 16, for outputs that are rounded to 8. One (2^-8 of an adapter's share lost) / two, us: 64 tokens of 16 adapters of rank 32, 4096 -> 6144 24.2 / 24.3, 32 of 1024 -> 4096 10.3 / 10.4, 8 of
+// 12288 -> 4096 21.0 / 21.0, 200 beside a product apart 50.8 / 51.1; one / three with outputs in 32 bits: 33.2 / 33.7, 14.2 / 14.6, 42.9 / 43.2, 50.7 / 51.4.
+constexpr int NO_SLOT = 0x7fffffff, TERM_PIECES = 2;
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -171,7 +173,7 @@ __device__ __forceinline__ void group_tokens(TokenGroups<MOST>& g, int M, int e,
 // added to *cell(token, i) for the lane's rows. An instruction is 16 rows and the eight tokens of a group; a group and 32 of the rank's numbers are an item, the next one's asked
 // for ahead of this one's instructions. ready: called before the first of v is read. v: float32 [.., parts * rank], by the tokens of g. One warp a scheduler has nothing to hide its
 // trips to shared memory behind, so an item makes few: its tokens, then all of its cells at once.
-template <int MOST, typename Ready, typename Cell>
+template <int PIECES, int MOST, typename Ready, typename Cell>
 __device__ __forceinline__ void warp_terms(const Adapters& ad, const float* v, const TokenGroups<MOST>& g, int M, int first, int step, const int (&n)[4], const bool (&has)[4],
                                            Ready ready, Cell cell) {
   const int lane = threadIdx.x & 31, col = lane >> 2, t4 = lane & 3, numbers = ad.parts * ad.rank, rows = ad.ends[MAX_PARTS - 1];
@@ -239,10 +241,20 @@ __device__ __forceinline__ void warp_terms(const Adapters& ad, const float* v, c
       float acc[2][4] = {};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(it.v[k][0].x, it.v[k][0].y), hi = __floats2bfloat162_rn(it.v[k][1].x, it.v[k][1].y);
+        float2 left[2] = {it.v[k][0], it.v[k][1]};  // of v behind the pieces so far
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-          mma_16816(acc[m], it.b[k][m][0], it.b[k][m][1], it.b[k][m][2], it.b[k][m][3], *reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        for (int piece = 0; piece < PIECES; ++piece) {
+          uint32_t b[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const __nv_bfloat162 now = __floats2bfloat162_rn(left[h].x, left[h].y);
+            const float2 back = __bfloat1622float2(now);
+            left[h] = make_float2(left[h].x - back.x, left[h].y - back.y);
+            b[h] = *reinterpret_cast<const uint32_t*>(&now);
+          }
+#pragma unroll
+          for (int m = 0; m < 2; ++m) mma_16816(acc[m], it.b[k][m][0], it.b[k][m][1], it.b[k][m][2], it.b[k][m][3], b[0], b[1]);
+        }
       }
 #pragma unroll
       for (int q = 0; q < 2; ++q)

@@ -719,7 +719,7 @@ __device__ __forceinline__ void epilogue_sync(int id) { asm volatile("bar.sync %
 // every CTA of the cluster adding up the tokens that fall to it, in the order of the slices.
 // The weights of the first stages are asked for before the wait on the kernels launched earlier
 // (they do not depend on them), the activations after it.
-// ADAPTED: beside the product the terms of the tokens' low-rank adapters, sum_j B_s[n, j] v[t, j] with v an earlier kernel's (rounded to bfloat16 here). The warps that
+// ADAPTED: beside the product the terms of the tokens' low-rank adapters, sum_j B_s[n, j] v[t, j] with v an earlier kernel's (16 bits of it here). The warps that
 // store the outputs have nothing to do while the weights stream, and work out terms then: tokens in the order of their adapters, eight of one adapter at most times the
 // warp's 32 rows of B an instruction; a cluster's CTAs share the adapters out, and a term enters the sum over the slices with the CTA that made it. One rounding.
 // (Terms as k-blocks of the tensor cores, as in the 2-CTA kernel, cost a copy of 128 short rows for each adapter of the step: 42.9 us at 64 tokens of 16 adapters, rank 32,
@@ -887,7 +887,7 @@ gemm_tc_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         if (term.tickets == nullptr) pdl_wait();
         if (term.tickets != nullptr && !__all_sync(0xffffffffu, tickets_reach(term.tickets + 1, units)) && lane == 0) atomicExch(status, 19);
       };
-      warp_terms(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i) { return part + tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i; });
+      warp_terms<TERM_PIECES>(ad, term.v, tokens, M, rank, slices, n, has, ready, [&](int tok, int i) { return part + tok * TC_BM + quad * 32 + (lane >> 2) + 8 * i; });
       if (term.tickets == nullptr) pdl_wait();
       __syncwarp();
     }
