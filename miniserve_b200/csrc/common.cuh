@@ -92,6 +92,11 @@ __device__ __forceinline__ uint4 float_to_bf16x8(const float (&f)[8]) {
   return v;
 }
 
+// A CTA may touch another one's shared memory once that one is known to have started: all threads of a cluster arrive when they start, and wait ahead of the first such access, by
+// when the others have long been there.
+__device__ __forceinline__ void cluster_started_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_started_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // ---- programmatic dependent launch

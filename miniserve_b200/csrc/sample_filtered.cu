@@ -218,6 +218,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   const int ctas = cl.ctas, rank = cl.rank, r = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const double u = uniform64 ? reinterpret_cast<const double*>(uniform)[r] : (double)reinterpret_cast<const float*>(uniform)[r];
   if (!(u >= 0.0 && u < 1.0)) return;  // (the whole cluster)
+  cluster_started_arrive();
   const float t = temperature[r];
   const int k = top_k ? top_k[r] : 0;
   const float p = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
@@ -258,6 +259,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   for (int i = tid; i < BINS; i += SF_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0;
   if (tid == 0) sh.listed = 0;
   u64 best = order_of(top), lowest = low < INFINITY ? (u64)~order_of(low) : 0;
+  cluster_started_wait();
   cl.reduce<true>(best, lowest);
   const float zmax = logit_of(best << INDEX_BITS);
   const float* mine = staged ? sf_logits : xs;
