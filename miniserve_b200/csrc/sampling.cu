@@ -308,6 +308,7 @@ sample_cluster_kernel(int* __restrict__ tokens, const float* __restrict__ logits
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int r = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster_started_arrive();
   pdl_prologue(logits, temperature, top_p, seed, counter);
   const float* lg = logits + (size_t)r * vocab;
   const float t = temperature[r], tp = top_p[r];
@@ -321,17 +322,20 @@ sample_cluster_kernel(int* __restrict__ tokens, const float* __restrict__ logits
       const float x = lg[begin + i];
       if (x > b.val) { b.val = x; b.idx = begin + i; }
     }
+    cluster_started_wait();
   } else if (tp >= 1.f) {
     const uint32_t key = mix32((uint32_t)seed[r] ^ mix32((uint32_t)counter[r]));
     for (int i = tid; i < n; i += NC_THREADS) {
       const float x = lg[begin + i] / t + gumbel(key, (uint32_t)(begin + i));
       if (x > b.val) { b.val = x; b.idx = begin + i; }
     }
+    cluster_started_wait();
   } else {
     const float inv_t = 1.0f / t;
     Nucleus nu;
     float one[1] = {-INFINITY};
     for (int i = tid; i < n; i += NC_THREADS) one[0] = fmaxf(one[0], lg[begin + i] * inv_t);
+    cluster_started_wait();
     nc_all_reduce<1, true>(one, sh, buf, cluster, rank, ctas);
     nu.zmax = one[0];
     one[0] = 0.f;

@@ -24,7 +24,10 @@ def body(name: str, kernel: str) -> str:
 
 
 # (file, kernel, what reaches another CTA's memory)
-@pytest.mark.parametrize("name,kernel,reach", [("sample_filtered.cu", "sample_filtered_kernel", r"cl\.reduce<|cl\.tell\(|map_shared_rank\(")])
+@pytest.mark.parametrize("name,kernel,reach", [("sample_filtered.cu", "sample_filtered_kernel", r"cl\.reduce<|cl\.tell\(|map_shared_rank\("),
+                                               ("sampling.cu", "sample_cluster_kernel", r"nc_all_reduce<|map_shared_rank\("),
+                                               ("gated_recurrence.cu", "rglru_scan_kernel", r"map_shared_rank\("), ("gemm_tc.cu", "gemm_tc_pair_kernel", r"mbar_arrive_first_cta\("),
+                                               ("gemm_tc.cu", "gemm_tc_decode_kernel", r"mapa|shared::cluster\.f32"), ("gemm_tc.cu", "adapter_v_kernel", r"mapa|ld\.shared::cluster")])
 def test_a_barrier_stands_ahead_of_the_first_access(name, kernel, reach):
     text = body(name, kernel)
     first = re.search(reach, text)

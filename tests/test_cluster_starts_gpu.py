@@ -31,3 +31,21 @@ def test_filtered_rows_of_few_tokens_a_cta(vocab, rows):
         ops.sample_filtered(out, logits, t, u, top_k=k, top_p=p)
     want = [-7 if i % 4 == 3 else plain(logits[i], f32(0.9), float(u[i]), int(k[i]), f32(0.7)) for i in range(rows)]
     assert all(out.tolist() == want for out in tokens)
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+def test_nucleus_rows_of_few_tokens_a_cta(rows):
+    """Rows by top_p, by temperature alone and greedy ones, a cluster each: the same tokens in every launch, and of the greedy rows the first of the likeliest."""
+    from miniserve_b200 import ops
+
+    logits, _ = peaked(rows, 16385, 2)
+    scratch = torch.empty(rows * ops.nucleus_bytes(), dtype=torch.uint8, device="cuda")
+    kinds = [(0.9, 0.7), (1.1, 1.0), (0.0, 1.0)]
+    t, p = (torch.tensor([kinds[i % 3][q] for i in range(rows)], device="cuda") for q in range(2))
+    seed, counter = torch.arange(rows, device="cuda"), torch.arange(rows, device="cuda") + 5
+    tokens = [torch.full((rows,), -7, dtype=torch.int32, device="cuda") for _ in range(200)]
+    for out in tokens:
+        ops.sample(out, logits, temperature=t, top_p=p, seed=seed, counter=counter, scratch=scratch)
+    first = tokens[0].tolist()
+    assert all(out.tolist() == first for out in tokens)
+    assert all(first[i] == int(logits[i].argmax()) for i in range(2, rows, 3)) and all(0 <= x < 16385 for x in first)
