@@ -206,7 +206,7 @@ class Engine:
     def capture_graphs(self, modes=("greedy",), context_lengths=(0,), prompt_tokens: int = 0) -> int:
         """Capture the decode graphs of every batch bucket now (while the engine is idle) instead
         of at their first use; returns how many were captured. ``modes``: of "greedy",
-        "temperature", "top_p", "filtered" (top_k or min_p). ``context_lengths``: lengths that requests will reach; the graphs of
+        "temperature", "top_p", "filtered" (all that sample have top_k or min_p), "temperature+filtered" and "top_p+filtered" (some have). ``context_lengths``: lengths that requests will reach; the graphs of
         every class of context length from the shortest's to the longest's are captured (those for short
         contexts by default). ``prompt_tokens``: also capture the step graphs that lone prompts of up to so
         many tokens meet (no more than a step's token budget), so that the first requests replay them."""

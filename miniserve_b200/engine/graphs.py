@@ -133,10 +133,18 @@ class DecodeGraphs:
             "temperature": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n),
             "top_p": lambda n: dict(temperatures=[1.0] * n, top_ps=[0.5] * n, seeds=[0] * n, counters=[0] * n),
             "filtered": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n, top_ks=[2] * n),
+            # one row with top_k beside rows drawn by noise
+            "temperature+filtered": lambda n: dict(temperatures=[1.0] * n, top_ps=[1.0] * n, seeds=[0] * n, counters=[0] * n, top_ks=[2] + [0] * (n - 1)),
+            "top_p+filtered": lambda n: dict(temperatures=[1.0] * n, top_ps=[0.5] * n, seeds=[0] * n, counters=[0] * n, top_ks=[2] + [0] * (n - 1)),
         }
+        unknown = [m for m in modes if m not in sampling_for]
+        if unknown:
+            raise ValueError(f"no sampling modes {unknown}; there are {list(sampling_for)}")
         before = len(self._graphs)
         for mode, klass, adapter in ((m, k, a) for m in modes for k in classes for a in ((-1, 0) if sf.low_rank else (-1,))):
             for bucket in self.buckets:
+                if bucket == 1 and mode.endswith("+filtered"):
+                    continue  # (a single row is one or the other)
                 caches = [sf.cache.new_request() for _ in range(bucket)]
                 try:
                     self.run([StepRow(c, [0], (0,), adapter=adapter) for c in caches], sampling_for[mode](bucket), klass=klass)
