@@ -20,6 +20,26 @@ _PREFIX = "base_model.model."
 _ENDS = {".lora_A.weight": 0, ".lora_B.weight": 1}
 
 
+def _config(folder: Path) -> dict:
+    """What ``adapter_config.json`` says, ``r`` a number."""
+    try:
+        cfg = json.loads((folder / "adapter_config.json").read_text())
+    except FileNotFoundError:
+        raise FileNotFoundError(f"no adapter_config.json in {folder}") from None
+    try:
+        cfg["r"] = int(cfg["r"])
+    except (KeyError, TypeError, ValueError):
+        raise ValueError(f"adapter_config.json in {folder} says no rank (r)") from None
+    return cfg
+
+
+def rank_of(source: "str | Path | Mapping[str, torch.Tensor]") -> int:
+    """The rank of an adapter, in a folder or as tensors by name."""
+    if isinstance(source, (str, Path)):
+        return _config(Path(source))["r"]
+    return max((t.shape[0] for key, t in source.items() if key.endswith(".lora_A.weight") and t.dim()), default=1)
+
+
 class AdapterStore:
     def __init__(self, model, slots: int, rank: int):
         """Room for ``slots`` adapters of a rank up to ``rank`` (made up to a multiple of 8) beside every projection of ``model`` that takes them."""
@@ -114,16 +134,13 @@ class AdapterStore:
     def _read(self, folder: Path) -> tuple[dict, float]:
         from safetensors.torch import load_file
 
-        try:
-            cfg = json.loads((folder / "adapter_config.json").read_text())
-        except FileNotFoundError:
-            raise FileNotFoundError(f"no adapter_config.json in {folder}") from None
+        cfg = _config(folder)
         odd = [k for k in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "fan_in_fan_out") if cfg.get(k)]
         if cfg.get("bias", "none") not in ("none", None):
             odd.append(f"bias={cfg['bias']}")
         if odd:
             raise ValueError(f"the adapter in {folder} has what there is nothing for here: {', '.join(odd)}")
-        r = int(cfg["r"])
+        r = cfg["r"]
         files = sorted(folder.glob("*.safetensors"))
         if not files:
             raise FileNotFoundError(f"no .safetensors files in {folder}")

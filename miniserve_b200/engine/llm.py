@@ -13,6 +13,7 @@ from typing import Sequence
 import torch
 
 from ..config.presets import preset
+from .adapters import rank_of
 from .engine import Engine
 from .loader import load_model, random_model
 from .request import SamplingParams
@@ -28,9 +29,12 @@ class LLM:
         keywords are the engine's (``kv_pool_tokens``, ``page_size``, ``max_running``,
         ``max_prefill_tokens``, ``chunked_prefill_size``, ``seed``, ``cuda_graph``,
         ``cuda_graph_max_bs``, ``step_graphs``, ``overlap``, ``kv_cache_dtype``, ``max_adapters``, ``max_adapter_rank``). ``adapters``: folders of low-rank
-        adapters to load, by the names that requests will call them (room for so many unless ``max_adapters`` says more)."""
+        adapters to load, by the names that requests will call them (room for so many of their ranks unless ``max_adapters`` and ``max_adapter_rank`` say more)."""
         if (model is None) == (random is None):
             raise ValueError("give either a model folder or random=PRESET")
+        if adapters:
+            engine_kwargs["max_adapters"] = max(len(adapters), engine_kwargs.get("max_adapters") or 0)
+            engine_kwargs["max_adapter_rank"] = max(*map(rank_of, adapters.values()), engine_kwargs.get("max_adapter_rank", 16))
         if model is not None:
             self.raw_config, self.config, self.model = load_model(model, dtype, device)
         else:
@@ -38,8 +42,6 @@ class LLM:
             big = (raw.get("hidden_size") or raw.get("width", 0)) * (raw.get("num_hidden_layers") or len(raw.get("layers", ()))) > 4096
             self.raw_config, self.config, self.model = random_model(raw, weights_seed, dtype, device,
                                                                     draw_on_device=big)
-        if adapters:
-            engine_kwargs["max_adapters"] = max(len(adapters), engine_kwargs.get("max_adapters") or 0)
         self.engine = Engine(self.model, **engine_kwargs)
         for name, folder in (adapters or {}).items():
             self.engine.load_adapter(name, folder)
