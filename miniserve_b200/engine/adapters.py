@@ -146,7 +146,11 @@ class AdapterStore:
             raise FileNotFoundError(f"no .safetensors files in {folder}")
         tensors: dict = {}
         for f in files:
-            tensors.update(load_file(str(f)))
+            more = load_file(str(f))
+            twice = sorted(tensors.keys() & more.keys())
+            if twice:
+                raise ValueError(f"{f} holds tensors that another file of {folder} holds too: {', '.join(twice[:4])}")
+            tensors.update(more)
         alpha = float(cfg.get("lora_alpha", r))
         return tensors, alpha / (math.sqrt(r) if cfg.get("use_rslora") else r)
 
@@ -161,7 +165,10 @@ class AdapterStore:
             if matrix not in self.places:
                 wrong.append(f"{key}: no projection here that takes an adapter")
                 continue
-            halves.setdefault(matrix, [None, None])[_ENDS[end]] = t
+            half = halves.setdefault(matrix, [None, None])
+            if half[_ENDS[end]] is not None:
+                wrong.append(f"{at}: given twice, with {_PREFIX} in front and without")
+            half[_ENDS[end]] = t
         ranks = set()
         for matrix, (a, b) in halves.items():
             low, _, first, behind = self.places[matrix]

@@ -1,0 +1,46 @@
+"""Adapters whose files leave more than one reading are refused, without a GPU."""
+
+from __future__ import annotations
+
+import json
+
+import pytest
+import torch
+from safetensors.torch import save_file
+
+from miniserve_b200.engine.adapters import AdapterStore
+
+from .test_adapters_engine import model, tensors
+
+PREFIX = "base_model.model."
+
+
+def written(path, parts, **config):
+    path.mkdir(exist_ok=True)
+    (path / "adapter_config.json").write_text(json.dumps({**dict(r=4, lora_alpha=8), **config}))
+    for name, part in parts.items():
+        save_file(part, str(path / name))
+    return path
+
+
+def test_a_matrix_that_is_named_in_both_ways():
+    m = model()
+    store, given = AdapterStore(m, 1, 8), tensors(m, 4, only="q_proj")
+    key = next(k for k in given if k.endswith("lora_B.weight"))
+    with pytest.raises(ValueError, match="given twice"):
+        store.load("x", {**given, key[len(PREFIX):]: given[key] + 1})
+    assert not store.names
+    store.load("x", {k[len(PREFIX):] if i % 2 else k: t for i, (k, t) in enumerate(given.items())})
+
+
+def test_a_tensor_that_two_files_hold(tmp_path):
+    m = model()
+    given = tensors(m, 4, only="q_proj")
+    keys = sorted(given)
+    halves = {"a.safetensors": {k: given[k] for k in keys[:3]}, "b.safetensors": {k: given[k] for k in keys[3:]}}
+    store = AdapterStore(m, 2, 8)
+    store.load("x", written(tmp_path / "good", halves))
+    halves["b.safetensors"][keys[0]] = torch.zeros_like(given[keys[0]])
+    with pytest.raises(ValueError, match="holds too"):
+        store.load("y", written(tmp_path / "bad", halves))
+    assert list(store.names) == ["x"]
