@@ -85,16 +85,16 @@ class AdapterStore:
         free = [s for s in range(self.slots) if s not in self.names.values()]
         if not free:
             raise ValueError(f"all {self.slots} adapters' places are taken ({', '.join(sorted(self.names))}): unload one, or ask for more (max_adapters)")
-        factor = None
+        factor = said = None
         if isinstance(source, (str, Path)):
-            tensors, factor = self._read(Path(source))
+            tensors, factor, said = self._read(Path(source))
             if alpha is not None:
                 raise ValueError("alpha is what the adapter's folder says")
         else:
             tensors = dict(source)
         if not math.isfinite(factor if factor is not None else 1.0 if alpha is None else alpha):
             raise ValueError(f"adapter {name!r} has a factor that is not finite")
-        pairs = self._pairs(name, tensors)
+        pairs = self._pairs(name, tensors, said)
         slot = free[0]
         self._settle()  # (a step in flight may still read what the place held)
         for low in self.products.values():
@@ -131,7 +131,8 @@ class AdapterStore:
         except KeyError:
             raise ValueError(f"no adapter named {name!r}; there are {sorted(self.names)}") from None
 
-    def _read(self, folder: Path) -> tuple[dict, float]:
+    def _read(self, folder: Path) -> tuple[dict, float, int]:
+        """The tensors, the factor and the rank that the folder's configuration says."""
         from safetensors.torch import load_file
 
         cfg = _config(folder)
@@ -152,10 +153,10 @@ class AdapterStore:
                 raise ValueError(f"{f} holds tensors that another file of {folder} holds too: {', '.join(twice[:4])}")
             tensors.update(more)
         alpha = float(cfg.get("lora_alpha", r))
-        return tensors, alpha / (math.sqrt(r) if cfg.get("use_rslora") else r)
+        return tensors, alpha / (math.sqrt(r) if cfg.get("use_rslora") else r), r
 
-    def _pairs(self, name: str, tensors: Mapping[str, torch.Tensor]) -> dict[str, tuple]:
-        """(A, B) by the model's matrix, or one error about all that does not fit."""
+    def _pairs(self, name: str, tensors: Mapping[str, torch.Tensor], said: int | None = None) -> dict[str, tuple]:
+        """(A, B) by the model's matrix, or one error about all that does not fit (``said``: the rank that they should have)."""
         halves: dict[str, list] = {}
         wrong: list[str] = []
         for key, t in tensors.items():
@@ -182,6 +183,8 @@ class AdapterStore:
                     wrong.append(f"{matrix}: numbers that are not finite (other requests' tokens would meet them)")
                 if not 1 <= a.shape[0] <= self.rank:
                     wrong.append(f"{matrix}: rank {a.shape[0]}, there is room for 1 to {self.rank} (max_adapter_rank)")
+        if said is not None and ranks and ranks != {said}:
+            wrong.append(f"tensors of rank {', '.join(map(str, sorted(ranks)))} beside a configuration that says {said} (the factor follows from it)")
         if len(ranks) > 1:
             wrong.append(f"ranks {sorted(ranks)}: all of an adapter's are one")
         if not halves and not wrong:

@@ -44,3 +44,13 @@ def test_a_tensor_that_two_files_hold(tmp_path):
     with pytest.raises(ValueError, match="holds too"):
         store.load("y", written(tmp_path / "bad", halves))
     assert list(store.names) == ["x"]
+
+
+def test_a_rank_that_is_not_the_tensors(tmp_path):
+    """The factor is lora_alpha over the rank, so the two have to agree."""
+    m = model()
+    store = AdapterStore(m, 1, 8)
+    with pytest.raises(ValueError, match="says 8"):
+        store.load("x", written(tmp_path / "bad", {"a.safetensors": tensors(m, 4, only="q_proj")}, r=8))
+    assert not store.names
+    store.load("x", written(tmp_path / "bad", {}, r=4))
