@@ -136,9 +136,11 @@ class AdapterStore:
         from safetensors.torch import load_file
 
         cfg = _config(folder)
-        odd = [k for k in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "fan_in_fan_out") if cfg.get(k)]
+        odd = [k for k in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "layer_replication", "fan_in_fan_out", "alora_invocation_tokens") if cfg.get(k)]
         if cfg.get("bias", "none") not in ("none", None):
             odd.append(f"bias={cfg['bias']}")
+        if str(cfg.get("peft_type") or "LORA").upper() != "LORA":
+            odd.append(f"peft_type={cfg['peft_type']}")
         if odd:
             raise ValueError(f"the adapter in {folder} has what there is nothing for here: {', '.join(odd)}")
         r = cfg["r"]

@@ -54,3 +54,14 @@ def test_a_rank_that_is_not_the_tensors(tmp_path):
         store.load("x", written(tmp_path / "bad", {"a.safetensors": tensors(m, 4, only="q_proj")}, r=8))
     assert not store.names
     store.load("x", written(tmp_path / "bad", {}, r=4))
+
+
+def test_kinds_of_adapters_that_there_is_nothing_for(tmp_path):
+    """Adapters that count behind certain tokens alone, and methods of other names."""
+    m = model()
+    given = {"a.safetensors": tensors(m, 4, only="q_proj")}
+    for i, extra in enumerate((dict(alora_invocation_tokens=[5, 7]), dict(peft_type="ADALORA"))):
+        with pytest.raises(ValueError, match="nothing for here"):
+            AdapterStore(m, 1, 8).load("x", written(tmp_path / str(i), given, **extra))
+    for i, extra in enumerate((dict(alora_invocation_tokens=None, peft_type="LORA"), dict(peft_type=None))):
+        AdapterStore(m, 1, 8).load("x", written(tmp_path / f"good{i}", given, **extra))
