@@ -92,25 +92,29 @@ class AdapterStore:
                 raise ValueError("alpha is what the adapter's folder says")
         else:
             tensors = dict(source)
-        if not math.isfinite(factor if factor is not None else 1.0 if alpha is None else alpha):
+        if factor is None and alpha is not None and not math.isfinite(alpha):
             raise ValueError(f"adapter {name!r} has a factor that is not finite")
         pairs = self._pairs(name, tensors, said)
+        if factor is None:
+            factor = 1.0 if alpha is None else float(alpha) / next(iter(pairs.values()))[0].shape[0]
+        if not abs(factor) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"adapter {name!r} has a factor that is not finite in 32 bits: {factor}")
         slot = free[0]
         self._settle()  # (a step in flight may still read what the place held)
         for low in self.products.values():
             low.scale[slot] = 0.0
-        used: dict[int, tuple] = {}
+        used: dict[int, ops.LowRank] = {}
         for matrix, (a, b) in pairs.items():
             low, part, first, behind = self.places[matrix]
             r = a.shape[0]
             if id(low) not in used:
                 low.a[slot].zero_()
                 low.b[slot].zero_()
-                used[id(low)] = (low, r)
+                used[id(low)] = low
             low.a[slot, part * low.rank:part * low.rank + r] = a.to(low.a.dtype)
             low.b[slot, first:behind, :r] = b.to(low.b.dtype)
-        for low, r in used.values():
-            low.scale[slot] = factor if factor is not None else (1.0 if alpha is None else float(alpha) / r)
+        for low in used.values():
+            low.scale[slot] = factor
         self._settle()  # (steps may run on another stream)
         self.names[name] = slot
         return slot

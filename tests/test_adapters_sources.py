@@ -65,3 +65,15 @@ def test_kinds_of_adapters_that_there_is_nothing_for(tmp_path):
             AdapterStore(m, 1, 8).load("x", written(tmp_path / str(i), given, **extra))
     for i, extra in enumerate((dict(alora_invocation_tokens=None, peft_type="LORA"), dict(peft_type=None))):
         AdapterStore(m, 1, 8).load("x", written(tmp_path / f"good{i}", given, **extra))
+
+
+def test_a_factor_that_32_bits_do_not_hold(tmp_path):
+    m = model()
+    store, given = AdapterStore(m, 1, 8), tensors(m, 4, only="q_proj")
+    with pytest.raises(ValueError, match="32 bits"):
+        store.load("x", given, alpha=1e39 * 4)
+    with pytest.raises(ValueError, match="32 bits"):
+        store.load("x", written(tmp_path / "bad", {"a.safetensors": given}, lora_alpha=-1e40))
+    assert not store.names and not any(bool(low.scale.any()) for low in store.products.values())
+    store.load("x", given, alpha=4e38)
+    assert all(bool(torch.isfinite(low.scale).all()) for low in store.products.values())
