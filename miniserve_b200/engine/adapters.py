@@ -30,6 +30,8 @@ def _config(folder: Path) -> dict:
         cfg["r"] = int(cfg["r"])
     except (KeyError, TypeError, ValueError):
         raise ValueError(f"adapter_config.json in {folder} says no rank (r)") from None
+    if cfg["r"] < 1:
+        raise ValueError(f"adapter_config.json in {folder} says a rank of {cfg['r']}")
     return cfg
 
 

@@ -77,3 +77,10 @@ def test_a_factor_that_32_bits_do_not_hold(tmp_path):
     assert not store.names and not any(bool(low.scale.any()) for low in store.products.values())
     store.load("x", given, alpha=4e38)
     assert all(bool(torch.isfinite(low.scale).all()) for low in store.products.values())
+
+
+def test_a_rank_of_nothing(tmp_path):
+    m = model()
+    for r in (0, -4):
+        with pytest.raises(ValueError, match="says a rank"):
+            AdapterStore(m, 1, 8).load("x", written(tmp_path / "bad", {"a.safetensors": tensors(m, 4, only="q_proj")}, r=r))
