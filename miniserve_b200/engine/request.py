@@ -86,7 +86,7 @@ class SamplingParams:
             (self.max_new_tokens >= 1, f"max_new_tokens={self.max_new_tokens}: a request produces at least one token"),
             (self.temperature >= 0, f"temperature={self.temperature}: cannot be negative (0 is greedy)"),  # NaN fails too
             (0 < self.top_p <= 1, f"top_p={self.top_p}: a probability mass in (0, 1]"),
-            (self.top_k >= 0 and self.top_k == int(self.top_k) and self.top_k < 1 << 31, f"top_k={self.top_k}: a number of tokens (0: all)"),
+            (0 <= self.top_k < 1 << 31 and self.top_k == int(self.top_k), f"top_k={self.top_k}: a number of tokens (0: all)"),
             (0 <= self.min_p <= 1, f"min_p={self.min_p}: a share of the most likely token's probability in [0, 1]"),
             (self.seed is None or 0 <= self.seed < 1 << 32, f"seed={self.seed}: an unsigned 32-bit number, or None"),
         ]
