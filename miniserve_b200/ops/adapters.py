@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import struct
 import sys
+import threading
 from contextlib import nullcontext
 from ctypes import c_char_p, c_int, c_longlong, c_ulonglong, c_void_p
 from dataclasses import dataclass
@@ -89,6 +90,7 @@ class AdapterRows:
         self.rows, self.tokens, self.index = slot_of_row.shape[0], row_of_token.shape[0], slot_of_row.get_device()
         self._plans: dict = {}  # (slots, stream, capture) -> (what the tensors' versions were, the plan)
         self._tickets: dict = {}
+        self._taking = threading.Lock()
         if self.index >= 0:
             self.status = _ops().device_status(slot_of_row.device).data_ptr()
             self.middle = struct.pack("3Q2i", slot_of_row.data_ptr(), row_of_token.data_ptr(), self.status, self.rows, 0)
@@ -115,13 +117,14 @@ class AdapterRows:
     def tickets(self, stream: int) -> int:
         """The address of two zeros on the device that no launch has had: a launch leaves its counts in them."""
         key = (stream, _lib().ms_adapter_capture_id(stream))
-        held = self._tickets.get(key)
-        if held is None or held[1] == held[2]:
-            with on_stream(stream, self.slot_of_row.device):
-                zeros = torch.zeros(2 * TICKETS, dtype=torch.int32, device=self.slot_of_row.device)
-            held = self._tickets[key] = [zeros, zeros.data_ptr(), zeros.data_ptr() + 8 * TICKETS]
-        held[1] += 8
-        return held[1] - 8
+        with self._taking:  # (two host threads: a pair is one launch's)
+            held = self._tickets.get(key)
+            if held is None or held[1] == held[2]:
+                with on_stream(stream, self.slot_of_row.device):
+                    zeros = torch.zeros(2 * TICKETS, dtype=torch.int32, device=self.slot_of_row.device)
+                held = self._tickets[key] = [zeros, zeros.data_ptr(), zeros.data_ptr() + 8 * TICKETS]
+            held[1] += 8
+            return held[1] - 8
 
 
 class _Plan:
