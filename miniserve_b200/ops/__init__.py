@@ -486,6 +486,10 @@ def qkv_norm_rope_kv(q_out: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         adapters.check(x, w_qkv, None, low_rank, adapter_rows, False)
         if t == 0:
             return
+        if torch.cuda.current_device() != low_rank.index:  # (as the other adapted products: on the tensors' device)
+            with torch.cuda.device(low_rank.index):
+                return qkv_norm_rope_kv(q_out, k_pool, v_pool, x, w_qkv, q_norm_w, k_norm_w, cos_sin, eps, positions, row_of_token, page_indptr, page_indices, page_size, stream,
+                                        low_rank, adapter_rows)
         product, v = adapters.product(x, low_rank, adapter_rows, _stream(stream))
     native.kernel_check(lib.ms_gemm_tc_qkv_bf16(
         _ptr(q_out), _ptr(x), _ptr(w_qkv), t, x.shape[1], nq, nkv, _ptr(k_pool), _ptr(v_pool), _ptr(q_norm_w), _ptr(k_norm_w),
