@@ -182,12 +182,13 @@ def run(state):
         if case["kind"] == "sample":
             ops.sample_filtered(st["tokens"], st["logits"], st["temperature"], st["uniform"], top_k=st["top_k"], top_p=st["top_p"], min_p=st["min_p"])
             return st["tokens"]
-        if "low_rank" not in st:  # the weights as the engine holds them, and what it makes once per step for all layers
+        if "low_rank" not in st:  # the weights as the engine holds them
             ends = [sum(_parts(case)[:i + 1]) for i in range(len(_parts(case)))]
             st["low_rank"] = ops.LowRank(st["a"], st["b"], st["scale"], tuple(ends))
-            st["adapter_rows"] = ops.AdapterRows(st["slot_of_row"], st["row_of_token"])
+        # a step's, made in the pass with all that products make of it (a model's layers share one)
+        rows = ops.AdapterRows(st["slot_of_row"], st["row_of_token"])
         product = ops.linear_silu_mul if case["kind"] == "glu" else ops.linear
-        product(st["x"], st["w"], out=st["out"], low_rank=st["low_rank"], adapter_rows=st["adapter_rows"])
+        product(st["x"], st["w"], out=st["out"], low_rank=st["low_rank"], adapter_rows=rows)
         return st["out"]
     if case["kind"] == "sample":
         return _plain_sample(st)
