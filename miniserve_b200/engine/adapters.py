@@ -1,7 +1,7 @@
 """The low-rank adapters that an engine holds beside its model's projections, a slot each (``AdapterStore``).
 
 An adapter comes as a folder with ``adapter_config.json`` (``r``, ``lora_alpha``) and safetensors, or as its tensors: for each adapted matrix ``<matrix>.lora_A.weight``
-[r, inputs] and ``<matrix>.lora_B.weight`` [outputs, r], ``<matrix>.weight`` being the model's tensor, with or without ``base_model.model.`` in front. It adds
+[r, inputs] and ``<matrix>.lora_B.weight`` [outputs, r], ``<matrix>.weight`` (or ``<matrix>``) being the model's tensor, with or without ``base_model.model.`` in front. It adds
 alpha / r B A x to the matrix's product. Which matrices may have one is the parts' to say (``Part.adapted_products``); others are refused, all that is wrong in one error.
 """
 
@@ -170,7 +170,8 @@ class AdapterStore:
         for key, t in tensors.items():
             at = key[len(_PREFIX):] if key.startswith(_PREFIX) else key
             end = next((e for e in _ENDS if at.endswith(e)), None)
-            matrix = at[:-len(end)] + ".weight" if end else None
+            stem = at[:-len(end)] if end else None
+            matrix = stem if stem in self.places else f"{stem}.weight"
             if matrix not in self.places:
                 wrong.append(f"{key}: no projection here that takes an adapter")
                 continue
