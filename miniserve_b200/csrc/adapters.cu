@@ -184,8 +184,8 @@ adapter_expand_kernel(float* out, const float* y, const float* v, const Adapters
 
 // The same for bfloat16 adapters on the tensor cores: up to 32 tokens a block, and 128 columns (GATED: 64 gate and their 64 up columns) at a time of every gridDim.x-th such
 // tile; the product's numbers of the next one are asked for ahead. A warp has 32 columns, four of them (a set) all columns, and the sets share the tokens' adapters out.
-// Bound by the trips for B and v of each group of eight tokens: us, tokens of one adapter / of 16, rank 16, 4,096 columns: 64 5.1 / 8.8, 512 9.5 / 18.3 (one tile of columns a block, 512
-// threads: 16.6 / 35.9); 2 x 12,288 columns, 64 10.9 / 19.4. Three blocks a multiprocessor spill registers: 8.5 / 17.3, 19.9 / 48.3.
+// Bound by the trips for B and v of each group of eight tokens: us, tokens of one adapter / of 16, rank 16, 4,096 columns: 64 5.2 / 9.5, 512 9.7 / 19.2 (in 32 bits 5.4 / 9.7 and 9.8 / 19.7; one tile of columns a block, 512
+// threads: 16.6 / 35.9); 2 x 12,288 columns, 64 10.9 / 20.0. Three blocks a multiprocessor spill registers: 8.5 / 17.3, 19.9 / 48.3.
 constexpr int EXPAND_TOKENS = 32, EXPAND_COLS = 128, EXPAND_SETS = 2, EXPAND_THREADS = EXPAND_SETS * 128, EXPAND_RESIDENT = 2;
 template <typename O, bool GATED>
 __global__ void __launch_bounds__(EXPAND_THREADS, EXPAND_RESIDENT)

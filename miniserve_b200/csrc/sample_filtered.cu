@@ -7,7 +7,7 @@
 //
 // Masses are integers: exp(z - max) in 64-bit floating point, times 2^bits, rounded to the nearest (bits: as many as leave room for the sum of the whole row, at most
 // 45). Sums of integers do not depend on their order, so the same row gives the same token whatever adds it up, and borders fall where 64 bits put them: a
-// mass is off by 2^-46 of the likeliest token's at most, and tokens below that have none.
+// mass is off by 2^-(bits + 1) of the likeliest token's at most (2^-46 up to 131,072 tokens, 2^-45 for 151,936, 2^-43 for 2^20), and tokens below that have none.
 #include <cfloat>
 
 #include <cooperative_groups.h>
@@ -280,7 +280,7 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
   // the least logit that is not below 2^-3 of a mass (rounded up, so that no logit from it on is either)
   const float from = zmax < INFINITY ? __double2float_ru((double)zmax - (double)(bits + 3) * STEPS / steps) : INFINITY;
   const Scale f{zmax, fmaxf(from, -FLT_MAX), zmax < INFINITY ? (double)zmax : 0.0, steps, bits, sh.powers};
-  // Bins by the fall below the largest: up to the least finite logit, and no further than masses go (2^-46 is 31.9 falls of T).
+  // Bins by the fall below the largest: up to the least finite logit, and no further than masses go (2^-46, the least there is, is 31.9 falls of T).
   const float floor_ = logit_of(((u64)~(uint32_t)lowest) << INDEX_BITS);
   const float width = fminf((float)BINS / fmaxf(fminf(zmax - floor_, 32.f * t), 1e-35f), 1e37f);
   auto bin_of = [&](float x) { return x == zmax ? 0 : (int)fminf((zmax - x) * width, (float)(BINS - 1)); };
@@ -382,7 +382,8 @@ sample_filtered_kernel(int* __restrict__ tokens, const float* __restrict__ logit
     group.sync();
     return mass;
   };
-  // The cut itself, the place at which `enough` comes true, within bin said[0]: by its places sorted in the first CTA; of more than those hold, by halving the range.
+  // The cut itself, the place at which `enough` comes true, within bin said[0]: by its places sorted in the first CTA; of more than those hold, by halving the range, a pass
+  // and a meeting for each of some 40 bits (by top-p of 151,936 tokens, us, one row and 8: logits that are whole numbers 145 and 219; one token far below the rest, which makes the bins wide, 190 and 307; else 33 and 43).
   auto settle = [&](auto enough, u64 all_count, u64 all_mass) {
     const int bin = (int)sh.said[0];
     const u64 cb = sh.said[1], mb = sh.said[2], members = sh.said[3];

@@ -244,7 +244,8 @@ def product(x: torch.Tensor, low_rank: LowRank, rows: AdapterRows, stream: int) 
 
 def way_of(tokens: int, outputs: int, inputs: int, rank: int, gated: bool, sms: int) -> str:
     """The way of a bfloat16 product with adapters. "stream": the weight-streaming kernel of decode steps, a thread's terms behind an output's sum. "decode": the swapped-operand tcgen05 kernel of decode steps, the terms on its idle epilogue warps. "pair": the 2-CTA tcgen05 kernel, which
-    takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it, the terms added behind.
+    takes the adapters in its own sums. "apart": the shared product in float32 wherever ``linear`` sends it (beyond 16 rows of bfloat16 the vendor
+    library's), the terms added behind.
 
     Up to 16 tokens stream, where k is at most 2,048, the weight at most 12 MiB and tokens times rank at most 256. decode / stream, us, behind a norm: 8 tokens of rank 16, 1024 -> 4096 9.1 / 6.9,
     1 token 7.4 / 6.2, 16 10.4 / 8.4, 8 of rank 32 9.3 / 8.9, gated 1024 -> 2 x 3 Ki 9.6 / 7.7 (rank 32: 9.9 / 11.0), 2048 -> 1024 8.1 / 7.3; but 16 tokens of 2048 -> 4096 10.6 / 11.1, 8 of
