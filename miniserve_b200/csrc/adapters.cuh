@@ -109,7 +109,7 @@ __device__ __forceinline__ float adapter_dot(const T* row, const float* v, int r
 
 // ---- terms of few tokens on the tensor cores: sum_j B_s[n, j] v[t, j], v as the sum of PIECES bfloat16 numbers: three hold all of its 24 bits, for outputs in
 // 32 bits; two hold 16, for outputs that are rounded to 8. One (2^-8 of an adapter's share lost) / two, us: 64 tokens of 16 adapters of rank 32, 4096 -> 6144 24.2 / 24.3, 32 of 1024 -> 4096 10.3 / 10.4, 8 of
-// 12288 -> 4096 21.0 / 21.0, 200 beside a product apart 50.8 / 51.1; one / three with outputs in 32 bits: 33.2 / 33.7, 14.2 / 14.6, 42.9 / 43.2, 50.7 / 51.4.
+// 12288 -> 4096 21.0 / 21.0, 200 beside a product apart 50.8 / 51.1; one / three with outputs in 32 bits: 33.2 / 33.8, 14.2 / 14.6, 42.9 / 43.3, 50.7 / 51.4.
 constexpr int NO_SLOT = 0x7fffffff, TERM_PIECES = 2;
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -249,7 +249,8 @@ __device__ __forceinline__ void warp_terms(const Adapters& ad, const float* v, c
           for (int h = 0; h < 2; ++h) {
             const __nv_bfloat162 now = __floats2bfloat162_rn(left[h].x, left[h].y);
             const float2 back = __bfloat1622float2(now);
-            left[h] = make_float2(left[h].x - back.x, left[h].y - back.y);
+            left[h].x = fabsf(back.x) < INFINITY ? left[h].x - back.x : 0.f;  // (infinity and NaN leave nothing)
+            left[h].y = fabsf(back.y) < INFINITY ? left[h].y - back.y : 0.f;
             b[h] = *reinterpret_cast<const uint32_t*>(&now);
           }
 #pragma unroll
