@@ -103,19 +103,15 @@ class AdapterStore:
             raise ValueError(f"adapter {name!r} has a factor that is not finite in 32 bits: {factor}")
         slot = free[0]
         self._settle()  # (a step in flight may still read what the place held)
-        for low in self.products.values():
+        for low in self.products.values():  # (beside all matrices: an earlier adapter's numbers, times a factor of 0, need not be 0)
             low.scale[slot] = 0.0
-        used: dict[int, ops.LowRank] = {}
+            low.a[slot].zero_()
+            low.b[slot].zero_()
         for matrix, (a, b) in pairs.items():
             low, part, first, behind = self.places[matrix]
             r = a.shape[0]
-            if id(low) not in used:
-                low.a[slot].zero_()
-                low.b[slot].zero_()
-                used[id(low)] = low
             low.a[slot, part * low.rank:part * low.rank + r] = a.to(low.a.dtype)
             low.b[slot, first:behind, :r] = b.to(low.b.dtype)
-        for low in used.values():
             low.scale[slot] = factor
         self._settle()  # (steps may run on another stream)
         self.names[name] = slot

@@ -84,3 +84,14 @@ def test_a_rank_of_nothing(tmp_path):
     for r in (0, -4):
         with pytest.raises(ValueError, match="says a rank"):
             AdapterStore(m, 1, 8).load("x", written(tmp_path / "bad", {"a.safetensors": tensors(m, 4, only="q_proj")}, r=r))
+
+
+def test_a_place_keeps_nothing_beside_the_matrices_that_the_next_adapter_does_not_have():
+    """A factor of 0 is not enough: numbers of an earlier adapter may give an infinity, which times 0 is no number."""
+    m = model()
+    store = AdapterStore(m, 1, 8)
+    store.load("wide", {k: 1e38 * t.sign() for k, t in tensors(m, 8).items()})
+    store.unload("wide")
+    store.load("narrow", tensors(m, 2, 1, only="k_proj"))
+    for (_, product), low in store.products.items():
+        assert bool(low.a[0].any()) == bool(low.b[0].any()) == bool(low.scale[0]) == (product == "qkv")
