@@ -22,7 +22,7 @@ from .. import ops
 
 
 def _mix32(x: np.ndarray) -> np.ndarray:
-    """Two rounds of x = ((x >> 16) ^ x) * 0x45D9F3B, then (x >> 16) ^ x, of unsigned 32-bit numbers (held in 64 bits)."""
+    """Two rounds of x = ((x >> 16) ^ x) * 0x45D9F3B, then (x >> 16) ^ x, of unsigned 32-bit numbers (held in 64 bits): Thomas Mueller's integer hash."""
     for _ in range(2):
         x = (((x >> 16) ^ x) * 0x45D9F3B) & 0xFFFFFFFF
     return (x >> 16) ^ x
